@@ -43,7 +43,9 @@ extern "C" {
  * activations; 3: linear + residual add; 4: reference platform switch,
  * weight budget, graph staleness check, grouped linears; 5: RMSNorm, gated
  * RMSNorm and RMSNorm + grouped linears; 6: their MLIR C-interface entries
- * and the bf16 group entries; 7: the accumulation switch).  The model ABI of
+ * and the bf16 group entries; 7: the accumulation switch, later joined by
+ * the residual-add norm and the mixture-of-experts entries, which change
+ * nothing that was there).  The model ABI of
  * the AOT library (llmcp_model_abi_version() == 2,
  * include/llmcp/Support/AotAbi.h:12) is not changed by this library. */
 #define LLMCP_Q8_ABI_VERSION 7
@@ -370,6 +372,41 @@ int llmcp_q8_rmsnorm_linear_group_bf16(
     llmcp_memref_bf16_2d *const *outputs, const int32_t *activations,
     int32_t execution_mode);
 
+/* Rows as Q8_1: `values` int8 [rows, cols], `scales` f32 [rows, cols / 32],
+ * both dense row-major in device memory, as llmcp_q8_quantize_activations
+ * writes them; values 16 B aligned. */
+typedef struct {
+  int8_t *values;
+  float *scales;
+  int64_t rows, cols;
+} llmcp_q8_rows;
+
+/* The residual's addition and the norm after it, with the normed rows as
+ * Q8_1 for the products that follow (llmcp_q8_expert_mlp_rows): sum = input +
+ * residual [M, H], rounded to the rows' type; rstd = f32(1 / sqrt(mean of
+ * sum^2 + eps)); normed = (sum * rstd) * w in f32, rounded to the type, with w
+ * + 1 in place of w when zero_centered; quantized = the Q8_1 of normed as
+ * stored.  H % 32 == 0, at most 32768.  normed or quantized may be null, not
+ * both; sum and normed may each take the memory of input or residual (same
+ * strides), but not each other's.  No counterpart in the reference, which
+ * has llmcp.add and llmcp.rms_norm apart: the sum of squares is taken in
+ * f64, so the bits do not depend on its order and are not those of
+ * llmcp_q8_rmsnorm, whose f32 sum is serial (they agree to about H * 2^-24;
+ * this one is the nearer to the exact norm).  The weight must be 16 B
+ * aligned (8 B for bf16), quantized->values 16 B; declines otherwise. */
+int llmcp_q8_add_rmsnorm(llmcp_q8_ctx *ctx, const llmcp_memref_f32_2d *input,
+                         const llmcp_memref_f32_2d *residual,
+                         const llmcp_memref_f32_1d *weight, float eps,
+                         int32_t zero_centered, llmcp_memref_f32_2d *sum,
+                         llmcp_memref_f32_2d *normed, llmcp_q8_rows *quantized);
+
+/* bf16 rows and weight. */
+int llmcp_q8_add_rmsnorm_bf16(llmcp_q8_ctx *ctx, const llmcp_memref_bf16_2d *input,
+                              const llmcp_memref_bf16_2d *residual,
+                              const llmcp_memref_bf16_1d *weight, float eps,
+                              int32_t zero_centered, llmcp_memref_bf16_2d *sum,
+                              llmcp_memref_bf16_2d *normed, llmcp_q8_rows *quantized);
+
 /* Fused SwiGLU hidden: h = silu(x . Wg^T) * (x . Wu^T), the pair
  * `linear{activation=silu}` + `mul` that FuseSiluMul produces
  * (FuseLinearActivations.cpp:27-43, LowerToLinalg.cpp:377-393). */
@@ -405,6 +442,101 @@ int llmcp_q8_mlp_bf16(llmcp_q8_ctx *ctx, const llmcp_memref_bf16_2d *input,
                       const llmcp_memref_i8_1d *w_down,
                       llmcp_memref_bf16_2d *hidden,
                       llmcp_memref_bf16_2d *output, int32_t execution_mode);
+
+/* ---- mixture of experts (no counterpart in the reference, whose model is
+ * dense).  A slot is a (token, choice) pair: token t's slots are t * top_k ..
+ * t * top_k + top_k - 1, and experts[slot] (int32, device memory, dense [M,
+ * top_k]) names the expert of each, -1 for none.  An id that is neither an
+ * expert nor -1 counts as none and sets the context's error flag
+ * (llmcp_q8_ctx_check).  Workspaces grow on the first call of a size: make
+ * it eagerly before capturing it into a graph. */
+
+/* Most experts of a stack and most choices per token. */
+#define LLMCP_Q8_MAX_EXPERTS 1024
+#define LLMCP_Q8_MAX_TOP_K 32
+
+/* Uploads a stack of `experts` q8_0_p4 tensors [rows, cols], one after
+ * another (the p4 bytes of one tensor [experts * rows, cols]), laid out once
+ * on the device for the expert entries, which alone take it: a weight
+ * descriptor of the stack's p4 size, experts * rows * (cols + cols / 16), whose
+ * data is host_p4.  rows % 8 == 0, cols % 32 == 0; an expert's device copy
+ * must stay below 4 GiB (declined otherwise).  llmcp_q8_release and the
+ * weight budget apply as to llmcp_q8_upload_p4. */
+int llmcp_q8_upload_experts_p4(llmcp_q8_ctx *ctx, const void *host_p4, int64_t experts,
+                               int64_t rows, int64_t cols, float *repack_ms);
+
+/* Same for a stack already in device memory, which may be freed by the
+ * caller after this call returns (llmcp_q8_register_device_p4). */
+int llmcp_q8_register_device_experts_p4(llmcp_q8_ctx *ctx, const void *dev_p4, int64_t experts,
+                                        int64_t rows, int64_t cols, float *repack_ms);
+
+/* The choice of experts from the router's logits [M, E]: per row the top_k
+ * largest logits in descending order (ties: the lowest index first) into
+ * experts [M, top_k], and scale times their softmax weights into weights [M,
+ * top_k] (f32): exp(l - max) over the sum of all E of them, or of the
+ * chosen ones when normalize.  A logit of -inf or NaN is masked: it is
+ * never chosen and adds nothing to a sum; a row with fewer than top_k others
+ * ends in slots of expert -1 and weight 0.  Logits of +inf share the row's
+ * weight.  E up to LLMCP_Q8_MAX_EXPERTS, top_k up to LLMCP_Q8_MAX_TOP_K and
+ * E (declined otherwise). */
+int llmcp_q8_route(llmcp_q8_ctx *ctx, const llmcp_memref_f32_2d *logits, int32_t top_k,
+                   int32_t normalize, float scale, int32_t *experts, float *weights);
+
+/* bf16 logits (widened exactly). */
+int llmcp_q8_route_bf16(llmcp_q8_ctx *ctx, const llmcp_memref_bf16_2d *logits, int32_t top_k,
+                        int32_t normalize, float scale, int32_t *experts, float *weights);
+
+/* Products grouped by expert: output row s, of M * top_k, is act(x . W_e^T)
+ * with e = experts[s] and x the input's row s / top_k (input of M rows) or s
+ * (input of M * top_k rows).  Each row is bit for bit what llmcp_q8_linear
+ * gives with that expert's weight (the platform's epilogue in block order, in
+ * either accumulation mode); rows of slots without an expert are zero. */
+int llmcp_q8_expert_linear(llmcp_q8_ctx *ctx, const llmcp_memref_f32_2d *input,
+                           const int32_t *experts, int32_t top_k,
+                           const llmcp_memref_i8_1d *weight, llmcp_memref_f32_2d *output,
+                           int32_t activation);
+
+/* bf16 input and output (as llmcp_q8_linear_bf16 per row). */
+int llmcp_q8_expert_linear_bf16(llmcp_q8_ctx *ctx, const llmcp_memref_bf16_2d *input,
+                                const int32_t *experts, int32_t top_k,
+                                const llmcp_memref_i8_1d *weight, llmcp_memref_bf16_2d *output,
+                                int32_t activation);
+
+/* The experts' SwiGLU MLPs and their sum: for each slot h = silu(x . Wg_e^T) *
+ * (x . Wu_e^T) and o = h . Wd_e^T as llmcp_q8_mlp gives them with the expert's
+ * weights, then output[t] = residual[t] + sum over the token's slots, in
+ * order, of weights[slot] * o[slot], an f32 FMA chain from the residual
+ * rounded once.  weights (f32 [M, top_k], nullable: all 1), residual
+ * (nullable: zero; it may be the output's memory).  Slots without an expert
+ * add nothing; a token with none gives its residual.  w_gate and w_up are
+ * stacks of [F, H] (F % 32 == 0), w_down of [H, F]. */
+int llmcp_q8_expert_mlp(llmcp_q8_ctx *ctx, const llmcp_memref_f32_2d *input,
+                        const int32_t *experts, const float *weights, int32_t top_k,
+                        const llmcp_memref_i8_1d *w_gate, const llmcp_memref_i8_1d *w_up,
+                        const llmcp_memref_i8_1d *w_down, const llmcp_memref_f32_2d *residual,
+                        llmcp_memref_f32_2d *output);
+
+/* bf16 input, residual and output; h's factors, h and o are rounded to bf16
+ * as in llmcp_q8_mlp_bf16. */
+int llmcp_q8_expert_mlp_bf16(llmcp_q8_ctx *ctx, const llmcp_memref_bf16_2d *input,
+                             const int32_t *experts, const float *weights, int32_t top_k,
+                             const llmcp_memref_i8_1d *w_gate, const llmcp_memref_i8_1d *w_up,
+                             const llmcp_memref_i8_1d *w_down,
+                             const llmcp_memref_bf16_2d *residual, llmcp_memref_bf16_2d *output);
+
+/* The same on rows that are quantized already (llmcp_q8_add_rmsnorm,
+ * llmcp_q8_quantize_activations). */
+int llmcp_q8_expert_mlp_rows(llmcp_q8_ctx *ctx, const llmcp_q8_rows *input,
+                             const int32_t *experts, const float *weights, int32_t top_k,
+                             const llmcp_memref_i8_1d *w_gate, const llmcp_memref_i8_1d *w_up,
+                             const llmcp_memref_i8_1d *w_down,
+                             const llmcp_memref_f32_2d *residual, llmcp_memref_f32_2d *output);
+int llmcp_q8_expert_mlp_rows_bf16(llmcp_q8_ctx *ctx, const llmcp_q8_rows *input,
+                                  const int32_t *experts, const float *weights, int32_t top_k,
+                                  const llmcp_memref_i8_1d *w_gate, const llmcp_memref_i8_1d *w_up,
+                                  const llmcp_memref_i8_1d *w_down,
+                                  const llmcp_memref_bf16_2d *residual,
+                                  llmcp_memref_bf16_2d *output);
 
 /* llmcp.lm_head (LowerToLinalg.cpp:729-765): f32 logits [M,V] over the tied
  * table, plus the first-maximum index of the last row written to

@@ -93,6 +93,12 @@ EXPORTS = [
     "_mlir_ciface_llmcp_q8_gated_rmsnorm", "_mlir_ciface_llmcp_q8_gated_rmsnorm_bf16",
     "_mlir_ciface_llmcp_q8_rmsnorm_linear_group3_bf16",
     "_mlir_ciface_llmcp_q8_rmsnorm_linear_group4_bf16",
+    "llmcp_q8_add_rmsnorm", "llmcp_q8_add_rmsnorm_bf16",
+    "llmcp_q8_upload_experts_p4", "llmcp_q8_register_device_experts_p4",
+    "llmcp_q8_route", "llmcp_q8_route_bf16",
+    "llmcp_q8_expert_linear", "llmcp_q8_expert_linear_bf16",
+    "llmcp_q8_expert_mlp", "llmcp_q8_expert_mlp_bf16",
+    "llmcp_q8_expert_mlp_rows", "llmcp_q8_expert_mlp_rows_bf16",
 ]
 
 
@@ -203,7 +209,15 @@ def lib():
             I32, [P, P, ctypes.c_float, I32, P] + [P] * 6 + [I32] * 4),
         "_mlir_ciface_llmcp_q8_rmsnorm_linear_group4_bf16": (
             I32, [P, P, ctypes.c_float, I32, P] + [P] * 8 + [I32] * 5),
+        "llmcp_q8_upload_experts_p4": (I, [P, P, I64, I64, I64, F]),
+        "llmcp_q8_register_device_experts_p4": (I, [P, P, I64, I64, I64, F]),
     }
+    for t in ("", "_bf16"):
+        sig["llmcp_q8_add_rmsnorm" + t] = (I, [P, P, P, P, ctypes.c_float, I32, P, P, P])
+        sig["llmcp_q8_route" + t] = (I, [P, P, I32, I32, ctypes.c_float, P, P])
+        sig["llmcp_q8_expert_linear" + t] = (I, [P, P, P, I32, P, P, I32])
+        sig["llmcp_q8_expert_mlp" + t] = (I, [P, P, P, P, I32, P, P, P, P, P])
+        sig["llmcp_q8_expert_mlp_rows" + t] = (I, [P, P, P, P, I32, P, P, P, P, P])
     for name, (res, args) in sig.items():
         fn = getattr(L, name)
         fn.restype = res
@@ -278,6 +292,27 @@ class DeviceBuffer:
             pass
 
 
+class MemRefRows(ctypes.Structure):
+    """llmcp_q8_rows."""
+    _fields_ = [("values", ctypes.c_void_p), ("scales", ctypes.c_void_p),
+                ("rows", ctypes.c_int64), ("cols", ctypes.c_int64)]
+
+
+class Q8Rows:
+    """Rows as Q8_1 in device memory: int8 values [rows, cols] and f32 scales
+    [rows, cols / 32]."""
+
+    def __init__(self, values, scales, rows, cols):
+        self.values, self.scales, self.rows, self.cols = values, scales, rows, cols
+
+    def memref(self):
+        return MemRefRows(_ptr(self.values), _ptr(self.scales), self.rows, self.cols)
+
+
+def _ptr(buf):
+    return buf.ptr if hasattr(buf, "ptr") else buf
+
+
 class Weight:
     """A q8_0_p4 tensor [rows, cols] known to the library's registry."""
 
@@ -289,6 +324,23 @@ class Weight:
     @property
     def nbytes(self):
         return p4_bytes(self.rows, self.cols)
+
+    def memref(self):
+        return i8_memref(self.key, self.nbytes)
+
+
+class Experts:
+    """A stack of q8_0_p4 tensors [experts, rows, cols] in the registry."""
+
+    def __init__(self, ctx, key_ptr, experts, rows, cols, owner=None, repack_ms=None):
+        self.ctx, self.key, self.experts = ctx, key_ptr, experts
+        self.rows, self.cols = rows, cols
+        self.owner = owner  # keeps the host/device bytes alive
+        self.repack_ms = repack_ms
+
+    @property
+    def nbytes(self):
+        return p4_bytes(self.experts * self.rows, self.cols)
 
     def memref(self):
         return i8_memref(self.key, self.nbytes)
@@ -415,6 +467,24 @@ class Context:
         return Weight(self, buf.ptr, rows, cols, owner=buf,
                       repack_ms=ms.value if time_repack else None)
 
+    def upload_experts_p4(self, host_p4, experts, rows, cols, time_repack=False):
+        """A stack of `experts` tensors [rows, cols], their p4 bytes one after
+        another."""
+        host = np.ascontiguousarray(host_p4, dtype=np.uint8)
+        ms = ctypes.c_float(0.0)
+        check(lib().llmcp_q8_upload_experts_p4(self.handle, host.ctypes.data, experts, rows, cols,
+                                               ctypes.byref(ms) if time_repack else None))
+        return Experts(self, host.ctypes.data, experts, rows, cols, owner=host,
+                       repack_ms=ms.value if time_repack else None)
+
+    def register_device_experts_p4(self, buf, experts, rows, cols, time_repack=False):
+        ms = ctypes.c_float(0.0)
+        check(lib().llmcp_q8_register_device_experts_p4(
+            self.handle, buf.ptr, experts, rows, cols,
+            ctypes.byref(ms) if time_repack else None))
+        return Experts(self, buf.ptr, experts, rows, cols, owner=buf,
+                       repack_ms=ms.value if time_repack else None)
+
     def synthesize_p4(self, seed, rows, cols, stddev=0.02, keep_f32=False):
         """Device-generated N(0, stddev^2) weights packed to q8_0_p4.
         Returns (p4 DeviceBuffer, f32 DeviceBuffer or None)."""
@@ -516,6 +586,52 @@ class Context:
         check(self._entry("llmcp_q8_rmsnorm_linear_group", dtype)(
             self.handle, ctypes.byref(xi), ctypes.byref(wv), float(eps),
             1 if zero_centered else 0, ctypes.byref(no), n, wp, yp, acts, MODE[mode]))
+
+    def add_rmsnorm(self, x, r, w, total, m, h, normed=None, quantized=None, eps=1e-6,
+                    zero_centered=False, dtype="f32"):
+        """total = x + r; normed = RMSNorm(total) with weight w [h]; quantized
+        (a Q8Rows) the Q8_1 of normed.  One of the two may be None."""
+        xi, ri, so = (f32_memref(_ptr(b), m, h) for b in (x, r, total))
+        no = f32_memref(_ptr(normed), m, h) if normed is not None else None
+        qo = quantized.memref() if quantized is not None else None
+        wv = i8_memref(_ptr(w), h)
+        check(self._entry("llmcp_q8_add_rmsnorm", dtype)(
+            self.handle, ctypes.byref(xi), ctypes.byref(ri), ctypes.byref(wv), float(eps),
+            1 if zero_centered else 0, ctypes.byref(so),
+            ctypes.byref(no) if no is not None else None,
+            ctypes.byref(qo) if qo is not None else None))
+
+    def route(self, logits, m, experts, top_k, ids, weights, normalize=True, scale=1.0,
+              dtype="f32"):
+        """ids [m, top_k] (int32) and weights [m, top_k] (f32) of the top_k
+        largest of each row's logits [m, experts] (of dtype)."""
+        li = f32_memref(_ptr(logits), m, experts)
+        check(self._entry("llmcp_q8_route", dtype)(
+            self.handle, ctypes.byref(li), int(top_k), 1 if normalize else 0, float(scale),
+            _ptr(ids), _ptr(weights)))
+
+    def expert_linear(self, x, ids, m, top_k, w, y, per_slot=False, activation="none",
+                      dtype="f32"):
+        """y [m * top_k, w.rows]: slot s is act(x row . W[ids[s]]^T), the row
+        s // top_k of x [m, K], or with per_slot row s of x [m * top_k, K]."""
+        xi = f32_memref(_ptr(x), m * top_k if per_slot else m, w.cols)
+        yo = f32_memref(_ptr(y), m * top_k, w.rows)
+        check(self._entry("llmcp_q8_expert_linear", dtype)(
+            self.handle, ctypes.byref(xi), _ptr(ids), int(top_k), ctypes.byref(w.memref()),
+            ctypes.byref(yo), ACT[activation]))
+
+    def expert_mlp(self, x, ids, weights, m, top_k, wg, wu, wd, y, residual=None, dtype="f32"):
+        """y = residual + sum over a token's slots of weights * the expert's
+        SwiGLU MLP of x [m, H] (of dtype, or a Q8Rows)."""
+        rows = isinstance(x, Q8Rows)
+        xi = x.memref() if rows else f32_memref(_ptr(x), m, wg.cols)
+        ri = f32_memref(_ptr(residual), m, wd.rows) if residual is not None else None
+        yo = f32_memref(_ptr(y), m, wd.rows)
+        check(self._entry("llmcp_q8_expert_mlp_rows" if rows else "llmcp_q8_expert_mlp", dtype)(
+            self.handle, ctypes.byref(xi), _ptr(ids),
+            _ptr(weights) if weights is not None else None, int(top_k),
+            ctypes.byref(wg.memref()), ctypes.byref(wu.memref()), ctypes.byref(wd.memref()),
+            ctypes.byref(ri) if ri is not None else None, ctypes.byref(yo)))
 
     def swiglu(self, x, wg, wu, h, m, mode="decode", dtype="f32"):
         xi = f32_memref(x.ptr if hasattr(x, "ptr") else x, m, wg.cols)

@@ -14,7 +14,7 @@ LIB = os.path.join(HERE, "libllmcp_q8.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 SOURCES = ["q8_kernels.hip", "q8_gemv_fma.hip", "q8_gemm.hip", "q8_gemm16.hip",
-           "q8_microbench.hip",
+           "q8_experts.hip", "q8_add_rmsnorm.hip", "q8_microbench.hip",
            "q8_runtime.cpp"]
 
 ROOT = os.path.dirname(HERE)

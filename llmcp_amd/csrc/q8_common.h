@@ -51,6 +51,27 @@ __host__ __device__ constexpr int seg_for(int64_t units) {
   return units == 18 ? 6 : (units == 8 ? 4 : 1);
 }
 
+// Device layout of a stack of experts, [rows, cols] each: an expert is its
+// tiles of 16 rows (the last one padded with zero rows), a tile `steps` of
+// four blocks of K (padded with zero blocks), 2 KiB each, and then `stages`
+// of 512 B of scales for four steps each.  In a step lane l = 16 q + r of a
+// wave finds its MFMA operands, values 8q .. 8q+7 of the tile's row r, at
+// p * 1024 + 16 l for blocks 2p and 2p + 1 (8 B each), in a stage of scales
+// the f16 scales of row r and blocks q, 4 + q, 8 + q, 12 + q at 8 l: every
+// load of a wave is one contiguous run, straight into the registers that the
+// MFMAs read.  (The unit layout serves the GEMV's lanes of consecutive
+// blocks; MFMA operands read from it are 16 B pieces 256 B apart.)
+constexpr int kMaxExperts = 1024;
+struct ExpertLayout {
+  int32_t steps, stages, tiles;
+  int64_t tile_bytes;
+  __host__ __device__ int64_t expert_bytes() const { return tiles * tile_bytes; }
+};
+inline ExpertLayout expert_layout(int64_t rows, int64_t cols) {
+  const int64_t steps = (cols / kBlock + 3) / 4, stages = (steps + 3) / 4;
+  return {(int32_t)steps, (int32_t)stages, (int32_t)((rows + 15) / 16), steps * 2048 + stages * 512};
+}
+
 // Buffer extent and scalar offset of the DMA of stage t of `stages`, `offset`
 // bytes from a base address: the whole 4 GiB that an unsigned offset reaches,
 // or, past the last stage, nothing at offset 0.  A raw buffer load is in range

@@ -211,6 +211,74 @@ hipError_t launch_gated_rmsnorm(const void *x, const void *gate, bool bf16,
                                 int64_t groups, int64_t g, const float *w, float eps,
                                 bool gate_activated, void *y, hipStream_t s);
 
+// Residual add + RMSNorm (q8_add_rmsnorm.hip) of m rows of width h (h % 32 ==
+// 0, at most kAddNormMaxCols): s = x + r, y (nullable) the norm of s, q / qs
+// (nullable) the Q8_1 of y, dense.  Rows and w share their type.  s and y may
+// take the place of x or r.
+constexpr int64_t kAddNormMaxCols = 32768;
+hipError_t launch_add_rmsnorm(const void *x, int64_t ldx, const void *r, int64_t ldr, bool bf16,
+                              int64_t m, int64_t h, const void *w, float eps, bool zero_centered,
+                              void *s, int64_t lds, void *y, int64_t ldy, int8_t *q, float *qs,
+                              hipStream_t stream);
+
+// ---- experts (q8_experts.hip)
+
+// p4 bytes (device) of a stack of experts [rows, cols] -> ExpertLayout.
+hipError_t launch_repack_experts(const uint8_t *p4, uint8_t *out, int64_t experts, int64_t rows,
+                                 int64_t cols, hipStream_t s);
+
+// The top_k largest of `experts` logits per row (ties: lowest index) and
+// their softmax weights, over all or (normalize) the chosen ones, times
+// scale; NaN and -inf are not chosen (id -1, weight 0).  ids, weights [m,
+// top_k].
+constexpr int kMaxTopK = 32;
+hipError_t launch_route(const void *logits, bool bf16, int64_t ld, int64_t m, int32_t experts,
+                        int32_t top_k, bool normalize, float scale, int32_t *ids, float *weights,
+                        hipStream_t s);
+
+// Up to this many slots each workgroup finds the slots of its expert itself;
+// more are sorted by launch_expert_plan first.
+constexpr int64_t kDirectSlots = 256;
+// Slots per tile for `slots` over `experts`, the tiles of launch_expert_plan
+// at most, and its ints (0: no plan).
+int32_t expert_tile_rows(int64_t slots, int64_t experts);
+int64_t expert_max_tiles(int64_t slots, int64_t experts);
+int64_t expert_plan_ints(int64_t slots, int64_t experts);
+hipError_t launch_expert_plan(const int32_t *ids, int64_t slots, int32_t experts, int32_t *plan,
+                              int32_t *err_flag, hipStream_t s);
+
+// y[slot] = act(row of the slot . W[ids[slot]]^T), or (up non-null) the Q8_1
+// of silu(row . W^T) * (row . up^T) into hq / hs; slots without an expert
+// give rows of zeros (the Q8_1 is left alone).  The weights are stacks in
+// ExpertLayout, each expert below 4 GiB.
+struct ExpertLaunch {
+  const int8_t *qa = nullptr;    // dense Q8_1 rows, 16 B aligned
+  const float *sa = nullptr;
+  int32_t per_row = 1;           // slots per input row
+  const int32_t *ids = nullptr;  // [slots]
+  int64_t slots = 0;
+  int32_t experts = 0;
+  const int32_t *plan = nullptr; // launch_expert_plan's, null up to kDirectSlots
+  int32_t *err_flag = nullptr;   // without a plan: set by an id out of range
+  const uint8_t *w = nullptr, *up = nullptr;
+  int64_t rows = 0, cols = 0;    // N and K of an expert
+  int activation = 0;
+  bool fma = true;
+  bool bf16 = false;             // y's type (up: both factors and h rounded)
+  void *y = nullptr;             // [slots, ldy]
+  int64_t ldy = 0;
+  int8_t *hq = nullptr;          // [slots, rows]
+  float *hs = nullptr;           // [slots, rows / 32]
+};
+hipError_t launch_experts(const ExpertLaunch &l, hipStream_t s);
+
+// y[t] = residual[t] (nullable) + sum over j < top_k, in order, of w[t, j]
+// (nullable: 1) * o[t * top_k + j] by f32 FMA; o dense [m * top_k, cols] of
+// y's type, cols % 4 == 0.  residual may be y.
+hipError_t launch_expert_combine(const void *o, const int32_t *ids, const float *w, int32_t top_k,
+                                 int32_t experts, int64_t m, int64_t cols, const void *residual,
+                                 int64_t ldr, void *y, int64_t ldy, bool bf16, hipStream_t s);
+
 hipError_t launch_embedding(const int64_t *tokens, int64_t count,
                             const uint8_t *table, int64_t rows, int64_t cols,
                             void *out, bool out_bf16, int64_t ldo,

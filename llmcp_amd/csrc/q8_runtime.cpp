@@ -30,6 +30,8 @@
 using namespace llmcp_q8;
 
 static_assert(LLMCP_Q8_MAX_GROUP == kMaxGroup, "group size of the C ABI");
+static_assert(LLMCP_Q8_MAX_EXPERTS == kMaxExperts && LLMCP_Q8_MAX_TOP_K == kMaxTopK,
+              "expert limits of the C ABI");
 
 namespace {
 
@@ -77,6 +79,7 @@ struct Tensor {
   uint64_t dev_bytes = 0;
   int64_t rows = 0;
   int64_t cols = 0;
+  int64_t experts = 0;     // > 0: a stack of so many [rows, cols], ExpertLayout
 };
 
 }  // namespace
@@ -113,6 +116,13 @@ struct llmcp_q8_ctx {
   // Tests only (llmcp_q8_test_ctx_gemm_splits): K splits forced on every
   // splittable GEMM of this context in SPLIT_K mode; 0 = chosen by shape.
   int32_t test_splits = 0;
+  // Mixture of experts, grown on demand: the slots sorted by expert, the
+  // SwiGLU's rows as Q8_1 and the experts' outputs.
+  int32_t *plan = nullptr;
+  int8_t *expert_hq = nullptr;
+  float *expert_hs = nullptr;
+  uint8_t *expert_out = nullptr;
+  uint64_t plan_bytes = 0, expert_hq_bytes = 0, expert_hs_bytes = 0, expert_out_bytes = 0;
   // Cap on device bytes of registered weights (0: none).
   uint64_t weight_budget = 0;
   uint64_t weight_bytes = 0;
@@ -153,9 +163,10 @@ const Tensor *find_tensor(llmcp_q8_ctx *ctx, const void *addr) {
 }
 
 // Weight descriptor -> registered tensor, with the verifier's size rule
-// (LLMCPOps.cpp:57-65: size == N * (K + K/16)).
+// (LLMCPOps.cpp:57-65: size == N * (K + K/16)).  `stack`: a stack of experts,
+// and no other tensor; without it never one.
 int resolve_weight(llmcp_q8_ctx *ctx, const llmcp_memref_i8_1d *w,
-                   const Tensor **out) {
+                   const Tensor **out, bool stack = false) {
   if (!w || !w->data) return fail(LLMCP_Q8_EINVAL, "null weight descriptor");
   const void *addr = w->data + w->offset;
   const Tensor *t = find_tensor(ctx, addr);
@@ -165,6 +176,11 @@ int resolve_weight(llmcp_q8_ctx *ctx, const llmcp_memref_i8_1d *w,
   if (w->strides[0] != 1 || (uint64_t)w->sizes[0] != t->key_bytes)
     return fail(LLMCP_Q8_DECLINED,
                 "q8_0_p4 weight size must be N * (K + (K/32)*2)");
+  if ((t->experts > 0) != stack)
+    return fail(LLMCP_Q8_DECLINED,
+                stack ? "weight %p is not a stack of experts"
+                      : "weight %p is a stack of experts: only the expert entries take it",
+                addr);
   *out = t;
   return LLMCP_Q8_OK;
 }
@@ -360,17 +376,25 @@ int ensure_decode_scratch(llmcp_q8_ctx *ctx, int64_t rows, int64_t cols) {
   return grow(ctx, ctx->hf, ctx->hf_bytes, (uint64_t)rows * 4, "mlp hidden");
 }
 
+// Bytes of a p4 tensor, or of a stack of `experts` of them.
+uint64_t p4_bytes_for(int64_t rows, int64_t cols, int64_t experts) {
+  return (uint64_t)std::max<int64_t>(experts, 1) * (uint64_t)rows * (uint64_t)(cols / kBlock) * 34u;
+}
+
 // Repacks device p4 bytes into a new device tensor for `key` (not yet
-// registered).  The weight budget counts `pending` bytes staged alongside.
+// registered), experts > 0: a stack of so many.  The weight budget counts
+// `pending` bytes staged alongside.
 int stage_from_device_p4(llmcp_q8_ctx *ctx, const void *key,
                          const uint8_t *dev_p4, int64_t rows, int64_t cols,
-                         float *repack_ms, uint64_t pending, Tensor &t) {
+                         float *repack_ms, uint64_t pending, Tensor &t, int64_t experts = 0) {
   t = Tensor();
   t.key = (uintptr_t)key;
   t.rows = rows;
   t.cols = cols;
-  t.key_bytes = (uint64_t)rows * (uint64_t)(cols / kBlock) * 34u;
-  t.dev_bytes = (uint64_t)device_bytes_for(rows, cols);
+  t.experts = experts;
+  t.key_bytes = p4_bytes_for(rows, cols, experts);
+  t.dev_bytes = experts ? (uint64_t)(experts * expert_layout(rows, cols).expert_bytes())
+                        : (uint64_t)device_bytes_for(rows, cols);
   if (ctx->weight_budget &&
       ctx->weight_bytes + pending + t.dev_bytes > ctx->weight_budget)
     return fail(LLMCP_Q8_ENOMEM,
@@ -392,7 +416,8 @@ int stage_from_device_p4(llmcp_q8_ctx *ctx, const void *key,
     if (err == hipSuccess) err = hipEventRecord(e0, ctx->stream);
   }
   if (err == hipSuccess)
-    err = launch_repack(dev_p4, t.dev, rows, cols, ctx->stream);
+    err = experts ? launch_repack_experts(dev_p4, t.dev, experts, rows, cols, ctx->stream)
+                  : launch_repack(dev_p4, t.dev, rows, cols, ctx->stream);
   if (err == hipSuccess && repack_ms) {
     err = hipEventRecord(e1, ctx->stream);
     if (err == hipSuccess) err = hipEventSynchronize(e1);
@@ -420,6 +445,7 @@ int commit_tensors(llmcp_q8_ctx *ctx, std::vector<Tensor> &staged) {
   };
   // workspace for each tensor's input row (and h for the MLP's down GEMV)
   for (const Tensor &t : staged) {
+    if (t.experts) continue;  // (an expert entry's depends on the slots)
     int rc = ensure_decode_scratch(ctx, t.rows, t.cols);
     if (rc) {
       drop_staged();
@@ -459,10 +485,10 @@ int commit_tensors(llmcp_q8_ctx *ctx, std::vector<Tensor> &staged) {
 // One tensor: stage and commit.
 int register_from_device_p4(llmcp_q8_ctx *ctx, const void *key,
                             const uint8_t *dev_p4, int64_t rows, int64_t cols,
-                            float *repack_ms) {
+                            float *repack_ms, int64_t experts = 0) {
   std::vector<Tensor> staged(1);
   int rc = stage_from_device_p4(ctx, key, dev_p4, rows, cols, repack_ms, 0,
-                                staged[0]);
+                                staged[0], experts);
   if (rc) return rc;
   return commit_tensors(ctx, staged);
 }
@@ -470,8 +496,8 @@ int register_from_device_p4(llmcp_q8_ctx *ctx, const void *key,
 // Host p4 bytes -> device staging copy -> staged tensor.
 int stage_from_host_p4(llmcp_q8_ctx *ctx, const void *host_p4, int64_t rows,
                        int64_t cols, float *repack_ms, uint64_t pending,
-                       Tensor &t) {
-  const uint64_t bytes = (uint64_t)rows * (uint64_t)(cols / kBlock) * 34u;
+                       Tensor &t, int64_t experts = 0) {
+  const uint64_t bytes = p4_bytes_for(rows, cols, experts);
   uint8_t *staging = nullptr;
   if (hipMalloc(&staging, bytes) != hipSuccess)
     return fail(LLMCP_Q8_ENOMEM, "staging of %llu bytes",
@@ -479,7 +505,7 @@ int stage_from_host_p4(llmcp_q8_ctx *ctx, const void *host_p4, int64_t rows,
   hipError_t e = hipMemcpyAsync(staging, host_p4, bytes, hipMemcpyHostToDevice,
                                 ctx->stream);
   int rc = e == hipSuccess ? stage_from_device_p4(ctx, host_p4, staging, rows,
-                                                  cols, repack_ms, pending, t)
+                                                  cols, repack_ms, pending, t, experts)
                            : hip_fail(e, "upload");
   (void)hipStreamSynchronize(ctx->stream);
   (void)hipFree(staging);
@@ -489,6 +515,20 @@ int stage_from_host_p4(llmcp_q8_ctx *ctx, const void *host_p4, int64_t rows,
 bool packable(int64_t rows, int64_t cols) {
   // isQ8PackedShape (Q8PackedLayout.h:38-42).
   return rows > 0 && cols > 0 && rows % 8 == 0 && cols % kBlock == 0;
+}
+
+// What the expert kernels can address: each expert's tiles at 32-bit offsets.
+int check_stack(int64_t experts, int64_t rows, int64_t cols) {
+  if (!packable(rows, cols))
+    return fail(LLMCP_Q8_DECLINED, "packed Q8_0 requires rows %% 8 == 0 and cols %% 32 == 0");
+  if (experts < 1 || experts > kMaxExperts)
+    return fail(LLMCP_Q8_DECLINED, "a stack of %lld experts (1 to %d)", (long long)experts,
+                kMaxExperts);
+  if (rows > 1ll << 31 || cols > 1ll << 31 ||
+      expert_layout(rows, cols).tile_bytes > 0xFFFFFFFFll / ((rows + 15) / 16))
+    return fail(LLMCP_Q8_DECLINED, "an expert of [%lld, %lld] reaches 4 GiB", (long long)rows,
+                (long long)cols);
+  return LLMCP_Q8_OK;
 }
 
 uint32_t rd32(const uint8_t *p) {
@@ -606,6 +646,10 @@ int llmcp_q8_ctx_destroy(llmcp_q8_ctx *ctx) {
     if (ctx->hf) (void)hipFree(ctx->hf);
     if (ctx->up) (void)hipFree(ctx->up);
     if (ctx->part) (void)hipFree(ctx->part);
+    if (ctx->plan) (void)hipFree(ctx->plan);
+    if (ctx->expert_hq) (void)hipFree(ctx->expert_hq);
+    if (ctx->expert_hs) (void)hipFree(ctx->expert_hs);
+    if (ctx->expert_out) (void)hipFree(ctx->expert_out);
     {
       std::lock_guard<std::mutex> lock(g_graph_mutex);
       for (auto it = g_graphs.begin(); it != g_graphs.end();)
@@ -846,6 +890,30 @@ int llmcp_q8_register_device_p4(llmcp_q8_ctx *ctx, const void *dev_p4,
     if (rc) return rc;
     return register_from_device_p4(ctx, dev_p4, (const uint8_t *)dev_p4, rows,
                                    cols, repack_ms);
+  });
+}
+
+int llmcp_q8_upload_experts_p4(llmcp_q8_ctx *ctx, const void *host_p4, int64_t experts,
+                               int64_t rows, int64_t cols, float *repack_ms) {
+  return guarded([&]() -> int {
+    if (!ctx || !host_p4) return fail(LLMCP_Q8_EINVAL, "null argument");
+    int rc = check_stack(experts, rows, cols);
+    if (rc || (rc = set_device(ctx))) return rc;
+    std::vector<Tensor> staged(1);
+    rc = stage_from_host_p4(ctx, host_p4, rows, cols, repack_ms, 0, staged[0], experts);
+    if (rc) return rc;
+    return commit_tensors(ctx, staged);
+  });
+}
+
+int llmcp_q8_register_device_experts_p4(llmcp_q8_ctx *ctx, const void *dev_p4, int64_t experts,
+                                        int64_t rows, int64_t cols, float *repack_ms) {
+  return guarded([&]() -> int {
+    if (!ctx || !dev_p4) return fail(LLMCP_Q8_EINVAL, "null argument");
+    int rc = check_stack(experts, rows, cols);
+    if (rc || (rc = set_device(ctx))) return rc;
+    return register_from_device_p4(ctx, dev_p4, (const uint8_t *)dev_p4, rows, cols, repack_ms,
+                                   experts);
   });
 }
 
@@ -1562,6 +1630,219 @@ static int swiglu_impl(llmcp_q8_ctx *ctx, const Rows &in,
                      (const float *)g.data, g.ld);
 }
 
+// ---------------------------------------------- residual add + RMSNorm --
+
+static int add_rmsnorm_impl(llmcp_q8_ctx *ctx, const Rows &in, const Rows &res,
+                            const NormWeight &nw, float eps, int32_t zero_centered,
+                            const Rows &sum, const Rows *normed, const llmcp_q8_rows *q) {
+  int rc = check_norm(in, nw, sum);
+  if (rc) return rc;
+  if (res.rows != in.rows || res.cols != in.cols ||
+      (normed && (normed->rows != in.rows || normed->cols != in.cols)))
+    return fail(LLMCP_Q8_DECLINED, "residual and normed rows must be [M, H] like the input");
+  if (!normed && !q) return fail(LLMCP_Q8_EINVAL, "neither normed nor quantized rows are asked for");
+  if (normed && normed->data == sum.data)
+    return fail(LLMCP_Q8_EINVAL, "sum and normed rows must not share memory");
+  if (q && (!q->values || !q->scales)) return fail(LLMCP_Q8_EINVAL, "null Q8_1 rows");
+  if (q && (q->rows != in.rows || q->cols != in.cols))
+    return fail(LLMCP_Q8_DECLINED, "Q8_1 rows must be [M, H] like the input");
+  if (q && ((uintptr_t)q->values % 16 != 0 || (uintptr_t)q->scales % 4 != 0))
+    return fail(LLMCP_Q8_DECLINED, "Q8_1 values must be 16 B aligned, scales 4 B");
+  if (in.cols > kAddNormMaxCols)
+    return fail(LLMCP_Q8_DECLINED, "residual norm width %lld above %lld", (long long)in.cols,
+                (long long)kAddNormMaxCols);
+  if (in.rows > 0xFFFFFFFFll / 1024)
+    return fail(LLMCP_Q8_DECLINED, "too many rows for one launch (%lld)", (long long)in.rows);
+  if (in.rows == 0) return LLMCP_Q8_OK;
+  if ((rc = set_device(ctx))) return rc;
+  hipError_t e = launch_add_rmsnorm(
+      in.data, in.ld, res.data, res.ld, in.bf16, in.rows, in.cols, nw.data, eps, zero_centered != 0,
+      sum.data, sum.ld, normed ? normed->data : nullptr, normed ? normed->ld : 0,
+      q ? q->values : nullptr, q ? q->scales : nullptr, ctx->stream);
+  if (e != hipSuccess) return hip_fail(e, "residual norm launch");
+  return LLMCP_Q8_OK;
+}
+
+// --------------------------------------------------- mixture of experts --
+
+static int route_impl(llmcp_q8_ctx *ctx, const Rows &logits, int32_t top_k, int32_t normalize,
+                      float scale, int32_t *experts, float *weights) {
+  if (!experts || !weights) return fail(LLMCP_Q8_EINVAL, "null argument");
+  if (logits.cols > kMaxExperts)
+    return fail(LLMCP_Q8_DECLINED, "%lld experts (up to %d)", (long long)logits.cols, kMaxExperts);
+  if (top_k < 1 || top_k > kMaxTopK || top_k > logits.cols)
+    return fail(LLMCP_Q8_DECLINED, "top_k %d of %lld experts (1 to %d)", top_k,
+                (long long)logits.cols, kMaxTopK);
+  if (logits.rows > 0xFFFFFFFFll / 64 - 4)
+    return fail(LLMCP_Q8_DECLINED, "too many rows for one launch (%lld)", (long long)logits.rows);
+  if (logits.rows == 0) return LLMCP_Q8_OK;
+  int rc = set_device(ctx);
+  if (rc) return rc;
+  hipError_t e = launch_route(logits.data, logits.bf16, logits.ld, logits.rows,
+                              (int32_t)logits.cols, top_k, normalize != 0, scale, experts, weights,
+                              ctx->stream);
+  if (e != hipSuccess) return hip_fail(e, "route launch");
+  return LLMCP_Q8_OK;
+}
+
+// Rows that experts read: f32 / bf16 rows or Q8_1 rows.
+struct ExpertRows {
+  const Rows *x = nullptr;
+  const llmcp_q8_rows *q = nullptr;
+  int64_t rows = 0, cols = 0;
+};
+
+// Whether the slots and their rows are within what a launch addresses: slots
+// and a product's workgroups (16 slots by 32 columns at the smallest) in 32
+// bits of work-items.
+static int check_slots(const ExpertRows &in, const int32_t *experts, int32_t top_k, int64_t slots,
+                       int64_t widest) {
+  if (!experts) return fail(LLMCP_Q8_EINVAL, "null expert ids");
+  if (top_k < 1 || top_k > kMaxTopK)
+    return fail(LLMCP_Q8_DECLINED, "top_k %d (1 to %d)", top_k, kMaxTopK);
+  if (slots > 1ll << 30 || (slots / 16 + kMaxExperts + 1) * ((widest + 31) / 32 + 1) > 0xFFFFFFull ||
+      slots * (widest / 4) > 0xFFFFFF00ll || in.rows * (in.cols / 4) > 0xFFFFFF00ll)
+    return fail(LLMCP_Q8_DECLINED, "too many slots for one launch (%lld)", (long long)slots);
+  return LLMCP_Q8_OK;
+}
+
+// The rows' Q8_1: as given, or quantized into the workspace.
+static int expert_quantize(llmcp_q8_ctx *ctx, const ExpertRows &in, ExpertLaunch &l) {
+  if (in.q) {
+    l.qa = in.q->values;
+    l.sa = in.q->scales;
+    return LLMCP_Q8_OK;
+  }
+  const int64_t blocks = in.cols / kBlock;
+  int rc = ensure_scratch(ctx, (uint64_t)(in.rows * in.cols), (uint64_t)(in.rows * blocks * 4));
+  if (rc) return rc;
+  hipError_t e = launch_quantize(in.x->data, in.x->bf16, in.rows, in.x->ld, in.cols, ctx->qa,
+                                 in.cols, ctx->sa, blocks, blocks, ctx->stream);
+  if (e != hipSuccess) return hip_fail(e, "quantize launch");
+  l.qa = ctx->qa;
+  l.sa = ctx->sa;
+  return LLMCP_Q8_OK;
+}
+
+static int expert_plan(llmcp_q8_ctx *ctx, const int32_t *experts, int64_t slots, int64_t count,
+                       ExpertLaunch &l) {
+  l.ids = experts;
+  l.slots = slots;
+  l.experts = (int32_t)count;
+  l.err_flag = ctx->err_flag;
+  l.fma = ctx->fma();
+  if (slots <= kDirectSlots) return LLMCP_Q8_OK;
+  int rc = grow(ctx, ctx->plan, ctx->plan_bytes, (uint64_t)expert_plan_ints(slots, count) * 4,
+                "expert plan");
+  if (rc) return rc;
+  hipError_t e = launch_expert_plan(experts, slots, (int32_t)count, ctx->plan, ctx->err_flag,
+                                    ctx->stream);
+  if (e != hipSuccess) return hip_fail(e, "expert plan launch");
+  l.plan = ctx->plan;
+  return LLMCP_Q8_OK;
+}
+
+static int expert_linear_impl(llmcp_q8_ctx *ctx, const Rows &x, const int32_t *experts,
+                              int32_t top_k, const llmcp_memref_i8_1d *weight, const Rows &out,
+                              int32_t activation) {
+  const Tensor *w = nullptr;
+  int rc = resolve_weight(ctx, weight, &w, true);
+  if (rc) return rc;
+  ExpertRows in;
+  in.x = &x;
+  in.rows = x.rows;
+  in.cols = x.cols;
+  if (x.cols != w->cols)
+    return fail(LLMCP_Q8_DECLINED, "input K %lld != expert K %lld", (long long)x.cols,
+                (long long)w->cols);
+  if (out.cols != w->rows)
+    return fail(LLMCP_Q8_DECLINED, "output N %lld != expert N %lld", (long long)out.cols,
+                (long long)w->rows);
+  if (activation < LLMCP_Q8_ACT_NONE || activation > LLMCP_Q8_ACT_SOFTPLUS)
+    return fail(LLMCP_Q8_DECLINED, "unsupported activation %d", activation);
+  const int64_t slots = out.rows;
+  if ((rc = check_slots(in, experts, top_k, slots, std::max(w->rows, w->cols)))) return rc;
+  if (slots % top_k != 0 || (x.rows != slots && x.rows != slots / top_k))
+    return fail(LLMCP_Q8_DECLINED, "output of %lld rows needs an input of %lld or %lld / top_k",
+                (long long)slots, (long long)slots, (long long)slots);
+  if (slots == 0) return LLMCP_Q8_OK;
+  if ((rc = set_device(ctx))) return rc;
+  ExpertLaunch l;
+  if ((rc = expert_quantize(ctx, in, l)) || (rc = expert_plan(ctx, experts, slots, w->experts, l)))
+    return rc;
+  l.per_row = x.rows == slots ? 1 : top_k;
+  l.w = w->dev;
+  l.rows = w->rows;
+  l.cols = w->cols;
+  l.activation = activation;
+  l.bf16 = out.bf16;
+  l.y = out.data;
+  l.ldy = out.ld;
+  hipError_t e = launch_experts(l, ctx->stream);
+  if (e != hipSuccess) return hip_fail(e, "expert launch");
+  return LLMCP_Q8_OK;
+}
+
+static int expert_mlp_impl(llmcp_q8_ctx *ctx, const ExpertRows &in, const int32_t *experts,
+                           const float *weights, int32_t top_k, const llmcp_memref_i8_1d *w_gate,
+                           const llmcp_memref_i8_1d *w_up, const llmcp_memref_i8_1d *w_down,
+                           const Rows *residual, const Rows &out) {
+  const Tensor *wg = nullptr, *wu = nullptr, *wd = nullptr;
+  int rc = resolve_weight(ctx, w_gate, &wg, true);
+  if (!rc) rc = resolve_weight(ctx, w_up, &wu, true);
+  if (!rc) rc = resolve_weight(ctx, w_down, &wd, true);
+  if (rc) return rc;
+  if (wg->rows != wu->rows || wg->cols != wu->cols || wd->cols != wg->rows ||
+      wd->rows != wg->cols || wg->experts != wu->experts || wg->experts != wd->experts)
+    return fail(LLMCP_Q8_DECLINED, "gate/up [F,H] and down [H,F] stacks differ");
+  const int64_t f = wg->rows, h = wg->cols, m = out.rows;
+  if (f % kBlock) return fail(LLMCP_Q8_DECLINED, "MLP width must be a multiple of 32");
+  if (in.cols != h || out.cols != h || in.rows != m)
+    return fail(LLMCP_Q8_DECLINED, "MLP input/output must be [M, H] row-major");
+  if (residual && (residual->rows != m || residual->cols != h))
+    return fail(LLMCP_Q8_DECLINED, "residual must be [M, H] like the output");
+  if (m > 1ll << 30) return fail(LLMCP_Q8_DECLINED, "too many tokens (%lld)", (long long)m);
+  const int64_t slots = m * top_k;
+  if ((rc = check_slots(in, experts, top_k, slots, std::max(f, h)))) return rc;
+  if (m == 0) return LLMCP_Q8_OK;
+  if ((rc = set_device(ctx))) return rc;
+  if ((rc = grow(ctx, ctx->expert_hq, ctx->expert_hq_bytes, (uint64_t)(slots * f), "expert hidden")) ||
+      (rc = grow(ctx, ctx->expert_hs, ctx->expert_hs_bytes, (uint64_t)(slots * (f / kBlock) * 4),
+                 "expert hidden scales")) ||
+      (rc = grow(ctx, ctx->expert_out, ctx->expert_out_bytes,
+                 (uint64_t)(slots * h) * (out.bf16 ? 2 : 4), "expert outputs")))
+    return rc;
+  ExpertLaunch l;
+  if ((rc = expert_quantize(ctx, in, l)) || (rc = expert_plan(ctx, experts, slots, wg->experts, l)))
+    return rc;
+  l.per_row = top_k;
+  l.w = wg->dev;
+  l.up = wu->dev;
+  l.rows = f;
+  l.cols = h;
+  l.bf16 = out.bf16;
+  l.hq = ctx->expert_hq;
+  l.hs = ctx->expert_hs;
+  hipError_t e = launch_experts(l, ctx->stream);
+  if (e != hipSuccess) return hip_fail(e, "expert SwiGLU launch");
+  l.qa = ctx->expert_hq;
+  l.sa = ctx->expert_hs;
+  l.per_row = 1;
+  l.w = wd->dev;
+  l.up = nullptr;
+  l.rows = h;
+  l.cols = f;
+  l.y = ctx->expert_out;
+  l.ldy = h;
+  e = launch_experts(l, ctx->stream);
+  if (e != hipSuccess) return hip_fail(e, "expert down launch");
+  e = launch_expert_combine(ctx->expert_out, experts, weights, top_k, (int32_t)wg->experts, m, h,
+                            residual ? residual->data : nullptr, residual ? residual->ld : 0,
+                            out.data, out.ld, out.bf16, ctx->stream);
+  if (e != hipSuccess) return hip_fail(e, "expert combine launch");
+  return LLMCP_Q8_OK;
+}
+
 static int lm_head_impl(llmcp_q8_ctx *ctx, const Rows &in,
                         const llmcp_memref_i8_1d *table, const Rows &logits,
                         int64_t *argmax_dev, int32_t execution_mode,
@@ -1934,6 +2215,166 @@ int llmcp_q8_swiglu_bf16(llmcp_q8_ctx *ctx, const llmcp_memref_bf16_2d *input,
     if (!view_of(input, true, in) || !view_of(output, true, out))
       return fail(LLMCP_Q8_DECLINED, kDenseMsg);
     return swiglu_impl(ctx, in, w_gate, w_up, out, execution_mode);
+  });
+}
+
+// ---- residual add + norm, experts
+
+int llmcp_q8_add_rmsnorm(llmcp_q8_ctx *ctx, const llmcp_memref_f32_2d *input,
+                         const llmcp_memref_f32_2d *residual, const llmcp_memref_f32_1d *weight,
+                         float eps, int32_t zero_centered, llmcp_memref_f32_2d *sum,
+                         llmcp_memref_f32_2d *normed, llmcp_q8_rows *quantized) {
+  return guarded([&]() -> int {
+    if (!ctx || !weight) return fail(LLMCP_Q8_EINVAL, "null argument");
+    Rows in, res, s, y;
+    NormWeight nw;
+    if (!view_of(input, false, in) || !view_of(residual, false, res) || !view_of(sum, false, s) ||
+        (normed && !view_of(normed, false, y)) || !norm_weight_of(weight, false, nw))
+      return fail(LLMCP_Q8_DECLINED, kDenseMsg);
+    return add_rmsnorm_impl(ctx, in, res, nw, eps, zero_centered, s, normed ? &y : nullptr, quantized);
+  });
+}
+
+int llmcp_q8_route(llmcp_q8_ctx *ctx, const llmcp_memref_f32_2d *logits, int32_t top_k,
+                   int32_t normalize, float scale, int32_t *experts, float *weights) {
+  return guarded([&]() -> int {
+    if (!ctx) return fail(LLMCP_Q8_EINVAL, "null context");
+    Rows l;
+    if (!view_of(logits, false, l)) return fail(LLMCP_Q8_DECLINED, kDenseMsg);
+    return route_impl(ctx, l, top_k, normalize, scale, experts, weights);
+  });
+}
+
+int llmcp_q8_expert_linear(llmcp_q8_ctx *ctx, const llmcp_memref_f32_2d *input,
+                           const int32_t *experts, int32_t top_k, const llmcp_memref_i8_1d *weight,
+                           llmcp_memref_f32_2d *output, int32_t activation) {
+  return guarded([&]() -> int {
+    if (!ctx) return fail(LLMCP_Q8_EINVAL, "null context");
+    Rows in, out;
+    if (!view_of(input, false, in) || !view_of(output, false, out))
+      return fail(LLMCP_Q8_DECLINED, kDenseMsg);
+    return expert_linear_impl(ctx, in, experts, top_k, weight, out, activation);
+  });
+}
+
+int llmcp_q8_expert_mlp(llmcp_q8_ctx *ctx, const llmcp_memref_f32_2d *input,
+                        const int32_t *experts, const float *weights, int32_t top_k,
+                        const llmcp_memref_i8_1d *w_gate, const llmcp_memref_i8_1d *w_up,
+                        const llmcp_memref_i8_1d *w_down, const llmcp_memref_f32_2d *residual,
+                        llmcp_memref_f32_2d *output) {
+  return guarded([&]() -> int {
+    if (!ctx) return fail(LLMCP_Q8_EINVAL, "null context");
+    Rows x, r, out;
+    if (!view_of(input, false, x) || (residual && !view_of(residual, false, r)) ||
+        !view_of(output, false, out))
+      return fail(LLMCP_Q8_DECLINED, kDenseMsg);
+    ExpertRows in;
+    in.x = &x;
+    in.rows = x.rows;
+    in.cols = x.cols;
+    return expert_mlp_impl(ctx, in, experts, weights, top_k, w_gate, w_up, w_down,
+                           residual ? &r : nullptr, out);
+  });
+}
+
+int llmcp_q8_expert_mlp_rows(llmcp_q8_ctx *ctx, const llmcp_q8_rows *input,
+                             const int32_t *experts, const float *weights, int32_t top_k,
+                             const llmcp_memref_i8_1d *w_gate, const llmcp_memref_i8_1d *w_up,
+                             const llmcp_memref_i8_1d *w_down, const llmcp_memref_f32_2d *residual,
+                             llmcp_memref_f32_2d *output) {
+  return guarded([&]() -> int {
+    if (!ctx || !input || !input->values || !input->scales)
+      return fail(LLMCP_Q8_EINVAL, "null argument");
+    if ((uintptr_t)input->values % 16 != 0 || (uintptr_t)input->scales % 4 != 0)
+      return fail(LLMCP_Q8_DECLINED, "Q8_1 values must be 16 B aligned, scales 4 B");
+    Rows r, out;
+    if ((residual && !view_of(residual, false, r)) || !view_of(output, false, out))
+      return fail(LLMCP_Q8_DECLINED, kDenseMsg);
+    ExpertRows in;
+    in.q = input;
+    in.rows = input->rows;
+    in.cols = input->cols;
+    return expert_mlp_impl(ctx, in, experts, weights, top_k, w_gate, w_up, w_down,
+                           residual ? &r : nullptr, out);
+  });
+}
+
+int llmcp_q8_add_rmsnorm_bf16(llmcp_q8_ctx *ctx, const llmcp_memref_bf16_2d *input,
+                         const llmcp_memref_bf16_2d *residual, const llmcp_memref_bf16_1d *weight,
+                         float eps, int32_t zero_centered, llmcp_memref_bf16_2d *sum,
+                         llmcp_memref_bf16_2d *normed, llmcp_q8_rows *quantized) {
+  return guarded([&]() -> int {
+    if (!ctx || !weight) return fail(LLMCP_Q8_EINVAL, "null argument");
+    Rows in, res, s, y;
+    NormWeight nw;
+    if (!view_of(input, true, in) || !view_of(residual, true, res) || !view_of(sum, true, s) ||
+        (normed && !view_of(normed, true, y)) || !norm_weight_of(weight, true, nw))
+      return fail(LLMCP_Q8_DECLINED, kDenseMsg);
+    return add_rmsnorm_impl(ctx, in, res, nw, eps, zero_centered, s, normed ? &y : nullptr, quantized);
+  });
+}
+
+int llmcp_q8_route_bf16(llmcp_q8_ctx *ctx, const llmcp_memref_bf16_2d *logits, int32_t top_k,
+                   int32_t normalize, float scale, int32_t *experts, float *weights) {
+  return guarded([&]() -> int {
+    if (!ctx) return fail(LLMCP_Q8_EINVAL, "null context");
+    Rows l;
+    if (!view_of(logits, true, l)) return fail(LLMCP_Q8_DECLINED, kDenseMsg);
+    return route_impl(ctx, l, top_k, normalize, scale, experts, weights);
+  });
+}
+
+int llmcp_q8_expert_linear_bf16(llmcp_q8_ctx *ctx, const llmcp_memref_bf16_2d *input,
+                           const int32_t *experts, int32_t top_k, const llmcp_memref_i8_1d *weight,
+                           llmcp_memref_bf16_2d *output, int32_t activation) {
+  return guarded([&]() -> int {
+    if (!ctx) return fail(LLMCP_Q8_EINVAL, "null context");
+    Rows in, out;
+    if (!view_of(input, true, in) || !view_of(output, true, out))
+      return fail(LLMCP_Q8_DECLINED, kDenseMsg);
+    return expert_linear_impl(ctx, in, experts, top_k, weight, out, activation);
+  });
+}
+
+int llmcp_q8_expert_mlp_bf16(llmcp_q8_ctx *ctx, const llmcp_memref_bf16_2d *input,
+                        const int32_t *experts, const float *weights, int32_t top_k,
+                        const llmcp_memref_i8_1d *w_gate, const llmcp_memref_i8_1d *w_up,
+                        const llmcp_memref_i8_1d *w_down, const llmcp_memref_bf16_2d *residual,
+                        llmcp_memref_bf16_2d *output) {
+  return guarded([&]() -> int {
+    if (!ctx) return fail(LLMCP_Q8_EINVAL, "null context");
+    Rows x, r, out;
+    if (!view_of(input, true, x) || (residual && !view_of(residual, true, r)) ||
+        !view_of(output, true, out))
+      return fail(LLMCP_Q8_DECLINED, kDenseMsg);
+    ExpertRows in;
+    in.x = &x;
+    in.rows = x.rows;
+    in.cols = x.cols;
+    return expert_mlp_impl(ctx, in, experts, weights, top_k, w_gate, w_up, w_down,
+                           residual ? &r : nullptr, out);
+  });
+}
+
+int llmcp_q8_expert_mlp_rows_bf16(llmcp_q8_ctx *ctx, const llmcp_q8_rows *input,
+                             const int32_t *experts, const float *weights, int32_t top_k,
+                             const llmcp_memref_i8_1d *w_gate, const llmcp_memref_i8_1d *w_up,
+                             const llmcp_memref_i8_1d *w_down, const llmcp_memref_bf16_2d *residual,
+                             llmcp_memref_bf16_2d *output) {
+  return guarded([&]() -> int {
+    if (!ctx || !input || !input->values || !input->scales)
+      return fail(LLMCP_Q8_EINVAL, "null argument");
+    if ((uintptr_t)input->values % 16 != 0 || (uintptr_t)input->scales % 4 != 0)
+      return fail(LLMCP_Q8_DECLINED, "Q8_1 values must be 16 B aligned, scales 4 B");
+    Rows r, out;
+    if ((residual && !view_of(residual, true, r)) || !view_of(output, true, out))
+      return fail(LLMCP_Q8_DECLINED, kDenseMsg);
+    ExpertRows in;
+    in.q = input;
+    in.rows = input->rows;
+    in.cols = input->cols;
+    return expert_mlp_impl(ctx, in, experts, weights, top_k, w_gate, w_up, w_down,
+                           residual ? &r : nullptr, out);
   });
 }
 
