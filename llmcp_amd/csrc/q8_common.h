@@ -53,23 +53,22 @@ __host__ __device__ constexpr int seg_for(int64_t units) {
 
 // Device layout of a stack of experts, [rows, cols] each: an expert is its
 // tiles of 16 rows (the last one padded with zero rows), a tile `steps` of
-// four blocks of K (padded with zero blocks), 2 KiB each, and then `stages`
-// of 512 B of scales for four steps each.  In a step lane l = 16 q + r of a
-// wave finds its MFMA operands, values 8q .. 8q+7 of the tile's row r, at
-// p * 1024 + 16 l for blocks 2p and 2p + 1 (8 B each), in a stage of scales
-// the f16 scales of row r and blocks q, 4 + q, 8 + q, 12 + q at 8 l: every
-// load of a wave is one contiguous run, straight into the registers that the
-// MFMAs read.  (The unit layout serves the GEMV's lanes of consecutive
-// blocks; MFMA operands read from it are 16 B pieces 256 B apart.)
+// four blocks of K (padded with zero blocks), 2 KiB of values each, and then
+// 128 B of scales for each.  A block of a tile is 512 B, [half][row][16 B]:
+// 16 rows of an MFMA operand on 32 x 32 tiles as they are, and two blocks
+// (1 KiB, lane l's 16 B at 16 l) after two lane swaps those on 16 x 16 tiles.
+// Every load of a wave is one or two contiguous runs, straight into the
+// registers that the MFMAs read.  (The unit layout serves the GEMV's lanes
+// of consecutive blocks; MFMA operands read from it are 16 B pieces 256 B
+// apart.)  The f16 scales of a step are [row][block].
 constexpr int kMaxExperts = 1024;
 struct ExpertLayout {
-  int32_t steps, stages, tiles;
-  int64_t tile_bytes;
-  __host__ __device__ int64_t expert_bytes() const { return tiles * tile_bytes; }
+  int32_t steps, tiles;
+  __host__ __device__ int64_t tile_bytes() const { return (int64_t)steps * 2176; }
+  __host__ __device__ int64_t expert_bytes() const { return tiles * tile_bytes(); }
 };
 inline ExpertLayout expert_layout(int64_t rows, int64_t cols) {
-  const int64_t steps = (cols / kBlock + 3) / 4, stages = (steps + 3) / 4;
-  return {(int32_t)steps, (int32_t)stages, (int32_t)((rows + 15) / 16), steps * 2048 + stages * 512};
+  return {(int32_t)((cols / kBlock + 3) / 4), (int32_t)((rows + 15) / 16)};
 }
 
 // Buffer extent and scalar offset of the DMA of stage t of `stages`, `offset`

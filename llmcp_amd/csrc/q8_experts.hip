@@ -4,8 +4,8 @@
 // The function per row is the other GEMMs': exact int32 block dots, acc =
 // fma(f32(I), sa * dw, acc) or acc + f32(I) * (sa * dw) in block order, so a
 // slot's result is bit for bit what the linear of its expert gives.  A
-// workgroup takes up to 16 RT slots of one expert and a range of the
-// weight's columns; its four waves hold NB tiles of 16 columns each.
+// workgroup takes up to 16, 32 or 64 slots of one expert and a range of the
+// weight's columns.
 #include "q8_kernels.h"
 
 #include <algorithm>
@@ -18,54 +18,43 @@ namespace {
 
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v2i __attribute__((ext_vector_type(2)));
+typedef int v16i __attribute__((ext_vector_type(16)));
 typedef float v16f __attribute__((ext_vector_type(16)));
-
-constexpr int kStageBlocks = 16;               // blocks of K per stage
-constexpr int kStageSteps = 4;                 // of four blocks each
-constexpr int kTileQs = kStageBlocks * 512;    // values of 16 rows and a stage
-constexpr int kTileScales = kStageBlocks * 64; // f32 scales of the same
+typedef float v32f __attribute__((ext_vector_type(32)));
 
 // ------------------------------------------------------------ repack ---- //
 
-// One thread per (tile, step, lane): the lane's MFMA operands of the step's
-// four blocks and their scale (the layout: ExpertLayout in q8_common.h).
+// One thread per (tile, step, lane): 16 B of two of the step's four blocks and
+// one scale (the layout: ExpertLayout in q8_common.h).
 __global__ void repack_experts_kernel(const uint8_t *__restrict__ p4, uint8_t *__restrict__ out,
                                       int64_t experts, int64_t rows, int64_t blocks,
                                       ExpertLayout lay) {
   const int64_t t = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  const int64_t steps = (int64_t)lay.stages * kStageSteps;  // scales cover whole stages
   const int lane = (int)(t & 63), li = lane & 15, lq = lane >> 4;
   const int64_t unit = t >> 6;
-  const int64_t tile = unit / steps;
-  const int step = (int)(unit - tile * steps);
+  const int64_t tile = unit / lay.steps;
+  const int step = (int)(unit - tile * lay.steps);
   if (tile >= experts * lay.tiles) return;
   const int64_t e = tile / lay.tiles;
   const int64_t row = (tile - e * lay.tiles) * 16 + li;
-  uint8_t *base = out + tile * lay.tile_bytes;
-  uint32_t w[4][2] = {};
-  uint16_t scale = 0;
-  if (row < rows) {
-    const int64_t g = (e * rows + row) / kLanes;
-    const int r = (int)((e * rows + row) % kLanes);
+  uint8_t *base = out + tile * lay.tile_bytes();
+  const int64_t g = (e * rows + row) / kLanes;
+  const int r = (int)((e * rows + row) % kLanes);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int64_t b = 4 * step + i;
-      if (b >= blocks) continue;
+  for (int p = 0; p < 2; ++p) {
+    uint32_t w[4] = {0, 0, 0, 0};
+    const int64_t b = 4 * step + 2 * p + (lq >> 1);
+    if (row < rows && b < blocks) {
       const uint8_t *rec = p4 + (g * blocks + b) * kRecord;
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
-        w[i][c] = *(const uint32_t *)(rec + 8 + 16 * (2 * lq + c) + 4 * r);
+      for (int c = 0; c < 4; ++c) w[c] = *(const uint32_t *)(rec + 8 + 16 * (4 * (lq & 1) + c) + 4 * r);
     }
-    const int64_t b = 4 * step + lq;
-    if (b < blocks) scale = *(const uint16_t *)(p4 + (g * blocks + b) * kRecord + 2 * r);
+    *(uint4 *)(base + step * 2048 + p * 1024 + lane * 16) = make_uint4(w[0], w[1], w[2], w[3]);
   }
-  if (step < lay.steps) {
-#pragma unroll
-    for (int p = 0; p < 2; ++p)
-      *(uint4 *)(base + step * 2048 + p * 1024 + lane * 16) =
-          make_uint4(w[2 * p][0], w[2 * p][1], w[2 * p + 1][0], w[2 * p + 1][1]);
-  }
-  *(uint16_t *)(base + lay.steps * 2048 + (step >> 2) * 512 + lane * 8 + 2 * (step & 3)) = scale;
+  const int64_t b = 4 * step + lq;
+  uint16_t scale = 0;
+  if (row < rows && b < blocks) scale = *(const uint16_t *)(p4 + (g * blocks + b) * kRecord + 2 * r);
+  *(uint16_t *)(base + lay.steps * 2048 + step * 128 + li * 8 + lq * 2) = scale;
 }
 
 // -------------------------------------------------------------- plan ---- //
@@ -75,88 +64,137 @@ __device__ __forceinline__ int group_of(int id, int experts) {
   return (unsigned)id < (unsigned)experts ? id : experts;
 }
 
-// Slots sorted by group and the tiles to compute, by one workgroup: plan[0]
-// = tiles, then {group, first, count} per tile, then the slots.  An id that
-// is neither an expert nor -1 sets the error flag.  The order of a group's
-// slots is that of the atomics; no result depends on it.
-__global__ __launch_bounds__(1024) void expert_plan_kernel(const int32_t *__restrict__ ids,
-                                                           int32_t slots, int32_t experts,
-                                                           int32_t rows, int32_t max_tiles,
-                                                           int32_t *__restrict__ plan,
-                                                           int32_t *__restrict__ err) {
-  __shared__ int count[kMaxExperts + 1], start[kMaxExperts + 2], tile0[kMaxExperts + 2];
-  __shared__ int part[2][16];
+// The tiles to compute, by one workgroup: {group, slots} of max_tiles tiles
+// (0 slots: none), then tile_rows slots of each.  A group's tiles are
+// consecutive and alike; tile i of T takes place (i % C) * 8 + i / C with C =
+// ceil(T / 8), so that with places dealt to the XCDs in turn each XCD gets
+// whole runs of them, an expert's on one or two.  An id that is neither an
+// expert nor -1 sets the error flag.  The order of a group's slots is that of
+// the atomics; no result depends on it.
+__device__ void expert_plan(const int32_t *__restrict__ ids, int32_t slots, int32_t experts,
+                            int32_t tile_rows, int32_t max_tiles, int32_t *__restrict__ plan,
+                            int32_t *__restrict__ err) {
+  __shared__ int count[kMaxExperts + 1], tile0[kMaxExperts + 1], per[kMaxExperts + 1];
+  __shared__ int part[16];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   for (int i = t; i <= experts; i += 1024) count[i] = 0;
   __syncthreads();
+  // eight ids per thread in flight together, here and below (one by one, each
+  // waiting for its load, 32768 slots took 40 us)
+  constexpr int kBatch = 8;
   bool bad = false;
-  for (int s = t; s < slots; s += 1024) {
-    const int id = ids[s];
-    bad |= id < -1 || id >= experts;
-    atomicAdd(&count[group_of(id, experts)], 1);
+  for (int s0 = t; s0 < slots; s0 += 1024 * kBatch) {
+    int id[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) id[k] = ids[min(s0 + 1024 * k, slots - 1)];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k)
+      if (s0 + 1024 * k < slots) {
+        bad |= id[k] < -1 || id[k] >= experts;
+        atomicAdd(&count[group_of(id[k], experts)], 1);
+      }
   }
   if (__ballot(bad) && lane == 0) *err = 1;
   __syncthreads();
-  // exclusive prefix sums of the slots and the tiles of the groups
-  int base_s = 0, base_t = 0;
+  // the groups' first tiles (an exclusive prefix sum) and slots per tile, in
+  // whole MFMA tiles
+  const int step = min(tile_rows, 16);
+  int total = 0;
   for (int g0 = 0; g0 <= experts; g0 += 1024) {
     const int g = g0 + t;
     const int c = g <= experts ? count[g] : 0;
-    const int n = (c + rows - 1) / rows;
-    int ps = c, pt = n;
+    const int n = (c + tile_rows - 1) / tile_rows;
+    int pt = n;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-      const int us = __shfl_up(ps, d), ut = __shfl_up(pt, d);
-      if (lane >= d) ps += us, pt += ut;
+      const int u = __shfl_up(pt, d);
+      if (lane >= d) pt += u;
     }
-    if (lane == 63) part[0][wave] = ps, part[1][wave] = pt;
+    if (lane == 63) part[wave] = pt;
     __syncthreads();
-    int os = base_s, ot = base_t;
+    int before = total;
     for (int w = 0; w < 16; ++w) {
-      if (w < wave) os += part[0][w], ot += part[1][w];
-      base_s += part[0][w], base_t += part[1][w];
+      if (w < wave) before += part[w];
+      total += part[w];
     }
-    if (g <= experts) start[g] = os + ps - c, tile0[g] = ot + pt - n;
+    if (g <= experts) {
+      tile0[g] = before + pt - n;
+      per[g] = n ? ((c + step - 1) / step + n - 1) / n * step : step;
+    }
     __syncthreads();
   }
-  if (t == 0) plan[0] = min(base_t, max_tiles);
-  int32_t *const tiles = plan + 4, *const order = tiles + 4 * max_tiles;
+  const int run = (total + 7) / 8;
+  auto place = [&](int i) { return (i % run) * 8 + i / run; };
+  for (int i = t; i < max_tiles; i += 1024) plan[2 * i + 1] = 0;
+  __syncthreads();
   for (int g = t; g <= experts; g += 1024) {
-    const int c = count[g], n = (c + rows - 1) / rows;
-    // a group's tiles alike, in whole 16-row tiles
-    const int per = n ? ((c + 15) / 16 + n - 1) / n * 16 : 0;
-    for (int i = 0; i < n; ++i) {
-      const int at = tile0[g] + i;
-      if (at >= max_tiles) break;
-      const int f = min(i * per, c);
-      *(v4i *)(tiles + 4 * at) = v4i{g, start[g] + f, min(per, c - f), 0};
-    }
+    const int c = count[g];
+    for (int i = 0; i * per[g] < c; ++i)
+      *(v2i *)(plan + 2 * place(tile0[g] + i)) = v2i{g, min(per[g], c - i * per[g])};
   }
   __syncthreads();
   for (int g = t; g <= experts; g += 1024) count[g] = 0;
   __syncthreads();
-  for (int s = t; s < slots; s += 1024) {
-    const int g = group_of(ids[s], experts);
-    order[start[g] + atomicAdd(&count[g], 1)] = s;
+  int32_t *const rows = plan + 2 * max_tiles;
+  for (int s0 = t; s0 < slots; s0 += 1024 * kBatch) {
+    int id[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) id[k] = ids[min(s0 + 1024 * k, slots - 1)];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int s = s0 + 1024 * k;
+      if (s >= slots) continue;
+      const int g = group_of(id[k], experts);
+      const int i = atomicAdd(&count[g], 1);
+      rows[(int64_t)place(tile0[g] + i / per[g]) * tile_rows + i % per[g]] = s;
+    }
   }
 }
 
-// -------------------------------------------------------------- GEMM ---- //
+// What comes before the products of many slots: workgroup 0 plans, the
+// others quantize the rows (x null: nothing to quantize).
+__global__ __launch_bounds__(1024) void expert_prepare_kernel(
+    const int32_t *__restrict__ ids, int32_t slots, int32_t experts, int32_t tile_rows,
+    int32_t max_tiles, int32_t *__restrict__ plan, int32_t *__restrict__ err,
+    const void *__restrict__ x, int bf16, int aligned, int64_t ldx, int64_t m, int32_t blocks,
+    int8_t *__restrict__ qa, float *__restrict__ sa) {
+  if (blockIdx.x == 0) return expert_plan(ids, slots, experts, tile_rows, max_tiles, plan, err);
+  const int64_t unit = ((int64_t)blockIdx.x - 1) * 128 + (threadIdx.x >> 3);  // (row, block)
+  const int64_t row = unit / blocks;
+  const int b = (int)(unit - row * blocks), p = threadIdx.x & 7;
+  const bool live = row < m;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (live) v = load_act4(x, row * ldx + b * kBlock + 4 * p, bf16 != 0, aligned != 0);
+  int32_t q;
+  float s;
+  quantize_block8(v, live, &q, &s);
+  if (!live) return;
+  *(int32_t *)(qa + unit * kBlock + 4 * p) = q;
+  if (p == 0) sa[unit] = s;
+}
+
+// ---------------------------------------------------------- products ---- //
 
 struct ExpertArgs {
   const int8_t *qa;    // Q8_1 rows [.., 32 blocks], dense
   const float *sa;     // their scales [.., blocks]
+  const void *x;       // few slots: the rows themselves, quantized by each
+  int64_t ldx;         //   workgroup (x_type 1: f32, 2: bf16)
+  int32_t x_type;      // 0: qa / sa
+  int32_t x_aligned;
   int32_t per_row;     // slots per input row: slot s reads row s / per_row
   const int32_t *ids;  // [slots]
   int32_t *err;        // without a plan: set by an id that is out of range
   int32_t slots, experts;
-  const int32_t *plan; // expert_plan_kernel's, or null: a tile per slot that
-  int32_t max_tiles;   //   is the first of its group (or of 16 RT of them)
+  const int32_t *plan; // expert_plan's, or null: a tile per slot that is the
+  int32_t max_tiles;   //   first of its group (or of 16 of them)
   const uint8_t *w0, *w1;
   ExpertLayout lay;
   int32_t blocks;      // K / 32
   int32_t rows;        // N of an expert
   int32_t n_groups;    // column ranges
+  int32_t repeat;      // column ranges that a workgroup takes one after another
+  int64_t in_rows;     // rows of qa / sa
   int32_t act;
   int32_t y_bf16, vec; // vec: y takes stores of four values
   void *y;             // [slots, ldy]
@@ -165,316 +203,25 @@ struct ExpertArgs {
   float *hs;
 };
 
-template <int RT, int NB, bool DUAL>
-struct ExpertShape {
-  static constexpr int COLS = 64 * NB / (DUAL ? 2 : 1);  // columns of a workgroup
-  static constexpr int STAGE = RT * (kTileQs + kTileScales);
-  static constexpr int HLD = COLS + 4;                   // h rows in LDS
-  static_assert(RT * 16 * HLD * 4 * (NB == 1 ? 2 : 1) <= 2 * STAGE, "h fits the ring");
-};
-
-// The slots of the workgroup's tile into `rows` (LDS): returns their number,
-// 0 for a workgroup with nothing to do, and their group.
-__device__ __forceinline__ int expert_tile(const ExpertArgs &p, int tile_rows, int &ng, int &group,
-                                           int *rows, int *shared) {
-  if (p.plan) {
-    // equal shares of consecutive (tile, column range) pairs per XCD: a
-    // tile's rows and an expert's weight are fetched into one L2
-    const int total = __builtin_amdgcn_readfirstlane(p.plan[0]) * p.n_groups;
-    const int share = (total + 7) / 8, i = blockIdx.x >> 3;
-    const int at = (blockIdx.x & 7) * share + i;
-    if (i >= share || at >= total) return 0;
-    const int tile = at / p.n_groups;
-    ng = at - tile * p.n_groups;
-    const v4i e = *(const v4i *)(p.plan + 4 + 4 * (int64_t)tile);
-    group = __builtin_amdgcn_readfirstlane(e[0]);
-    const int count = __builtin_amdgcn_readfirstlane(e[2]);
-    if ((int)threadIdx.x < count)
-      rows[threadIdx.x] = p.plan[4 + 4 * (int64_t)p.max_tiles + e[1] + threadIdx.x];
-    __syncthreads();
-    return count;
-  }
-  const int s = blockIdx.x / p.n_groups;
-  ng = blockIdx.x - s * p.n_groups;
-  const int id = __builtin_amdgcn_readfirstlane(p.ids[s]);
-  group = group_of(id, p.experts);
-  if (ng == 0 && threadIdx.x == 0 && (id < -1 || id >= p.experts)) *p.err = 1;
-  if (threadIdx.x < 64) {
-    // the slots of this group before s, and from s on
-    int before = 0, after = 0;
-    const int lane = threadIdx.x;
-    for (int c = 0; c < p.slots; c += 64) {
-      const int i = c + lane;
-      const bool hit = i < p.slots && group_of(p.ids[i], p.experts) == group;
-      before += __popcll(__ballot(hit && i < s));
-    }
-    if (before % tile_rows == 0)
-      for (int c = s & ~63; c < p.slots; c += 64) {
-        const int i = c + lane;
-        const bool hit = i >= s && i < p.slots && group_of(p.ids[i], p.experts) == group;
-        const uint64_t m = __ballot(hit);
-        const int at = after + __popcll(m & ((1ull << lane) - 1));
-        if (hit && at < tile_rows) rows[at] = i;
-        after += __popcll(m);
-      }
-    if (lane == 0) *shared = min(after, tile_rows);
-  }
-  __syncthreads();
-  return __builtin_amdgcn_readfirstlane(*shared);
+// The plan's tile and the column range of this workgroup; its slots into
+// `rows` (LDS, no barrier).  Returns the number of slots.
+__device__ __forceinline__ int planned_tile(const ExpertArgs &p, int tile_rows, int &ng, int &group,
+                                            int *rows) {
+  const int i = blockIdx.x >> 3;
+  const int tile = i / p.n_groups * 8 + (blockIdx.x & 7);
+  ng = i - i / p.n_groups * p.n_groups;
+  if ((int)threadIdx.x < tile_rows)
+    rows[threadIdx.x] = p.plan[2 * (int64_t)p.max_tiles + (int64_t)tile * tile_rows + threadIdx.x];
+  const v2i e = *(const v2i *)(p.plan + 2 * (int64_t)tile);
+  group = __builtin_amdgcn_readfirstlane(e[0]);
+  return __builtin_amdgcn_readfirstlane(e[1]);
 }
 
-// The workgroup's sums over NRT 16-row tiles of slots (NRT <= RT).
-template <int NRT, int RT, int NB, bool FMA, bool DUAL>
-__device__ __forceinline__ void expert_sums(const ExpertArgs &p, int count, const int *rows,
-                                            const uint8_t *const (&wt)[NB], uint8_t *smem,
-                                            float (&acc)[NB][RT][4]) {
-  constexpr int STAGE = ExpertShape<RT, NB, DUAL>::STAGE;
-  const int tid = threadIdx.x, lane = tid & 63, li = lane & 15, lq = lane >> 4;
-  const int steps = p.lay.steps, stages = p.lay.stages;
-  // ---- rows into LDS: thread (row li, 16 B piece g and g + 16 of 32)
-  const int g = tid >> 4;
-  const int8_t *src[NRT];
-  const float *ssrc[NRT];
-  bool live[NRT];
-#pragma unroll
-  for (int r = 0; r < NRT; ++r) {
-    const int i = 16 * r + li;
-    live[r] = i < count;
-    const int64_t row = rows[live[r] ? i : 0] / p.per_row;
-    src[r] = p.qa + row * p.blocks * kBlock;
-    ssrc[r] = p.sa + row * p.blocks;
-  }
-  v4i av[NRT][2];
-  float as[NRT];
-  auto load_rows = [&](int stage) __attribute__((always_inline)) {
-    const int b0 = stage * kStageBlocks;
-#pragma unroll
-    for (int r = 0; r < NRT; ++r) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int b = min(b0 + 8 * h + (g >> 1), p.blocks - 1);
-        av[r][h] = *(const v4i *)(src[r] + b * kBlock + 16 * (g & 1));
-      }
-      as[r] = ssrc[r][min(b0 + g, p.blocks - 1)];
-    }
-  };
-  auto store_rows = [&](int stage) __attribute__((always_inline)) {
-    uint8_t *const at = smem + (stage & 1) * STAGE;
-    const int b0 = stage * kStageBlocks;
-#pragma unroll
-    for (int r = 0; r < NRT; ++r) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int b = 8 * h + (g >> 1);
-        v4i v = av[r][h];
-        if (!live[r] || b0 + b >= p.blocks) v = v4i{0, 0, 0, 0};
-        uint8_t *const to = at + r * kTileQs + (b >> 1) * 1024 + 2 * (g & 1) * 256 + li * 16 + (b & 1) * 8;
-        *(v2i *)to = v2i{v[0], v[1]};
-        *(v2i *)(to + 256) = v2i{v[2], v[3]};
-      }
-      const bool ok = live[r] && b0 + g < p.blocks;
-      *(float *)(at + RT * kTileQs + r * kTileScales + g * 64 + li * 4) = ok ? as[r] : 0.0f;
-    }
-  };
-  // ---- weights: a stage of each tile in registers, each step's replaced by
-  // the next stage's as soon as its MFMAs have taken it
-  v4i wq[NB][kStageSteps][2];
-  uint2 wd[NB], wdn[NB];
-  auto load_step = [&](int stage, int q) __attribute__((always_inline)) {
-    const int st = min(stage * kStageSteps + q, steps - 1);
-#pragma unroll
-    for (int t = 0; t < NB; ++t)
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-        wq[t][q][j] = __builtin_nontemporal_load(
-            (const v4i *)(wt[t] + (uint32_t)st * 2048u + j * 1024 + lane * 16));
-  };
-  auto load_scales = [&](int stage, uint2 (&d)[NB]) __attribute__((always_inline)) {
-    const int sg = min(stage, stages - 1);
-#pragma unroll
-    for (int t = 0; t < NB; ++t)
-      d[t] = *(const uint2 *)(wt[t] + (uint32_t)steps * 2048u + sg * 512 + lane * 8);
-  };
-  load_rows(0);
-  load_scales(0, wd);
-#pragma unroll
-  for (int q = 0; q < kStageSteps; ++q) load_step(0, q);
-  store_rows(0);
-  __syncthreads();
-#pragma unroll
-  for (int t = 0; t < NB; ++t)
-#pragma unroll
-    for (int r = 0; r < NRT; ++r)
-#pragma unroll
-      for (int v = 0; v < 4; ++v) acc[t][r][v] = 0.0f;
-
-  for (int s = 0; s < stages; ++s) {
-    const uint8_t *const at = smem + (s & 1) * STAGE;
-    load_rows(s + 1 < stages ? s + 1 : s);
-    load_scales(s + 1, wdn);
-#pragma unroll
-    for (int q = 0; q < kStageSteps; ++q) {
-      if (s * kStageSteps + q >= steps) break;
-#pragma unroll
-      for (int r = 0; r < NRT; ++r) {
-        const v4i a0 = *(const v4i *)(at + r * kTileQs + (2 * q) * 1024 + lane * 16);
-        const v4i a1 = *(const v4i *)(at + r * kTileQs + (2 * q + 1) * 1024 + lane * 16);
-        const float sa = *(const float *)(at + RT * kTileQs + r * kTileScales + (4 * q + lq) * 64 + li * 4);
-#pragma unroll
-        for (int t = 0; t < NB; ++t) {
-          const uint32_t dw = q < 2 ? wd[t].x : wd[t].y;
-          const v16f z = {};
-          const v16f f = __builtin_amdgcn_mfma_f32_16x16x1f32(
-              half_bits_to_float((q & 1) ? dw >> 16 : dw & 0xffffu), sa, z, 0, 0, 0);
-          v4i c[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const v4i w = wq[t][q][j >> 1], a = j < 2 ? a0 : a1;
-            const v2i wv = (j & 1) ? v2i{w[2], w[3]} : v2i{w[0], w[1]};
-            const v2i xv = (j & 1) ? v2i{a[2], a[3]} : v2i{a[0], a[1]};
-            c[j] = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, wv),
-                                                         __builtin_bit_cast(long, xv),
-                                                         v4i{0, 0, 0, 0}, 0, 0, 0);
-          }
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int v = 0; v < 4; ++v) {
-              const float dot = (float)c[j][v];
-              if (FMA) {
-                acc[t][r][v] = __builtin_fmaf(dot, f[4 * j + v], acc[t][r][v]);
-              } else {
-                const float contrib = dot * f[4 * j + v];
-                acc[t][r][v] = acc[t][r][v] + contrib;
-              }
-            }
-        }
-      }
-      load_step(s + 1, q);
-    }
-#pragma unroll
-    for (int t = 0; t < NB; ++t) wd[t] = wdn[t];
-    if (s + 1 < stages) store_rows(s + 1);
-    __syncthreads();
-  }
-}
-
-template <int NRT, int RT, int NB, bool FMA, bool DUAL>
-__device__ __forceinline__ void expert_tile_run(const ExpertArgs &p, int ng, int group, int count,
-                                                const int *rows, uint8_t *smem) {
-  typedef ExpertShape<RT, NB, DUAL> Sh;
-  const int lane = threadIdx.x & 63, li = lane & 15, lq = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int col0 = ng * Sh::COLS;
-  // the wave's tiles of 16 columns (a wave past the last repeats it)
-  const uint8_t *wt[NB];
-  int tile[NB];
-#pragma unroll
-  for (int t = 0; t < NB; ++t) {
-    const bool up = DUAL && (NB == 2 ? t == 1 : (wave & 1) != 0);
-    const int i = DUAL ? (NB == 2 ? wave : wave >> 1) : wave * NB + t;
-    tile[t] = col0 / 16 + i;
-    const int c = min(tile[t], p.lay.tiles - 1);
-    wt[t] = (up ? p.w1 : p.w0) + (int64_t)group * p.lay.expert_bytes() + (uint32_t)c * (uint32_t)p.lay.tile_bytes;
-  }
-  float acc[NB][RT][4];
-  expert_sums<NRT, RT, NB, FMA, DUAL>(p, count, rows, wt, smem, acc);
-
-  if constexpr (!DUAL) {
-#pragma unroll
-    for (int t = 0; t < NB; ++t) {
-      const int n = tile[t] * 16 + 4 * lq;
-#pragma unroll
-      for (int r = 0; r < NRT; ++r) {
-        float o[4];
-#pragma unroll
-        for (int v = 0; v < 4; ++v) o[v] = acc[t][r][v];
-        activate_array(o, p.act);
-        const int i = 16 * r + li;
-        if (i >= count || n >= p.rows) continue;
-        const int64_t at = (int64_t)rows[i] * p.ldy + n;
-        if (p.y_bf16) {
-          uint16_t h[4];
-#pragma unroll
-          for (int v = 0; v < 4; ++v) h[v] = float_to_bf16(o[v]);
-          uint16_t *const y = (uint16_t *)p.y + at;
-          if (p.vec) {
-            *(uint2 *)y = make_uint2(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16);
-          } else {
-#pragma unroll
-            for (int v = 0; v < 4; ++v) y[v] = h[v];
-          }
-        } else {
-          float *const y = (float *)p.y + at;
-          if (p.vec) {
-            *(float4 *)y = make_float4(o[0], o[1], o[2], o[3]);
-          } else {
-#pragma unroll
-            for (int v = 0; v < 4; ++v) y[v] = o[v];
-          }
-        }
-      }
-    }
-  } else {
-    // h = silu(gate) * up through LDS (the ring's place: the last barrier of
-    // the sums lies behind every read of it), then its Q8_1 by rows
-    float *const hb = (float *)smem, *const ub = hb + RT * 16 * Sh::HLD;
-    const int c = 16 * (NB == 2 ? wave : wave >> 1) + 4 * lq;
-    const bool bf16 = p.y_bf16 != 0;
-#pragma unroll
-    for (int r = 0; r < NRT; ++r) {
-      float o[4];
-      if constexpr (NB == 2) {
-#pragma unroll
-        for (int v = 0; v < 4; ++v) o[v] = acc[0][r][v];
-        activate_array(o, ACT_SILU);
-#pragma unroll
-        for (int v = 0; v < 4; ++v)
-          o[v] = bf16 ? bf16_to_float(float_to_bf16(o[v])) * bf16_to_float(float_to_bf16(acc[NB - 1][r][v]))
-                      : o[v] * acc[NB - 1][r][v];
-      } else {
-#pragma unroll
-        for (int v = 0; v < 4; ++v) o[v] = acc[0][r][v];
-        if (!(wave & 1)) activate_array(o, ACT_SILU);
-        if (bf16) {
-#pragma unroll
-          for (int v = 0; v < 4; ++v) o[v] = bf16_to_float(float_to_bf16(o[v]));
-        }
-      }
-      float *const to = (NB == 1 && (wave & 1)) ? ub : hb;
-      *(float4 *)(to + (16 * r + li) * Sh::HLD + c) = make_float4(o[0], o[1], o[2], o[3]);
-    }
-    __syncthreads();
-    constexpr int NBLK = Sh::COLS / 32;
-    const int l8 = threadIdx.x & 7;
-    for (int u = threadIdx.x >> 3; u < NRT * 16 * NBLK; u += 32) {
-      const int r = u / NBLK, b = u - r * NBLK;
-      float4 v = *(const float4 *)(hb + r * Sh::HLD + 32 * b + 4 * l8);
-      if constexpr (NB == 1) {
-        const float4 w = *(const float4 *)(ub + r * Sh::HLD + 32 * b + 4 * l8);
-        v = make_float4(v.x * w.x, v.y * w.y, v.z * w.z, v.w * w.w);
-      }
-      if (bf16)
-        v = make_float4(bf16_to_float(float_to_bf16(v.x)), bf16_to_float(float_to_bf16(v.y)),
-                        bf16_to_float(float_to_bf16(v.z)), bf16_to_float(float_to_bf16(v.w)));
-      int32_t q;
-      float s;
-      quantize_block8(v, true, &q, &s);
-      const int n = col0 + 32 * b;
-      if (r < count && n < p.rows) {
-        const int64_t slot = rows[r];
-        *(int32_t *)(p.hq + slot * p.rows + n + 4 * l8) = q;
-        if (l8 == 0) p.hs[slot * (p.rows / kBlock) + n / kBlock] = s;
-      }
-    }
-  }
-}
-
-// Rows of slots without an expert: zeros.
-template <int COLS>
-__device__ __forceinline__ void expert_zero_rows(const ExpertArgs &p, int ng, int count, const int *rows) {
-  for (int i = threadIdx.x; i < count * COLS; i += 256) {
-    const int r = i / COLS, n = ng * COLS + i % COLS;
+// Rows of slots without an expert: zeros in columns [col0, col0 + cols).
+__device__ __forceinline__ void expert_zero_rows(const ExpertArgs &p, int col0, int cols, int count,
+                                                 const int *rows) {
+  for (int i = threadIdx.x; i < count * cols; i += 256) {
+    const int r = i / cols, n = col0 + i % cols;
     if (n >= p.rows) continue;
     const int64_t at = (int64_t)rows[r] * p.ldy + n;
     if (p.y_bf16) ((uint16_t *)p.y)[at] = 0;
@@ -482,27 +229,611 @@ __device__ __forceinline__ void expert_zero_rows(const ExpertArgs &p, int ng, in
   }
 }
 
-template <int RT, int NB, bool FMA, bool DUAL>
-__global__ __launch_bounds__(256, 2) void expert_kernel(const ExpertArgs p) {
+__device__ __forceinline__ float as_bf16(float v) { return bf16_to_float(float_to_bf16(v)); }
+
+// One step of the platform's chain: acc + dot * f.
+template <bool FMA>
+__device__ __forceinline__ float chain(int dot, float f, float acc) {
+  if (FMA) return __builtin_fmaf((float)dot, f, acc);
+  const float contrib = (float)dot * f;
+  return acc + contrib;
+}
+
+// A barrier that waits for this wave's LDS operations and nothing else: the
+// global loads in flight stay there (__syncthreads waits for them too).
+__device__ __forceinline__ void lds_barrier() {
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+}
+
+typedef unsigned v4u __attribute__((ext_vector_type(4)));
+
+// silu for a result that is rounded to bf16 next: the rounded values of
+// silu_f32 (activate_array), most of them without its f64 exponential.  In
+// f32, exp(-v) = 2^h (1 + l ln 2) with h + l = -v log2(e), h its rounding; the
+// hardware's 2^x and 1/x are good to one step (2^-23), so the result is
+// within 3 * 2^-23 of silu and silu_f32's four roundings 4 * 2^-24: the two
+// differ by less than 2^-20, 16 steps of f32 at the least.  Where no midpoint
+// of bf16 lies within 16 steps both round to the same value; where one does
+// (one value in 2000), or where |v| leaves the range of that reckoning, the
+// array is done again exactly.
+template <int N>
+__device__ __forceinline__ void silu_for_bf16(float (&v)[N]) {
+  float r[N];
+  bool slow = false;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float x = v[i], h = x * -1.44269502f;
+    const float l = __builtin_fmaf(x, -1.92596303e-8f, __builtin_fmaf(x, -1.44269502f, -h));
+    const float e0 = __builtin_amdgcn_exp2f(h);
+    const float e = __builtin_fmaf(e0, l * 0.693147182f, e0);
+    r[i] = x * __builtin_amdgcn_rcpf(1.0f + e);
+    const uint32_t low = __builtin_bit_cast(uint32_t, r[i]) & 0xffffu;
+    const float a = fabsf(x);
+    slow |= low - (0x8000u - 17u) <= 34u || !(a < 80.0f) || (a < 0x1p-100f && x != 0.0f);
+  }
+  if (__builtin_amdgcn_ballot_w64(slow) == 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = r[i];
+  } else {
+    activate_array(v, ACT_SILU);
+  }
+}
+
+// The Q8_1 of h in LDS ([slot][ld] f32, 32 columns from col0 on per block)
+// into hq / hs; threads in groups of eight.
+__device__ __forceinline__ void store_h(const ExpertArgs &p, const float *hb, int ld, int nblk,
+                                        int col0, int count, const int *rows) {
+  const int l8 = threadIdx.x & 7;
+  const int units = (count * nblk + 7) & ~7;  // whole waves
+  for (int u = threadIdx.x >> 3; u < units; u += 32) {
+    const int r = min(u / nblk, count - 1), b = u % nblk;
+    const float4 v = *(const float4 *)(hb + r * ld + 32 * b + 4 * l8);
+    int32_t q;
+    float s;
+    quantize_block8(v, true, &q, &s);
+    const int n = col0 + 32 * b;
+    if (u < count * nblk && n < p.rows) {
+      const int64_t slot = rows[r];
+      *(int32_t *)(p.hq + slot * p.rows + n + 4 * l8) = q;
+      if (l8 == 0) p.hs[slot * (p.rows / kBlock) + n / kBlock] = s;
+    }
+  }
+}
+
+// ---- few slots per expert: up to 4 NV = 4, 8 or 16, on 16 x 16 tiles
+//
+// Bound by the stream of the weights.  The rows are the A operand and the
+// weights B, so a result's slot is its register and lane quarter: slot i is
+// put at row 4 (i % 4) + i / 4, and 4 NV slots need NV of the four registers
+// of each MFMA result: the epilogue of a step of four blocks is 8 NV
+// operations.  Each wave streams its tiles of 16 columns straight into the
+// registers that the MFMAs read, a ring of kFewRing steps, without a pause
+// from tile to tile; the rows stay in LDS for all of them.  A step issues its
+// MFMAs, reads the next step's rows and then runs the epilogue of the step
+// before, so that a lone wave waits for none of them.
+//
+// LDS: [slots][a_ld] values (a block pair's 64 B: quarter, block parity,
+// eight values), [slots][s_ld] scales.
+
+struct FewLds {
+  int steps2;      // steps rounded up to a pair
+  int a_ld, s_ld;  // of a row of values (bytes) and of scales (floats)
+  __host__ __device__ static FewLds of(int steps) {
+    // rows 16 B apart modulo 256 B, scales an odd number of 16 B: what the
+    // lanes of one read take lies in different banks
+    const int s2 = (steps + 1) & ~1;
+    return {s2, s2 * 128 + 16, 4 * (s2 + 1)};
+  }
+  __host__ __device__ int bytes(int n) const { return n * (a_ld + 4 * s_ld); }
+};
+constexpr int kFewHLd = 36;
+constexpr int kFewBox = 2 * 4 * 64 * 4 + 16 * kFewHLd * 4;  // DUAL: up sums, h
+constexpr int kFewLdsMost = 159 * 1024;
+constexpr int kFewRing = 6;  // steps of a wave's tile in flight
+
+// The ring's place q takes step st of the tile at byte `tile` of the expert
+// (st >= live: zeros, without touching memory).  No load is branched around:
+// the compiler counts the loads in flight to know which have come.
+struct FewRing {
+  v4u w[kFewRing][2];
+  uint32_t d[kFewRing];
+};
+__device__ __forceinline__ void few_load(FewRing &ring, int q, const uint8_t *wexp, uint32_t tile,
+                                         int st, int live, int steps, int lane) {
+  const DmaStage a = dma_stage(st, live, tile + (uint32_t)st * 2048u);
+  const DmaStage b = dma_stage(st, live, tile + (uint32_t)steps * 2048u + (uint32_t)st * 128u);
+  const __amdgpu_buffer_rsrc_t r =
+      __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(wexp), 0, a.extent, 0x00020000);
+  constexpr int kNt = 2;  // non-temporal: read once
+  ring.w[q][0] = __builtin_amdgcn_raw_buffer_load_b128(r, lane * 16, a.offset, kNt);
+  ring.w[q][1] = __builtin_amdgcn_raw_buffer_load_b128(r, lane * 16 + 1024, a.offset, kNt);
+  ring.d[q] = __builtin_amdgcn_raw_buffer_load_b16(r, (lane & 15) * 8 + (lane >> 4) * 2, b.offset, kNt);
+}
+
+// A step's dots (four blocks) and scale products.
+struct FewDots {
+  v4i c[4];
+  v16f f;
+};
+
+template <int NV, bool FMA, bool DUAL>
+__device__ __forceinline__ void few_run(const ExpertArgs &p, int ng, int count, const int *rows,
+                                        const uint8_t *wexp, FewRing &ring, const uint8_t *smem,
+                                        int used, float *box) {
+  const int lane = threadIdx.x & 63, li = lane & 15, lq = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int steps = p.lay.steps;
+  const FewLds lds = FewLds::of(steps);
+  const int stages = (lds.steps2 + kFewRing - 1) / kFewRing;
+  // the slot at MFMA row li (any other's data for a row past the last)
+  const int mine = min((li >> 2) + 4 * (li & 3), count - 1);
+  const uint8_t *const a = smem + mine * lds.a_ld + lq * 16;
+  const float *const sa = (const float *)(smem + used * lds.a_ld) + mine * lds.s_ld + lq;
+  const uint32_t tile_bytes = (uint32_t)p.lay.tile_bytes();
+  auto tile_of = [&](int it) {
+    return DUAL ? (ng * p.repeat + it) * 2 + (wave >> 1) : (ng * p.repeat + it) * 4 + wave;
+  };
+  v4i x0, x1;
+  float sx;
+  auto read_rows = [&](int st) __attribute__((always_inline)) {
+    x0 = *(const v4i *)(a + st * 128);
+    x1 = *(const v4i *)(a + st * 128 + 64);
+    sx = sa[4 * st];
+  };
+  auto dots = [&](FewDots &o, const v4u (&w)[2], uint32_t d) __attribute__((always_inline)) {
+    const v16f z = {};
+    o.f = __builtin_amdgcn_mfma_f32_16x16x1f32(sx, half_bits_to_float(d), z, 0, 0, 0);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      // lanes 0-31 hold the pair's even block, 32-63 the odd one; the swap
+      // leaves each block its own operand, eights 0, 2, 1, 3
+      const v4i x = j ? x1 : x0;
+      const auto lo = __builtin_amdgcn_permlane32_swap(w[j][0], w[j][2], false, false);
+      const auto hi = __builtin_amdgcn_permlane32_swap(w[j][1], w[j][3], false, false);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const v2i wv = {(int)lo[k], (int)hi[k]};
+        const v2i xv = {x[2 * k], x[2 * k + 1]};
+        o.c[2 * j + k] = __builtin_amdgcn_mfma_i32_16x16x32_i8(
+            __builtin_bit_cast(long, xv), __builtin_bit_cast(long, wv), v4i{0, 0, 0, 0}, 0, 0, 0);
+      }
+    }
+  };
+  float acc[NV];
+  auto epilogue = [&](const FewDots &o) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int v = 0; v < NV; ++v) acc[v] = chain<FMA>(o.c[j][v], o.f[4 * j + v], acc[v]);
+  };
+  read_rows(0);
+  for (int it = 0; it < p.repeat; ++it) {
+    const uint32_t cur = (uint32_t)min(tile_of(it), p.lay.tiles - 1) * tile_bytes;
+    const uint32_t next = (uint32_t)min(tile_of(it + 1), p.lay.tiles - 1) * tile_bytes;
+    const int after = it + 1 < p.repeat ? steps : 0;  // live steps of the next tile
+#pragma unroll
+    for (int v = 0; v < NV; ++v) acc[v] = 0.0f;
+    FewDots even, odd = {};  // (the step before the first: nothing to add)
+    for (int s = 0; s < stages; ++s) {
+      const bool last = s + 1 == stages;
+      const uint32_t from = last ? next : cur;
+      const int st0 = last ? 0 : kFewRing * (s + 1), live = last ? after : steps;
+      static_for<kFewRing / 2>([&](auto Q) __attribute__((always_inline)) {
+        constexpr int q = 2 * decltype(Q)::value;
+        const int st = kFewRing * s + q;
+        if (st < lds.steps2) {
+          dots(even, ring.w[q], ring.d[q]);
+          read_rows(st + 1);
+          __builtin_amdgcn_sched_barrier(0);
+          epilogue(odd);
+          dots(odd, ring.w[q + 1], ring.d[q + 1]);
+          read_rows(st + 2 == lds.steps2 ? 0 : st + 2);
+          __builtin_amdgcn_sched_barrier(0);
+          epilogue(even);
+        }
+        few_load(ring, q, wexp, from, st0 + q, live, steps, lane);
+        few_load(ring, q + 1, wexp, from, st0 + q + 1, live, steps, lane);
+      });
+    }
+    epilogue(odd);
+    const int n = tile_of(it) * 16 + li;
+    if constexpr (!DUAL) {
+      activate_array(acc, p.act);
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        const int i = 4 * v + lq;
+        if (i >= count || n >= p.rows) continue;
+        const int64_t at = (int64_t)rows[i] * p.ldy + n;
+        if (p.y_bf16) ((uint16_t *)p.y)[at] = float_to_bf16(acc[v]);
+        else ((float *)p.y)[at] = acc[v];
+      }
+    } else {
+      // the up wave's sums to the gate wave, h to LDS, its Q8_1 by rows
+      float *const ub = box + (wave >> 1) * 256, *const hb = box + 512;
+      if (wave & 1) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) ub[v * 64 + lane] = acc[v];
+      }
+      lds_barrier();
+      if (!(wave & 1)) {
+        if (p.y_bf16) silu_for_bf16(acc);
+        else activate_array(acc, ACT_SILU);
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+          const float u = ub[v * 64 + lane];
+          const float h = p.y_bf16 ? as_bf16(as_bf16(acc[v]) * as_bf16(u)) : acc[v] * u;
+          hb[(4 * v + lq) * kFewHLd + 16 * (wave >> 1) + li] = h;
+        }
+      }
+      lds_barrier();
+      store_h(p, hb, kFewHLd, 1, (ng * p.repeat + it) * 32, count, rows);
+    }
+  }
+}
+
+template <int NV, bool FMA, bool DUAL>
+__global__ __launch_bounds__(256, 3) void expert_few_kernel(const ExpertArgs p) {
 #ifdef __HIP_DEVICE_COMPILE__
-  typedef ExpertShape<RT, NB, DUAL> Sh;
-  __shared__ __align__(1024) uint8_t smem[2 * Sh::STAGE];
-  __shared__ int rows[16 * RT], shared;
-  int ng = 0, group = 0;
-  const int count = expert_tile(p, 16 * RT, ng, group, rows, &shared);
-  if (count == 0) return;
+  constexpr int TILE = 4 * NV;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ int rows[TILE];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int steps = p.lay.steps;
+  int ng = 0, group = 0, count = 0;
+  if (p.plan) {
+    count = planned_tile(p, TILE, ng, group, rows);
+    if (count == 0) return;
+  } else {
+    // every wave looks over all slots: those of this group before s, and the
+    // tile's from s on
+    const int s = blockIdx.x / p.n_groups;
+    ng = blockIdx.x - s * p.n_groups;
+    int id[kDirectSlots / 64];
+#pragma unroll
+    for (int c = 0; c < kDirectSlots / 64; ++c) id[c] = p.ids[min(64 * c + lane, p.slots - 1)];
+    int own = 0;
+#pragma unroll
+    for (int c = 0; c < kDirectSlots / 64; ++c)
+      if (s >> 6 == c) own = __builtin_amdgcn_readlane(id[c], s & 63);
+    group = group_of(own, p.experts);
+    if (ng == 0 && tid == 0 && (own < -1 || own >= p.experts)) *p.err = 1;
+    int before = 0;
+#pragma unroll
+    for (int c = 0; c < kDirectSlots / 64; ++c) {
+      const int i = 64 * c + lane;
+      const bool hit = i < p.slots && group_of(id[c], p.experts) == group;
+      before += __popcll(__ballot(hit && i < s));
+      const uint64_t m = __ballot(hit && i >= s);
+      const int at = count + __popcll(m & ((1ull << lane) - 1));
+      if (wave == 0 && hit && i >= s && at < TILE) rows[at] = i;
+      count += __popcll(m);
+    }
+    if (before % TILE != 0) return;
+    count = min(count, TILE);
+  }
+  const int cols = (DUAL ? 32 : 64) * p.repeat;
   if (group >= p.experts) {
-    if constexpr (!DUAL) expert_zero_rows<Sh::COLS>(p, ng, count, rows);
+    __syncthreads();
+    if constexpr (!DUAL) expert_zero_rows(p, ng * cols, cols, count, rows);
     return;
   }
-  const int nrt = (count + 15) >> 4;
-  if (RT == 1 || nrt == 1) return expert_tile_run<1, RT, NB, FMA, DUAL>(p, ng, group, count, rows, smem);
-  if constexpr (RT >= 2)
-    if (RT == 2 || nrt == 2) return expert_tile_run<2, RT, NB, FMA, DUAL>(p, ng, group, count, rows, smem);
-  if constexpr (RT >= 4) {
-    if (nrt == 3) return expert_tile_run<3, RT, NB, FMA, DUAL>(p, ng, group, count, rows, smem);
-    return expert_tile_run<4, RT, NB, FMA, DUAL>(p, ng, group, count, rows, smem);
+  // the weights' first steps on their way before anything waits for the rows
+  const uint8_t *const wexp = (DUAL && (wave & 1) ? p.w1 : p.w0) + (int64_t)group * p.lay.expert_bytes();
+  FewRing ring;
+  {
+    const int tile = DUAL ? ng * p.repeat * 2 + (wave >> 1) : ng * p.repeat * 4 + wave;
+    const uint32_t at = (uint32_t)min(tile, p.lay.tiles - 1) * (uint32_t)p.lay.tile_bytes();
+#pragma unroll
+    for (int q = 0; q < kFewRing; ++q) few_load(ring, q, wexp, at, q, steps, steps, lane);
   }
+  lds_barrier();
+  // ---- the rows' Q8_1 into LDS, eight lanes per block
+  const FewLds lds = FewLds::of(steps);
+  const int used = min(TILE, p.slots);  // rows that the LDS holds
+  float *const ls = (float *)(smem + used * lds.a_ld);
+  {
+    const int l8 = tid & 7, padded = 4 * lds.steps2;
+    for (int u0 = 0; u0 < count * padded; u0 += 128) {
+      // four blocks per thread group at once: their loads in flight together
+      float4 v[4];
+      int32_t q[4];
+      float sc[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int u = min(u0 + 32 * k + (tid >> 3), count * padded - 1);
+        const int r = u / padded, b = min(u - r * padded, p.blocks - 1);
+        const int64_t row = rows[r] / p.per_row;
+        if (p.x_type) {
+          v[k] = load_act4(p.x, row * p.ldx + b * kBlock + 4 * l8, p.x_type == 2, p.x_aligned != 0);
+        } else {
+          q[k] = *(const int32_t *)(p.qa + (row * p.blocks + b) * kBlock + 4 * l8);
+          sc[k] = p.sa[row * p.blocks + b];
+        }
+      }
+      if (p.x_type) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) quantize_block8(v[k], true, &q[k], &sc[k]);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int u = u0 + 32 * k + (tid >> 3);
+        if (u >= count * padded) continue;
+        const int r = u / padded, b = u - r * padded;
+        const int quarter = (l8 >> 1 & 1) * 2 + (l8 >> 2);  // eights 0, 2, 1, 3
+        *(int32_t *)(smem + r * lds.a_ld + (b >> 1) * 64 + quarter * 16 + (b & 1) * 8 + (l8 & 1) * 4) = q[k];
+        if (l8 == 0) ls[r * lds.s_ld + b] = b < p.blocks ? sc[k] : 0.0f;
+      }
+    }
+  }
+  lds_barrier();
+  float *const box = (float *)(smem + lds.bytes(used));
+  few_run<NV, FMA, DUAL>(p, ng, count, rows, wexp, ring, smem, used, box);
+#endif
+}
+
+// ---- many slots per expert: up to 64, on 32 x 32 tiles
+//
+// Bound by the exact epilogue, a convert and an FMA per result and block,
+// and by the MFMAs, which do not run under it.  The weights are the A
+// operand: two tiles of 16 rows side by side, for a SwiGLU 16 columns of
+// gate and of up, whose results land in the same lane.
+// v_mfma_i32_32x32x32_i8 gives a block's dots; v_mfma_f32_32x32x1_2b_f32 two
+// scale tiles, of the two tiles of 32 slots (TT = 2) or of two blocks (TT =
+// 1): a unit is two dots and their scales.  Three waves per SIMD cover each
+// other's latencies.  The rows pass through an LDS ring of three steps of four
+// blocks, loaded a step before they are stored there, one barrier a step; a
+// workgroup takes `repeat` column ranges without a pause in either stream.
+
+template <int TT>
+struct ManyLds {
+  // of a step: [tile of 32 slots][block][half][slot][16 B], halves 16 B apart
+  // modulo 256 B and scales [block][slot], blocks 64 B apart modulo 256 B, so
+  // that the stores, eight pieces of a row or four scales side by side, lie
+  // in different banks
+  static constexpr int HALF = 528, BLOCK = 2 * HALF, TILE = 4 * BLOCK;
+  static constexpr int SBLOCK = TT * 128 + 64;
+  static constexpr int A = TT * TILE, BUF = A + 4 * SBLOCK;
+  static constexpr int RING = 3 * BUF;
+  static constexpr int HLD = 68;
+  static constexpr int H = TT * 32 * HLD * 4;
+};
+
+template <int TT, bool FMA, bool DUAL>
+__device__ __forceinline__ void many_run(const ExpertArgs &p, int ng, int group, int count,
+                                         const int *rows, uint8_t *smem, float *hb) {
+  typedef ManyLds<TT> L;
+  constexpr int U = TT == 2 ? 4 : 2;  // units per step
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int steps = p.lay.steps;
+  // ---- weights: the lane's row of 32 (lanes 16-31 and 48-63: of the second
+  // tile) and half of each block, a step in registers, each block replaced
+  // by the next step's once its MFMA has taken it
+  const int64_t expert = (int64_t)group * p.lay.expert_bytes();
+  const int second = lane >> 4 & 1;
+  const uint8_t *const wbase = (DUAL && second ? p.w1 : p.w0) + expert;
+  const uint32_t tile_bytes = (uint32_t)p.lay.tile_bytes();
+  // the first of the wave's tiles in column range r
+  auto tile_of = [&](int r) { return DUAL ? r * 4 + wave : r * 8 + wave * 2; };
+  const uint8_t *wp, *dp;  // of the step to load next
+  auto seek = [&](int r) __attribute__((always_inline)) {
+    const int t = min(tile_of(r) + (DUAL ? 0 : second), p.lay.tiles - 1);
+    wp = wbase + (uint32_t)t * tile_bytes + hi * 256 + (lane & 15) * 16;
+    dp = wbase + (uint32_t)t * tile_bytes + (uint32_t)steps * 2048u + (lane & 15) * 8;
+  };
+  v4i wq[4];
+  uint2 wd;
+  // ---- rows: thread (slot tid / 8, 16 B piece tid % 8 of a step's 128 B) and
+  // (slot tid / 4, scale tid % 4): a row's bytes of a step side by side in a
+  // wave, so that it asks for few lines.  Past a row's last block they read
+  // the next row's data or (past the last row) zeros, against weights of zero.
+  const __amdgpu_buffer_rsrc_t rq = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<int8_t *>(p.qa), 0, (int)(uint32_t)(p.in_rows * p.blocks * kBlock), 0x00020000);
+  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<float *>(p.sa), 0, (int)(uint32_t)(p.in_rows * p.blocks * 4), 0x00020000);
+  const int piece = tid & 7, sblock = tid & 3;
+  uint32_t src[TT];
+#pragma unroll
+  for (int t = 0; t < TT; ++t)
+    src[t] = (uint32_t)(rows[min(32 * t + (tid >> 3), count - 1)] / p.per_row) * (uint32_t)(p.blocks * kBlock) +
+             16 * piece;
+  const int sslot = (tid >> 2) & (32 * TT - 1);  // (TT = 1: the upper threads repeat)
+  const uint32_t ssrc =
+      (uint32_t)(rows[min(sslot, count - 1)] / p.per_row) * (uint32_t)(p.blocks * 4) + 4 * sblock;
+  v4u xv[TT];
+  float xs;
+  auto load_rows = [&](int step) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < TT; ++t) xv[t] = __builtin_amdgcn_raw_buffer_load_b128(rq, src[t], step * 128, 0);
+    xs = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, ssrc, step * 16, 0));
+    xs = 4 * step + sblock < p.blocks ? xs : 0.0f;  // (no inf against a weight of zero)
+  };
+  uint8_t *const to = smem + piece * L::HALF + (tid >> 3) * 16;
+  uint8_t *const sto = smem + L::A + sblock * L::SBLOCK + sslot * 4;
+  auto store_rows = [&](int buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < TT; ++t) *(v4u *)(to + buf * L::BUF + t * L::TILE) = xv[t];
+    *(float *)(sto + buf * L::BUF) = xs;
+  };
+  // ---- a unit's operands
+  v4i x0, x1;  // TT = 2: the block's two slot tiles, TT = 1: two blocks
+  float sx;
+  const uint8_t *const from = smem + hi * L::HALF + l32 * 16;
+  const uint8_t *const sfrom = smem + L::A + (TT == 2 ? lane * 4 : hi * L::SBLOCK + l32 * 4);
+  auto read_rows = [&](int buf, int u) __attribute__((always_inline)) {
+    const uint8_t *const at = from + buf * L::BUF;
+    x0 = *(const v4i *)(at + (TT == 2 ? u : 2 * u) * L::BLOCK);
+    x1 = *(const v4i *)(at + (TT == 2 ? L::TILE + u * L::BLOCK : (2 * u + 1) * L::BLOCK));
+    sx = *(const float *)(sfrom + buf * L::BUF + (TT == 2 ? u : 2 * u) * L::SBLOCK);
+  };
+  auto scale = [&](int b) __attribute__((always_inline)) -> float {
+    const uint32_t d = b < 2 ? wd.x : wd.y;
+    return half_bits_to_float((b & 1) ? d >> 16 : d & 0xffffu);
+  };
+  float acc[TT][16];
+  const v16i zi = {};
+  const v32f zf = {};
+  auto clear = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < TT; ++t)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) acc[t][v] = 0.0f;
+  };
+
+  // the steps of all column ranges in one sequence: `step` of the range that
+  // is computed, `ahead` of the rows that are loaded (they start over with
+  // each range)
+  const int r0 = ng * p.repeat;
+  const int ranges = min(p.repeat, (p.lay.tiles + (DUAL ? 4 : 8) - 1) / (DUAL ? 4 : 8) - r0);
+  int ahead = 0;
+  auto advance = [&]() { ahead = ahead + 1 == steps ? 0 : ahead + 1; };
+  load_rows(ahead);
+  advance();
+  seek(r0);
+#pragma unroll
+  for (int b = 0; b < 4; ++b) wq[b] = *(const v4i *)(wp + b * 512);
+  wd = *(const uint2 *)dp;
+  store_rows(0);
+  load_rows(ahead);
+  advance();
+  store_rows(1);
+  load_rows(ahead);
+  advance();
+  lds_barrier();
+  read_rows(0, 0);
+  clear();
+  int range = 0, step = 0;
+  int buf = 0, buf1 = 1, buf2 = 2;  // the ring's places of steps 0, + 1, + 2
+  for (;;) {
+    // (that place's last read, of the step before, lies behind a barrier)
+    store_rows(buf2);
+    load_rows(ahead);
+    advance();
+    float dw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) dw[u] = TT == 2 ? scale(u) : hi ? scale(2 * u + 1) : scale(2 * u);
+    // the next step's weights: of this range, or the first of the next one
+    // (of this one again behind the last)
+    const bool done = step + 1 == steps;
+    if (done) {
+      seek(r0 + min(range + 1, ranges - 1));
+    } else {
+      wp += 2048;
+      dp += 128;
+    }
+    wd = *(const uint2 *)dp;
+    static_for<U>([&](auto UU) __attribute__((always_inline)) {
+      constexpr int u = decltype(UU)::value;
+      constexpr int b0 = TT == 2 ? u : 2 * u, b1 = TT == 2 ? u : 2 * u + 1;
+      const v16i d0 = __builtin_amdgcn_mfma_i32_32x32x32_i8(wq[b0], x0, zi, 0, 0, 0);
+      const v32f f = __builtin_amdgcn_mfma_f32_32x32x1f32(dw[u], sx, zf, 0, 0, 0);
+      const v16i d1 = __builtin_amdgcn_mfma_i32_32x32x32_i8(wq[b1], x1, zi, 0, 0, 0);
+      wq[b0] = *(const v4i *)(wp + b0 * 512);
+      if constexpr (b1 != b0) wq[b1] = *(const v4i *)(wp + b1 * 512);
+      // (or the MFMAs, pure operations, are moved down to their first use)
+      asm volatile("" ::"v"(d0), "v"(f), "v"(d1));
+      read_rows(u + 1 == U ? buf1 : buf, (u + 1) % U);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int v = 0; v < 16; ++v) acc[0][v] = chain<FMA>(d0[v], f[v], acc[0][v]);
+#pragma unroll
+      for (int v = 0; v < 16; ++v) acc[TT - 1][v] = chain<FMA>(d1[v], f[16 + v], acc[TT - 1][v]);
+#pragma unroll
+      for (int t = 0; t < TT; ++t)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) asm volatile("" : "+v"(acc[t][v]));
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (u == U - 2) lds_barrier();
+    });
+    ++step;
+    const int free = buf;
+    buf = buf1, buf1 = buf2, buf2 = free;
+    if (!done) continue;
+    const int tile0 = tile_of(r0 + range);
+    if constexpr (!DUAL) {
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        const int i = 32 * t + l32;
+        const int64_t base = (int64_t)rows[min(i, count - 1)] * p.ldy;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float o[4];
+#pragma unroll
+          for (int v = 0; v < 4; ++v) o[v] = acc[t][4 * j + v];
+          activate_array(o, p.act);
+          const int n = tile0 * 16 + 8 * j + 4 * hi;
+          if (i >= count || n >= p.rows) continue;
+          if (p.y_bf16) {
+            uint16_t h[4];
+#pragma unroll
+            for (int v = 0; v < 4; ++v) h[v] = float_to_bf16(o[v]);
+            uint16_t *const y = (uint16_t *)p.y + base + n;
+            if (p.vec) {
+              *(uint2 *)y = make_uint2(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16);
+            } else {
+#pragma unroll
+              for (int v = 0; v < 4; ++v) y[v] = h[v];
+            }
+          } else {
+            float *const y = (float *)p.y + base + n;
+            if (p.vec) {
+              *(float4 *)y = make_float4(o[0], o[1], o[2], o[3]);
+            } else {
+#pragma unroll
+              for (int v = 0; v < 4; ++v) y[v] = o[v];
+            }
+          }
+        }
+      }
+    } else {
+      // h through LDS, then its Q8_1 by rows
+#pragma unroll
+      for (int t = 0; t < TT; ++t)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float o[4];
+#pragma unroll
+          for (int v = 0; v < 4; ++v) o[v] = acc[t][4 * j + v];
+          if (p.y_bf16) silu_for_bf16(o);
+          else activate_array(o, ACT_SILU);
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const float u = acc[t][8 + 4 * j + v];
+            o[v] = p.y_bf16 ? as_bf16(as_bf16(o[v]) * as_bf16(u)) : o[v] * u;
+          }
+          *(float4 *)(hb + (32 * t + l32) * L::HLD + 16 * wave + 8 * j + 4 * hi) =
+              make_float4(o[0], o[1], o[2], o[3]);
+        }
+      lds_barrier();
+      store_h(p, hb, L::HLD, 2, (r0 + range) * 64, count, rows);
+      // (the next write of hb lies behind the barriers of the next range)
+    }
+    if (++range == ranges) break;
+    step = 0;
+    clear();
+  }
+}
+
+template <int TT, bool FMA, bool DUAL>
+__global__ __launch_bounds__(256, 3) void expert_many_kernel(const ExpertArgs p) {
+#ifdef __HIP_DEVICE_COMPILE__
+  __shared__ __align__(1024) uint8_t smem[ManyLds<TT>::RING];
+  __shared__ __align__(16) float hb[DUAL ? ManyLds<TT>::H / 4 : 4];
+  __shared__ int rows[32 * TT];
+  int ng, group;
+  const int count = planned_tile(p, 32 * TT, ng, group, rows);
+  if (count == 0) return;
+  lds_barrier();
+  if (group >= p.experts) {
+    if constexpr (!DUAL) expert_zero_rows(p, ng * 128 * p.repeat, 128 * p.repeat, count, rows);
+    return;
+  }
+  if (TT == 1 || count <= 32) many_run<1, FMA, DUAL>(p, ng, group, count, rows, smem, hb);
+  else many_run<TT, FMA, DUAL>(p, ng, group, count, rows, smem, hb);
 #endif
 }
 
@@ -510,7 +841,9 @@ __global__ __launch_bounds__(256, 2) void expert_kernel(const ExpertArgs p) {
 
 // y[t] = residual[t] + sum over its slots j, in order, of w[t, j] * o[t, j]:
 // an f32 FMA chain from the residual (or zero), rounded once; slots without
-// an expert add nothing.  Four columns per thread.
+// an expert add nothing.  Four columns per thread; eight slots' loads go out
+// together (a slot without an expert loads the first one's: its row is never
+// written, so it is not used).
 template <bool BF16>
 __global__ __launch_bounds__(256) void expert_combine_kernel(
     const void *__restrict__ o, const int32_t *__restrict__ ids, const float *__restrict__ w,
@@ -523,16 +856,27 @@ __global__ __launch_bounds__(256) void expert_combine_kernel(
   const int c = 4 * (int)(i - t * quads);
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
   if (residual) v = load_act4(residual, t * ldr + c, BF16, raligned != 0);
-  for (int j = 0; j < top_k; ++j) {
-    const int64_t s = t * top_k + j;
-    const int id = ids[s];
-    if ((unsigned)id >= (unsigned)experts) continue;
-    const float f = w ? w[s] : 1.0f;
-    const float4 x = load_act4(o, s * cols + c, BF16, true);
-    v.x = __builtin_fmaf(f, x.x, v.x);
-    v.y = __builtin_fmaf(f, x.y, v.y);
-    v.z = __builtin_fmaf(f, x.z, v.z);
-    v.w = __builtin_fmaf(f, x.w, v.w);
+  constexpr int K = 8;
+  for (int j0 = 0; j0 < top_k; j0 += K) {
+    int id[K];
+    float f[K];
+    uint4 x[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int64_t s = t * top_k + min(j0 + k, top_k - 1);
+      id[k] = j0 + k < top_k ? ids[s] : -1;
+      f[k] = w ? w[s] : 1.0f;
+      x[k] = load_raw4<BF16, true>(o, s * cols + c);
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if ((unsigned)id[k] >= (unsigned)experts) continue;
+      const float4 a = act4_of_raw<BF16>(x[k]);
+      v.x = __builtin_fmaf(f[k], a.x, v.x);
+      v.y = __builtin_fmaf(f[k], a.y, v.y);
+      v.z = __builtin_fmaf(f[k], a.z, v.z);
+      v.w = __builtin_fmaf(f[k], a.w, v.w);
+    }
   }
   if (BF16) {
     uint16_t *const to = (uint16_t *)y + t * ldy + c;
@@ -634,7 +978,7 @@ hipError_t launch_repack_experts(const uint8_t *p4, uint8_t *out, int64_t expert
                                  int64_t cols, hipStream_t s) {
   const ExpertLayout lay = expert_layout(rows, cols);
   // a launch holds fewer than 2^32 threads: experts in as many as it takes
-  const int64_t per = (int64_t)lay.tiles * lay.stages * kStageSteps * 64;
+  const int64_t per = (int64_t)lay.tiles * lay.steps * 64;
   const int64_t most = std::max<int64_t>(1, ((1ll << 31) / per));
   for (int64_t e = 0; e < experts; e += most) {
     const int64_t n = std::min(most, experts - e);
@@ -647,39 +991,73 @@ hipError_t launch_repack_experts(const uint8_t *p4, uint8_t *out, int64_t expert
   return hipSuccess;
 }
 
-int32_t expert_tile_rows(int64_t slots, int64_t experts) {
-  const int64_t mean = slots / std::max<int64_t>(1, std::min(slots, experts));
-  return mean <= 10 ? 16 : mean <= 20 ? 32 : 64;
+int32_t expert_tile_rows(int64_t slots, int64_t experts, int64_t widest) {
+  const int64_t some = std::max<int64_t>(1, std::min(slots, experts));
+  const int64_t mean = slots / some;
+  int32_t rows = slots * 2 <= 3 * some ? 4 : mean <= 4 ? 8 : mean <= 10 ? 16 : mean <= 28 ? 32 : 64;
+  // the few-slot kernel keeps its rows in LDS
+  const FewLds lds = FewLds::of((int)((widest / kBlock + 3) / 4));
+  while (rows > 4 && rows <= 16 && lds.bytes(rows) + kFewBox > kFewLdsMost / 2) rows /= 2;
+  return rows <= 16 && lds.bytes(rows) + kFewBox > kFewLdsMost ? 32 : rows;
 }
 
-int64_t expert_max_tiles(int64_t slots, int64_t experts) {
-  return slots / expert_tile_rows(slots, experts) + std::min(slots, experts + 1);
+bool expert_planned(int64_t slots, int32_t tile_rows) {
+  return slots > kDirectSlots || tile_rows > 16;
 }
 
-int64_t expert_plan_ints(int64_t slots, int64_t experts) {
-  return slots <= kDirectSlots ? 0 : 4 + 4 * expert_max_tiles(slots, experts) + slots;
+int64_t expert_max_tiles(int64_t slots, int64_t experts, int32_t tile_rows) {
+  return (slots / tile_rows + std::min(slots, experts + 1) + 7) / 8 * 8;
 }
 
-hipError_t launch_expert_plan(const int32_t *ids, int64_t slots, int32_t experts, int32_t *plan,
-                              int32_t *err_flag, hipStream_t s) {
-  hipLaunchKernelGGL(expert_plan_kernel, dim3(1), dim3(1024), 0, s, ids, (int32_t)slots, experts,
-                     expert_tile_rows(slots, experts), (int32_t)expert_max_tiles(slots, experts), plan,
-                     err_flag);
+int64_t expert_plan_ints(int64_t slots, int64_t experts, int32_t tile_rows) {
+  return expert_max_tiles(slots, experts, tile_rows) * (2 + tile_rows);
+}
+
+hipError_t launch_expert_prepare(const int32_t *ids, int64_t slots, int32_t experts,
+                                 int32_t tile_rows, int32_t *plan, int32_t *err_flag, const void *x, bool bf16, int64_t m, int64_t ldx,
+                                 int64_t cols, int8_t *qa, float *sa, hipStream_t s) {
+  const int64_t wgs = 1 + (x ? (m * (cols / kBlock) + 127) / 128 : 0);
+  if (wgs * 1024 > 0xFFFFFFFFll) return hipErrorInvalidConfiguration;
+  const int aligned = (uintptr_t)x % (bf16 ? 8 : 16) == 0 && ldx % 4 == 0;
+  hipLaunchKernelGGL(expert_prepare_kernel, dim3((unsigned)wgs), dim3(1024), 0, s, ids, (int32_t)slots,
+                     experts, tile_rows, (int32_t)expert_max_tiles(slots, experts, tile_rows), plan,
+                     err_flag, x, bf16 ? 1 : 0, aligned, ldx, m, (int32_t)(cols / kBlock), qa, sa);
   return hipGetLastError();
 }
 
-template <int RT, int NB, bool DUAL>
-static hipError_t launch_shape(ExpertArgs &a, bool fma, hipStream_t s) {
-  constexpr int COLS = ExpertShape<RT, NB, DUAL>::COLS;
-  a.n_groups = (a.rows + COLS - 1) / COLS;
-  const int64_t wgs = a.plan ? ((int64_t)a.max_tiles * a.n_groups + 7) / 8 * 8
-                             : (int64_t)a.slots * a.n_groups;
+// Column ranges of `cols` columns per workgroup for about `tiles` tiles with
+// work: as many as leave `fill` workgroups per CU.
+static void set_repeat(ExpertArgs &a, int64_t tiles, int cols, int fill) {
+  const int64_t groups = (a.rows + cols - 1) / cols;
+  const int64_t want = std::max<int64_t>(1, tiles * groups / ((int64_t)fill * cu_count()));
+  a.n_groups = (int32_t)((groups + std::min(want, groups) - 1) / std::min(want, groups));
+  a.repeat = (int32_t)((groups + a.n_groups - 1) / a.n_groups);
+}
+
+template <int NV, bool DUAL>
+static hipError_t launch_few(ExpertArgs &a, bool fma, hipStream_t s) {
+  const int64_t tiles = a.plan ? a.max_tiles : a.slots;
+  set_repeat(a, std::min(a.slots, a.experts), DUAL ? 32 : 64, 8);
+  const int64_t wgs = tiles * a.n_groups;
   // HIP bounds a grid's work-items by 2^32 - 1
   if (wgs * 256 > 0xFFFFFFFFll) return hipErrorInvalidConfiguration;
+  const size_t lds = FewLds::of(a.lay.steps).bytes(std::min(4 * NV, a.slots)) + (DUAL ? kFewBox : 0);
   if (fma)
-    hipLaunchKernelGGL((expert_kernel<RT, NB, true, DUAL>), dim3((unsigned)wgs), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((expert_few_kernel<NV, true, DUAL>), dim3((unsigned)wgs), dim3(256), lds, s, a);
   else
-    hipLaunchKernelGGL((expert_kernel<RT, NB, false, DUAL>), dim3((unsigned)wgs), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((expert_few_kernel<NV, false, DUAL>), dim3((unsigned)wgs), dim3(256), lds, s, a);
+  return hipGetLastError();
+}
+
+template <int TT, bool DUAL>
+static hipError_t launch_many(ExpertArgs &a, bool fma, hipStream_t s) {
+  set_repeat(a, std::max(a.slots / (32 * TT), std::min(a.slots, a.experts)), DUAL ? 64 : 128, 12);
+  const int64_t wgs = (int64_t)a.max_tiles * a.n_groups;
+  if (wgs * 256 > 0xFFFFFFFFll) return hipErrorInvalidConfiguration;
+  if (fma)
+    hipLaunchKernelGGL((expert_many_kernel<TT, true, DUAL>), dim3((unsigned)wgs), dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((expert_many_kernel<TT, false, DUAL>), dim3((unsigned)wgs), dim3(256), 0, s, a);
   return hipGetLastError();
 }
 
@@ -687,13 +1065,18 @@ hipError_t launch_experts(const ExpertLaunch &l, hipStream_t s) {
   ExpertArgs a = {};
   a.qa = l.qa;
   a.sa = l.sa;
+  a.x = l.x;
+  a.ldx = l.ldx;
+  a.x_type = l.x ? (l.bf16 ? 2 : 1) : 0;
+  a.x_aligned = (uintptr_t)l.x % (l.bf16 ? 8 : 16) == 0 && l.ldx % 4 == 0 ? 1 : 0;
   a.per_row = l.per_row;
+  a.in_rows = l.in_rows;
   a.ids = l.ids;
   a.err = l.err_flag;
   a.slots = (int32_t)l.slots;
   a.experts = l.experts;
   a.plan = l.plan;
-  a.max_tiles = (int32_t)expert_max_tiles(l.slots, l.experts);
+  a.max_tiles = (int32_t)expert_max_tiles(l.slots, l.experts, l.tile_rows);
   a.w0 = l.w;
   a.w1 = l.up;
   a.lay = expert_layout(l.rows, l.cols);
@@ -707,13 +1090,17 @@ hipError_t launch_experts(const ExpertLaunch &l, hipStream_t s) {
   a.hq = l.hq;
   a.hs = l.hs;
   const bool dual = l.up != nullptr;
-  switch (expert_tile_rows(l.slots, l.experts)) {
+  switch (l.tile_rows) {
+    case 4:
+      return dual ? launch_few<1, true>(a, l.fma, s) : launch_few<1, false>(a, l.fma, s);
+    case 8:
+      return dual ? launch_few<2, true>(a, l.fma, s) : launch_few<2, false>(a, l.fma, s);
     case 16:
-      return dual ? launch_shape<1, 1, true>(a, l.fma, s) : launch_shape<1, 1, false>(a, l.fma, s);
+      return dual ? launch_few<4, true>(a, l.fma, s) : launch_few<4, false>(a, l.fma, s);
     case 32:
-      return dual ? launch_shape<2, 2, true>(a, l.fma, s) : launch_shape<2, 2, false>(a, l.fma, s);
+      return dual ? launch_many<1, true>(a, l.fma, s) : launch_many<1, false>(a, l.fma, s);
     default:
-      return dual ? launch_shape<4, 2, true>(a, l.fma, s) : launch_shape<4, 2, false>(a, l.fma, s);
+      return dual ? launch_many<2, true>(a, l.fma, s) : launch_many<2, false>(a, l.fma, s);
   }
 }
 

@@ -236,16 +236,20 @@ hipError_t launch_route(const void *logits, bool bf16, int64_t ld, int64_t m, in
                         int32_t top_k, bool normalize, float scale, int32_t *ids, float *weights,
                         hipStream_t s);
 
-// Up to this many slots each workgroup finds the slots of its expert itself;
-// more are sorted by launch_expert_plan first.
+// Slots per tile for `slots` over `experts` (4, 8, 16, 32 or 64) of weights and rows
+// up to `widest` wide; whether the tiles are planned (launch_expert_prepare)
+// or each workgroup finds the slots of its expert itself, up to kDirectSlots
+// of them; a plan's tiles at most, and its ints.
 constexpr int64_t kDirectSlots = 256;
-// Slots per tile for `slots` over `experts`, the tiles of launch_expert_plan
-// at most, and its ints (0: no plan).
-int32_t expert_tile_rows(int64_t slots, int64_t experts);
-int64_t expert_max_tiles(int64_t slots, int64_t experts);
-int64_t expert_plan_ints(int64_t slots, int64_t experts);
-hipError_t launch_expert_plan(const int32_t *ids, int64_t slots, int32_t experts, int32_t *plan,
-                              int32_t *err_flag, hipStream_t s);
+int32_t expert_tile_rows(int64_t slots, int64_t experts, int64_t widest);
+bool expert_planned(int64_t slots, int32_t tile_rows);
+int64_t expert_max_tiles(int64_t slots, int64_t experts, int32_t tile_rows);
+int64_t expert_plan_ints(int64_t slots, int64_t experts, int32_t tile_rows);
+// The plan and, x non-null, the Q8_1 of its m rows into qa / sa (dense).
+hipError_t launch_expert_prepare(const int32_t *ids, int64_t slots, int32_t experts,
+                                 int32_t tile_rows, int32_t *plan, int32_t *err_flag, const void *x,
+                                 bool bf16, int64_t m, int64_t ldx, int64_t cols, int8_t *qa,
+                                 float *sa, hipStream_t s);
 
 // y[slot] = act(row of the slot . W[ids[slot]]^T), or (up non-null) the Q8_1
 // of silu(row . W^T) * (row . up^T) into hq / hs; slots without an expert
@@ -254,11 +258,15 @@ hipError_t launch_expert_plan(const int32_t *ids, int64_t slots, int32_t experts
 struct ExpertLaunch {
   const int8_t *qa = nullptr;    // dense Q8_1 rows, 16 B aligned
   const float *sa = nullptr;
+  const void *x = nullptr;       // or (no plan) the rows, quantized by each
+  int64_t ldx = 0;               // workgroup; of y's type
   int32_t per_row = 1;           // slots per input row
+  int64_t in_rows = 0;           // rows of qa / sa; qa below 4 GiB
   const int32_t *ids = nullptr;  // [slots]
   int64_t slots = 0;
   int32_t experts = 0;
-  const int32_t *plan = nullptr; // launch_expert_plan's, null up to kDirectSlots
+  int32_t tile_rows = 16;        // expert_tile_rows
+  const int32_t *plan = nullptr; // launch_expert_prepare's, if expert_planned
   int32_t *err_flag = nullptr;   // without a plan: set by an id out of range
   const uint8_t *w = nullptr, *up = nullptr;
   int64_t rows = 0, cols = 0;    // N and K of an expert

@@ -525,7 +525,7 @@ int check_stack(int64_t experts, int64_t rows, int64_t cols) {
     return fail(LLMCP_Q8_DECLINED, "a stack of %lld experts (1 to %d)", (long long)experts,
                 kMaxExperts);
   if (rows > 1ll << 31 || cols > 1ll << 31 ||
-      expert_layout(rows, cols).tile_bytes > 0xFFFFFFFFll / ((rows + 15) / 16))
+      expert_layout(rows, cols).tile_bytes() > 0xFFFFFFFFll / ((rows + 15) / 16))
     return fail(LLMCP_Q8_DECLINED, "an expert of [%lld, %lld] reaches 4 GiB", (long long)rows,
                 (long long)cols);
   return LLMCP_Q8_OK;
@@ -1685,6 +1685,10 @@ static int route_impl(llmcp_q8_ctx *ctx, const Rows &logits, int32_t top_k, int3
   return LLMCP_Q8_OK;
 }
 
+// Up to this many rows are quantized by the workgroups that read them, without
+// a launch of their own.
+constexpr int64_t kFewRowsQuantized = 4;
+
 // Rows that experts read: f32 / bf16 rows or Q8_1 rows.
 struct ExpertRows {
   const Rows *x = nullptr;
@@ -1692,53 +1696,58 @@ struct ExpertRows {
   int64_t rows = 0, cols = 0;
 };
 
-// Whether the slots and their rows are within what a launch addresses: slots
-// and a product's workgroups (16 slots by 32 columns at the smallest) in 32
-// bits of work-items.
+// Whether the slots and their rows are within what a launch addresses: a
+// product's workgroups (16 slots by 32 columns at the smallest) in 32 bits of
+// work-items, Q8_1 rows (the input's and the hidden ones) in 32 bits of bytes.
 static int check_slots(const ExpertRows &in, const int32_t *experts, int32_t top_k, int64_t slots,
                        int64_t widest) {
   if (!experts) return fail(LLMCP_Q8_EINVAL, "null expert ids");
   if (top_k < 1 || top_k > kMaxTopK)
     return fail(LLMCP_Q8_DECLINED, "top_k %d (1 to %d)", top_k, kMaxTopK);
   if (slots > 1ll << 30 || (slots / 16 + kMaxExperts + 1) * ((widest + 31) / 32 + 1) > 0xFFFFFFull ||
-      slots * (widest / 4) > 0xFFFFFF00ll || in.rows * (in.cols / 4) > 0xFFFFFF00ll)
+      slots * widest > 0xFFFFFF00ll || in.rows * in.cols > 0xFFFFFF00ll)
     return fail(LLMCP_Q8_DECLINED, "too many slots for one launch (%lld)", (long long)slots);
   return LLMCP_Q8_OK;
 }
 
-// The rows' Q8_1: as given, or quantized into the workspace.
-static int expert_quantize(llmcp_q8_ctx *ctx, const ExpertRows &in, ExpertLaunch &l) {
-  if (in.q) {
-    l.qa = in.q->values;
-    l.sa = in.q->scales;
-    return LLMCP_Q8_OK;
-  }
-  const int64_t blocks = in.cols / kBlock;
-  int rc = ensure_scratch(ctx, (uint64_t)(in.rows * in.cols), (uint64_t)(in.rows * blocks * 4));
-  if (rc) return rc;
-  hipError_t e = launch_quantize(in.x->data, in.x->bf16, in.rows, in.x->ld, in.cols, ctx->qa,
-                                 in.cols, ctx->sa, blocks, blocks, ctx->stream);
-  if (e != hipSuccess) return hip_fail(e, "quantize launch");
-  l.qa = ctx->qa;
-  l.sa = ctx->sa;
-  return LLMCP_Q8_OK;
-}
-
-static int expert_plan(llmcp_q8_ctx *ctx, const int32_t *experts, int64_t slots, int64_t count,
-                       ExpertLaunch &l) {
+// What the products need first: the rows' Q8_1 (as given, quantized here, or
+// left to the workgroups) and the plan of many slots.
+static int expert_prepare(llmcp_q8_ctx *ctx, const ExpertRows &in, const int32_t *experts,
+                          int64_t slots, int64_t count, int64_t widest, ExpertLaunch &l) {
   l.ids = experts;
+  l.tile_rows = expert_tile_rows(slots, count, widest);
   l.slots = slots;
   l.experts = (int32_t)count;
   l.err_flag = ctx->err_flag;
   l.fma = ctx->fma();
-  if (slots <= kDirectSlots) return LLMCP_Q8_OK;
-  int rc = grow(ctx, ctx->plan, ctx->plan_bytes, (uint64_t)expert_plan_ints(slots, count) * 4,
-                "expert plan");
-  if (rc) return rc;
-  hipError_t e = launch_expert_plan(experts, slots, (int32_t)count, ctx->plan, ctx->err_flag,
-                                    ctx->stream);
-  if (e != hipSuccess) return hip_fail(e, "expert plan launch");
-  l.plan = ctx->plan;
+  const bool planned = expert_planned(slots, l.tile_rows);
+  const int64_t blocks = in.cols / kBlock;
+  int rc;
+  if (in.q) {
+    l.qa = in.q->values;
+    l.sa = in.q->scales;
+  } else if (!planned && in.rows <= kFewRowsQuantized) {
+    l.x = in.x->data;
+    l.ldx = in.x->ld;
+  } else {
+    if ((rc = ensure_scratch(ctx, (uint64_t)(in.rows * in.cols), (uint64_t)(in.rows * blocks * 4))))
+      return rc;
+    l.qa = ctx->qa;
+    l.sa = ctx->sa;
+  }
+  hipError_t e = hipSuccess;
+  if (planned) {
+    if ((rc = grow(ctx, ctx->plan, ctx->plan_bytes, (uint64_t)expert_plan_ints(slots, count, l.tile_rows) * 4, "expert plan")))
+      return rc;
+    l.plan = ctx->plan;
+    e = launch_expert_prepare(experts, slots, (int32_t)count, l.tile_rows, ctx->plan, ctx->err_flag,
+                              in.x ? in.x->data : nullptr, in.x && in.x->bf16, in.rows,
+                              in.x ? in.x->ld : 0, in.cols, ctx->qa, ctx->sa, ctx->stream);
+  } else if (in.x && !l.x) {
+    e = launch_quantize(in.x->data, in.x->bf16, in.rows, in.x->ld, in.cols, ctx->qa, in.cols,
+                        ctx->sa, blocks, blocks, ctx->stream);
+  }
+  if (e != hipSuccess) return hip_fail(e, "expert preparation launch");
   return LLMCP_Q8_OK;
 }
 
@@ -1768,9 +1777,9 @@ static int expert_linear_impl(llmcp_q8_ctx *ctx, const Rows &x, const int32_t *e
   if (slots == 0) return LLMCP_Q8_OK;
   if ((rc = set_device(ctx))) return rc;
   ExpertLaunch l;
-  if ((rc = expert_quantize(ctx, in, l)) || (rc = expert_plan(ctx, experts, slots, w->experts, l)))
-    return rc;
+  if ((rc = expert_prepare(ctx, in, experts, slots, w->experts, w->cols, l))) return rc;
   l.per_row = x.rows == slots ? 1 : top_k;
+  l.in_rows = x.rows;
   l.w = w->dev;
   l.rows = w->rows;
   l.cols = w->cols;
@@ -1813,9 +1822,9 @@ static int expert_mlp_impl(llmcp_q8_ctx *ctx, const ExpertRows &in, const int32_
                  (uint64_t)(slots * h) * (out.bf16 ? 2 : 4), "expert outputs")))
     return rc;
   ExpertLaunch l;
-  if ((rc = expert_quantize(ctx, in, l)) || (rc = expert_plan(ctx, experts, slots, wg->experts, l)))
-    return rc;
+  if ((rc = expert_prepare(ctx, in, experts, slots, wg->experts, std::max(f, h), l))) return rc;
   l.per_row = top_k;
+  l.in_rows = m;
   l.w = wg->dev;
   l.up = wu->dev;
   l.rows = f;
@@ -1827,7 +1836,9 @@ static int expert_mlp_impl(llmcp_q8_ctx *ctx, const ExpertRows &in, const int32_
   if (e != hipSuccess) return hip_fail(e, "expert SwiGLU launch");
   l.qa = ctx->expert_hq;
   l.sa = ctx->expert_hs;
+  l.x = nullptr;
   l.per_row = 1;
+  l.in_rows = slots;
   l.w = wd->dev;
   l.up = nullptr;
   l.rows = h;
