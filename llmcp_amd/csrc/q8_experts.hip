@@ -64,113 +64,139 @@ __device__ __forceinline__ int group_of(int id, int experts) {
   return (unsigned)id < (unsigned)experts ? id : experts;
 }
 
-// The tiles to compute, by one workgroup: {group, slots} of max_tiles tiles
-// (0 slots: none), then tile_rows slots of each.  A group's tiles are
-// consecutive and alike; tile i of T takes place (i % C) * 8 + i / C with C =
-// ceil(T / 8), so that with places dealt to the XCDs in turn each XCD gets
-// whole runs of them, an expert's on one or two.  An id that is neither an
-// expert nor -1 sets the error flag.  The order of a group's slots is that of
-// the atomics; no result depends on it.
+// The tiles to compute, by one workgroup: {group, first, slots} of max_tiles
+// tiles (0 slots: none), then the slots sorted by group, a tile's from `first`
+// on.  A group's tiles are consecutive and alike; tile i of T takes place (i %
+// C) * 8 + i / C with C = ceil(T / 8), so that with places dealt to the XCDs in
+// turn each XCD gets whole runs of them, an expert's on one or two.  An id
+// that is neither an expert nor -1 sets the error flag.  The order of a
+// group's slots is that of the atomics; no result depends on it.
 __device__ void expert_plan(const int32_t *__restrict__ ids, int32_t slots, int32_t experts,
                             int32_t tile_rows, int32_t max_tiles, int32_t *__restrict__ plan,
                             int32_t *__restrict__ err) {
-  __shared__ int count[kMaxExperts + 1], tile0[kMaxExperts + 1], per[kMaxExperts + 1];
-  __shared__ int part[16];
+  // groups 0 .. experts, the last the slots without one
+  __shared__ int count[kMaxExperts + 1], before[kMaxExperts + 1], tile0[kMaxExperts + 1];
+  __shared__ int part[2][16];
+  constexpr int kKeep = 32;
+  __shared__ __align__(16) uint16_t order[1024 * kKeep];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   for (int i = t; i <= experts; i += 1024) count[i] = 0;
+  for (int i = t; i < max_tiles; i += 1024) plan[4 * i + 2] = 0;
   __syncthreads();
-  // eight ids per thread in flight together, here and below (one by one, each
-  // waiting for its load, 32768 slots took 40 us)
-  constexpr int kBatch = 8;
+  // A thread's ids, all in flight together (one by one 32768 slots took 40
+  // us), and their places in their groups, kept in registers up to kKeep
+  // ids; beyond, in batches that are gone through twice.
+  uint32_t held[kKeep];  // group << 20 | place in it (at most 2^20 slots)
   bool bad = false;
-  for (int s0 = t; s0 < slots; s0 += 1024 * kBatch) {
-    int id[kBatch];
+  const __amdgpu_buffer_rsrc_t ri =
+      __builtin_amdgcn_make_buffer_rsrc(const_cast<int32_t *>(ids), 0, slots * 4, 0x00020000);
+  auto count_in = [&](int s0) __attribute__((always_inline)) {
 #pragma unroll
-    for (int k = 0; k < kBatch; ++k) id[k] = ids[min(s0 + 1024 * k, slots - 1)];
+    for (int k = 0; k < kKeep; ++k)
+      held[k] = __builtin_amdgcn_raw_buffer_load_b32(ri, (s0 + 1024 * k + t) * 4, 0, 0);
 #pragma unroll
-    for (int k = 0; k < kBatch; ++k)
-      if (s0 + 1024 * k < slots) {
-        bad |= id[k] < -1 || id[k] >= experts;
-        atomicAdd(&count[group_of(id[k], experts)], 1);
-      }
-  }
+    for (int k = 0; k < kKeep; ++k) {
+      if (s0 + 1024 * k + t >= slots) continue;
+      const int id = (int)held[k], g = group_of(id, experts);
+      bad |= id < -1 || id >= experts;
+      held[k] = (uint32_t)g << 20 | (uint32_t)atomicAdd(&count[g], 1);
+    }
+  };
+  for (int s0 = 0; s0 < slots; s0 += 1024 * kKeep) count_in(s0);
   if (__ballot(bad) && lane == 0) *err = 1;
   __syncthreads();
-  // the groups' first tiles (an exclusive prefix sum) and slots per tile, in
-  // whole MFMA tiles
-  const int step = min(tile_rows, 16);
-  int total = 0;
+  // the groups' first slots and tiles (exclusive prefix sums); then a tile's
+  // header by the thread of its group
+  const int step = min(tile_rows, 16);  // a tile holds whole MFMA tiles
+  int total = 0, sorted = 0;
   for (int g0 = 0; g0 <= experts; g0 += 1024) {
     const int g = g0 + t;
     const int c = g <= experts ? count[g] : 0;
     const int n = (c + tile_rows - 1) / tile_rows;
-    int pt = n;
+    int pt = n, ps = c;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-      const int u = __shfl_up(pt, d);
-      if (lane >= d) pt += u;
+      const int u = __shfl_up(pt, d), v = __shfl_up(ps, d);
+      if (lane >= d) pt += u, ps += v;
     }
-    if (lane == 63) part[wave] = pt;
+    if (lane == 63) part[0][wave] = pt, part[1][wave] = ps;
     __syncthreads();
-    int before = total;
+    int tiles = total, above = sorted;
     for (int w = 0; w < 16; ++w) {
-      if (w < wave) before += part[w];
-      total += part[w];
+      if (w < wave) tiles += part[0][w], above += part[1][w];
+      total += part[0][w], sorted += part[1][w];
     }
-    if (g <= experts) {
-      tile0[g] = before + pt - n;
-      per[g] = n ? ((c + step - 1) / step + n - 1) / n * step : step;
-    }
+    if (g <= experts) before[g] = above + ps - c, tile0[g] = tiles + pt - n;
     __syncthreads();
   }
-  const int run = (total + 7) / 8;
-  auto place = [&](int i) { return (i % run) * 8 + i / run; };
-  for (int i = t; i < max_tiles; i += 1024) plan[2 * i + 1] = 0;
-  __syncthreads();
+  const int run = max((total + 7) / 8, 1);
   for (int g = t; g <= experts; g += 1024) {
-    const int c = count[g];
-    for (int i = 0; i * per[g] < c; ++i)
-      *(v2i *)(plan + 2 * place(tile0[g] + i)) = v2i{g, min(per[g], c - i * per[g])};
+    const int c = count[g], n = (c + tile_rows - 1) / tile_rows;
+    const int per = n ? ((c + step - 1) / step + n - 1) / n * step : step;
+    int r = tile0[g] % run, x = tile0[g] / run;
+    for (int f = 0; f < c; f += per) {
+      *(v4i *)(plan + 4 * (8 * r + x)) = v4i{g, before[g] + f, min(per, c - f), 0};
+      if (++r == run) r = 0, ++x;
+    }
+  }
+  int32_t *const sorted_slots = plan + 4 * max_tiles;
+  if (slots <= 1024 * kKeep) {
+    // through LDS, to be written side by side (scattered from this one
+    // workgroup, a line per slot, 32768 of them took 15 us)
+#pragma unroll
+    for (int k = 0; k < kKeep; ++k)
+      if (1024 * k + t < slots) order[before[held[k] >> 20] + (held[k] & 0xFFFFFu)] = (uint16_t)(1024 * k + t);
+    __syncthreads();
+    for (int i = 2 * t; i < slots; i += 2048) {
+      const uint32_t two = *(const uint32_t *)(order + i);
+      *(v2i *)(sorted_slots + i) = v2i{(int)(two & 0xffffu), (int)(two >> 16)};  // (one past an odd end)
+    }
+    return;
   }
   __syncthreads();
   for (int g = t; g <= experts; g += 1024) count[g] = 0;
   __syncthreads();
-  int32_t *const rows = plan + 2 * max_tiles;
-  for (int s0 = t; s0 < slots; s0 += 1024 * kBatch) {
-    int id[kBatch];
+  for (int s0 = 0; s0 < slots; s0 += 1024 * kKeep) {
+    count_in(s0);
 #pragma unroll
-    for (int k = 0; k < kBatch; ++k) id[k] = ids[min(s0 + 1024 * k, slots - 1)];
-#pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      const int s = s0 + 1024 * k;
-      if (s >= slots) continue;
-      const int g = group_of(id[k], experts);
-      const int i = atomicAdd(&count[g], 1);
-      rows[(int64_t)place(tile0[g] + i / per[g]) * tile_rows + i % per[g]] = s;
-    }
+    for (int k = 0; k < kKeep; ++k)
+      if (s0 + 1024 * k + t < slots)
+        sorted_slots[before[held[k] >> 20] + (held[k] & 0xFFFFFu)] = s0 + 1024 * k + t;
   }
 }
 
 // What comes before the products of many slots: workgroup 0 plans, the
 // others quantize the rows (x null: nothing to quantize).
+constexpr int kQuantUnits = 4;
 __global__ __launch_bounds__(1024) void expert_prepare_kernel(
     const int32_t *__restrict__ ids, int32_t slots, int32_t experts, int32_t tile_rows,
     int32_t max_tiles, int32_t *__restrict__ plan, int32_t *__restrict__ err,
     const void *__restrict__ x, int bf16, int aligned, int64_t ldx, int64_t m, int32_t blocks,
     int8_t *__restrict__ qa, float *__restrict__ sa) {
   if (blockIdx.x == 0) return expert_plan(ids, slots, experts, tile_rows, max_tiles, plan, err);
-  const int64_t unit = ((int64_t)blockIdx.x - 1) * 128 + (threadIdx.x >> 3);  // (row, block)
-  const int64_t row = unit / blocks;
-  const int b = (int)(unit - row * blocks), p = threadIdx.x & 7;
-  const bool live = row < m;
-  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (live) v = load_act4(x, row * ldx + b * kBlock + 4 * p, bf16 != 0, aligned != 0);
-  int32_t q;
-  float s;
-  quantize_block8(v, live, &q, &s);
-  if (!live) return;
-  *(int32_t *)(qa + unit * kBlock + 4 * p) = q;
-  if (p == 0) sa[unit] = s;
+  // (row, block) units, eight threads each, kQuantUnits in flight per thread
+  // (the plan's registers leave room for one workgroup per CU)
+  const int p = threadIdx.x & 7;
+  const int64_t u0 = ((int64_t)blockIdx.x - 1) * 128 * kQuantUnits + (threadIdx.x >> 3);
+  const int64_t units = m * blocks;
+  float4 v[kQuantUnits];
+#pragma unroll
+  for (int k = 0; k < kQuantUnits; ++k) {
+    const uint32_t u = (uint32_t)min(u0 + 128 * k, units - 1);
+    const uint32_t row = u / (uint32_t)blocks;
+    v[k] = load_act4(x, (int64_t)row * ldx + (int64_t)(u - row * (uint32_t)blocks) * kBlock + 4 * p,
+                     bf16 != 0, aligned != 0);
+  }
+#pragma unroll
+  for (int k = 0; k < kQuantUnits; ++k) {
+    const int64_t u = u0 + 128 * k;
+    int32_t q;
+    float s;
+    quantize_block8(v[k], true, &q, &s);
+    if (u >= units) continue;
+    *(int32_t *)(qa + u * kBlock + 4 * p) = q;
+    if (p == 0) sa[u] = s;
+  }
 }
 
 // ---------------------------------------------------------- products ---- //
@@ -205,16 +231,15 @@ struct ExpertArgs {
 
 // The plan's tile and the column range of this workgroup; its slots into
 // `rows` (LDS, no barrier).  Returns the number of slots.
-__device__ __forceinline__ int planned_tile(const ExpertArgs &p, int tile_rows, int &ng, int &group,
-                                            int *rows) {
+__device__ __forceinline__ int planned_tile(const ExpertArgs &p, int &ng, int &group, int *rows) {
   const int i = blockIdx.x >> 3;
   const int tile = i / p.n_groups * 8 + (blockIdx.x & 7);
   ng = i - i / p.n_groups * p.n_groups;
-  if ((int)threadIdx.x < tile_rows)
-    rows[threadIdx.x] = p.plan[2 * (int64_t)p.max_tiles + (int64_t)tile * tile_rows + threadIdx.x];
-  const v2i e = *(const v2i *)(p.plan + 2 * (int64_t)tile);
+  const v4i e = *(const v4i *)(p.plan + 4 * (int64_t)tile);
   group = __builtin_amdgcn_readfirstlane(e[0]);
-  return __builtin_amdgcn_readfirstlane(e[1]);
+  const int count = __builtin_amdgcn_readfirstlane(e[2]);
+  if ((int)threadIdx.x < count) rows[threadIdx.x] = p.plan[4 * (int64_t)p.max_tiles + e[1] + threadIdx.x];
+  return count;
 }
 
 // Rows of slots without an expert: zeros in columns [col0, col0 + cols).
@@ -485,7 +510,7 @@ __global__ __launch_bounds__(256, 3) void expert_few_kernel(const ExpertArgs p) 
   const int steps = p.lay.steps;
   int ng = 0, group = 0, count = 0;
   if (p.plan) {
-    count = planned_tile(p, TILE, ng, group, rows);
+    count = planned_tile(p, ng, group, rows);
     if (count == 0) return;
   } else {
     // every wave looks over all slots: those of this group before s, and the
@@ -825,7 +850,7 @@ __global__ __launch_bounds__(256, 3) void expert_many_kernel(const ExpertArgs p)
   __shared__ __align__(16) float hb[DUAL ? ManyLds<TT>::H / 4 : 4];
   __shared__ int rows[32 * TT];
   int ng, group;
-  const int count = planned_tile(p, 32 * TT, ng, group, rows);
+  const int count = planned_tile(p, ng, group, rows);
   if (count == 0) return;
   lds_barrier();
   if (group >= p.experts) {
@@ -1010,13 +1035,14 @@ int64_t expert_max_tiles(int64_t slots, int64_t experts, int32_t tile_rows) {
 }
 
 int64_t expert_plan_ints(int64_t slots, int64_t experts, int32_t tile_rows) {
-  return expert_max_tiles(slots, experts, tile_rows) * (2 + tile_rows);
+  return 4 * expert_max_tiles(slots, experts, tile_rows) + slots + 1;
 }
 
 hipError_t launch_expert_prepare(const int32_t *ids, int64_t slots, int32_t experts,
                                  int32_t tile_rows, int32_t *plan, int32_t *err_flag, const void *x, bool bf16, int64_t m, int64_t ldx,
                                  int64_t cols, int8_t *qa, float *sa, hipStream_t s) {
-  const int64_t wgs = 1 + (x ? (m * (cols / kBlock) + 127) / 128 : 0);
+  const int64_t per = 128 * kQuantUnits;
+  const int64_t wgs = 1 + (x ? (m * (cols / kBlock) + per - 1) / per : 0);
   if (wgs * 1024 > 0xFFFFFFFFll) return hipErrorInvalidConfiguration;
   const int aligned = (uintptr_t)x % (bf16 ? 8 : 16) == 0 && ldx % 4 == 0;
   hipLaunchKernelGGL(expert_prepare_kernel, dim3((unsigned)wgs), dim3(1024), 0, s, ids, (int32_t)slots,
@@ -1051,7 +1077,7 @@ static hipError_t launch_few(ExpertArgs &a, bool fma, hipStream_t s) {
 
 template <int TT, bool DUAL>
 static hipError_t launch_many(ExpertArgs &a, bool fma, hipStream_t s) {
-  set_repeat(a, std::max(a.slots / (32 * TT), std::min(a.slots, a.experts)), DUAL ? 64 : 128, 12);
+  set_repeat(a, std::max(a.slots / (32 * TT), std::min(a.slots, a.experts)), DUAL ? 64 : 128, 20);
   const int64_t wgs = (int64_t)a.max_tiles * a.n_groups;
   if (wgs * 256 > 0xFFFFFFFFll) return hipErrorInvalidConfiguration;
   if (fma)

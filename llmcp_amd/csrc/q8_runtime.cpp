@@ -1704,7 +1704,7 @@ static int check_slots(const ExpertRows &in, const int32_t *experts, int32_t top
   if (!experts) return fail(LLMCP_Q8_EINVAL, "null expert ids");
   if (top_k < 1 || top_k > kMaxTopK)
     return fail(LLMCP_Q8_DECLINED, "top_k %d (1 to %d)", top_k, kMaxTopK);
-  if (slots > 1ll << 30 || (slots / 16 + kMaxExperts + 1) * ((widest + 31) / 32 + 1) > 0xFFFFFFull ||
+  if (slots > kMaxSlots || (slots / 16 + kMaxExperts + 1) * ((widest + 31) / 32 + 1) > 0xFFFFFFull ||
       slots * widest > 0xFFFFFF00ll || in.rows * in.cols > 0xFFFFFF00ll)
     return fail(LLMCP_Q8_DECLINED, "too many slots for one launch (%lld)", (long long)slots);
   return LLMCP_Q8_OK;
