@@ -383,6 +383,72 @@ struct FewDots {
   v4i c[4];
   v16f f;
 };
+// A step's rows: the MFMA operands of its two block pairs, the lane's scale.
+struct FewRows {
+  v4i x[2];
+  float s;
+};
+
+__device__ __forceinline__ void few_dots(FewDots &o, const FewRows &x, const v4u (&w)[2], uint32_t d) {
+  const v16f z = {};
+  o.f = __builtin_amdgcn_mfma_f32_16x16x1f32(x.s, half_bits_to_float(d), z, 0, 0, 0);
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    // lanes 0-31 hold the pair's even block, 32-63 the odd one; the swap
+    // leaves each block its own operand, eights 0, 2, 1, 3
+    const auto lo = __builtin_amdgcn_permlane32_swap(w[j][0], w[j][2], false, false);
+    const auto hi = __builtin_amdgcn_permlane32_swap(w[j][1], w[j][3], false, false);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const v2i wv = {(int)lo[k], (int)hi[k]};
+      const v2i xv = {x.x[j][2 * k], x.x[j][2 * k + 1]};
+      o.c[2 * j + k] = __builtin_amdgcn_mfma_i32_16x16x32_i8(
+          __builtin_bit_cast(long, xv), __builtin_bit_cast(long, wv), v4i{0, 0, 0, 0}, 0, 0, 0);
+    }
+  }
+}
+
+// One tile: acc = the chains of 4 NV slots over its steps.  The ring holds
+// the tile's first steps and goes on to `after` steps of the tile at `next`;
+// x holds step 0's rows, at the end as well (read_rows reads a step's).
+template <int NV, bool FMA, class ReadRows>
+__device__ __forceinline__ void few_tile(FewRing &ring, const uint8_t *wexp, uint32_t cur,
+                                         uint32_t next, int after, int steps, FewRows &x,
+                                         ReadRows &&read_rows, float (&acc)[NV]) {
+  const int lane = threadIdx.x & 63;
+  const int steps2 = (steps + 1) & ~1, stages = (steps2 + kFewRing - 1) / kFewRing;
+  auto epilogue = [&](const FewDots &o) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int v = 0; v < NV; ++v) acc[v] = chain<FMA>(o.c[j][v], o.f[4 * j + v], acc[v]);
+  };
+#pragma unroll
+  for (int v = 0; v < NV; ++v) acc[v] = 0.0f;
+  FewDots even, odd = {};  // (the step before the first: nothing to add)
+  for (int s = 0; s < stages; ++s) {
+    const bool last = s + 1 == stages;
+    const uint32_t from = last ? next : cur;
+    const int st0 = last ? 0 : kFewRing * (s + 1), live = last ? after : steps;
+    static_for<kFewRing / 2>([&](auto Q) __attribute__((always_inline)) {
+      constexpr int q = 2 * decltype(Q)::value;
+      const int st = kFewRing * s + q;
+      if (st < steps2) {
+        few_dots(even, x, ring.w[q], ring.d[q]);
+        read_rows(x, st + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        epilogue(odd);
+        few_dots(odd, x, ring.w[q + 1], ring.d[q + 1]);
+        read_rows(x, st + 2 == steps2 ? 0 : st + 2);
+        __builtin_amdgcn_sched_barrier(0);
+        epilogue(even);
+      }
+      few_load(ring, q, wexp, from, st0 + q, live, steps, lane);
+      few_load(ring, q + 1, wexp, from, st0 + q + 1, live, steps, lane);
+    });
+  }
+  epilogue(odd);
+}
 
 template <int NV, bool FMA, bool DUAL>
 __device__ __forceinline__ void few_run(const ExpertArgs &p, int ng, int count, const int *rows,
@@ -392,7 +458,6 @@ __device__ __forceinline__ void few_run(const ExpertArgs &p, int ng, int count, 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int steps = p.lay.steps;
   const FewLds lds = FewLds::of(steps);
-  const int stages = (lds.steps2 + kFewRing - 1) / kFewRing;
   // the slot at MFMA row li (any other's data for a row past the last)
   const int mine = min((li >> 2) + 4 * (li & 3), count - 1);
   const uint8_t *const a = smem + mine * lds.a_ld + lq * 16;
@@ -401,69 +466,18 @@ __device__ __forceinline__ void few_run(const ExpertArgs &p, int ng, int count, 
   auto tile_of = [&](int it) {
     return DUAL ? (ng * p.repeat + it) * 2 + (wave >> 1) : (ng * p.repeat + it) * 4 + wave;
   };
-  v4i x0, x1;
-  float sx;
-  auto read_rows = [&](int st) __attribute__((always_inline)) {
-    x0 = *(const v4i *)(a + st * 128);
-    x1 = *(const v4i *)(a + st * 128 + 64);
-    sx = sa[4 * st];
+  auto read_rows = [&](FewRows &x, int st) __attribute__((always_inline)) {
+    x.x[0] = *(const v4i *)(a + st * 128);
+    x.x[1] = *(const v4i *)(a + st * 128 + 64);
+    x.s = sa[4 * st];
   };
-  auto dots = [&](FewDots &o, const v4u (&w)[2], uint32_t d) __attribute__((always_inline)) {
-    const v16f z = {};
-    o.f = __builtin_amdgcn_mfma_f32_16x16x1f32(sx, half_bits_to_float(d), z, 0, 0, 0);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      // lanes 0-31 hold the pair's even block, 32-63 the odd one; the swap
-      // leaves each block its own operand, eights 0, 2, 1, 3
-      const v4i x = j ? x1 : x0;
-      const auto lo = __builtin_amdgcn_permlane32_swap(w[j][0], w[j][2], false, false);
-      const auto hi = __builtin_amdgcn_permlane32_swap(w[j][1], w[j][3], false, false);
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const v2i wv = {(int)lo[k], (int)hi[k]};
-        const v2i xv = {x[2 * k], x[2 * k + 1]};
-        o.c[2 * j + k] = __builtin_amdgcn_mfma_i32_16x16x32_i8(
-            __builtin_bit_cast(long, xv), __builtin_bit_cast(long, wv), v4i{0, 0, 0, 0}, 0, 0, 0);
-      }
-    }
-  };
-  float acc[NV];
-  auto epilogue = [&](const FewDots &o) __attribute__((always_inline)) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int v = 0; v < NV; ++v) acc[v] = chain<FMA>(o.c[j][v], o.f[4 * j + v], acc[v]);
-  };
-  read_rows(0);
+  FewRows x;
+  read_rows(x, 0);
   for (int it = 0; it < p.repeat; ++it) {
-    const uint32_t cur = (uint32_t)min(tile_of(it), p.lay.tiles - 1) * tile_bytes;
-    const uint32_t next = (uint32_t)min(tile_of(it + 1), p.lay.tiles - 1) * tile_bytes;
-    const int after = it + 1 < p.repeat ? steps : 0;  // live steps of the next tile
-#pragma unroll
-    for (int v = 0; v < NV; ++v) acc[v] = 0.0f;
-    FewDots even, odd = {};  // (the step before the first: nothing to add)
-    for (int s = 0; s < stages; ++s) {
-      const bool last = s + 1 == stages;
-      const uint32_t from = last ? next : cur;
-      const int st0 = last ? 0 : kFewRing * (s + 1), live = last ? after : steps;
-      static_for<kFewRing / 2>([&](auto Q) __attribute__((always_inline)) {
-        constexpr int q = 2 * decltype(Q)::value;
-        const int st = kFewRing * s + q;
-        if (st < lds.steps2) {
-          dots(even, ring.w[q], ring.d[q]);
-          read_rows(st + 1);
-          __builtin_amdgcn_sched_barrier(0);
-          epilogue(odd);
-          dots(odd, ring.w[q + 1], ring.d[q + 1]);
-          read_rows(st + 2 == lds.steps2 ? 0 : st + 2);
-          __builtin_amdgcn_sched_barrier(0);
-          epilogue(even);
-        }
-        few_load(ring, q, wexp, from, st0 + q, live, steps, lane);
-        few_load(ring, q + 1, wexp, from, st0 + q + 1, live, steps, lane);
-      });
-    }
-    epilogue(odd);
+    float acc[NV];
+    few_tile<NV, FMA>(ring, wexp, (uint32_t)min(tile_of(it), p.lay.tiles - 1) * tile_bytes,
+                      (uint32_t)min(tile_of(it + 1), p.lay.tiles - 1) * tile_bytes,
+                      it + 1 < p.repeat ? steps : 0, steps, x, read_rows, acc);
     const int n = tile_of(it) * 16 + li;
     if constexpr (!DUAL) {
       activate_array(acc, p.act);
@@ -597,6 +611,82 @@ __global__ __launch_bounds__(256, 3) void expert_few_kernel(const ExpertArgs p) 
   lds_barrier();
   float *const box = (float *)(smem + lds.bytes(used));
   few_run<NV, FMA, DUAL>(p, ng, count, rows, wexp, ring, smem, used, box);
+#endif
+}
+
+// ---- few tokens: the down products and their weighted sum in one launch
+//
+// A workgroup per token and tile of 16 columns, a wave per slot (in turns
+// beyond eight): each streams its expert's tile with its one row of h in
+// LDS, and the results, rounded to the output's type, are added in slot
+// order by sixteen lanes (expert_combine_kernel's sum).  An expert that two
+// tokens share is read twice.
+
+constexpr int kTokenWaves = 8;
+
+// LDS of a wave: its row's values, natural order, and scales, each of a pair
+// of steps more than the row may have.
+__host__ __device__ inline int token_lds(int steps) { return ((steps + 1) & ~1) * (128 + 16); }
+
+template <bool FMA, bool BF16>
+__global__ __launch_bounds__(64 * kTokenWaves) void expert_token_kernel(
+    const ExpertArgs p, const float *__restrict__ weights, int32_t top_k, const void *residual,
+    int64_t ldr, void *y, int64_t ldy) {
+#ifdef __HIP_DEVICE_COMPILE__
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ float sums[kMaxTopK][16];
+  const int lane = threadIdx.x & 63, li = lane & 15, lq = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const int64_t token = blockIdx.y;
+  const int tile = blockIdx.x, steps = p.lay.steps;
+  uint8_t *const mine = smem + wave * token_lds(steps);
+  float *const ls = (float *)(mine + ((steps + 1) & ~1) * 128);
+  for (int j = wave; j < top_k; j += waves) {
+    const int64_t slot = token * top_k + j;
+    const int id = __builtin_amdgcn_readfirstlane(p.ids[slot]);
+    if ((unsigned)id >= (unsigned)p.experts) continue;  // uniform per wave
+    const uint8_t *const wexp = p.w0 + (int64_t)id * p.lay.expert_bytes();
+    const uint32_t at = (uint32_t)tile * (uint32_t)p.lay.tile_bytes();
+    FewRing ring;
+#pragma unroll
+    for (int q = 0; q < kFewRing; ++q) few_load(ring, q, wexp, at, q, steps, steps, lane);
+    const int8_t *const row = p.qa + slot * p.blocks * kBlock;
+    for (int b = lane; b < 2 * p.blocks; b += 64) *(v4i *)(mine + 16 * b) = *(const v4i *)(row + 16 * b);
+    // (a block past the last must have a finite scale; its weights are zero)
+    for (int b = lane; b < 4 * ((steps + 1) & ~1); b += 64)
+      ls[b] = b < p.blocks ? p.sa[slot * p.blocks + b] : 0.0f;
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the wave's own stores
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    // every MFMA row reads the one row: eights 0, 2, 1, 3 of a block
+    const uint8_t *const a = mine + ((lq & 1) * 2 + (lq >> 1)) * 8;
+    auto read_rows = [&](FewRows &x, int st) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const v2i v = *(const v2i *)(a + st * 128 + i * 32);
+        x.x[i >> 1][2 * (i & 1)] = v[0], x.x[i >> 1][2 * (i & 1) + 1] = v[1];
+      }
+      x.s = ls[4 * st + lq];
+    };
+    FewRows x;
+    read_rows(x, 0);
+    float acc[1];
+    few_tile<1, FMA>(ring, wexp, at, at, 0, steps, x, read_rows, acc);
+    if (lq == 0) sums[j][li] = BF16 ? as_bf16(acc[0]) : acc[0];
+  }
+  __syncthreads();
+  const int n = tile * 16 + threadIdx.x;
+  if (threadIdx.x >= 16 || n >= p.rows) return;
+  float v = 0.0f;
+  if (residual)
+    v = BF16 ? bf16_to_float(((const uint16_t *)residual)[token * ldr + n])
+             : ((const float *)residual)[token * ldr + n];
+  for (int j = 0; j < top_k; ++j) {
+    const int64_t slot = token * top_k + j;
+    if ((unsigned)p.ids[slot] >= (unsigned)p.experts) continue;
+    v = __builtin_fmaf(weights ? weights[slot] : 1.0f, sums[j][threadIdx.x], v);
+  }
+  if (BF16) ((uint16_t *)y)[token * ldy + n] = float_to_bf16(v);
+  else ((float *)y)[token * ldy + n] = v;
 #endif
 }
 
@@ -1087,7 +1177,7 @@ static hipError_t launch_many(ExpertArgs &a, bool fma, hipStream_t s) {
   return hipGetLastError();
 }
 
-hipError_t launch_experts(const ExpertLaunch &l, hipStream_t s) {
+static ExpertArgs expert_args(const ExpertLaunch &l) {
   ExpertArgs a = {};
   a.qa = l.qa;
   a.sa = l.sa;
@@ -1115,6 +1205,11 @@ hipError_t launch_experts(const ExpertLaunch &l, hipStream_t s) {
   a.vec = (uintptr_t)l.y % (l.bf16 ? 8 : 16) == 0 && l.ldy % 4 == 0 ? 1 : 0;
   a.hq = l.hq;
   a.hs = l.hs;
+  return a;
+}
+
+hipError_t launch_experts(const ExpertLaunch &l, hipStream_t s) {
+  ExpertArgs a = expert_args(l);
   const bool dual = l.up != nullptr;
   switch (l.tile_rows) {
     case 4:
@@ -1128,6 +1223,31 @@ hipError_t launch_experts(const ExpertLaunch &l, hipStream_t s) {
     default:
       return dual ? launch_many<2, true>(a, l.fma, s) : launch_many<2, false>(a, l.fma, s);
   }
+}
+
+bool expert_token_takes(int64_t m, int32_t top_k, int64_t experts, int64_t cols) {
+  // an expert's weight read once per token, a launch less: as long as few
+  // tokens share one
+  const int64_t slots = m * top_k;
+  return (m == 1 || slots * 4 <= experts) &&
+         std::min(top_k, kTokenWaves) * token_lds(expert_layout(16, cols).steps) <= 150 * 1024;
+}
+
+hipError_t launch_expert_token(const ExpertLaunch &l, const float *weights, int32_t top_k, int64_t m,
+                               const void *residual, int64_t ldr, void *y, int64_t ldy, hipStream_t s) {
+  const ExpertArgs a = expert_args(l);
+  const int waves = std::min(top_k, kTokenWaves);
+  const dim3 grid((unsigned)a.lay.tiles, (unsigned)m), wg(64 * waves);
+  const size_t lds = (size_t)waves * token_lds(a.lay.steps);
+  if (l.fma && l.bf16)
+    hipLaunchKernelGGL((expert_token_kernel<true, true>), grid, wg, lds, s, a, weights, top_k, residual, ldr, y, ldy);
+  else if (l.fma)
+    hipLaunchKernelGGL((expert_token_kernel<true, false>), grid, wg, lds, s, a, weights, top_k, residual, ldr, y, ldy);
+  else if (l.bf16)
+    hipLaunchKernelGGL((expert_token_kernel<false, true>), grid, wg, lds, s, a, weights, top_k, residual, ldr, y, ldy);
+  else
+    hipLaunchKernelGGL((expert_token_kernel<false, false>), grid, wg, lds, s, a, weights, top_k, residual, ldr, y, ldy);
+  return hipGetLastError();
 }
 
 hipError_t launch_expert_combine(const void *o, const int32_t *ids, const float *w, int32_t top_k,

@@ -281,6 +281,12 @@ struct ExpertLaunch {
 };
 hipError_t launch_experts(const ExpertLaunch &l, hipStream_t s);
 
+// Down products (l: qa / sa the hidden rows, one per slot) and the weighted
+// sum below in one launch, for few tokens.
+bool expert_token_takes(int64_t m, int32_t top_k, int64_t experts, int64_t cols);
+hipError_t launch_expert_token(const ExpertLaunch &l, const float *weights, int32_t top_k, int64_t m,
+                               const void *residual, int64_t ldr, void *y, int64_t ldy, hipStream_t s);
+
 // y[t] = residual[t] (nullable) + sum over j < top_k, in order, of w[t, j]
 // (nullable: 1) * o[t * top_k + j] by f32 FMA; o dense [m * top_k, cols] of
 // y's type, cols % 4 == 0.  residual may be y.
