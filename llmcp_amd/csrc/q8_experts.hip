@@ -1015,15 +1015,37 @@ __global__ __launch_bounds__(256) void expert_combine_kernel(
 // ------------------------------------------------------------- route ---- //
 
 // Order of f32 logits as unsigned: NaN and -inf (never chosen) 0, then
-// ascending with the value.
+// ascending with the value (zeros of both signs alike); and back.
 __device__ __forceinline__ uint32_t logit_key(float v) {
   const uint32_t u = __builtin_bit_cast(uint32_t, v);
   const uint32_t k = (u >> 31) ? ~u : u | 0x80000000u;
   return !(v > -__builtin_inff()) ? 0u : (v == 0.0f ? 0x80000000u : k);
 }
+__device__ __forceinline__ float key_logit(uint32_t k) {
+  return __builtin_bit_cast(float, (k >> 31) ? k & 0x7FFFFFFFu : ~k);
+}
+
+// The wave's largest v, in scalar registers (row shifts and row broadcasts; a
+// lane without a source keeps its own).
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_max(uint32_t v) {
+  const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xf, 0xf, false);
+  return o > v ? o : v;
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+  v = dpp_max<0x111>(v);  // row_shr:1, 2, 4, 8
+  v = dpp_max<0x112>(v);
+  v = dpp_max<0x114>(v);
+  v = dpp_max<0x118>(v);
+  v = dpp_max<0x142>(v);  // row_bcast:15, 31
+  v = dpp_max<0x143>(v);
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
 
 // One wave per row, PER logits per lane (logit i in lane i % 64): top_k
-// rounds, each the largest (key, lowest index) of the wave.
+// rounds, each the wave's largest key and the lowest index that has it; then
+// the chosen ones' exponentials side by side, one per lane.  Latency bound
+// for few rows: a round is six lane moves and a ballot per 64 logits.
 template <bool BF16, int PER>
 __global__ __launch_bounds__(256) void route_kernel(const void *__restrict__ logits, int64_t ld,
                                                     int64_t m, int32_t experts, int32_t top_k,
@@ -1044,46 +1066,41 @@ __global__ __launch_bounds__(256) void route_kernel(const void *__restrict__ log
                   : ((const float *)logits)[row * ld + e];
     key[i] = logit_key(l[i]);
   }
-  // round 0's winner is the row's maximum: exp(l - max) needs it first
-  float top = 0.0f, total = 0.0f, mine = 0.0f;
+  uint32_t first = 0, mine = 0;  // the largest key, and this lane's round's
   int id = -1;
   for (int j = 0; j < top_k; ++j) {
-    // the largest key first, then the lowest index
-    uint64_t best = 0;
+    uint32_t most = key[0];
+#pragma unroll
+    for (int i = 1; i < PER; ++i) most = key[i] > most ? key[i] : most;
+    most = wave_max(most);
+    if (most == 0) break;  // only masked logits are left
+    if (j == 0) first = most;
+    int e = -1;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const uint64_t k = (uint64_t)key[i] << 32 | (uint32_t)~(64 * i + lane);
-      best = key[i] && k > best ? k : best;
+      const uint64_t hit = __ballot(key[i] == most);
+      const bool here = e < 0 && hit != 0;
+      e = here ? 64 * i + __builtin_ctzll(hit | 1ull << 63) : e;
+      if (here && lane == (e & 63)) key[i] = 0;
     }
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) {
-      const uint64_t o = __shfl_xor((unsigned long long)best, d);
-      best = o > best ? o : best;
-    }
-    if (best == 0) break;  // only masked logits are left
-    const int e = (int)~(uint32_t)best;
-    float v = 0.0f;
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-      if (64 * i + lane == e) v = l[i], key[i] = 0;
-    v = __shfl(v, e & 63);
-    if (j == 0) top = v;
-    // (the maximum itself gives 1, also where it is infinite)
-    const float p = v == top ? 1.0f : exp_f32(v - top);
-    total += p;
-    if (lane == j) id = e, mine = p;
+    if (lane == j) id = e, mine = most;
   }
+  const float top = key_logit(first);
+  // (the maximum itself gives 1, also where it is infinite)
+  auto weight = [&](float v) { return v == top ? 1.0f : exp_f32(v - top); };
+  const float p = id >= 0 ? weight(key_logit(mine)) : 0.0f;
+  float total = p;
   if (!normalize) {
     total = 0.0f;
 #pragma unroll
     for (int i = 0; i < PER; ++i)
-      if (l[i] > -__builtin_inff()) total += l[i] == top ? 1.0f : exp_f32(l[i] - top);
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) total += __shfl_xor(total, d);
+      if (l[i] > -__builtin_inff()) total += weight(l[i]);
   }
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) total += __shfl_xor(total, d);
   if (lane < top_k) {
     ids[row * top_k + lane] = id;
-    weights[row * top_k + lane] = id >= 0 ? mine / total * scale : 0.0f;
+    weights[row * top_k + lane] = id >= 0 ? p / total * scale : 0.0f;
   }
 }
 
