@@ -727,7 +727,10 @@ __device__ __forceinline__ void many_run(const ExpertArgs &p, int ng, int group,
   const int steps = p.lay.steps;
   // ---- weights: the lane's row of 32 (lanes 16-31 and 48-63: of the second
   // tile) and half of each block, a step in registers, each block replaced
-  // by the next step's once its MFMA has taken it
+  // by the next step's once its MFMA has taken it.  (Two steps ahead, with
+  // two waves per SIMD or with spills, four waves, and non-temporal loads
+  // were all slower for tiles of 32 slots bound by this stream: 333 tokens
+  // over 128 experts, 102 + 59 us, 105 + 64, 133 + 90, 125 + 72, 103 + 68.)
   const int64_t expert = (int64_t)group * p.lay.expert_bytes();
   const int second = lane >> 4 & 1;
   const uint8_t *const wbase = (DUAL && second ? p.w1 : p.w0) + expert;
@@ -742,6 +745,7 @@ __device__ __forceinline__ void many_run(const ExpertArgs &p, int ng, int group,
   };
   v4i wq[4];
   uint2 wd;
+  auto load_block = [&](int b) __attribute__((always_inline)) { wq[b] = *(const v4i *)(wp + b * 512); };
   // ---- rows: thread (slot tid / 8, 16 B piece tid % 8 of a step's 128 B) and
   // (slot tid / 4, scale tid % 4): a row's bytes of a step side by side in a
   // wave, so that it asks for few lines.  Past a row's last block they read
@@ -799,19 +803,32 @@ __device__ __forceinline__ void many_run(const ExpertArgs &p, int ng, int group,
       for (int v = 0; v < 16; ++v) acc[t][v] = 0.0f;
   };
 
-  // the steps of all column ranges in one sequence: `step` of the range that
-  // is computed, `ahead` of the rows that are loaded (they start over with
-  // each range)
+  // the steps of all column ranges in one sequence: `step` of `range` is
+  // computed, `ahead` the step of the rows that are loaded next (they start
+  // over with each range), `wstep` of `wrange` that of the weights (the last
+  // range again behind the last)
   const int r0 = ng * p.repeat;
   const int ranges = min(p.repeat, (p.lay.tiles + (DUAL ? 4 : 8) - 1) / (DUAL ? 4 : 8) - r0);
-  int ahead = 0;
+  int range = 0, step = 0, ahead = 0, wstep = 0, wrange = 0;
+  int buf = 0, buf1 = 1, buf2 = 2;  // the ring's places of steps 0, + 1, + 2
   auto advance = [&]() { ahead = ahead + 1 == steps ? 0 : ahead + 1; };
+  auto next_weights = [&]() __attribute__((always_inline)) {
+    if (++wstep == steps) {
+      wstep = 0;
+      wrange = min(wrange + 1, ranges - 1);
+      seek(r0 + wrange);
+    } else {
+      wp += 2048;
+      dp += 128;
+    }
+  };
   load_rows(ahead);
   advance();
   seek(r0);
 #pragma unroll
-  for (int b = 0; b < 4; ++b) wq[b] = *(const v4i *)(wp + b * 512);
+  for (int b = 0; b < 4; ++b) load_block(b);
   wd = *(const uint2 *)dp;
+  next_weights();
   store_rows(0);
   load_rows(ahead);
   advance();
@@ -821,8 +838,6 @@ __device__ __forceinline__ void many_run(const ExpertArgs &p, int ng, int group,
   lds_barrier();
   read_rows(0, 0);
   clear();
-  int range = 0, step = 0;
-  int buf = 0, buf1 = 1, buf2 = 2;  // the ring's places of steps 0, + 1, + 2
   for (;;) {
     // (that place's last read, of the step before, lies behind a barrier)
     store_rows(buf2);
@@ -830,16 +845,8 @@ __device__ __forceinline__ void many_run(const ExpertArgs &p, int ng, int group,
     advance();
     float dw[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) dw[u] = TT == 2 ? scale(u) : hi ? scale(2 * u + 1) : scale(2 * u);
-    // the next step's weights: of this range, or the first of the next one
-    // (of this one again behind the last)
-    const bool done = step + 1 == steps;
-    if (done) {
-      seek(r0 + min(range + 1, ranges - 1));
-    } else {
-      wp += 2048;
-      dp += 128;
-    }
+    for (int u = 0; u < U; ++u)
+      dw[u] = TT == 2 ? scale(u) : hi ? scale(2 * u + 1) : scale(2 * u);
     wd = *(const uint2 *)dp;
     static_for<U>([&](auto UU) __attribute__((always_inline)) {
       constexpr int u = decltype(UU)::value;
@@ -847,8 +854,8 @@ __device__ __forceinline__ void many_run(const ExpertArgs &p, int ng, int group,
       const v16i d0 = __builtin_amdgcn_mfma_i32_32x32x32_i8(wq[b0], x0, zi, 0, 0, 0);
       const v32f f = __builtin_amdgcn_mfma_f32_32x32x1f32(dw[u], sx, zf, 0, 0, 0);
       const v16i d1 = __builtin_amdgcn_mfma_i32_32x32x32_i8(wq[b1], x1, zi, 0, 0, 0);
-      wq[b0] = *(const v4i *)(wp + b0 * 512);
-      if constexpr (b1 != b0) wq[b1] = *(const v4i *)(wp + b1 * 512);
+      load_block(b0);
+      if constexpr (b1 != b0) load_block(b1);
       // (or the MFMAs, pure operations, are moved down to their first use)
       asm volatile("" ::"v"(d0), "v"(f), "v"(d1));
       read_rows(u + 1 == U ? buf1 : buf, (u + 1) % U);
@@ -864,10 +871,10 @@ __device__ __forceinline__ void many_run(const ExpertArgs &p, int ng, int group,
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (u == U - 2) lds_barrier();
     });
-    ++step;
+    next_weights();
     const int free = buf;
     buf = buf1, buf1 = buf2, buf2 = free;
-    if (!done) continue;
+    if (++step < steps) continue;
     const int tile0 = tile_of(r0 + range);
     if constexpr (!DUAL) {
 #pragma unroll
