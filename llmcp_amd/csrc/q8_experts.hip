@@ -307,6 +307,13 @@ __device__ __forceinline__ void silu_for_bf16(float (&v)[N]) {
   }
 }
 
+// A product's activation before its store.
+template <int N>
+__device__ __forceinline__ void activate_out(float (&v)[N], int act, int bf16) {
+  if (act == ACT_SILU && bf16) silu_for_bf16(v);
+  else activate_array(v, act);
+}
+
 // The Q8_1 of h in LDS ([slot][ld] f32, 32 columns from col0 on per block)
 // into hq / hs; threads in groups of eight.
 __device__ __forceinline__ void store_h(const ExpertArgs &p, const float *hb, int ld, int nblk,
@@ -480,7 +487,7 @@ __device__ __forceinline__ void few_run(const ExpertArgs &p, int ng, int count, 
                       it + 1 < p.repeat ? steps : 0, steps, x, read_rows, acc);
     const int n = tile_of(it) * 16 + li;
     if constexpr (!DUAL) {
-      activate_array(acc, p.act);
+      activate_out(acc, p.act, p.y_bf16);
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
         const int i = 4 * v + lq;
@@ -498,8 +505,7 @@ __device__ __forceinline__ void few_run(const ExpertArgs &p, int ng, int count, 
       }
       lds_barrier();
       if (!(wave & 1)) {
-        if (p.y_bf16) silu_for_bf16(acc);
-        else activate_array(acc, ACT_SILU);
+        activate_out(acc, ACT_SILU, p.y_bf16);
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
           const float u = ub[v * 64 + lane];
@@ -526,6 +532,53 @@ __global__ __launch_bounds__(256, 3) void expert_few_kernel(const ExpertArgs p) 
   if (p.plan) {
     count = planned_tile(p, ng, group, rows);
     if (count == 0) return;
+  } else if constexpr (NV > 1) {
+    // the slots counted by group, tile blockIdx.x / n_groups of the groups'
+    // tiles found (counts do not depend on the atomics' order), its slots in
+    // their own order
+    __shared__ int hist[kDirectSlots], found[2];
+    const int tile = blockIdx.x / p.n_groups;
+    ng = blockIdx.x - tile * p.n_groups;
+    hist[tid] = 0;
+    if (tid == 0) found[0] = -1;
+    const int id = p.ids[min(tid, p.slots - 1)];
+    lds_barrier();
+    if (tid < p.slots) atomicAdd(&hist[group_of(id, p.experts)], 1);
+    if (blockIdx.x == 0 && (id < -1 || id >= p.experts)) *p.err = 1;
+    lds_barrier();
+    if (wave == 0) {
+      int n[4], sum = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) sum += n[k] = (hist[4 * lane + k] + TILE - 1) / TILE;
+      int before = sum;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int u = __shfl_up(before, d);
+        if (lane >= d) before += u;
+      }
+      before -= sum;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (tile >= before && tile < before + n[k]) found[0] = 4 * lane + k, found[1] = tile - before;
+        before += n[k];
+      }
+    }
+    lds_barrier();
+    group = __builtin_amdgcn_readfirstlane(found[0]);
+    if (group < 0) return;
+    const int first = __builtin_amdgcn_readfirstlane(found[1]) * TILE;
+    count = min(__builtin_amdgcn_readfirstlane(hist[group]) - first, TILE);
+    if (wave == 0) {
+      int before = 0;
+      for (int c = 0; c < p.slots; c += 64) {
+        const int i = c + lane;
+        const bool hit = i < p.slots && group_of(p.ids[min(i, p.slots - 1)], p.experts) == group;
+        const uint64_t m = __ballot(hit);
+        const int at = before + __popcll(m & ((1ull << lane) - 1)) - first;
+        if (hit && at >= 0 && at < TILE) rows[at] = i;
+        before += __popcll(m);
+      }
+    }
   } else {
     // every wave looks over all slots: those of this group before s, and the
     // tile's from s on
@@ -570,43 +623,65 @@ __global__ __launch_bounds__(256, 3) void expert_few_kernel(const ExpertArgs p) 
     for (int q = 0; q < kFewRing; ++q) few_load(ring, q, wexp, at, q, steps, steps, lane);
   }
   lds_barrier();
-  // ---- the rows' Q8_1 into LDS, eight lanes per block
+  // ---- the rows' Q8_1 into LDS
   const FewLds lds = FewLds::of(steps);
   const int used = min(TILE, p.slots);  // rows that the LDS holds
   float *const ls = (float *)(smem + used * lds.a_ld);
-  {
-    const int l8 = tid & 7, padded = 4 * lds.steps2;
-    for (int u0 = 0; u0 < count * padded; u0 += 128) {
-      // four blocks per thread group at once: their loads in flight together
+  if (p.x_type) {
+    // quantized here, eight lanes per block, four blocks of each in flight
+    const int l8 = tid & 7;
+    for (int u0 = 0; u0 < count * p.blocks; u0 += 128) {
       float4 v[4];
-      int32_t q[4];
-      float sc[4];
+      int r[4], b[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int u = min(u0 + 32 * k + (tid >> 3), count * padded - 1);
-        const int r = u / padded, b = min(u - r * padded, p.blocks - 1);
-        const int64_t row = rows[r] / p.per_row;
-        if (p.x_type) {
-          v[k] = load_act4(p.x, row * p.ldx + b * kBlock + 4 * l8, p.x_type == 2, p.x_aligned != 0);
-        } else {
-          q[k] = *(const int32_t *)(p.qa + (row * p.blocks + b) * kBlock + 4 * l8);
-          sc[k] = p.sa[row * p.blocks + b];
-        }
-      }
-      if (p.x_type) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) quantize_block8(v[k], true, &q[k], &sc[k]);
+        const int u = min(u0 + 32 * k + (tid >> 3), count * p.blocks - 1);
+        r[k] = u / p.blocks, b[k] = u - r[k] * p.blocks;
+        v[k] = load_act4(p.x, (int64_t)(rows[r[k]] / p.per_row) * p.ldx + b[k] * kBlock + 4 * l8,
+                         p.x_type == 2, p.x_aligned != 0);
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int u = u0 + 32 * k + (tid >> 3);
-        if (u >= count * padded) continue;
-        const int r = u / padded, b = u - r * padded;
+        int32_t q;
+        float sc;
+        quantize_block8(v[k], true, &q, &sc);
+        if (u0 + 32 * k + (tid >> 3) >= count * p.blocks) continue;
         const int quarter = (l8 >> 1 & 1) * 2 + (l8 >> 2);  // eights 0, 2, 1, 3
-        *(int32_t *)(smem + r * lds.a_ld + (b >> 1) * 64 + quarter * 16 + (b & 1) * 8 + (l8 & 1) * 4) = q[k];
-        if (l8 == 0) ls[r * lds.s_ld + b] = b < p.blocks ? sc[k] : 0.0f;
+        *(int32_t *)(smem + r[k] * lds.a_ld + (b[k] >> 1) * 64 + quarter * 16 + (b[k] & 1) * 8 +
+                     (l8 & 1) * 4) = q;
+        if (l8 == 0) ls[r[k] * lds.s_ld + b[k]] = sc;
       }
     }
+  } else {
+    // a half block and a scale per thread, four of each in flight
+    const int halves = 2 * p.blocks;
+    for (int u0 = 0; u0 < count * halves; u0 += 1024) {
+      v4i v[4];
+      float sc[4];
+      int r[4], h[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int u = min(u0 + 256 * k + tid, count * halves - 1);
+        r[k] = u / halves, h[k] = u - r[k] * halves;
+        const int64_t row = rows[r[k]] / p.per_row;
+        v[k] = *(const v4i *)(p.qa + (row * p.blocks) * kBlock + 16 * h[k]);
+        sc[k] = p.sa[row * p.blocks + (h[k] >> 1)];
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (u0 + 256 * k + tid >= count * halves) continue;
+        const int b = h[k] >> 1;
+        uint8_t *const to = smem + r[k] * lds.a_ld + (b >> 1) * 64 + (h[k] & 1) * 16 + (b & 1) * 8;
+        *(v2i *)to = v2i{v[k][0], v[k][1]};
+        *(v2i *)(to + 32) = v2i{v[k][2], v[k][3]};
+        if (!(h[k] & 1)) ls[r[k] * lds.s_ld + b] = sc[k];
+      }
+    }
+  }
+  // blocks past the last: weights of zero against any values, scales of zero
+  for (int u = tid; u < count * 8; u += 256) {
+    const int b = p.blocks + (u & 7);
+    if (b < 4 * lds.steps2) ls[(u >> 3) * lds.s_ld + b] = 0.0f;
   }
   lds_barrier();
   float *const box = (float *)(smem + lds.bytes(used));
@@ -886,7 +961,7 @@ __device__ __forceinline__ void many_run(const ExpertArgs &p, int ng, int group,
           float o[4];
 #pragma unroll
           for (int v = 0; v < 4; ++v) o[v] = acc[t][4 * j + v];
-          activate_array(o, p.act);
+          activate_out(o, p.act, p.y_bf16);
           const int n = tile0 * 16 + 8 * j + 4 * hi;
           if (i >= count || n >= p.rows) continue;
           if (p.y_bf16) {
@@ -920,8 +995,7 @@ __device__ __forceinline__ void many_run(const ExpertArgs &p, int ng, int group,
           float o[4];
 #pragma unroll
           for (int v = 0; v < 4; ++v) o[v] = acc[t][4 * j + v];
-          if (p.y_bf16) silu_for_bf16(o);
-          else activate_array(o, ACT_SILU);
+          activate_out(o, ACT_SILU, p.y_bf16);
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
             const float u = acc[t][8 + 4 * j + v];
@@ -1140,8 +1214,8 @@ int32_t expert_tile_rows(int64_t slots, int64_t experts, int64_t widest) {
   return rows <= 16 && lds.bytes(rows) + kFewBox > kFewLdsMost ? 32 : rows;
 }
 
-bool expert_planned(int64_t slots, int32_t tile_rows) {
-  return slots > kDirectSlots || tile_rows > 16;
+bool expert_planned(int64_t slots, int64_t experts, int32_t tile_rows) {
+  return slots > kDirectSlots || tile_rows > 16 || (tile_rows > 4 && experts >= kDirectSlots);
 }
 
 int64_t expert_max_tiles(int64_t slots, int64_t experts, int32_t tile_rows) {
@@ -1176,7 +1250,9 @@ static void set_repeat(ExpertArgs &a, int64_t tiles, int cols, int fill) {
 
 template <int NV, bool DUAL>
 static hipError_t launch_few(ExpertArgs &a, bool fma, hipStream_t s) {
-  const int64_t tiles = a.plan ? a.max_tiles : a.slots;
+  const int64_t tiles = a.plan ? a.max_tiles
+                        : NV == 1 ? a.slots
+                                  : a.slots / (4 * NV) + std::min(a.slots, a.experts + 1);
   set_repeat(a, std::min(a.slots, a.experts), DUAL ? 32 : 64, 8);
   const int64_t wgs = tiles * a.n_groups;
   // HIP bounds a grid's work-items by 2^32 - 1

@@ -243,7 +243,7 @@ hipError_t launch_route(const void *logits, bool bf16, int64_t ld, int64_t m, in
 constexpr int64_t kDirectSlots = 256;
 constexpr int64_t kMaxSlots = 1 << 20;  // of a plan
 int32_t expert_tile_rows(int64_t slots, int64_t experts, int64_t widest);
-bool expert_planned(int64_t slots, int32_t tile_rows);
+bool expert_planned(int64_t slots, int64_t experts, int32_t tile_rows);
 int64_t expert_max_tiles(int64_t slots, int64_t experts, int32_t tile_rows);
 int64_t expert_plan_ints(int64_t slots, int64_t experts, int32_t tile_rows);
 // The plan and, x non-null, the Q8_1 of its m rows into qa / sa (dense).

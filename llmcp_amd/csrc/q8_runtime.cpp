@@ -1732,7 +1732,7 @@ static int expert_prepare(llmcp_q8_ctx *ctx, const ExpertRows &in, const int32_t
   l.experts = (int32_t)count;
   l.err_flag = ctx->err_flag;
   l.fma = ctx->fma();
-  const bool planned = expert_planned(slots, l.tile_rows);
+  const bool planned = expert_planned(slots, count, l.tile_rows);
   const int64_t blocks = in.cols / kBlock;
   int rc;
   if (in.q) {

@@ -97,6 +97,26 @@ def test_expert_linear_bitwise(ctx, oracle, m, top_k, e, n, k, dtype):
         st.release()
 
 
+# (tokens, top_k, experts, n, k): rows too wide for sixteen, eight and any of
+# them in a workgroup's LDS; a plan of more slots than are sorted through LDS,
+# of the most experts, and of a slot more than a workgroup looks over itself
+@pytest.mark.parametrize("m,top_k,e,n,k", [
+    (40, 2, 8, 24, 8192), (12, 1, 2, 16, 16416), (3, 2, 4, 16, 45056), (17000, 2, 5, 8, 32),
+    (32768, 1, 3, 8, 32), (32769, 1, 70, 8, 32), (400, 4, 1024, 8, 32), (257, 1, 300, 8, 32),
+    (256, 1, 200, 8, 32), (250, 1, 100, 24, 64)])
+def test_expert_linear_limits(ctx, oracle, m, top_k, e, n, k):
+    rng = np.random.default_rng(m + k)
+    st = Stack(ctx, oracle, rng, e, n, k)
+    try:
+        ids = rng.integers(-1, e, (m, top_k)).astype(np.int32)
+        x = rng.standard_normal((m, k)).astype(np.float32)
+        got = run_linear(ctx, oracle, st, x, ids, False, "none", "f32")
+        assert same(got, by_slot(ids, lambda i, r: oracle.linear(r, st.p4[i], n, epilogue=ctx.epilogue),
+                                 slot_rows(x, ids, False), n))
+    finally:
+        st.release()
+
+
 @pytest.mark.parametrize("m,top_k,e,only", [
     (60, 4, 64, [5]), (60, 4, 64, [0, 63, 7, 8]), (400, 2, 32, [31]), (400, 2, 32, [3, 3, 9])])
 def test_expert_linear_uneven(ctx, oracle, m, top_k, e, only):
@@ -236,7 +256,8 @@ def from_type(ctx, oracle, buf, shape, dtype):
 
 
 @pytest.mark.parametrize("m,top_k,e,h,f,masked", [
-    (1, 1, 1, 32, 32, 0.0), (1, 8, 12, 2560, 96, 0.0), (1, 8, 12, 160, 224, 0.4),
+    (1, 1, 1, 32, 32, 0.0), (1, 8, 12, 2560, 96, 0.0), (1, 12, 20, 96, 160, 0.2), (1, 32, 40, 64, 32, 0.0),
+    (3, 2, 40, 96, 64, 0.3), (5, 2, 40, 96, 64, 0.0), (11, 2, 40, 96, 64, 0.0), (1, 8, 12, 160, 224, 0.4),
     (2, 3, 4, 96, 64, 0.0), (16, 4, 24, 256, 96, 0.0), (60, 4, 3, 128, 160, 0.3),
     (33, 8, 9, 64, 32, 0.0), (150, 2, 7, 96, 192, 0.1), (300, 1, 1, 64, 96, 0.0),
     (130, 4, 100, 32, 64, 0.9)])
@@ -257,6 +278,33 @@ def test_expert_mlp(ctx, oracle, m, top_k, e, h, f, masked, dtype):
         empty = (ids < 0).all(1)
         if empty.any():  # a token without an expert: its residual
             assert np.array_equal(y[empty], r[empty] if residual else np.zeros((empty.sum(), h)))
+    finally:
+        for s in (gate, up, down):
+            s.release()
+
+
+def test_swiglu_rounds_as_the_oracle_over_the_gate_s_range(ctx, oracle):
+    """bf16: silu of gate sums of every size and of both signs, those next to
+    a rounding of bf16 among them, through one expert whose down weights
+    pick single columns of h apart."""
+    rng = np.random.default_rng(77)
+    h, f, m, dtype = 64, 64, 400, "bf16"
+    gate, up = Stack(ctx, oracle, rng, 1, f, h, 0.3), Stack(ctx, oracle, rng, 1, f, h, 0.3)
+    down = Stack(ctx, oracle, rng, 1, h, f)
+    bits, wide = oracle.f32_to_bf16_bits, oracle.bf16_bits_to_f32
+    try:
+        x = rng.standard_normal((m, h)) * 10.0 ** rng.uniform(-44, 3, (m, 1))
+        x = wide(bits(x.astype(np.float32)))
+        ids = np.zeros((m, 1), np.int32)
+        yd = ctx.alloc(m * h * 2)
+        ctx.expert_mlp(to_type(ctx, oracle, x, dtype), ctx.to_device(ids), None, m, 1, gate.t, up.t,
+                       down.t, yd, dtype=dtype)
+        _, ref, bound = mlp_reference(oracle, ctx.epilogue, x, ids, None, gate, up, down, None, dtype)
+        fine = np.isfinite(ref)
+        y = from_type(ctx, oracle, yd, (m, h), dtype)
+        assert np.array_equal(np.isfinite(y), fine)
+        # one slot of weight 1: the sum is o itself, already bf16
+        assert np.array_equal(y[fine], ref[fine].astype(np.float32))
     finally:
         for s in (gate, up, down):
             s.release()
@@ -433,6 +481,54 @@ def test_block_end_to_end(ctx, q8, oracle, m):
         ctx.release(router)
         for st in (gate, up, down):
             st.release()
+
+
+def test_two_contexts_streams_and_graphs(ctx, q8, oracle):
+    """Two contexts with the same weights on streams of their own, and two
+    graphs of one context that share its workspace, replayed in turn."""
+    rng = np.random.default_rng(12)
+    e, h, f, top_k, dtype = 6, 96, 64, 3, "bf16"
+    gate, up, down, _, _, _, _ = expert_mlp_case(ctx, oracle, rng, 4, top_k, e, h, f, dtype)
+    cases, refs = [], []
+    for m in (1, 100):
+        ids, x = choices(rng, m, top_k, e), rng.standard_normal((m, h)).astype(np.float32)
+        xb = oracle.f32_to_bf16_bits(x)
+        cases.append((m, ctx.to_device(xb), ctx.to_device(ids), ctx.alloc(m * h * 2)))
+        _, ref, bound = mlp_reference(oracle, ctx.epilogue, oracle.bf16_bits_to_f32(xb), ids, None,
+                                      gate, up, down, None, dtype)
+        refs.append((ref, bound))
+    other = q8.Context(0)
+    try:
+        other.set_platform(ctx.platform)
+        stacks = [other.upload_experts_p4(np.concatenate(s.p4), e, s.n, s.k) for s in (gate, up, down)]
+
+        def call(c, st, i, y=None):
+            m, x, ids, out = cases[i]
+            c.expert_mlp(x, ids, None, m, top_k, *st, y or out, dtype=dtype)
+        own = [s.t for s in (gate, up, down)]
+        for i in (1, 0):
+            call(ctx, own, i)
+        ctx.sync()
+        graphs = []
+        for i in (0, 1):
+            ctx.graph_begin()
+            call(ctx, own, i)
+            graphs.append(ctx.graph_end())
+        outs = [other.alloc(cases[i][0] * h * 2) for i in (0, 1)]
+        for rep in range(4):
+            for i in ((0, 1), (1, 0))[rep % 2]:
+                ctx.graph_launch(graphs[i])
+                call(other, stacks, 1 - i, outs[1 - i])
+        for c, bufs in ((ctx, [cases[0][3], cases[1][3]]), (other, outs)):
+            for buf, case, (ref, bound) in zip(bufs, cases, refs):
+                y = oracle.bf16_bits_to_f32(c.to_host(buf, (case[0], h), np.uint16))
+                assert (np.abs(y - ref) <= bound).all()
+        for g in graphs:
+            ctx.graph_destroy(g)
+    finally:
+        other.close()
+        for s in (gate, up, down):
+            s.release()
 
 
 # ------------------------------------------------------ registry, errors --
