@@ -7,6 +7,7 @@
 //   arena loader       lib/Runtime/WeightArena.cpp:27-131, include/llmcp/Support/PackedWeights.h
 //   arena writer       lib/Model/WeightPacker.cpp:126-160, :164-274
 //   packer             lib/Model/Quantization.cpp:92-116, :165-214
+#include <dlfcn.h>
 #include <hip/hip_runtime.h>
 #include <omp.h>
 
@@ -3182,8 +3183,16 @@ int llmcp_q8_microbench_epilogue(llmcp_q8_ctx *ctx, int32_t mode, int32_t blocks
   });
 }
 
+// Whether f is a kernel of this library.  Another's node may stand for more
+// than hipLaunchKernel takes (a module's function, a cooperative grid).
+static bool own_kernel(const void *f) {
+  static const char here = 0;
+  Dl_info a, b;
+  return dladdr(f, &a) && dladdr(&here, &b) && a.dli_fbase == b.dli_fbase;
+}
+
 // The kernels of a graph in order if it is nothing but a chain of up to
-// kMaxChain of them; empty otherwise.
+// kMaxChain of this library's; empty otherwise.
 static std::vector<hipKernelNodeParams> kernel_chain(hipGraph_t g) {
   size_t n = 0, m = 0;
   if (hipGraphGetNodes(g, nullptr, &n) != hipSuccess || n == 0 || n > kMaxChain) return {};
@@ -3205,7 +3214,8 @@ static std::vector<hipKernelNodeParams> kernel_chain(hipGraph_t g) {
     hipGraphNodeType type;
     hipKernelNodeParams k = {};
     if (hipGraphNodeGetType(at, &type) != hipSuccess || type != hipGraphNodeTypeKernel ||
-        hipGraphKernelNodeGetParams(at, &k) != hipSuccess || !k.func || !k.kernelParams || k.extra)
+        hipGraphKernelNodeGetParams(at, &k) != hipSuccess || !k.func || !k.kernelParams || k.extra ||
+        !own_kernel(k.func))
       return {};
     chain.push_back(k);
   }
