@@ -1786,11 +1786,13 @@ static int expert_linear_impl(llmcp_q8_ctx *ctx, const Rows &x, const int32_t *e
   if (activation < LLMCP_Q8_ACT_NONE || activation > LLMCP_Q8_ACT_SOFTPLUS)
     return fail(LLMCP_Q8_DECLINED, "unsupported activation %d", activation);
   const int64_t slots = out.rows;
-  if ((rc = check_slots(in, experts, top_k, slots, std::max(w->rows, w->cols)))) return rc;
-  if (slots % top_k != 0 || (x.rows != slots && x.rows != slots / top_k))
+  if (top_k > 0 && (slots % top_k != 0 || (x.rows != slots && x.rows != slots / top_k)))
     return fail(LLMCP_Q8_DECLINED, "output of %lld rows needs an input of %lld or %lld / top_k",
                 (long long)slots, (long long)slots, (long long)slots);
+  if ((rc = check_slots(in, experts, top_k, slots, std::max(w->rows, w->cols)))) return rc;
   if (slots == 0) return LLMCP_Q8_OK;
+  if (x.data == out.data)
+    return fail(LLMCP_Q8_EINVAL, "an expert linear's output must not take its input's memory");
   if ((rc = set_device(ctx))) return rc;
   ExpertLaunch l;
   if ((rc = expert_prepare(ctx, in, experts, slots, w->experts, w->cols, l))) return rc;

@@ -604,6 +604,7 @@ def test_expert_entries_refuse(ctx, q8, oracle):
             args[i] = bad
             assert linear(*args) == code, (i, code)
         assert linear(*ok, act=4) == q8.DECLINED
+        assert linear(*ok[:4], mr(buf.ptr, 4, 32)) == q8.EINVAL  # over its own input
         assert linear(mr(buf.ptr, 0, 64), buf.ptr, 2, w, mr(buf.ptr, 0, 32)) == q8.OK
         mlp = lambda x, y, wg, wu, wd, k=2, r=None: L.llmcp_q8_expert_mlp(  # noqa: E731
             ctx.handle, ref(x), buf.ptr, None, k, ref(wg.t.memref()), ref(wu.t.memref()),
