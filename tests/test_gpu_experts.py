@@ -283,6 +283,43 @@ def test_expert_mlp(ctx, oracle, m, top_k, e, h, f, masked, dtype):
             s.release()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("pad", [0, 3, 4])
+def test_expert_mlp_many_rows(ctx, q8, oracle, pad, dtype):
+    """Enough rows that the sum takes eight bf16 columns per thread, residual
+    and output with rows apart: the bits of calls on a few rows each."""
+    rng = np.random.default_rng(pad)
+    m, top_k, e, h, f = 4100, 3, 6, 1024, 32
+    stacks = [Stack(ctx, oracle, rng, e, n, k) for n, k in ((f, h), (f, h), (h, f))]
+    size, et = (2, np.uint16) if dtype == "bf16" else (4, np.float32)
+    try:
+        x, r = (rng.standard_normal((m, n)).astype(np.float32) for n in (h, h + pad))
+        ids = choices(rng, m, top_k, e, masked=0.2)
+        w = rng.standard_normal((m, top_k)).astype(np.float32)
+        xd, rd = to_type(ctx, oracle, x, dtype), to_type(ctx, oracle, r, dtype)
+        idd, wd = ctx.to_device(ids), ctx.to_device(w)
+        fill = np.full((m, h + pad), 7, et)
+        yd, part = ctx.to_device(fill), ctx.to_device(fill)
+        names = [ctypes.byref(s.t.memref()) for s in stacks]
+
+        def call(y, first, n):
+            at = lambda buf, row: buf.ptr + first * row  # noqa: E731
+            rows = [q8.f32_memref(at(b, k * size), n, h, k) for b, k in
+                    ((xd, h), (rd, h + pad), (y, h + pad))]
+            q8.check(getattr(q8.lib(), "llmcp_q8_expert_mlp" + ("_bf16" if dtype == "bf16" else ""))(
+                ctx.handle, ctypes.byref(rows[0]), at(idd, 4 * top_k), at(wd, 4 * top_k), top_k, *names,
+                ctypes.byref(rows[1]), ctypes.byref(rows[2])))
+        call(yd, 0, m)
+        for first in range(0, m, 400):
+            call(part, first, min(400, m - first))
+        a, b = (ctx.to_host(v, (m, h + pad), et) for v in (yd, part))
+        assert np.array_equal(a.view(np.uint8), b.view(np.uint8))
+        assert (a[:, h:] == 7).all() and np.isfinite(from_type(ctx, oracle, yd, (m, h + pad), dtype)).all()
+    finally:
+        for s in stacks:
+            s.release()
+
+
 def test_swiglu_rounds_as_the_oracle_over_the_gate_s_range(ctx, oracle):
     """bf16: silu of gate sums of every size and of both signs, those next to
     a rounding of bf16 among them, through one expert whose down weights
