@@ -717,20 +717,36 @@ __global__ __launch_bounds__(64 * kTokenWaves) void expert_token_kernel(
   const int tile = blockIdx.x, steps = p.lay.steps;
   uint8_t *const mine = smem + wave * token_lds(steps);
   float *const ls = (float *)(mine + ((steps + 1) & ~1) * 128);
+  // what the sum needs, on its way before the products
+  const int64_t choice = token * top_k + min(lane, top_k - 1);
+  const int ids = p.ids[choice];
+  const float factors = weights ? weights[choice] : 1.0f;
+  const int n = tile * 16 + li;
+  float v = 0.0f;
+  if (residual && wave == 0 && n < p.rows)
+    v = BF16 ? bf16_to_float(((const uint16_t *)residual)[token * ldr + n])
+             : ((const float *)residual)[token * ldr + n];
   for (int j = wave; j < top_k; j += waves) {
     const int64_t slot = token * top_k + j;
-    const int id = __builtin_amdgcn_readfirstlane(p.ids[slot]);
+    const int id = __builtin_amdgcn_readlane(ids, j);
     if ((unsigned)id >= (unsigned)p.experts) continue;  // uniform per wave
     const uint8_t *const wexp = p.w0 + (int64_t)id * p.lay.expert_bytes();
     const uint32_t at = (uint32_t)tile * (uint32_t)p.lay.tile_bytes();
+    // the row's first pieces before the weights, which then need not have come
+    // for them to be stored
+    const int8_t *const row = p.qa + slot * p.blocks * kBlock;
+    const float *const scales = p.sa + slot * p.blocks;
+    const v4i r0 = *(const v4i *)(row + 16 * min(lane, 2 * p.blocks - 1));
+    const float s0 = scales[min(lane, p.blocks - 1)];
     FewRing ring;
 #pragma unroll
     for (int q = 0; q < kFewRing; ++q) few_load(ring, q, wexp, at, q, steps, steps, lane);
-    const int8_t *const row = p.qa + slot * p.blocks * kBlock;
-    for (int b = lane; b < 2 * p.blocks; b += 64) *(v4i *)(mine + 16 * b) = *(const v4i *)(row + 16 * b);
     // (a block past the last must have a finite scale; its weights are zero)
-    for (int b = lane; b < 4 * ((steps + 1) & ~1); b += 64)
-      ls[b] = b < p.blocks ? p.sa[slot * p.blocks + b] : 0.0f;
+    const int padded = 4 * ((steps + 1) & ~1);
+    if (lane < 2 * p.blocks) *(v4i *)(mine + 16 * lane) = r0;
+    if (lane < padded) ls[lane] = lane < p.blocks ? s0 : 0.0f;
+    for (int b = lane + 64; b < 2 * p.blocks; b += 64) *(v4i *)(mine + 16 * b) = *(const v4i *)(row + 16 * b);
+    for (int b = lane + 64; b < padded; b += 64) ls[b] = b < p.blocks ? scales[b] : 0.0f;
     __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the wave's own stores
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
     // every MFMA row reads the one row: eights 0, 2, 1, 3 of a block
@@ -750,17 +766,13 @@ __global__ __launch_bounds__(64 * kTokenWaves) void expert_token_kernel(
     if (lq == 0) sums[j][li] = BF16 ? as_bf16(acc[0]) : acc[0];
   }
   __syncthreads();
-  const int n = tile * 16 + threadIdx.x;
-  if (threadIdx.x >= 16 || n >= p.rows) return;
-  float v = 0.0f;
-  if (residual)
-    v = BF16 ? bf16_to_float(((const uint16_t *)residual)[token * ldr + n])
-             : ((const float *)residual)[token * ldr + n];
+  if (wave != 0) return;
   for (int j = 0; j < top_k; ++j) {
-    const int64_t slot = token * top_k + j;
-    if ((unsigned)p.ids[slot] >= (unsigned)p.experts) continue;
-    v = __builtin_fmaf(weights ? weights[slot] : 1.0f, sums[j][threadIdx.x], v);
+    if ((unsigned)__builtin_amdgcn_readlane(ids, j) >= (unsigned)p.experts) continue;
+    const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, factors), j));
+    v = __builtin_fmaf(w, sums[j][li], v);
   }
+  if (lane >= 16 || n >= p.rows) return;
   if (BF16) ((uint16_t *)y)[token * ldy + n] = float_to_bf16(v);
   else ((float *)y)[token * ldy + n] = v;
 #endif
