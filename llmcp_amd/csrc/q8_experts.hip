@@ -368,14 +368,15 @@ constexpr int kFewLdsMost = 159 * 1024;
 constexpr int kFewRing = 6;  // steps of a wave's tile in flight
 
 // The ring's place q takes step st of the tile at byte `tile` of the expert
-// (st >= live: zeros, without touching memory).  No load is branched around:
+// (st >= live: zeros, without touching memory), the lane's scale from byte
+// scale_at of the step's.  No load is branched around:
 // the compiler counts the loads in flight to know which have come.
 struct FewRing {
   v4u w[kFewRing][2];
   uint32_t d[kFewRing];
 };
 __device__ __forceinline__ void few_load(FewRing &ring, int q, const uint8_t *wexp, uint32_t tile,
-                                         int st, int live, int steps, int lane) {
+                                         int st, int live, int steps, int lane, int scale_at) {
   const DmaStage a = dma_stage(st, live, tile + (uint32_t)st * 2048u);
   const DmaStage b = dma_stage(st, live, tile + (uint32_t)steps * 2048u + (uint32_t)st * 128u);
   const __amdgpu_buffer_rsrc_t r =
@@ -383,7 +384,7 @@ __device__ __forceinline__ void few_load(FewRing &ring, int q, const uint8_t *we
   constexpr int kNt = 2;  // non-temporal: read once
   ring.w[q][0] = __builtin_amdgcn_raw_buffer_load_b128(r, lane * 16, a.offset, kNt);
   ring.w[q][1] = __builtin_amdgcn_raw_buffer_load_b128(r, lane * 16 + 1024, a.offset, kNt);
-  ring.d[q] = __builtin_amdgcn_raw_buffer_load_b16(r, (lane & 15) * 8 + (lane >> 4) * 2, b.offset, kNt);
+  ring.d[q] = __builtin_amdgcn_raw_buffer_load_b16(r, scale_at, b.offset, kNt);
 }
 
 // A step's dots (four blocks) and scale products.
@@ -423,7 +424,7 @@ template <int NV, bool FMA, class ReadRows>
 __device__ __forceinline__ void few_tile(FewRing &ring, const uint8_t *wexp, uint32_t cur,
                                          uint32_t next, int after, int steps, FewRows &x,
                                          ReadRows &&read_rows, float (&acc)[NV]) {
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63, scale_at = (lane & 15) * 8 + (lane >> 4) * 2;
   const int steps2 = (steps + 1) & ~1, stages = (steps2 + kFewRing - 1) / kFewRing;
   auto epilogue = [&](const FewDots &o) __attribute__((always_inline)) {
 #pragma unroll
@@ -451,8 +452,8 @@ __device__ __forceinline__ void few_tile(FewRing &ring, const uint8_t *wexp, uin
         __builtin_amdgcn_sched_barrier(0);
         epilogue(even);
       }
-      few_load(ring, q, wexp, from, st0 + q, live, steps, lane);
-      few_load(ring, q + 1, wexp, from, st0 + q + 1, live, steps, lane);
+      few_load(ring, q, wexp, from, st0 + q, live, steps, lane, scale_at);
+      few_load(ring, q + 1, wexp, from, st0 + q + 1, live, steps, lane, scale_at);
     });
   }
   epilogue(odd);
@@ -621,7 +622,7 @@ __global__ __launch_bounds__(256, 3) void expert_few_kernel(const ExpertArgs p) 
     const int tile = DUAL ? ng * p.repeat * 2 + (wave >> 1) : ng * p.repeat * 4 + wave;
     const uint32_t at = (uint32_t)min(tile, p.lay.tiles - 1) * (uint32_t)p.lay.tile_bytes();
 #pragma unroll
-    for (int q = 0; q < kFewRing; ++q) few_load(ring, q, wexp, at, q, steps, steps, lane);
+    for (int q = 0; q < kFewRing; ++q) few_load(ring, q, wexp, at, q, steps, steps, lane, (lane & 15) * 8 + (lane >> 4) * 2);
   }
   lds_barrier();
   // ---- the rows' Q8_1 into LDS
@@ -690,11 +691,215 @@ __global__ __launch_bounds__(256, 3) void expert_few_kernel(const ExpertArgs p) 
 #endif
 }
 
-// ---- few tokens: the down products and their weighted sum in one launch
+// ---- few tokens: a slot's own row, no sharing
+//
+// A CU takes about 13 B a clock from beyond its L2 however few of the others
+// do (a workgroup that reads 174 KB takes 11 us whether there are 24 of them or
+// 240), so a token's products are as fast as the bytes are spread evenly, and
+// as what comes before the first and after the last load is short.
+
+// What a row is: Q8_1, or f32 or bf16 to be quantized here.
+enum { ROW_Q8 = 0, ROW_F32 = 1, ROW_BF16 = 2 };
+
+// A wave's part of a row in LDS, `count` blocks from `first` on: values in
+// order, scales (zero past the row's last block).  `start` issues the first
+// loads, `store` waits for them.
+template <int KIND, int U>
+struct TokenRow {
+  uint4 v[U];  // eight lanes per block
+  v4i q;       // ROW_Q8: half a block per lane, a scale per lane
+  float s;
+  __device__ __forceinline__ uint4 load(const ExpertArgs &p, int64_t row, int block) const {
+    const int64_t at = row * p.ldx + (int64_t)min(block, p.blocks - 1) * kBlock + 4 * (threadIdx.x & 7);
+    return load_raw4<KIND == ROW_BF16, true>(p.x, at);
+  }
+  __device__ __forceinline__ void start(const ExpertArgs &p, int64_t row, int first) {
+    const int lane = threadIdx.x & 63;
+    if constexpr (KIND != ROW_Q8) {
+#pragma unroll
+      for (int k = 0; k < U; ++k) v[k] = load(p, row, first + 8 * k + (lane >> 3));
+    } else {
+      q = *(const v4i *)(p.qa + row * p.blocks * kBlock + 16 * min(2 * first + lane, 2 * p.blocks - 1));
+      s = p.sa[row * p.blocks + min(first + lane, p.blocks - 1)];
+    }
+  }
+  __device__ __forceinline__ void store(const ExpertArgs &p, int64_t row, int first, int count,
+                                        uint8_t *values, float *scales) {
+    const int lane = threadIdx.x & 63, l8 = lane & 7;
+    if constexpr (KIND != ROW_Q8) {
+      auto one = [&](uint4 x, int u) __attribute__((always_inline)) {
+        int32_t b;
+        float sc;
+        quantize_block8(act4_of_raw<KIND == ROW_BF16>(x), true, &b, &sc);
+        if (u >= count) return;
+        *(int32_t *)(values + u * kBlock + 4 * l8) = b;
+        if (l8 == 0) scales[u] = first + u < p.blocks ? sc : 0.0f;
+      };
+#pragma unroll
+      for (int k = 0; k < U; ++k)
+        if (8 * k < count) one(v[k], 8 * k + (lane >> 3));
+      for (int u = 8 * U; u < count; u += 8) one(load(p, row, first + u + (lane >> 3)), u + (lane >> 3));
+    } else {
+      const int8_t *const qrow = p.qa + row * p.blocks * kBlock;
+      const float *const srow = p.sa + row * p.blocks;
+      if (lane < 2 * count) *(v4i *)(values + 16 * lane) = q;
+      if (lane < count) scales[lane] = first + lane < p.blocks ? s : 0.0f;
+      for (int u = lane + 64; u < 2 * count; u += 64)
+        *(v4i *)(values + 16 * u) = *(const v4i *)(qrow + 16 * min(2 * first + u, 2 * p.blocks - 1));
+      for (int u = lane + 64; u < count; u += 64)
+        scales[u] = first + u < p.blocks ? srow[first + u] : 0.0f;
+    }
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the wave's own stores
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  }
+};
+
+// ---- the SwiGLU of a slot
+//
+// A workgroup takes 8 columns of gate and of up, two waves each, half of the
+// steps per wave.  A lane takes half a block of a row, four v_dot4; two steps
+// together give every lane a block's dot, which goes to LDS with the scale
+// product, and sixteen lanes run the chains over them in block order.  h is
+// left in the output's type; the down products quantize it.
+
+constexpr int kUpPairs = 5;  // pairs of steps of a wave in flight
+struct UpRing {
+  v4u w[kUpPairs][2];
+  uint32_t d[kUpPairs];
+};
+
+// Steps of a wave (an even number) and the LDS: the row, then [gate,
+// up][block][column] {dot, factor} of whole batches of the chain.
+constexpr int kUpBatch = 16;  // blocks read while as many before are added
+__host__ __device__ inline int token_up_steps(int steps) { return ((steps + 1) / 2 + 1) & ~1; }
+__host__ __device__ inline int token_up_blocks(int steps) { return (4 * steps + kUpBatch - 1) & -kUpBatch; }
+__host__ __device__ inline int token_up_lds(int steps) {
+  return 2 * token_up_steps(steps) * (128 + 16) + (2 * token_up_blocks(steps) + kUpBatch) * 8 * 8;
+}
+
+// The ring's place q takes steps st and st + 1 of the eight rows whose values
+// and scales begin at bytes `values` and `scales` of the expert; from `live` on
+// they are zeros, without touching memory.
+__device__ __forceinline__ void up_load(UpRing &ring, int q, const uint8_t *wexp, uint32_t values,
+                                        uint32_t scales, int st, int live, int lane) {
+  constexpr int kNt = 2;  // non-temporal: read once
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const DmaStage a = dma_stage(st + i, live, values + (uint32_t)(st + i) * 2048u);
+    const __amdgpu_buffer_rsrc_t r =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(wexp), 0, a.extent, 0x00020000);
+    ring.w[q][i] = __builtin_amdgcn_raw_buffer_load_b128(r, (lane >> 3) * 256 + (lane & 7) * 16, a.offset, kNt);
+  }
+  // the second step's by the lanes of second halves (if there is one)
+  const DmaStage d = dma_stage(st, live, scales + (uint32_t)st * 128u);
+  const __amdgpu_buffer_rsrc_t r =
+      __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(wexp), 0, d.extent, 0x00020000);
+  const int second = (st + 1 - live) >> 31 & 128;
+  ring.d[q] = __builtin_amdgcn_raw_buffer_load_b16(
+      r, (lane & 7) * 8 + (lane >> 4) * 2 + (lane & 8 ? second : 0), d.offset, kNt);
+}
+
+template <bool FMA, bool BF16, int KIND>
+__global__ __launch_bounds__(256) void expert_token_up_kernel(const ExpertArgs p) {
+#ifdef __HIP_DEVICE_COMPILE__
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int steps = p.lay.steps, slot = blockIdx.y;
+  const int64_t row = slot / p.per_row;
+  const int per = token_up_steps(steps);
+  const int first = min((wave >> 1) * per, steps), end = min(first + per, steps);
+  float *const scales = (float *)(smem + 2 * per * 128);
+  float2 *const box = (float2 *)(smem + 2 * per * (128 + 16));
+  // a quarter of the row per wave (an even number of blocks)
+  const int quarter = 2 * per;
+  TokenRow<KIND, 3> x;
+  x.start(p, row, wave * quarter);
+  const int id = __builtin_amdgcn_readfirstlane(p.ids[slot]);
+  if ((unsigned)id >= (unsigned)p.experts) {
+    if (blockIdx.x == 0 && threadIdx.x == 0 && id != -1) *p.err = 1;
+    return;
+  }
+  const uint8_t *const wexp = (wave & 1 ? p.w1 : p.w0) + (int64_t)id * p.lay.expert_bytes();
+  const uint32_t tile = (blockIdx.x >> 1) * (uint32_t)p.lay.tile_bytes();
+  const uint32_t wat = tile + (blockIdx.x & 1) * 128u, dat = tile + (uint32_t)steps * 2048u + (blockIdx.x & 1) * 64u;
+  UpRing ring;
+#pragma unroll
+  for (int q = 0; q < kUpPairs; ++q) up_load(ring, q, wexp, wat, dat, first + 2 * q, end, lane);
+  x.store(p, row, wave * quarter, quarter, smem + wave * quarter * kBlock, scales + wave * quarter);
+  // blocks of the last batch that no step writes
+  const int blocks = token_up_blocks(steps), written = 4 * ((steps + 1) & ~1);
+  for (int i = threadIdx.x; i < (blocks - written) * 16; i += 256)
+    box[(i & 8 ? blocks * 8 : 0) + (written + (i >> 4)) * 8 + (i & 7)] = make_float2(0.0f, 0.0f);
+  lds_barrier();
+  // lane: column lane % 8, half (lane / 8) % 2 of block lane / 16, of whose two
+  // steps it keeps that of its half
+  const bool upper = lane & 8;
+  auto pass = [&](int s, auto LOADS, auto FULL) __attribute__((always_inline)) {
+    const uint8_t *const xv = smem + s * 128 + (lane >> 3) * 16;
+    const float *const xs = scales + 4 * s + (upper ? 4 : 0) + (lane >> 4);
+    float2 *const to = box + (wave & 1) * blocks * 8 + ((s + (upper ? 1 : 0)) * 4 + (lane >> 4)) * 8 + (lane & 7);
+    static_for<kUpPairs>([&](auto Q) __attribute__((always_inline)) {
+      constexpr int q = decltype(Q)::value;
+      if (FULL || s + 2 * q < end) {
+        int c[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const v4i v = *(const v4i *)(xv + (2 * q + i) * 128);
+          c[i] = 0;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) c[i] = __builtin_amdgcn_sdot4((int)ring.w[q][i][k], v[k], c[i], false);
+        }
+        // the other half's part of this lane's step (row_ror:8)
+        const int send = upper ? c[0] : c[1];
+        const int dot = (upper ? c[1] : c[0]) + __builtin_amdgcn_update_dpp(0, send, 0x128, 0xf, 0xf, false);
+        to[2 * q * 32] = make_float2((float)dot, xs[8 * q] * half_bits_to_float(ring.d[q]));
+      }
+      if (LOADS) up_load(ring, q, wexp, wat, dat, s + 2 * (q + kUpPairs), end, lane);
+    });
+  };
+  int st = first;
+  for (; st + 2 * kUpPairs < end; st += 2 * kUpPairs) pass(st, std::true_type(), std::true_type());
+  if (st + 2 * kUpPairs == end) pass(st, std::false_type(), std::true_type());
+  else pass(st, std::false_type(), std::false_type());
+  lds_barrier();
+  if (wave != 0) return;
+  // lanes 0-7: the gate's columns, 8-15: the up's (the others repeat)
+  const float2 *t = box + (upper ? blocks * 8 : 0) + (lane & 7);
+  float acc[1] = {0.0f};
+  float2 v[kUpBatch];
+#pragma unroll
+  for (int k = 0; k < kUpBatch; ++k) v[k] = t[k * 8];
+  for (int b = 0; b < blocks; b += kUpBatch) {
+    float2 n[kUpBatch];  // (behind the last batch: memory that is not used)
+    t += kUpBatch * 8;
+#pragma unroll
+    for (int k = 0; k < kUpBatch; ++k) n[k] = t[k * 8];
+#pragma unroll
+    for (int k = 0; k < kUpBatch; ++k) {
+      if (FMA) {
+        acc[0] = __builtin_fmaf(v[k].x, v[k].y, acc[0]);
+      } else {
+        const float contrib = v[k].x * v[k].y;
+        acc[0] = acc[0] + contrib;
+      }
+      v[k] = n[k];
+    }
+  }
+  const float u = dpp_f32<0x128>(acc[0]);
+  activate_out(acc, ACT_SILU, BF16);
+  if (lane >= 8) return;
+  const int64_t at = (int64_t)slot * p.ldy + blockIdx.x * 8 + lane;
+  if (BF16) ((uint16_t *)p.y)[at] = float_to_bf16(as_bf16(acc[0]) * as_bf16(u));
+  else ((float *)p.y)[at] = acc[0] * u;
+#endif
+}
+
+// ---- their down products and weighted sum in one launch
 //
 // A workgroup per token and tile of 16 columns, a wave per slot (in turns
-// beyond eight): each streams its expert's tile with its one row of h in
-// LDS, and the results, rounded to the output's type, are added in slot
+// beyond eight): each streams its expert's tile with its one row of h,
+// quantized to LDS, and the results, rounded to the output's type, are added in slot
 // order by sixteen lanes (expert_combine_kernel's sum).  An expert that two
 // tokens share is read twice.
 
@@ -728,27 +933,17 @@ __global__ __launch_bounds__(64 * kTokenWaves) void expert_token_kernel(
              : ((const float *)residual)[token * ldr + n];
   for (int j = wave; j < top_k; j += waves) {
     const int64_t slot = token * top_k + j;
+    TokenRow<BF16 ? ROW_BF16 : ROW_F32, 3> x;  // on its way before the weights
+    x.start(p, slot, 0);
     const int id = __builtin_amdgcn_readlane(ids, j);
     if ((unsigned)id >= (unsigned)p.experts) continue;  // uniform per wave
     const uint8_t *const wexp = p.w0 + (int64_t)id * p.lay.expert_bytes();
     const uint32_t at = (uint32_t)tile * (uint32_t)p.lay.tile_bytes();
-    // the row's first pieces before the weights, which then need not have come
-    // for them to be stored
-    const int8_t *const row = p.qa + slot * p.blocks * kBlock;
-    const float *const scales = p.sa + slot * p.blocks;
-    const v4i r0 = *(const v4i *)(row + 16 * min(lane, 2 * p.blocks - 1));
-    const float s0 = scales[min(lane, p.blocks - 1)];
     FewRing ring;
 #pragma unroll
-    for (int q = 0; q < kFewRing; ++q) few_load(ring, q, wexp, at, q, steps, steps, lane);
-    // (a block past the last must have a finite scale; its weights are zero)
-    const int padded = 4 * ((steps + 1) & ~1);
-    if (lane < 2 * p.blocks) *(v4i *)(mine + 16 * lane) = r0;
-    if (lane < padded) ls[lane] = lane < p.blocks ? s0 : 0.0f;
-    for (int b = lane + 64; b < 2 * p.blocks; b += 64) *(v4i *)(mine + 16 * b) = *(const v4i *)(row + 16 * b);
-    for (int b = lane + 64; b < padded; b += 64) ls[b] = b < p.blocks ? scales[b] : 0.0f;
-    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the wave's own stores
-    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    for (int q = 0; q < kFewRing; ++q)
+      few_load(ring, q, wexp, at, q, steps, steps, lane, li * 8 + lq * 2);
+    x.store(p, slot, 0, 4 * ((steps + 1) & ~1), mine, ls);
     // every MFMA row reads the one row: eights 0, 2, 1, 3 of a block
     const uint8_t *const a = mine + ((lq & 1) * 2 + (lq >> 1)) * 8;
     auto read_rows = [&](FewRows &x, int st) __attribute__((always_inline)) {
@@ -759,10 +954,10 @@ __global__ __launch_bounds__(64 * kTokenWaves) void expert_token_kernel(
       }
       x.s = ls[4 * st + lq];
     };
-    FewRows x;
-    read_rows(x, 0);
+    FewRows first;
+    read_rows(first, 0);
     float acc[1];
-    few_tile<1, FMA>(ring, wexp, at, at, 0, steps, x, read_rows, acc);
+    few_tile<1, FMA>(ring, wexp, at, at, 0, steps, first, read_rows, acc);
     if (lq == 0) sums[j][li] = BF16 ? as_bf16(acc[0]) : acc[0];
   }
   __syncthreads();
@@ -1350,12 +1545,27 @@ hipError_t launch_experts(const ExpertLaunch &l, hipStream_t s) {
   }
 }
 
-bool expert_token_takes(int64_t m, int32_t top_k, int64_t experts, int64_t cols) {
-  // an expert's weight read once per token, a launch less: as long as few
-  // tokens share one
-  const int64_t slots = m * top_k;
-  return (m == 1 || slots * 4 <= experts) &&
-         std::min(top_k, kTokenWaves) * token_lds(expert_layout(16, cols).steps) <= 150 * 1024;
+bool expert_token_takes(int64_t m, int32_t top_k, int64_t experts, int64_t cols, int64_t width) {
+  // an expert's weight read once per slot: as long as few tokens share one
+  return (m == 1 || m * top_k * 4 <= experts) && token_up_lds(expert_layout(16, cols).steps) <= 150 * 1024 &&
+         std::min(top_k, kTokenWaves) * token_lds(expert_layout(16, width).steps) <= 150 * 1024;
+}
+
+template <bool FMA, bool BF16>
+static hipError_t launch_token_up(const ExpertArgs &a, hipStream_t s) {
+  const dim3 grid((unsigned)(a.rows / 8), (unsigned)a.slots), wg(256);
+  const size_t lds = (size_t)token_up_lds(a.lay.steps);
+  if (!a.x_type)
+    hipLaunchKernelGGL((expert_token_up_kernel<FMA, BF16, ROW_Q8>), grid, wg, lds, s, a);
+  else
+    hipLaunchKernelGGL((expert_token_up_kernel<FMA, BF16, BF16 ? ROW_BF16 : ROW_F32>), grid, wg, lds, s, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_expert_token_up(const ExpertLaunch &l, hipStream_t s) {
+  const ExpertArgs a = expert_args(l);
+  if (l.fma) return l.bf16 ? launch_token_up<true, true>(a, s) : launch_token_up<true, false>(a, s);
+  return l.bf16 ? launch_token_up<false, true>(a, s) : launch_token_up<false, false>(a, s);
 }
 
 hipError_t launch_expert_token(const ExpertLaunch &l, const float *weights, int32_t top_k, int64_t m,

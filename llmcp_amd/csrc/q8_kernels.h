@@ -281,9 +281,12 @@ struct ExpertLaunch {
 };
 hipError_t launch_experts(const ExpertLaunch &l, hipStream_t s);
 
-// Down products (l: qa / sa the hidden rows, one per slot) and the weighted
-// sum below in one launch, for few tokens.
-bool expert_token_takes(int64_t m, int32_t top_k, int64_t experts, int64_t cols);
+// The MLPs of few tokens, of [width, cols] experts, in two launches: the
+// SwiGLU products (l.up set, rows 16 B (bf16: 8 B) aligned or quantized, no
+// plan; h into y in the output's type, [slots, ldy]), and the down products
+// (l.x those rows) with the weighted sum below.
+bool expert_token_takes(int64_t m, int32_t top_k, int64_t experts, int64_t cols, int64_t width);
+hipError_t launch_expert_token_up(const ExpertLaunch &l, hipStream_t s);
 hipError_t launch_expert_token(const ExpertLaunch &l, const float *weights, int32_t top_k, int64_t m,
                                const void *residual, int64_t ldr, void *y, int64_t ldy, hipStream_t s);
 

@@ -1724,22 +1724,25 @@ static int check_slots(const ExpertRows &in, const int32_t *experts, int32_t top
 }
 
 // What the products need first: the rows' Q8_1 (as given, quantized here, or
-// left to the workgroups) and the plan of many slots.
+// left to the workgroups) and the plan of many slots (token: for the kernels
+// of few tokens, which need none).
 static int expert_prepare(llmcp_q8_ctx *ctx, const ExpertRows &in, const int32_t *experts,
-                          int64_t slots, int64_t count, int64_t widest, ExpertLaunch &l) {
+                          int64_t slots, int64_t count, int64_t widest, bool token,
+                          ExpertLaunch &l) {
   l.ids = experts;
   l.tile_rows = expert_tile_rows(slots, count, widest);
   l.slots = slots;
   l.experts = (int32_t)count;
   l.err_flag = ctx->err_flag;
   l.fma = ctx->fma();
-  const bool planned = expert_planned(slots, count, l.tile_rows);
+  const bool planned = !token && expert_planned(slots, count, l.tile_rows);
+  const bool aligned = in.x && (uintptr_t)in.x->data % (in.x->bf16 ? 8 : 16) == 0 && in.x->ld % 4 == 0;
   const int64_t blocks = in.cols / kBlock;
   int rc;
   if (in.q) {
     l.qa = in.q->values;
     l.sa = in.q->scales;
-  } else if (!planned && l.tile_rows == 4) {
+  } else if (token ? aligned : !planned && l.tile_rows == 4) {
     // the workgroups that read the rows quantize them, up to four each: a
     // launch less (M = 16 over 128 experts 2.5 .. 4.7 us of it against 2 in the
     // product; tiles of more slots would wait for their rows)
@@ -1795,7 +1798,7 @@ static int expert_linear_impl(llmcp_q8_ctx *ctx, const Rows &x, const int32_t *e
     return fail(LLMCP_Q8_EINVAL, "an expert linear's output must not take its input's memory");
   if ((rc = set_device(ctx))) return rc;
   ExpertLaunch l;
-  if ((rc = expert_prepare(ctx, in, experts, slots, w->experts, w->cols, l))) return rc;
+  if ((rc = expert_prepare(ctx, in, experts, slots, w->experts, w->cols, false, l))) return rc;
   l.per_row = x.rows == slots ? 1 : top_k;
   l.in_rows = x.rows;
   l.w = w->dev;
@@ -1833,14 +1836,16 @@ static int expert_mlp_impl(llmcp_q8_ctx *ctx, const ExpertRows &in, const int32_
   if ((rc = check_slots(in, experts, top_k, slots, std::max(f, h)))) return rc;
   if (m == 0) return LLMCP_Q8_OK;
   if ((rc = set_device(ctx))) return rc;
-  if ((rc = grow(ctx, ctx->expert_hq, ctx->expert_hq_bytes, (uint64_t)(slots * f), "expert hidden")) ||
-      (rc = grow(ctx, ctx->expert_hs, ctx->expert_hs_bytes, (uint64_t)(slots * (f / kBlock) * 4),
-                 "expert hidden scales")) ||
-      (rc = grow(ctx, ctx->expert_out, ctx->expert_out_bytes,
-                 (uint64_t)(slots * h) * (out.bf16 ? 2 : 4), "expert outputs")))
+  const bool token = expert_token_takes(m, top_k, wg->experts, h, f);
+  const uint64_t out_bytes = (uint64_t)(slots * (token ? f : h)) * (out.bf16 ? 2 : 4);
+  if (!token &&
+      ((rc = grow(ctx, ctx->expert_hq, ctx->expert_hq_bytes, (uint64_t)(slots * f), "expert hidden")) ||
+       (rc = grow(ctx, ctx->expert_hs, ctx->expert_hs_bytes, (uint64_t)(slots * (f / kBlock) * 4),
+                  "expert hidden scales"))))
     return rc;
+  if ((rc = grow(ctx, ctx->expert_out, ctx->expert_out_bytes, out_bytes, "expert outputs"))) return rc;
   ExpertLaunch l;
-  if ((rc = expert_prepare(ctx, in, experts, slots, wg->experts, std::max(f, h), l))) return rc;
+  if ((rc = expert_prepare(ctx, in, experts, slots, wg->experts, std::max(f, h), token, l))) return rc;
   l.per_row = top_k;
   l.in_rows = m;
   l.w = wg->dev;
@@ -1850,18 +1855,23 @@ static int expert_mlp_impl(llmcp_q8_ctx *ctx, const ExpertRows &in, const int32_
   l.bf16 = out.bf16;
   l.hq = ctx->expert_hq;
   l.hs = ctx->expert_hs;
-  hipError_t e = launch_experts(l, ctx->stream);
+  if (token) {
+    l.y = ctx->expert_out;
+    l.ldy = f;
+  }
+  hipError_t e = token ? launch_expert_token_up(l, ctx->stream) : launch_experts(l, ctx->stream);
   if (e != hipSuccess) return hip_fail(e, "expert SwiGLU launch");
   l.qa = ctx->expert_hq;
   l.sa = ctx->expert_hs;
-  l.x = nullptr;
+  l.x = token ? ctx->expert_out : nullptr;
+  l.ldx = token ? f : 0;
   l.per_row = 1;
   l.in_rows = slots;
   l.w = wd->dev;
   l.up = nullptr;
   l.rows = h;
   l.cols = f;
-  if (expert_token_takes(m, top_k, wd->experts, f)) {
+  if (token) {
     e = launch_expert_token(l, weights, top_k, m, residual ? residual->data : nullptr,
                             residual ? residual->ld : 0, out.data, out.ld, ctx->stream);
     if (e != hipSuccess) return hip_fail(e, "expert down launch");
