@@ -768,8 +768,8 @@ struct UpRing {
   uint32_t d[kUpPairs];
 };
 
-// Steps of a wave (an even number) and the LDS: the row, then [gate,
-// up][block][column] {dot, factor} of whole batches of the chain.
+// Steps of a wave (an even number) and the LDS: the row, then [gate, up][pair of
+// blocks][column][block] {dot, factor} of whole batches of the chain.
 constexpr int kUpBatch = 16;  // blocks read while as many before are added
 __host__ __device__ inline int token_up_steps(int steps) { return ((steps + 1) / 2 + 1) & ~1; }
 __host__ __device__ inline int token_up_blocks(int steps) { return (4 * steps + kUpBatch - 1) & -kUpBatch; }
@@ -824,13 +824,17 @@ __global__ __launch_bounds__(256) void expert_token_up_kernel(const ExpertArgs p
   const uint32_t tile = (blockIdx.x >> 1) * (uint32_t)p.lay.tile_bytes();
   const uint32_t wat = tile + (blockIdx.x & 1) * 128u, dat = tile + (uint32_t)steps * 2048u + (blockIdx.x & 1) * 64u;
   UpRing ring;
-#pragma unroll
-  for (int q = 0; q < kUpPairs; ++q) up_load(ring, q, wexp, wat, dat, first + 2 * q, end, lane);
-  x.store(p, row, wave * quarter, quarter, smem + wave * quarter * kBlock, scales + wave * quarter);
+  static_for<kUpPairs>([&](auto Q) __attribute__((always_inline)) {
+    constexpr int q = decltype(Q)::value;
+    up_load(ring, q, wexp, wat, dat, first + 2 * q, end, lane);
+    // (the later loads wait for room in the CU's queue as it is)
+    if constexpr (q == 1)
+      x.store(p, row, wave * quarter, quarter, smem + wave * quarter * kBlock, scales + wave * quarter);
+  });
   // blocks of the last batch that no step writes
   const int blocks = token_up_blocks(steps), written = 4 * ((steps + 1) & ~1);
   for (int i = threadIdx.x; i < (blocks - written) * 16; i += 256)
-    box[(i & 8 ? blocks * 8 : 0) + (written + (i >> 4)) * 8 + (i & 7)] = make_float2(0.0f, 0.0f);
+    box[(i & 8 ? blocks * 8 : 0) + written * 8 + (i >> 4) * 8 + (i & 7)] = make_float2(0.0f, 0.0f);
   lds_barrier();
   // lane: column lane % 8, half (lane / 8) % 2 of block lane / 16, of whose two
   // steps it keeps that of its half
@@ -838,7 +842,8 @@ __global__ __launch_bounds__(256) void expert_token_up_kernel(const ExpertArgs p
   auto pass = [&](int s, auto LOADS, auto FULL) __attribute__((always_inline)) {
     const uint8_t *const xv = smem + s * 128 + (lane >> 3) * 16;
     const float *const xs = scales + 4 * s + (upper ? 4 : 0) + (lane >> 4);
-    float2 *const to = box + (wave & 1) * blocks * 8 + ((s + (upper ? 1 : 0)) * 4 + (lane >> 4)) * 8 + (lane & 7);
+    float2 *const to = box + (wave & 1) * blocks * 8 + (s + (upper ? 1 : 0)) * 32 + (lane >> 5) * 16 +
+                       (lane & 7) * 2 + (lane >> 4 & 1);
     static_for<kUpPairs>([&](auto Q) __attribute__((always_inline)) {
       constexpr int q = decltype(Q)::value;
       if (FULL || s + 2 * q < end) {
@@ -865,26 +870,34 @@ __global__ __launch_bounds__(256) void expert_token_up_kernel(const ExpertArgs p
   lds_barrier();
   if (wave != 0) return;
   // lanes 0-7: the gate's columns, 8-15: the up's (the others repeat)
-  const float2 *t = box + (upper ? blocks * 8 : 0) + (lane & 7);
+  const float4 *t = (const float4 *)box + (upper ? blocks * 4 : 0) + (lane & 7);
   float acc[1] = {0.0f};
-  float2 v[kUpBatch];
+  constexpr int B = kUpBatch / 2;
+  auto read = [&](float4 (&v)[B], int b) __attribute__((always_inline)) {
 #pragma unroll
-  for (int k = 0; k < kUpBatch; ++k) v[k] = t[k * 8];
-  for (int b = 0; b < blocks; b += kUpBatch) {
-    float2 n[kUpBatch];  // (behind the last batch: memory that is not used)
-    t += kUpBatch * 8;
+    for (int k = 0; k < B; ++k) v[k] = t[(b / 2 + k) * 8];
+  };
+  auto add = [&](const float4 (&v)[B]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int k = 0; k < kUpBatch; ++k) n[k] = t[k * 8];
-#pragma unroll
-    for (int k = 0; k < kUpBatch; ++k) {
+    for (int k = 0; k < B; ++k) {
       if (FMA) {
         acc[0] = __builtin_fmaf(v[k].x, v[k].y, acc[0]);
+        acc[0] = __builtin_fmaf(v[k].z, v[k].w, acc[0]);
       } else {
-        const float contrib = v[k].x * v[k].y;
-        acc[0] = acc[0] + contrib;
+        const float c0 = v[k].x * v[k].y, c1 = v[k].z * v[k].w;
+        acc[0] = acc[0] + c0;
+        acc[0] = acc[0] + c1;
       }
-      v[k] = n[k];
     }
+  };
+  float4 even[B], odd[B];  // (behind the last batch: memory that is not used)
+  read(even, 0);
+  for (int b = 0; b < blocks; b += 2 * kUpBatch) {
+    read(odd, b + kUpBatch);
+    add(even);
+    if (b + kUpBatch >= blocks) break;
+    read(even, b + 2 * kUpBatch);
+    add(odd);
   }
   const float u = dpp_f32<0x128>(acc[0]);
   activate_out(acc, ACT_SILU, BF16);
