@@ -940,23 +940,24 @@ __global__ __launch_bounds__(64 * kTokenWaves) void expert_token_kernel(
   const int ids = p.ids[choice];
   const float factors = weights ? weights[choice] : 1.0f;
   const int n = tile * 16 + li;
-  float v = 0.0f;
+  uint32_t raw = 0;  // widened at the end: nothing waits for it here
   if (residual && wave == 0 && n < p.rows)
-    v = BF16 ? bf16_to_float(((const uint16_t *)residual)[token * ldr + n])
-             : ((const float *)residual)[token * ldr + n];
+    raw = BF16 ? ((const uint16_t *)residual)[token * ldr + n] : ((const uint32_t *)residual)[token * ldr + n];
   for (int j = wave; j < top_k; j += waves) {
     const int64_t slot = token * top_k + j;
     TokenRow<BF16 ? ROW_BF16 : ROW_F32, 3> x;  // on its way before the weights
     x.start(p, slot, 0);
-    const int id = __builtin_amdgcn_readlane(ids, j);
+    const int id = __builtin_amdgcn_readfirstlane(p.ids[slot]);
     if ((unsigned)id >= (unsigned)p.experts) continue;  // uniform per wave
     const uint8_t *const wexp = p.w0 + (int64_t)id * p.lay.expert_bytes();
     const uint32_t at = (uint32_t)tile * (uint32_t)p.lay.tile_bytes();
     FewRing ring;
-#pragma unroll
-    for (int q = 0; q < kFewRing; ++q)
+    static_for<kFewRing>([&](auto Q) __attribute__((always_inline)) {
+      constexpr int q = decltype(Q)::value;
       few_load(ring, q, wexp, at, q, steps, steps, lane, li * 8 + lq * 2);
-    x.store(p, slot, 0, 4 * ((steps + 1) & ~1), mine, ls);
+      // (the later loads wait for room in the CU's queue as it is)
+      if constexpr (q == 2) x.store(p, slot, 0, 4 * ((steps + 1) & ~1), mine, ls);
+    });
     // every MFMA row reads the one row: eights 0, 2, 1, 3 of a block
     const uint8_t *const a = mine + ((lq & 1) * 2 + (lq >> 1)) * 8;
     auto read_rows = [&](FewRows &x, int st) __attribute__((always_inline)) {
@@ -975,10 +976,18 @@ __global__ __launch_bounds__(64 * kTokenWaves) void expert_token_kernel(
   }
   __syncthreads();
   if (wave != 0) return;
-  for (int j = 0; j < top_k; ++j) {
-    if ((unsigned)__builtin_amdgcn_readlane(ids, j) >= (unsigned)p.experts) continue;
-    const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, factors), j));
-    v = __builtin_fmaf(w, sums[j][li], v);
+  float v = BF16 ? bf16_to_float(raw) : __uint_as_float(raw);
+  constexpr int K = 8;  // read together
+  for (int j0 = 0; j0 < top_k; j0 += K) {
+    float o[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) o[k] = sums[(j0 + k) & (kMaxTopK - 1)][li];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if (j0 + k >= top_k || (unsigned)__builtin_amdgcn_readlane(ids, j0 + k) >= (unsigned)p.experts) continue;
+      const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, factors), j0 + k));
+      v = __builtin_fmaf(w, o[k], v);
+    }
   }
   if (lane >= 16 || n >= p.rows) return;
   if (BF16) ((uint16_t *)y)[token * ldy + n] = float_to_bf16(v);
