@@ -91,11 +91,15 @@ __device__ void expert_plan(const int32_t *__restrict__ ids, int32_t slots, int3
   const __amdgpu_buffer_rsrc_t ri =
       __builtin_amdgcn_make_buffer_rsrc(const_cast<int32_t *>(ids), 0, slots * 4, 0x00020000);
   auto count_in = [&](int s0) __attribute__((always_inline)) {
-#pragma unroll
-    for (int k = 0; k < kKeep; ++k)
-      held[k] = __builtin_amdgcn_raw_buffer_load_b32(ri, (s0 + 1024 * k + t) * 4, 0, 0);
+    // (few slots: the rounds without one are not gone through)
 #pragma unroll
     for (int k = 0; k < kKeep; ++k) {
+      if (s0 + 1024 * k >= slots) break;
+      held[k] = __builtin_amdgcn_raw_buffer_load_b32(ri, (s0 + 1024 * k + t) * 4, 0, 0);
+    }
+#pragma unroll
+    for (int k = 0; k < kKeep; ++k) {
+      if (s0 + 1024 * k >= slots) break;
       if (s0 + 1024 * k + t >= slots) continue;
       const int id = (int)held[k], g = group_of(id, experts);
       bad |= id < -1 || id >= experts;
@@ -144,7 +148,7 @@ __device__ void expert_plan(const int32_t *__restrict__ ids, int32_t slots, int3
     // through LDS, to be written side by side (scattered from this one
     // workgroup, a line per slot, 32768 of them took 15 us)
 #pragma unroll
-    for (int k = 0; k < kKeep; ++k)
+    for (int k = 0; k < kKeep && 1024 * k < slots; ++k)
       if (1024 * k + t < slots) order[before[held[k] >> 20] + (held[k] & 0xFFFFFu)] = (uint16_t)(1024 * k + t);
     __syncthreads();
     for (int i = 2 * t; i < slots; i += 2048) {
@@ -204,7 +208,7 @@ __global__ __launch_bounds__(1024) void expert_prepare_kernel(
 struct ExpertArgs {
   const int8_t *qa;    // Q8_1 rows [.., 32 blocks], dense
   const float *sa;     // their scales [.., blocks]
-  const void *x;       // few slots: the rows themselves, quantized by each
+  const void *x;       // up to 4 slots: the rows themselves, quantized by each
   int64_t ldx;         //   workgroup (x_type 1: f32, 2: bf16)
   int32_t x_type;      // 0: qa / sa
   int32_t x_aligned;
@@ -629,32 +633,7 @@ __global__ __launch_bounds__(256, 3) void expert_few_kernel(const ExpertArgs p) 
   const FewLds lds = FewLds::of(steps);
   const int used = min(TILE, p.slots);  // rows that the LDS holds
   float *const ls = (float *)(smem + used * lds.a_ld);
-  if (p.x_type) {
-    // quantized here, eight lanes per block, four blocks of each in flight
-    const int l8 = tid & 7;
-    for (int u0 = 0; u0 < count * p.blocks; u0 += 128) {
-      float4 v[4];
-      int r[4], b[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int u = min(u0 + 32 * k + (tid >> 3), count * p.blocks - 1);
-        r[k] = u / p.blocks, b[k] = u - r[k] * p.blocks;
-        v[k] = load_act4(p.x, (int64_t)(rows[r[k]] / p.per_row) * p.ldx + b[k] * kBlock + 4 * l8,
-                         p.x_type == 2, p.x_aligned != 0);
-      }
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        int32_t q;
-        float sc;
-        quantize_block8(v[k], true, &q, &sc);
-        if (u0 + 32 * k + (tid >> 3) >= count * p.blocks) continue;
-        const int quarter = (l8 >> 1 & 1) * 2 + (l8 >> 2);  // eights 0, 2, 1, 3
-        *(int32_t *)(smem + r[k] * lds.a_ld + (b[k] >> 1) * 64 + quarter * 16 + (b[k] & 1) * 8 +
-                     (l8 & 1) * 4) = q;
-        if (l8 == 0) ls[r[k] * lds.s_ld + b[k]] = sc;
-      }
-    }
-  } else {
+  auto copy = [&]() __attribute__((always_inline)) {
     // a half block and a scale per thread, four of each in flight
     const int halves = 2 * p.blocks;
     for (int u0 = 0; u0 < count * halves; u0 += 1024) {
@@ -679,6 +658,40 @@ __global__ __launch_bounds__(256, 3) void expert_few_kernel(const ExpertArgs p) 
         if (!(h[k] & 1)) ls[r[k] * lds.s_ld + b] = sc[k];
       }
     }
+  };
+  // quantized here, eight lanes per block, four blocks of each in flight
+  auto quantize = [&](auto BF16, auto ALIGNED) __attribute__((always_inline)) {
+    const int l8 = tid & 7;
+    for (int u0 = 0; u0 < count * p.blocks; u0 += 128) {
+      uint4 v[4];
+      int r[4], b[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int u = min(u0 + 32 * k + (tid >> 3), count * p.blocks - 1);
+        r[k] = u / p.blocks, b[k] = u - r[k] * p.blocks;
+        v[k] = load_raw4<BF16(), ALIGNED()>(
+            p.x, (int64_t)(rows[r[k]] / p.per_row) * p.ldx + b[k] * kBlock + 4 * l8);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        int32_t q;
+        float sc;
+        quantize_block8(act4_of_raw<BF16()>(v[k]), true, &q, &sc);
+        if (u0 + 32 * k + (tid >> 3) >= count * p.blocks) continue;
+        const int quarter = (l8 >> 1 & 1) * 2 + (l8 >> 2);  // eights 0, 2, 1, 3
+        *(int32_t *)(smem + r[k] * lds.a_ld + (b[k] >> 1) * 64 + quarter * 16 + (b[k] & 1) * 8 +
+                     (l8 & 1) * 4) = q;
+        if (l8 == 0) ls[r[k] * lds.s_ld + b[k]] = sc;
+      }
+    }
+  };
+  if (NV > 1 || !p.x_type) {
+    copy();
+  } else if constexpr (NV == 1) {
+    const std::true_type yes;
+    const std::false_type no;
+    if (p.x_type == 2) p.x_aligned ? quantize(yes, yes) : quantize(yes, no);
+    else p.x_aligned ? quantize(no, yes) : quantize(no, no);
   }
   // blocks past the last: weights of zero against any values, scales of zero
   for (int u = tid; u < count * 8; u += 256) {
