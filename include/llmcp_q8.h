@@ -449,7 +449,11 @@ int llmcp_q8_mlp_bf16(llmcp_q8_ctx *ctx, const llmcp_memref_bf16_2d *input,
  * top_k]) names the expert of each, -1 for none.  An id that is neither an
  * expert nor -1 counts as none and sets the context's error flag
  * (llmcp_q8_ctx_check).  Workspaces grow on the first call of a size: make
- * it eagerly before capturing it into a graph. */
+ * it eagerly before capturing it into a graph.  A call takes up to 2^20 slots
+ * and rows (the input, and a row as wide as an expert's N or K per slot)
+ * whose Q8_1 values stay below 4 GiB; more is declined.  Which kernels run,
+ * and so the time, depends on the numbers of slots and experts, never on the
+ * ids: results are the same bits whichever run. */
 
 /* Most experts of a stack and most choices per token. */
 #define LLMCP_Q8_MAX_EXPERTS 1024
@@ -460,8 +464,9 @@ int llmcp_q8_mlp_bf16(llmcp_q8_ctx *ctx, const llmcp_memref_bf16_2d *input,
  * on the device for the expert entries, which alone take it: a weight
  * descriptor of the stack's p4 size, experts * rows * (cols + cols / 16), whose
  * data is host_p4.  rows % 8 == 0, cols % 32 == 0; an expert's device copy
- * must stay below 4 GiB (declined otherwise).  llmcp_q8_release and the
- * weight budget apply as to llmcp_q8_upload_p4. */
+ * must stay below 4 GiB (declined otherwise).  llmcp_q8_release, the weight
+ * budget and a second registration at one address apply as to
+ * llmcp_q8_upload_p4. */
 int llmcp_q8_upload_experts_p4(llmcp_q8_ctx *ctx, const void *host_p4, int64_t experts,
                                int64_t rows, int64_t cols, float *repack_ms);
 
@@ -490,7 +495,8 @@ int llmcp_q8_route_bf16(llmcp_q8_ctx *ctx, const llmcp_memref_bf16_2d *logits, i
  * with e = experts[s] and x the input's row s / top_k (input of M rows) or s
  * (input of M * top_k rows).  Each row is bit for bit what llmcp_q8_linear
  * gives with that expert's weight (the platform's epilogue in block order, in
- * either accumulation mode); rows of slots without an expert are zero. */
+ * either accumulation mode); rows of slots without an expert are zero.  The
+ * output must not take the input's memory. */
 int llmcp_q8_expert_linear(llmcp_q8_ctx *ctx, const llmcp_memref_f32_2d *input,
                            const int32_t *experts, int32_t top_k,
                            const llmcp_memref_i8_1d *weight, llmcp_memref_f32_2d *output,
@@ -507,7 +513,8 @@ int llmcp_q8_expert_linear_bf16(llmcp_q8_ctx *ctx, const llmcp_memref_bf16_2d *i
  * weights, then output[t] = residual[t] + sum over the token's slots, in
  * order, of weights[slot] * o[slot], an f32 FMA chain from the residual
  * rounded once.  weights (f32 [M, top_k], nullable: all 1), residual
- * (nullable: zero; it may be the output's memory).  Slots without an expert
+ * (nullable: zero; it may be the output's memory, as may the input, with the
+ * same strides).  Slots without an expert
  * add nothing; a token with none gives its residual.  w_gate and w_up are
  * stacks of [F, H] (F % 32 == 0), w_down of [H, F]. */
 int llmcp_q8_expert_mlp(llmcp_q8_ctx *ctx, const llmcp_memref_f32_2d *input,

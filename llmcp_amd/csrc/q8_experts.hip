@@ -71,6 +71,9 @@ __device__ __forceinline__ int group_of(int id, int experts) {
 // turn each XCD gets whole runs of them, an expert's on one or two.  An id
 // that is neither an expert nor -1 sets the error flag.  The order of a
 // group's slots is that of the atomics; no result depends on it.
+// Bound by latency, one workgroup's passes over the ids: with the rows' Q8_1
+// beside it 5.6 us for 640 or 2664 slots, 15.5 us for 32768 (and 4096 rows
+// of 2560).
 __device__ void expert_plan(const int32_t *__restrict__ ids, int32_t slots, int32_t experts,
                             int32_t tile_rows, int32_t max_tiles, int32_t *__restrict__ plan,
                             int32_t *__restrict__ err) {
@@ -350,7 +353,10 @@ __device__ __forceinline__ void store_h(const ExpertArgs &p, const float *hb, in
 // registers that the MFMAs read, a ring of kFewRing steps, without a pause
 // from tile to tile; the rows stay in LDS for all of them.  A step issues its
 // MFMAs, reads the next step's rows and then runs the epilogue of the step
-// before, so that a lone wave waits for none of them.
+// before, so that a lone wave waits for none of them.  Measured: 16 tokens
+// through 8 of 128 experts of [768, 2560], gate and up 62 us (344 MB, 5.5
+// TB/s), down 37 us (172 MB, 4.7 TB/s); what is missing to the 6.4 TB/s of a
+// plain read is the launch and the last workgroups.
 //
 // LDS: [slots][a_ld] values (a block pair's 64 B: quarter, block parity,
 // eight values), [slots][s_ld] scales.
@@ -773,7 +779,9 @@ struct TokenRow {
 // steps per wave.  A lane takes half a block of a row, four v_dot4; two steps
 // together give every lane a block's dot, which goes to LDS with the scale
 // product, and sixteen lanes run the chains over them in block order.  h is
-// left in the output's type; the down products quantize it.
+// left in the output's type; the down products quantize it.  Measured: 8
+// experts of [768, 2560], 33 MB, 8.2 us (11 to 12 on tiles of 16 columns, 32
+// per workgroup and 192 workgroups; a plain read of as much 7.1).
 
 constexpr int kUpPairs = 5;  // pairs of steps of a wave in flight
 struct UpRing {
@@ -927,7 +935,8 @@ __global__ __launch_bounds__(256) void expert_token_up_kernel(const ExpertArgs p
 // beyond eight): each streams its expert's tile with its one row of h,
 // quantized to LDS, and the results, rounded to the output's type, are added in slot
 // order by sixteen lanes (expert_combine_kernel's sum).  An expert that two
-// tokens share is read twice.
+// tokens share is read twice.  Measured: 8 experts of [2560, 768], 17 MB, 6.4
+// us: 160 workgroups that each read 104 KB at what a CU takes.
 
 constexpr int kTokenWaves = 8;
 
@@ -1020,6 +1029,10 @@ __global__ __launch_bounds__(64 * kTokenWaves) void expert_token_kernel(
 // other's latencies.  The rows pass through an LDS ring of three steps of four
 // blocks, loaded a step before they are stored there, one barrier a step; a
 // workgroup takes `repeat` column ranges without a pause in either stream.
+// Measured with 128 experts of [768, 2560], 8 per token: 4096 tokens, gate and
+// up 440 .. 460 us and down 265 us (258 + 129 GFLOP, 570 and 490 TOPS, where
+// convert, FMA and MFMAs alone reach 880); 333 tokens, TT = 1, 101 and 58 us
+// (538 and 269 MB of weights, 5.3 and 4.6 TB/s).
 
 template <int TT>
 struct ManyLds {
@@ -1382,6 +1395,7 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
 // rounds, each the wave's largest key and the lowest index that has it; then
 // the chosen ones' exponentials side by side, one per lane.  Latency bound
 // for few rows: a round is six lane moves and a ballot per 64 logits.
+// Measured: the 8 largest of 128, one row 3.4 us, 4096 rows 5.0.
 template <bool BF16, int PER>
 __global__ __launch_bounds__(256) void route_kernel(const void *__restrict__ logits, int64_t ld,
                                                     int64_t m, int32_t experts, int32_t top_k,

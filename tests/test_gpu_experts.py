@@ -320,6 +320,43 @@ def test_expert_mlp_many_rows(ctx, q8, oracle, pad, dtype):
             s.release()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("e,top_k,h,f", [(40, 4, 160, 96), (3, 5, 96, 64), (12, 9, 2560, 192)])
+def test_expert_mlp_alone_and_in_batches(ctx, q8, oracle, e, top_k, h, f, dtype):
+    """A token's bits do not depend on the tokens beside it: one at a time, a
+    few, many (each size has kernels of its own), rows as they are, at odd
+    addresses or as Q8_1, and the output over the input."""
+    rng = np.random.default_rng(e)
+    m = 90
+    gate, up, down, ids, p, x, _ = expert_mlp_case(ctx, oracle, rng, m, top_k, e, h, f, dtype, 0.1)
+    size, et = (2, np.uint16) if dtype == "bf16" else (4, np.float32)
+    try:
+        bits = oracle.f32_to_bf16_bits(x) if dtype == "bf16" else np.ascontiguousarray(x, np.float32)
+        xd, idd, pd, yd = ctx.to_device(bits), ctx.to_device(ids), ctx.to_device(p), ctx.alloc(m * h * size)
+        stacks = (gate.t, up.t, down.t)
+        ctx.expert_mlp(xd, idd, pd, m, top_k, *stacks, yd, dtype=dtype)
+        want = ctx.to_host(yd, (m, h), et).view(np.uint8)
+        for n in (1, 3, 17):
+            for first in range(0, m - n + 1, 6 if n == 1 else n):
+                ctx.expert_mlp(xd.ptr + first * h * size, idd.ptr + first * top_k * 4,
+                               pd.ptr + first * top_k * 4, n, top_k, *stacks, yd, dtype=dtype)
+                got = ctx.to_host(yd, (n, h), et).view(np.uint8)
+                assert np.array_equal(got, want[first:first + n]), (n, first)
+        odd = ctx.to_device(np.concatenate([bits.ravel()[:1], bits.ravel()]))
+        q, s = ctx.alloc(m * h), ctx.alloc(m * h // 8)
+        ctx.quantize(ctx.to_device(np.ascontiguousarray(x, np.float32)), m, h, q, s)
+        for n in (1, 17, m):
+            for rows in (odd.ptr + size, q8.Q8Rows(q, s, n, h)):
+                ctx.expert_mlp(rows, idd, pd, n, top_k, *stacks, yd, dtype=dtype)
+                assert np.array_equal(ctx.to_host(yd, (n, h), et).view(np.uint8), want[:n]), n
+            over = ctx.to_device(bits)
+            ctx.expert_mlp(over, idd, pd, n, top_k, *stacks, over, dtype=dtype)
+            assert np.array_equal(ctx.to_host(over, (n, h), et).view(np.uint8), want[:n]), n
+    finally:
+        for st in (gate, up, down):
+            st.release()
+
+
 def test_swiglu_rounds_as_the_oracle_over_the_gate_s_range(ctx, oracle):
     """bf16: silu of gate sums of every size and of both signs, those next to
     a rounding of bf16 among them, through one expert whose down weights
