@@ -66,10 +66,10 @@ __device__ __forceinline__ int group_of(int id, int experts) {
 
 // The tiles to compute, by one workgroup: {group, first, slots} of max_tiles
 // tiles (0 slots: none), then the slots sorted by group, a tile's from `first`
-// on.  A group's tiles are consecutive and alike; tile i of T takes place (i %
-// C) * 8 + i / C with C = ceil(T / 8), so that with places dealt to the XCDs in
-// turn each XCD gets whole runs of them, an expert's on one or two.  An id
-// that is neither an expert nor -1 sets the error flag.  The order of a
+// on.  A group's tiles are consecutive, full but the last; tile i of T takes
+// place (i % C) * 8 + i / C with C = ceil(T / 8), so that with places dealt to
+// the XCDs in turn each XCD gets whole runs of them, an expert's on one or two.
+// An id that is neither an expert nor -1 sets the error flag.  The order of a
 // group's slots is that of the atomics; no result depends on it.
 // Bound by latency, one workgroup's passes over the ids: with the rows' Q8_1
 // beside it 5.6 us for 640 or 2664 slots, 15.5 us for 32768 (and 4096 rows
@@ -114,7 +114,6 @@ __device__ void expert_plan(const int32_t *__restrict__ ids, int32_t slots, int3
   __syncthreads();
   // the groups' first slots and tiles (exclusive prefix sums); then a tile's
   // header by the thread of its group
-  const int step = min(tile_rows, 16);  // a tile holds whole MFMA tiles
   int total = 0, sorted = 0;
   for (int g0 = 0; g0 <= experts; g0 += 1024) {
     const int g = g0 + t;
@@ -138,11 +137,10 @@ __device__ void expert_plan(const int32_t *__restrict__ ids, int32_t slots, int3
   }
   const int run = max((total + 7) / 8, 1);
   for (int g = t; g <= experts; g += 1024) {
-    const int c = count[g], n = (c + tile_rows - 1) / tile_rows;
-    const int per = n ? ((c + step - 1) / step + n - 1) / n * step : step;
+    const int c = count[g];
     int r = tile0[g] % run, x = tile0[g] / run;
-    for (int f = 0; f < c; f += per) {
-      *(v4i *)(plan + 4 * (8 * r + x)) = v4i{g, before[g] + f, min(per, c - f), 0};
+    for (int f = 0; f < c; f += tile_rows) {
+      *(v4i *)(plan + 4 * (8 * r + x)) = v4i{g, before[g] + f, min(tile_rows, c - f), 0};
       if (++r == run) r = 0, ++x;
     }
   }
