@@ -357,6 +357,29 @@ def test_expert_mlp_alone_and_in_batches(ctx, q8, oracle, e, top_k, h, f, dtype)
             st.release()
 
 
+# H of several passes of a wave's ring (an odd number of steps, whole passes),
+# rows of more pieces than are asked for at once, F of several rings; H past
+# what the LDS of one token's kernels holds
+@pytest.mark.parametrize("e,top_k,h,f", [(2, 3, 4480, 1056), (2, 2, 5120, 64), (3, 9, 160, 2208),
+                                         (1, 2, 2592, 800), (2, 1, 23040, 32), (1, 1, 32768, 32)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_expert_mlp_one_wide_token(ctx, q8, oracle, e, top_k, h, f, dtype):
+    rng = np.random.default_rng(h + f)
+    gate, up, down, ids, p, x, r = expert_mlp_case(ctx, oracle, rng, 1, top_k, e, h, f, dtype)
+    try:
+        _, ref, bound = mlp_reference(oracle, ctx.epilogue, x, ids, p, gate, up, down, r, dtype)
+        q, s, yd = ctx.alloc(h), ctx.alloc(h // 8), ctx.alloc(h * 4)
+        ctx.quantize(ctx.to_device(np.ascontiguousarray(x, np.float32)), 1, h, q, s)
+        for rows in (to_type(ctx, oracle, x, dtype), q8.Q8Rows(q, s, 1, h)):
+            ctx.expert_mlp(rows, ctx.to_device(ids), ctx.to_device(p), 1, top_k, gate.t, up.t, down.t, yd,
+                           residual=to_type(ctx, oracle, r, dtype), dtype=dtype)
+            y = from_type(ctx, oracle, yd, (1, h), dtype).astype(np.float64)
+            assert (np.abs(y - ref) <= bound).all()
+    finally:
+        for st in (gate, up, down):
+            st.release()
+
+
 def test_swiglu_rounds_as_the_oracle_over_the_gate_s_range(ctx, oracle):
     """bf16: silu of gate sums of every size and of both signs, those next to
     a rounding of bf16 among them, through one expert whose down weights
