@@ -10,7 +10,8 @@
 // the row is split over lanes.  (The f64 work is a multiply and an add per
 // value of a row that is bound by memory.)  Measured in bf16, H = 2560, sum and
 // Q8_1 out: one row 3.9 us (the latency of two passes over the workgroup),
-// 4096 rows 20.5 us for 96 MB (4.7 TB/s; a copy reaches 5.3).
+// 4096 rows 19.4 us for 96 MB (4.9 TB/s; a copy reaches 5.3; 20.7 with the
+// loads one by one and the sum by LDS permutes).
 #include "q8_kernels.h"
 
 #include <algorithm>
@@ -51,6 +52,25 @@ __device__ __forceinline__ void load8(float (&v)[8], const void *p, int64_t i, i
   }
 }
 
+// Eight values as they are in memory, 16 B aligned: no conversion, so that the
+// loads behind one go out before it has come.
+template <bool BF16>
+struct Raw8 {
+  uint4 b[BF16 ? 1 : 2];
+  __device__ __forceinline__ void load(const void *p, int64_t i) {
+    const uint4 *const at = (const uint4 *)((const uint8_t *)p + i * (BF16 ? 2 : 4));
+#pragma unroll
+    for (int k = 0; k < (BF16 ? 1 : 2); ++k) b[k] = at[k];
+  }
+  __device__ __forceinline__ void widen(float (&v)[8]) const {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (BF16) v[k] = bf16_to_float(k & 1 ? word(b[0], k / 2) >> 16 : word(b[0], k / 2) & 0xffffu);
+      else v[k] = __uint_as_float(word(b[k / 4], k % 4));
+    }
+  }
+};
+
 // Stores eight values, rounding v to what is stored.
 template <bool BF16>
 __device__ __forceinline__ void store8(float (&v)[8], void *p, int64_t i, int aligned) {
@@ -83,43 +103,78 @@ __device__ __forceinline__ void store8(float (&v)[8], void *p, int64_t i, int al
   }
 }
 
+// v of the lane that CTRL names, 0 where there is none, added.
+template <int CTRL>
+__device__ __forceinline__ double dpp_add(double v) {
+  const int2 b = __builtin_bit_cast(int2, v);
+  const int2 o = make_int2(__builtin_amdgcn_update_dpp(0, b.x, CTRL, 0xf, 0xf, true),
+                           __builtin_amdgcn_update_dpp(0, b.y, CTRL, 0xf, 0xf, true));
+  return v + __builtin_bit_cast(double, o);
+}
+
 // A workgroup per row; thread t holds values 8 (t + i * threads) .. + 7 for
 // i < VPT in registers from the loads to the stores, so outputs may take the
-// inputs' memory.
-template <bool BF16, int VPT>
+// inputs' memory.  VEC: input rows and weight 16 B aligned, all their loads out
+// together.
+template <bool BF16, int VPT, bool VEC>
 __global__ __launch_bounds__(1024) void add_rmsnorm_kernel(const AddNormArgs p) {
   __shared__ double part[16];
   const int64_t row = blockIdx.x;
   const int t = threadIdx.x, threads = blockDim.x, vecs = p.h / 8;
   float v[VPT][8];
   double sum = 0.0;
+  float w[VPT][8];
+  if constexpr (VEC) {
+    Raw8<BF16> x[VPT], r[VPT], g[VPT];
 #pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    const int e = t + i * threads;
+    for (int i = 0; i < VPT; ++i) {
+      // (past the row: the last values again, taken out below)
+      const int e = min(t + i * threads, vecs - 1);
+      x[i].load(p.x, row * p.ldx + 8 * e);
+      r[i].load(p.r, row * p.ldr + 8 * e);
+    }
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[i][k] = 0.0f;
-    if (e < vecs) {
-      float r[8];
+    for (int i = 0; i < VPT; ++i) g[i].load(p.w, 8 * min(t + i * threads, vecs - 1));
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      float f[8];
+      x[i].widen(v[i]);
+      r[i].widen(f);
+      g[i].widen(w[i]);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[i][k] = v[i][k] + f[k];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int e = min(t + i * threads, vecs - 1);
+      float f[8];
       load8<BF16>(v[i], p.x, row * p.ldx + 8 * e, p.ax);
-      load8<BF16>(r, p.r, row * p.ldr + 8 * e, p.ar);
+      load8<BF16>(f, p.r, row * p.ldr + 8 * e, p.ar);
+      load8<BF16>(w[i], p.w, 8 * e, 1);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[i][k] = v[i][k] + r[k];
+      for (int k = 0; k < 8; ++k) v[i][k] = v[i][k] + f[k];
     }
   }
-  float w[VPT][8];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int e = t + i * threads;
     if (e < vecs) {
-      load8<BF16>(w[i], p.w, 8 * e, 1);
       store8<BF16>(v[i], p.s, row * p.lds + 8 * e, p.as);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[i][k] = 0.0f;
     }
 #pragma unroll
     for (int k = 0; k < 8; ++k) sum += (double)v[i][k] * (double)v[i][k];
   }
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) sum += __shfl_xor(sum, d);
-  if ((t & 63) == 0) part[t >> 6] = sum;
+  sum = dpp_add<0x111>(sum);  // row_shr:1, 2, 4, 8
+  sum = dpp_add<0x112>(sum);
+  sum = dpp_add<0x114>(sum);
+  sum = dpp_add<0x118>(sum);
+  sum = dpp_add<0x142>(sum);  // row_bcast:15, 31: the whole sum in lane 63
+  sum = dpp_add<0x143>(sum);
+  if ((t & 63) == 63) part[t >> 6] = sum;
   __syncthreads();
   sum = 0.0;
   for (int i = 0; i < threads / 64; ++i) sum += part[i];
@@ -171,12 +226,15 @@ hipError_t launch_add_rmsnorm_t(const AddNormArgs &a, int64_t m, hipStream_t s) 
   const int vecs = a.h / 8;
   const int threads = std::min(1024, (vecs + 63) / 64 * 64);
   const dim3 grid((unsigned)m), wg((unsigned)threads);
-  if (vecs <= 1024)
-    hipLaunchKernelGGL((add_rmsnorm_kernel<BF16, 1>), grid, wg, 0, s, a);
-  else if (vecs <= 2048)
-    hipLaunchKernelGGL((add_rmsnorm_kernel<BF16, 2>), grid, wg, 0, s, a);
-  else
-    hipLaunchKernelGGL((add_rmsnorm_kernel<BF16, 4>), grid, wg, 0, s, a);
+  const int most = BF16 ? 2 : 1;
+  const bool vec = a.ax == most && a.ar == most && (uintptr_t)a.w % 16 == 0;
+  const auto kernel = vec ? (vecs <= 1024   ? add_rmsnorm_kernel<BF16, 1, true>
+                             : vecs <= 2048 ? add_rmsnorm_kernel<BF16, 2, true>
+                                            : add_rmsnorm_kernel<BF16, 4, true>)
+                          : (vecs <= 1024   ? add_rmsnorm_kernel<BF16, 1, false>
+                             : vecs <= 2048 ? add_rmsnorm_kernel<BF16, 2, false>
+                                            : add_rmsnorm_kernel<BF16, 4, false>);
+  hipLaunchKernelGGL(kernel, grid, wg, 0, s, a);
   return hipGetLastError();
 }
 
