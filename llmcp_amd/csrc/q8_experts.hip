@@ -64,6 +64,21 @@ __device__ __forceinline__ int group_of(int id, int experts) {
   return (unsigned)id < (unsigned)experts ? id : experts;
 }
 
+// The sum of v over this lane and those before it (lane moves: a permute
+// through LDS takes over 100 clocks).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_plus(int v) {
+  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, true);
+}
+__device__ __forceinline__ int wave_scan(int v) {
+  v = dpp_plus<0x111, 0xf>(v);  // row_shr:1, 2, 4, 8
+  v = dpp_plus<0x112, 0xf>(v);
+  v = dpp_plus<0x114, 0xf>(v);
+  v = dpp_plus<0x118, 0xf>(v);
+  v = dpp_plus<0x142, 0xa>(v);  // row_bcast:15 into the odd rows, 31 into the upper half
+  return dpp_plus<0x143, 0xc>(v);
+}
+
 // The tiles to compute, by one workgroup: {group, first, slots} of max_tiles
 // tiles (0 slots: none), then the slots sorted by group, a tile's from `first`
 // on.  A group's tiles are consecutive, full but the last; tile i of T takes
@@ -119,12 +134,7 @@ __device__ void expert_plan(const int32_t *__restrict__ ids, int32_t slots, int3
     const int g = g0 + t;
     const int c = g <= experts ? count[g] : 0;
     const int n = (c + tile_rows - 1) / tile_rows;
-    int pt = n, ps = c;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int u = __shfl_up(pt, d), v = __shfl_up(ps, d);
-      if (lane >= d) pt += u, ps += v;
-    }
+    const int pt = wave_scan(n), ps = wave_scan(c);
     if (lane == 63) part[0][wave] = pt, part[1][wave] = ps;
     __syncthreads();
     int tiles = total, above = sorted;
@@ -560,13 +570,7 @@ __global__ __launch_bounds__(256, 3) void expert_few_kernel(const ExpertArgs p) 
       int n[4], sum = 0;
 #pragma unroll
       for (int k = 0; k < 4; ++k) sum += n[k] = (hist[4 * lane + k] + TILE - 1) / TILE;
-      int before = sum;
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const int u = __shfl_up(before, d);
-        if (lane >= d) before += u;
-      }
-      before -= sum;
+      int before = wave_scan(sum) - sum;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         if (tile >= before && tile < before + n[k]) found[0] = 4 * lane + k, found[1] = tile - before;
@@ -1389,6 +1393,21 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
   return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 
+// The wave's sum, in a scalar register.
+template <int CTRL>
+__device__ __forceinline__ float dpp_sum(float v) {
+  return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float wave_sum(float v) {
+  v = dpp_sum<0x111>(v);
+  v = dpp_sum<0x112>(v);
+  v = dpp_sum<0x114>(v);
+  v = dpp_sum<0x118>(v);
+  v = dpp_sum<0x142>(v);
+  v = dpp_sum<0x143>(v);
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
+
 // One wave per row, PER logits per lane (logit i in lane i % 64): top_k
 // rounds, each the wave's largest key and the lowest index that has it; then
 // the chosen ones' exponentials side by side, one per lane.  Latency bound
@@ -1444,8 +1463,7 @@ __global__ __launch_bounds__(256) void route_kernel(const void *__restrict__ log
     for (int i = 0; i < PER; ++i)
       if (l[i] > -__builtin_inff()) total += weight(l[i]);
   }
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) total += __shfl_xor(total, d);
+  total = wave_sum(total);
   if (lane < top_k) {
     ids[row * top_k + lane] = id;
     weights[row * top_k + lane] = id >= 0 ? p / total * scale : 0.0f;
