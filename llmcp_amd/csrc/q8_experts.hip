@@ -87,8 +87,8 @@ __device__ __forceinline__ int wave_scan(int v) {
 // An id that is neither an expert nor -1 sets the error flag.  The order of a
 // group's slots is that of the atomics; no result depends on it.
 // Bound by latency, one workgroup's passes over the ids: with the rows' Q8_1
-// beside it 5.6 us for 640 or 2664 slots, 15.5 us for 32768 (and 4096 rows
-// of 2560).
+// beside it 3.9 us for 640 slots (and as many rows of 768), 5.0 for 2664 (333
+// rows of 2560), 15 for 32768 (4096 rows).
 __device__ void expert_plan(const int32_t *__restrict__ ids, int32_t slots, int32_t experts,
                             int32_t tile_rows, int32_t max_tiles, int32_t *__restrict__ plan,
                             int32_t *__restrict__ err) {
@@ -97,7 +97,7 @@ __device__ void expert_plan(const int32_t *__restrict__ ids, int32_t slots, int3
   __shared__ int part[2][16];
   constexpr int kKeep = 32;
   __shared__ __align__(16) uint16_t order[1024 * kKeep];
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   for (int i = t; i <= experts; i += 1024) count[i] = 0;
   for (int i = t; i < max_tiles; i += 1024) plan[4 * i + 2] = 0;
   __syncthreads();
@@ -137,11 +137,11 @@ __device__ void expert_plan(const int32_t *__restrict__ ids, int32_t slots, int3
     const int pt = wave_scan(n), ps = wave_scan(c);
     if (lane == 63) part[0][wave] = pt, part[1][wave] = ps;
     __syncthreads();
-    int tiles = total, above = sorted;
-    for (int w = 0; w < 16; ++w) {
-      if (w < wave) tiles += part[0][w], above += part[1][w];
-      total += part[0][w], sorted += part[1][w];
-    }
+    // over the sixteen waves: each scans their sums itself
+    const int wt = wave_scan(part[0][lane & 15]), ws = wave_scan(part[1][lane & 15]);
+    const int tiles = total + (wave ? __builtin_amdgcn_readlane(wt, wave - 1) : 0);
+    const int above = sorted + (wave ? __builtin_amdgcn_readlane(ws, wave - 1) : 0);
+    total += __builtin_amdgcn_readlane(wt, 15), sorted += __builtin_amdgcn_readlane(ws, 15);
     if (g <= experts) before[g] = above + ps - c, tile0[g] = tiles + pt - n;
     __syncthreads();
   }
@@ -162,9 +162,11 @@ __device__ void expert_plan(const int32_t *__restrict__ ids, int32_t slots, int3
     for (int k = 0; k < kKeep && 1024 * k < slots; ++k)
       if (1024 * k + t < slots) order[before[held[k] >> 20] + (held[k] & 0xFFFFFu)] = (uint16_t)(1024 * k + t);
     __syncthreads();
-    for (int i = 2 * t; i < slots; i += 2048) {
-      const uint32_t two = *(const uint32_t *)(order + i);
-      *(v2i *)(sorted_slots + i) = v2i{(int)(two & 0xffffu), (int)(two >> 16)};  // (one past an odd end)
+#pragma unroll 8
+    for (int i = 4 * t; i < slots; i += 4096) {
+      const uint2 four = *(const uint2 *)(order + i);
+      *(v4i *)(sorted_slots + i) = v4i{(int)(four.x & 0xffffu), (int)(four.x >> 16),  // (up to
+                                       (int)(four.y & 0xffffu), (int)(four.y >> 16)};  // three past the end)
     }
     return;
   }
@@ -187,31 +189,38 @@ __global__ __launch_bounds__(1024) void expert_prepare_kernel(
     const int32_t *__restrict__ ids, int32_t slots, int32_t experts, int32_t tile_rows,
     int32_t max_tiles, int32_t *__restrict__ plan, int32_t *__restrict__ err,
     const void *__restrict__ x, int bf16, int aligned, int64_t ldx, int64_t m, int32_t blocks,
-    int8_t *__restrict__ qa, float *__restrict__ sa) {
+    int32_t per, int8_t *__restrict__ qa, float *__restrict__ sa) {
   if (blockIdx.x == 0) return expert_plan(ids, slots, experts, tile_rows, max_tiles, plan, err);
-  // (row, block) units, eight threads each, kQuantUnits in flight per thread
+  // (row, block) units, eight threads each, `per` of them in flight per thread
   // (the plan's registers leave room for one workgroup per CU)
   const int p = threadIdx.x & 7;
-  const int64_t u0 = ((int64_t)blockIdx.x - 1) * 128 * kQuantUnits + (threadIdx.x >> 3);
+  const int64_t u0 = ((int64_t)blockIdx.x - 1) * 128 * per + (threadIdx.x >> 3);
   const int64_t units = m * blocks;
-  float4 v[kQuantUnits];
+  auto quantize = [&](auto BF16, auto ALIGNED) __attribute__((always_inline)) {
+    uint4 v[kQuantUnits];
 #pragma unroll
-  for (int k = 0; k < kQuantUnits; ++k) {
-    const uint32_t u = (uint32_t)min(u0 + 128 * k, units - 1);
-    const uint32_t row = u / (uint32_t)blocks;
-    v[k] = load_act4(x, (int64_t)row * ldx + (int64_t)(u - row * (uint32_t)blocks) * kBlock + 4 * p,
-                     bf16 != 0, aligned != 0);
-  }
+    for (int k = 0; k < kQuantUnits; ++k) {
+      if (k >= per) break;
+      const uint32_t u = (uint32_t)min(u0 + 128 * k, units - 1);
+      const uint32_t row = u / (uint32_t)blocks;
+      v[k] = load_raw4<BF16(), ALIGNED()>(x, (int64_t)row * ldx + (int64_t)(u - row * (uint32_t)blocks) * kBlock + 4 * p);
+    }
 #pragma unroll
-  for (int k = 0; k < kQuantUnits; ++k) {
-    const int64_t u = u0 + 128 * k;
-    int32_t q;
-    float s;
-    quantize_block8(v[k], true, &q, &s);
-    if (u >= units) continue;
-    *(int32_t *)(qa + u * kBlock + 4 * p) = q;
-    if (p == 0) sa[u] = s;
-  }
+    for (int k = 0; k < kQuantUnits; ++k) {
+      if (k >= per) break;
+      const int64_t u = u0 + 128 * k;
+      int32_t q;
+      float s;
+      quantize_block8(act4_of_raw<BF16()>(v[k]), true, &q, &s);
+      if (u >= units) continue;
+      *(int32_t *)(qa + u * kBlock + 4 * p) = q;
+      if (p == 0) sa[u] = s;
+    }
+  };
+  const std::true_type yes;
+  const std::false_type no;
+  if (bf16) aligned ? quantize(yes, yes) : quantize(yes, no);
+  else aligned ? quantize(no, yes) : quantize(no, no);
 }
 
 // ---------------------------------------------------------- products ---- //
@@ -1508,19 +1517,21 @@ int64_t expert_max_tiles(int64_t slots, int64_t experts, int32_t tile_rows) {
 }
 
 int64_t expert_plan_ints(int64_t slots, int64_t experts, int32_t tile_rows) {
-  return 4 * expert_max_tiles(slots, experts, tile_rows) + slots + 1;
+  return 4 * expert_max_tiles(slots, experts, tile_rows) + (slots + 3) / 4 * 4;
 }
 
 hipError_t launch_expert_prepare(const int32_t *ids, int64_t slots, int32_t experts,
                                  int32_t tile_rows, int32_t *plan, int32_t *err_flag, const void *x, bool bf16, int64_t m, int64_t ldx,
                                  int64_t cols, int8_t *qa, float *sa, hipStream_t s) {
-  const int64_t per = 128 * kQuantUnits;
-  const int64_t wgs = 1 + (x ? (m * (cols / kBlock) + per - 1) / per : 0);
+  // one unit per thread as long as that leaves CUs without a workgroup
+  const int64_t units = x ? m * (cols / kBlock) : 0;
+  const int32_t per = units <= 128 * (int64_t)cu_count() ? 1 : kQuantUnits;
+  const int64_t wgs = 1 + (units + 128 * per - 1) / (128 * per);
   if (wgs * 1024 > 0xFFFFFFFFll) return hipErrorInvalidConfiguration;
   const int aligned = (uintptr_t)x % (bf16 ? 8 : 16) == 0 && ldx % 4 == 0;
   hipLaunchKernelGGL(expert_prepare_kernel, dim3((unsigned)wgs), dim3(1024), 0, s, ids, (int32_t)slots,
                      experts, tile_rows, (int32_t)expert_max_tiles(slots, experts, tile_rows), plan,
-                     err_flag, x, bf16 ? 1 : 0, aligned, ldx, m, (int32_t)(cols / kBlock), qa, sa);
+                     err_flag, x, bf16 ? 1 : 0, aligned, ldx, m, (int32_t)(cols / kBlock), per, qa, sa);
   return hipGetLastError();
 }
 
