@@ -451,7 +451,9 @@ int llmcp_q8_mlp_bf16(llmcp_q8_ctx *ctx, const llmcp_memref_bf16_2d *input,
  * (llmcp_q8_ctx_check).  Workspaces grow on the first call of a size: make
  * it eagerly before capturing it into a graph.  A call takes up to 2^20 slots
  * and rows (the input, and a row as wide as an expert's N or K per slot)
- * whose Q8_1 values stay below 4 GiB; more is declined.  Which kernels run,
+ * whose Q8_1 values stay below 4 GiB; more is declined, as are experts so wide
+ * (N or K past some 200000) that one launch could not hold their column
+ * ranges.  Which kernels run,
  * and so the time, depends on the numbers of slots and experts, never on the
  * ids: results are the same bits whichever run. */
 

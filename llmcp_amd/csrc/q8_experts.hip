@@ -203,7 +203,8 @@ __global__ __launch_bounds__(1024) void expert_prepare_kernel(
       if (k >= per) break;
       const uint32_t u = (uint32_t)min(u0 + 128 * k, units - 1);
       const uint32_t row = u / (uint32_t)blocks;
-      v[k] = load_raw4<BF16(), ALIGNED()>(x, (int64_t)row * ldx + (int64_t)(u - row * (uint32_t)blocks) * kBlock + 4 * p);
+      const uint32_t col = (u - row * (uint32_t)blocks) * kBlock + 4 * p;
+      v[k] = load_raw4<BF16(), ALIGNED()>(x, (int64_t)row * ldx + col);
     }
 #pragma unroll
     for (int k = 0; k < kQuantUnits; ++k) {
@@ -643,7 +644,8 @@ __global__ __launch_bounds__(256, 3) void expert_few_kernel(const ExpertArgs p) 
     const int tile = DUAL ? ng * p.repeat * 2 + (wave >> 1) : ng * p.repeat * 4 + wave;
     const uint32_t at = (uint32_t)min(tile, p.lay.tiles - 1) * (uint32_t)p.lay.tile_bytes();
 #pragma unroll
-    for (int q = 0; q < kFewRing; ++q) few_load(ring, q, wexp, at, q, steps, steps, lane, (lane & 15) * 8 + (lane >> 4) * 2);
+    for (int q = 0; q < kFewRing; ++q)
+      few_load(ring, q, wexp, at, q, steps, steps, lane, (lane & 15) * 8 + (lane >> 4) * 2);
   }
   lds_barrier();
   // ---- the rows' Q8_1 into LDS
@@ -854,7 +856,8 @@ __global__ __launch_bounds__(256) void expert_token_up_kernel(const ExpertArgs p
   }
   const uint8_t *const wexp = (wave & 1 ? p.w1 : p.w0) + (int64_t)id * p.lay.expert_bytes();
   const uint32_t tile = (blockIdx.x >> 1) * (uint32_t)p.lay.tile_bytes();
-  const uint32_t wat = tile + (blockIdx.x & 1) * 128u, dat = tile + (uint32_t)steps * 2048u + (blockIdx.x & 1) * 64u;
+  const uint32_t wat = tile + (blockIdx.x & 1) * 128u;
+  const uint32_t dat = tile + (uint32_t)steps * 2048u + (blockIdx.x & 1) * 64u;
   UpRing ring;
   static_for<kUpPairs>([&](auto Q) __attribute__((always_inline)) {
     constexpr int q = decltype(Q)::value;
@@ -1017,9 +1020,10 @@ __global__ __launch_bounds__(64 * kTokenWaves) void expert_token_kernel(
     for (int k = 0; k < K; ++k) o[k] = sums[(j0 + k) & (kMaxTopK - 1)][li];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      if (j0 + k >= top_k || (unsigned)__builtin_amdgcn_readlane(ids, j0 + k) >= (unsigned)p.experts) continue;
-      const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, factors), j0 + k));
-      v = __builtin_fmaf(w, o[k], v);
+      const int j = j0 + k;
+      if (j >= top_k || (unsigned)__builtin_amdgcn_readlane(ids, j) >= (unsigned)p.experts) continue;
+      const int w = __builtin_amdgcn_readlane(__builtin_bit_cast(int, factors), j);
+      v = __builtin_fmaf(__builtin_bit_cast(float, w), o[k], v);
     }
   }
   if (lane >= 16 || n >= p.rows) return;
@@ -1405,7 +1409,8 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
 // The wave's sum, in a scalar register.
 template <int CTRL>
 __device__ __forceinline__ float dpp_sum(float v) {
-  return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+  const int o = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true);
+  return v + __builtin_bit_cast(float, o);
 }
 __device__ __forceinline__ float wave_sum(float v) {
   v = dpp_sum<0x111>(v);
