@@ -182,6 +182,19 @@ __device__ void expert_plan(const int32_t *__restrict__ ids, int32_t slots, int3
   }
 }
 
+// quantize_block8 of N raw pieces side by side; again one by one for a rare
+// extreme scale.
+template <bool BF16, int N>
+__device__ __forceinline__ void quantize_pieces(const uint4 (&v)[N], int32_t (&q)[N], float (&s)[N]) {
+  bool slow = false;
+#pragma unroll
+  for (int k = 0; k < N; ++k) slow |= quantize_block8_fast(act4_of_raw<BF16>(v[k]), &q[k], &s[k]);
+  if (__builtin_amdgcn_ballot_w64(slow)) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) quantize_block8(act4_of_raw<BF16>(v[k]), true, &q[k], &s[k]);
+  }
+}
+
 // What comes before the products of many slots: workgroup 0 plans, the
 // others quantize the rows (x null: nothing to quantize).
 constexpr int kQuantUnits = 4;
@@ -200,22 +213,22 @@ __global__ __launch_bounds__(1024) void expert_prepare_kernel(
     uint4 v[kQuantUnits];
 #pragma unroll
     for (int k = 0; k < kQuantUnits; ++k) {
-      if (k >= per) break;
+      v[k] = make_uint4(0, 0, 0, 0);
+      if (k >= per) continue;
       const uint32_t u = (uint32_t)min(u0 + 128 * k, units - 1);
       const uint32_t row = u / (uint32_t)blocks;
       const uint32_t col = (u - row * (uint32_t)blocks) * kBlock + 4 * p;
       v[k] = load_raw4<BF16(), ALIGNED()>(x, (int64_t)row * ldx + col);
     }
+    int32_t q[kQuantUnits];
+    float s[kQuantUnits];
+    quantize_pieces<BF16()>(v, q, s);
 #pragma unroll
     for (int k = 0; k < kQuantUnits; ++k) {
-      if (k >= per) break;
       const int64_t u = u0 + 128 * k;
-      int32_t q;
-      float s;
-      quantize_block8(act4_of_raw<BF16()>(v[k]), true, &q, &s);
-      if (u >= units) continue;
-      *(int32_t *)(qa + u * kBlock + 4 * p) = q;
-      if (p == 0) sa[u] = s;
+      if (k >= per || u >= units) break;
+      *(int32_t *)(qa + u * kBlock + 4 * p) = q[k];
+      if (p == 0) sa[u] = s[k];
     }
   };
   const std::true_type yes;
@@ -693,6 +706,7 @@ __global__ __launch_bounds__(256, 3) void expert_few_kernel(const ExpertArgs p) 
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
+        // (side by side 2 % slower here: other workgroups fill the waits)
         int32_t q;
         float sc;
         quantize_block8(act4_of_raw<BF16()>(v[k]), true, &q, &sc);
@@ -759,18 +773,20 @@ struct TokenRow {
                                         uint8_t *values, float *scales) {
     const int lane = threadIdx.x & 63, l8 = lane & 7;
     if constexpr (KIND != ROW_Q8) {
-      auto one = [&](uint4 x, int u) __attribute__((always_inline)) {
-        int32_t b;
-        float sc;
-        quantize_block8(act4_of_raw<KIND == ROW_BF16>(x), true, &b, &sc);
+      auto put = [&](int32_t b, float sc, int u) __attribute__((always_inline)) {
         if (u >= count) return;
         *(int32_t *)(values + u * kBlock + 4 * l8) = b;
         if (l8 == 0) scales[u] = first + u < p.blocks ? sc : 0.0f;
       };
+      int32_t b[U];
+      float sc[U];
+      quantize_pieces<KIND == ROW_BF16>(v, b, sc);
 #pragma unroll
-      for (int k = 0; k < U; ++k)
-        if (8 * k < count) one(v[k], 8 * k + (lane >> 3));
-      for (int u = 8 * U; u < count; u += 8) one(load(p, row, first + u + (lane >> 3)), u + (lane >> 3));
+      for (int k = 0; k < U; ++k) put(b[k], sc[k], 8 * k + (lane >> 3));
+      for (int u = 8 * U; u < count; u += 8) {
+        quantize_block8(act4_of_raw<KIND == ROW_BF16>(load(p, row, first + u + (lane >> 3))), true, &b[0], &sc[0]);
+        put(b[0], sc[0], u + (lane >> 3));
+      }
     } else {
       const int8_t *const qrow = p.qa + row * p.blocks * kBlock;
       const float *const srow = p.sa + row * p.blocks;
@@ -793,7 +809,7 @@ struct TokenRow {
 // together give every lane a block's dot, which goes to LDS with the scale
 // product, and sixteen lanes run the chains over them in block order.  h is
 // left in the output's type; the down products quantize it.  Measured: 8
-// experts of [768, 2560], 33 MB, 8.2 us (11 to 12 on tiles of 16 columns, 32
+// experts of [768, 2560], 33 MB, 8.1 us (11 to 12 on tiles of 16 columns, 32
 // per workgroup and 192 workgroups; a plain read of as much 7.1).
 
 constexpr int kUpPairs = 5;  // pairs of steps of a wave in flight
@@ -949,7 +965,7 @@ __global__ __launch_bounds__(256) void expert_token_up_kernel(const ExpertArgs p
 // beyond eight): each streams its expert's tile with its one row of h,
 // quantized to LDS, and the results, rounded to the output's type, are added in slot
 // order by sixteen lanes (expert_combine_kernel's sum).  An expert that two
-// tokens share is read twice.  Measured: 8 experts of [2560, 768], 17 MB, 6.4
+// tokens share is read twice.  Measured: 8 experts of [2560, 768], 17 MB, 6.3
 // us: 160 workgroups that each read 104 KB at what a CU takes.
 
 constexpr int kTokenWaves = 8;
