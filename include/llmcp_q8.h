@@ -451,9 +451,9 @@ int llmcp_q8_mlp_bf16(llmcp_q8_ctx *ctx, const llmcp_memref_bf16_2d *input,
  * (llmcp_q8_ctx_check).  Workspaces grow on the first call of a size: make
  * it eagerly before capturing it into a graph.  A call takes up to 2^20 slots
  * and rows (the input, and a row as wide as an expert's N or K per slot)
- * whose Q8_1 values stay below 4 GiB; more is declined, as are experts so wide
- * (N or K past some 200000) that one launch could not hold their column
- * ranges.  Which kernels run,
+ * whose Q8_1 values stay below 4 GiB, and (slots / 16 + 1025) * (W / 32 + 1)
+ * below 2^24, W the wider of N and K rounded up to 32 (one launch's column
+ * ranges); more is declined.  Which kernels run,
  * and so the time, depends on the numbers of slots and experts, never on the
  * ids: results are the same bits whichever run. */
 
@@ -465,8 +465,9 @@ int llmcp_q8_mlp_bf16(llmcp_q8_ctx *ctx, const llmcp_memref_bf16_2d *input,
  * another (the p4 bytes of one tensor [experts * rows, cols]), laid out once
  * on the device for the expert entries, which alone take it: a weight
  * descriptor of the stack's p4 size, experts * rows * (cols + cols / 16), whose
- * data is host_p4.  rows % 8 == 0, cols % 32 == 0; an expert's device copy
- * must stay below 4 GiB (declined otherwise).  llmcp_q8_release, the weight
+ * data is host_p4.  rows % 8 == 0, cols % 32 == 0, each at most 523744 (what
+ * a call of one slot takes); an expert's device copy must stay below 4 GiB
+ * (declined otherwise).  llmcp_q8_release, the weight
  * budget and a second registration at one address apply as to
  * llmcp_q8_upload_p4. */
 int llmcp_q8_upload_experts_p4(llmcp_q8_ctx *ctx, const void *host_p4, int64_t experts,

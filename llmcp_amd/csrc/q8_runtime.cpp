@@ -528,6 +528,11 @@ bool packable(int64_t rows, int64_t cols) {
   return rows > 0 && cols > 0 && rows % 8 == 0 && cols % kBlock == 0;
 }
 
+// Widest N and K of an expert: with one slot check_slots still takes them.  Past
+// it no entry takes the stack, and from a K of 2^27 on the layout kernel's int
+// offsets in a tile (2 KiB of values per 128 of K) would not hold.
+constexpr int64_t kMaxExpertWidth = (0xFFFFFF / (kMaxExperts + 1) - 1) * 32;
+
 // What the expert kernels can address: each expert's tiles at 32-bit offsets.
 int check_stack(int64_t experts, int64_t rows, int64_t cols) {
   if (!packable(rows, cols))
@@ -535,8 +540,10 @@ int check_stack(int64_t experts, int64_t rows, int64_t cols) {
   if (experts < 1 || experts > kMaxExperts)
     return fail(LLMCP_Q8_DECLINED, "a stack of %lld experts (1 to %d)", (long long)experts,
                 kMaxExperts);
-  if (rows > 1ll << 31 || cols > 1ll << 31 ||
-      expert_layout(rows, cols).tile_bytes() > 0xFFFFFFFFll / ((rows + 15) / 16))
+  if (rows > kMaxExpertWidth || cols > kMaxExpertWidth)
+    return fail(LLMCP_Q8_DECLINED, "an expert of [%lld, %lld] (up to %lld wide)", (long long)rows,
+                (long long)cols, (long long)kMaxExpertWidth);
+  if (expert_layout(rows, cols).tile_bytes() > 0xFFFFFFFFll / ((rows + 15) / 16))
     return fail(LLMCP_Q8_DECLINED, "an expert of [%lld, %lld] reaches 4 GiB", (long long)rows,
                 (long long)cols);
   return LLMCP_Q8_OK;
@@ -774,6 +781,12 @@ int32_t llmcp_q8_test_gemm_plan(int64_t m, const int64_t *rows, int32_t count, i
   gemm16_instance(m, rows, count, cols, dual != 0, seg, row_tiles, col_tiles);
   *splits = gemm_splits_for(m, rows[0], cols, 0);
   return gemm16_takes(m, rows, count, cols, dual != 0) ? 1 : 0;
+}
+
+// Test hook, declared in no header of the product (no counterpart in the
+// reference): whether a stack of experts of this shape would be registered.
+int llmcp_q8_test_expert_stack(int64_t experts, int64_t rows, int64_t cols) {
+  return check_stack(experts, rows, cols);
 }
 
 int32_t llmcp_q8_get_platform(llmcp_q8_ctx *ctx) {
