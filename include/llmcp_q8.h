@@ -822,7 +822,11 @@ int llmcp_q8_microbench_epilogue(llmcp_q8_ctx *ctx, int32_t mode, int32_t blocks
  * holds the device addresses of the context's workspace and weights at
  * capture: graph_launch refuses it with LLMCP_Q8_ESTALE once any of them
  * was freed or reallocated (a call that grew the workspace, a weight
- * released or registered again). */
+ * released or registered again).  graph_launch replays a graph that is
+ * nothing but a chain of up to seven of this library's kernels by launching
+ * them in order on the context's stream, which takes less time than a HIP
+ * graph launch, and any other as the HIP graph it is.  (An error from a launch
+ * midway leaves those before it on the stream.) */
 int llmcp_q8_graph_begin(llmcp_q8_ctx *ctx);
 int llmcp_q8_graph_end(llmcp_q8_ctx *ctx, void **graph_exec);
 int llmcp_q8_graph_launch(llmcp_q8_ctx *ctx, void *graph_exec);

@@ -153,12 +153,14 @@ struct GraphInfo {
   std::vector<hipKernelNodeParams> chain;
 };
 // Longest chain of kernels that is replayed by launching them one after
-// another (kernel_chain).  Up to eight that takes the host no longer than
-// hipGraphLaunch does (linears of 2560 x 2560, chain against graph: 1 / 2 / 4
-// / 8 of them 2.7 / 5.2 / 10.3 / 21 us against 17.4 / 16.5 / 17.3 / 19.5; 16 of
-// them 43 against 21), and the replays follow each other more closely (2.9 /
-// 5.5 / 10.9 / 21.7 us each against 17.4 / 16.6 / 17.5 / 26.8).
-constexpr size_t kMaxChain = 8;
+// another (kernel_chain): up to here that takes the host less than
+// hipGraphLaunch does.  Host time of a replay of 1 / 2 / 4 / 6 / 7 / 8 linears
+// of 2560 x 2560 into an idle queue, us: 2.6 / 4.7 / 8.8 / 12.8 / 15.0 / 22.8 by
+// launches, 16.7 / 17.4 / 17.7 / 18.1 / 17.7 / 18.0 as a graph; of 256 x 2560 and
+// of 65536 x 2560 the same within 2 us.  The replays also follow each other more
+// closely (2.9 / 5.6 / 11.0 / 16.2 / 18.9 / 21.9 us each against 13.3 / 13.5 /
+// 17.1 / 21.8 / 24.5 / 27.3; seven of 65536 x 2560 174 against 178).
+constexpr size_t kMaxChain = 7;
 std::mutex g_graph_mutex;
 std::map<void *, GraphInfo> g_graphs;
 
@@ -3316,6 +3318,15 @@ int llmcp_q8_graph_launch(llmcp_q8_ctx *ctx, void *graph_exec) {
     HIP_TRY(hipGraphLaunch((hipGraphExec_t)graph_exec, ctx->stream));
     return LLMCP_Q8_OK;
   });
+}
+
+// Test hook, declared in no header of the product (no counterpart in the
+// reference): how many launches a replay of this graph is, 0 where it goes as
+// the graph it is, -1 for an unknown one.
+int32_t llmcp_q8_test_graph_chain(void *graph_exec) {
+  std::lock_guard<std::mutex> lock(g_graph_mutex);
+  auto it = g_graphs.find(graph_exec);
+  return it == g_graphs.end() ? -1 : (int32_t)it->second.chain.size();
 }
 
 int llmcp_q8_graph_destroy(void *graph_exec) {
