@@ -646,6 +646,15 @@ int llmcp_q8_selftest_quantizer(llmcp_q8_ctx *ctx, uint64_t *mismatches);
 int llmcp_q8_selftest_exp(llmcp_q8_ctx *ctx, uint64_t counts[4], float *inputs,
                           uint32_t *results, int64_t cap, int64_t *stored);
 
+/* Device self-test of the silu inside the experts' bf16 SwiGLU (no counterpart
+ * in the reference): where a result is rounded to bf16 next, an f32 form
+ * stands in for the epilogues' silu unless its value lies near a midpoint of
+ * bf16.  Over all 2^32 floats, counts[0] is the number of values of that form
+ * that would be taken and round to another bf16 (0 expected), counts[1]
+ * those of the whole function that do (0 expected), counts[2] those that the
+ * f32 form leaves to the other.  Synchronous. */
+int llmcp_q8_selftest_silu(llmcp_q8_ctx *ctx, uint64_t counts[3]);
+
 /* ---------------------------------------------------- offline packing -- */
 
 /* quantizeTensorQ8_0Packed (lib/Model/Quantization.cpp:165-214) on the host:

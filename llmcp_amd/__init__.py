@@ -75,6 +75,7 @@ EXPORTS = [
     "llmcp_q8_event_elapsed_ms", "llmcp_q8_graph_begin", "llmcp_q8_graph_end",
     "llmcp_q8_graph_launch", "llmcp_q8_graph_destroy",
     "llmcp_q8_device_bytes", "llmcp_q8_selftest_quantizer", "llmcp_q8_selftest_exp",
+    "llmcp_q8_selftest_silu",
     "llmcp_q8_linear_bf16", "llmcp_q8_swiglu_bf16", "llmcp_q8_mlp_bf16",
     "llmcp_q8_lm_head_bf16", "llmcp_q8_embedding_bf16", "llmcp_q8_lm_head_noalloc",
     "_mlir_ciface_llmcp_q8_linear_bf16", "_mlir_ciface_llmcp_q8_swiglu_bf16",
@@ -171,6 +172,7 @@ def lib():
         "llmcp_q8_graph_destroy": (I, [P]),
         "llmcp_q8_device_bytes": (U64, [P, P]),
         "llmcp_q8_selftest_quantizer": (I, [P, ctypes.POINTER(U64)]),
+        "llmcp_q8_selftest_silu": (I, [P, ctypes.POINTER(U64)]),
         "llmcp_q8_selftest_exp": (I, [P, ctypes.POINTER(U64), P, P, ctypes.c_int64,
                                       ctypes.POINTER(ctypes.c_int64)]),
         "llmcp_q8_linear_bf16": (I, [P, P, P, P, I32, I32]),
@@ -699,6 +701,14 @@ class Context:
         check(lib().llmcp_q8_selftest_exp(self.handle, counts, xs.ctypes.data,
                                           rs.ctypes.data, cap, ctypes.byref(k)))
         return tuple(int(c) for c in counts), xs[:k.value], rs[:k.value]
+
+    def selftest_silu(self):
+        """Exhaustive device check of the silu of the experts' bf16 SwiGLU:
+        (its f32 form's values that would be taken and round unlike silu,
+        the whole function's that do, values left to the exact form)."""
+        counts = (ctypes.c_uint64 * 3)()
+        check(lib().llmcp_q8_selftest_silu(self.handle, counts))
+        return tuple(int(c) for c in counts)
 
     # ---- timing
     def event(self):

@@ -318,31 +318,58 @@ typedef unsigned v4u __attribute__((ext_vector_type(4)));
 // f32, exp(-v) = 2^h (1 + l ln 2) with h + l = -v log2(e), h its rounding; the
 // hardware's 2^x and 1/x are good to one step (2^-23), so the result is
 // within 3 * 2^-23 of silu and silu_f32's four roundings 4 * 2^-24: the two
-// differ by less than 2^-20, 16 steps of f32 at the least.  Where no midpoint
-// of bf16 lies within 16 steps both round to the same value; where one does
+// differ by less than 2^-20, at most 16 steps of f32.  Where no midpoint
+// of bf16 lies within 17 steps both round to the same value; where one does
 // (one value in 2000), or where |v| leaves the range of that reckoning, the
-// array is done again exactly.  (Compared on the card over all 2^32 floats: no
-// difference.)
+// array is done again exactly.  (llmcp_q8_selftest_silu compares all 2^32
+// floats on the running card: no difference.)
+//
+// One value by the f32 form; sets `slow` where it is not to be taken.
+__device__ __forceinline__ float silu_bf16_fast(float x, bool &slow) {
+  const float h = x * -1.44269502f;
+  const float l = __builtin_fmaf(x, -1.92596303e-8f, __builtin_fmaf(x, -1.44269502f, -h));
+  const float e0 = __builtin_amdgcn_exp2f(h);
+  const float e = __builtin_fmaf(e0, l * 0.693147182f, e0);
+  const float r = x * __builtin_amdgcn_rcpf(1.0f + e);
+  const uint32_t low = __builtin_bit_cast(uint32_t, r) & 0xffffu;
+  const float a = fabsf(x);
+  slow |= low - (0x8000u - 17u) <= 34u || !(a < 80.0f) || (a < 0x1p-100f && x != 0.0f);
+  return r;
+}
 template <int N>
 __device__ __forceinline__ void silu_for_bf16(float (&v)[N]) {
   float r[N];
   bool slow = false;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float x = v[i], h = x * -1.44269502f;
-    const float l = __builtin_fmaf(x, -1.92596303e-8f, __builtin_fmaf(x, -1.44269502f, -h));
-    const float e0 = __builtin_amdgcn_exp2f(h);
-    const float e = __builtin_fmaf(e0, l * 0.693147182f, e0);
-    r[i] = x * __builtin_amdgcn_rcpf(1.0f + e);
-    const uint32_t low = __builtin_bit_cast(uint32_t, r[i]) & 0xffffu;
-    const float a = fabsf(x);
-    slow |= low - (0x8000u - 17u) <= 34u || !(a < 80.0f) || (a < 0x1p-100f && x != 0.0f);
-  }
+  for (int i = 0; i < N; ++i) r[i] = silu_bf16_fast(v[i], slow);
   if (__builtin_amdgcn_ballot_w64(slow) == 0) {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = r[i];
   } else {
     activate_array(v, ACT_SILU);
+  }
+}
+
+// Over the float bit patterns [lo, lo + 2^31): out[0] counts the f32 form's
+// values that would be taken and round to another bf16 than silu_f32 (each by
+// itself, whatever its neighbours need), out[1] silu_for_bf16's that do,
+// out[2] the values that the f32 form leaves.  NaNs are alike.
+__global__ __launch_bounds__(256) void selftest_silu_kernel(uint32_t lo, unsigned long long *out) {
+  const float v = __builtin_bit_cast(float, lo + blockIdx.x * 256u + threadIdx.x);
+  const uint16_t want = float_to_bf16(silu_f32(v));
+  bool slow = false;
+  const float r = silu_bf16_fast(v, slow);
+  float whole[1] = {v};
+  silu_for_bf16(whole);
+  auto unlike = [&](float x) {
+    const uint16_t got = float_to_bf16(x);
+    return got != want && !((got & 0x7fff) > 0x7f80 && (want & 0x7fff) > 0x7f80);
+  };
+  const uint64_t bad = __ballot(!slow && unlike(r)), off = __ballot(unlike(whole[0])), left = __ballot(slow);
+  if ((threadIdx.x & 63) == 0) {
+    if (bad) atomicAdd(out, (unsigned long long)__popcll(bad));
+    if (off) atomicAdd(out + 1, (unsigned long long)__popcll(off));
+    if (left) atomicAdd(out + 2, (unsigned long long)__popcll(left));
   }
 }
 
@@ -1515,6 +1542,15 @@ hipError_t launch_repack_experts(const uint8_t *p4, uint8_t *out, int64_t expert
                        cols / kBlock, lay);
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
+  }
+  return hipSuccess;
+}
+
+hipError_t launch_selftest_silu(unsigned long long *out, hipStream_t s) {
+  for (uint32_t half = 0; half < 2; ++half) {
+    hipLaunchKernelGGL(selftest_silu_kernel, dim3(1u << 23), dim3(256), 0, s, half << 31, out);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
   }
   return hipSuccess;
 }

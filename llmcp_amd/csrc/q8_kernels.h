@@ -227,6 +227,11 @@ hipError_t launch_add_rmsnorm(const void *x, int64_t ldx, const void *r, int64_t
 hipError_t launch_repack_experts(const uint8_t *p4, uint8_t *out, int64_t experts, int64_t rows,
                                  int64_t cols, hipStream_t s);
 
+// All floats through the SwiGLU's silu of a bf16 result: adds to out[3] the
+// values of its f32 form that would be taken and round unlike silu_f32, the whole
+// function's that do, and the values that the f32 form leaves.
+hipError_t launch_selftest_silu(unsigned long long *out, hipStream_t s);
+
 // The top_k largest of `experts` logits per row (ties: lowest index) and
 // their softmax weights, over all or (normalize) the chosen ones, times
 // scale; NaN and -inf are not chosen (id -1, weight 0).  ids, weights [m,

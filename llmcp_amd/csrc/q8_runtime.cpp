@@ -893,6 +893,27 @@ int llmcp_q8_selftest_exp(llmcp_q8_ctx *ctx, uint64_t counts[4], float *inputs,
   });
 }
 
+int llmcp_q8_selftest_silu(llmcp_q8_ctx *ctx, uint64_t counts[3]) {
+  return guarded([&]() -> int {
+    if (!ctx || !counts) return fail(LLMCP_Q8_EINVAL, "null argument");
+    int rc = set_device(ctx);
+    if (rc) return rc;
+    unsigned long long *out = nullptr;
+    unsigned long long host[3] = {0, 0, 0};
+    if (hipMalloc(&out, sizeof(host)) != hipSuccess)
+      return fail(LLMCP_Q8_ENOMEM, "silu self-test counters");
+    hipError_t e = hipMemsetAsync(out, 0, sizeof(host), ctx->stream);
+    if (e == hipSuccess) e = launch_selftest_silu(out, ctx->stream);
+    if (e == hipSuccess)
+      e = hipMemcpyAsync(host, out, sizeof(host), hipMemcpyDeviceToHost, ctx->stream);
+    if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);
+    (void)hipFree(out);
+    if (e != hipSuccess) return hip_fail(e, "silu self-test");
+    for (int i = 0; i < 3; ++i) counts[i] = host[i];
+    return LLMCP_Q8_OK;
+  });
+}
+
 // ------------------------------------------------------------- weights --
 
 int llmcp_q8_upload_p4(llmcp_q8_ctx *ctx, const void *host_p4, int64_t rows,
