@@ -1592,13 +1592,18 @@ hipError_t launch_expert_prepare(const int32_t *ids, int64_t slots, int32_t expe
   return hipGetLastError();
 }
 
-// Column ranges of `cols` columns per workgroup for about `tiles` tiles with
-// work: as many as leave `fill` workgroups per CU.
-static void set_repeat(ExpertArgs &a, int64_t tiles, int cols, int fill) {
-  const int64_t groups = (a.rows + cols - 1) / cols;
-  const int64_t want = std::max<int64_t>(1, tiles * groups / ((int64_t)fill * cu_count()));
-  a.n_groups = (int32_t)((groups + std::min(want, groups) - 1) / std::min(want, groups));
-  a.repeat = (int32_t)((groups + a.n_groups - 1) / a.n_groups);
+// Column ranges of 32 to 128 columns, `repeat` of them per workgroup: as many as
+// leave 8 workgroups (few slots) or 20 (many) per CU for about as many tiles as
+// there is work for.
+void expert_ranges(int64_t slots, int64_t experts, int32_t tile_rows, int64_t rows, bool dual,
+                   int32_t test_repeat, int32_t *n_groups, int32_t *repeat) {
+  const bool few = tile_rows <= 16;
+  const int64_t cols = (dual ? 32 : 64) * (few ? 1 : 2), groups = (rows + cols - 1) / cols;
+  const int64_t some = std::min(slots, experts), tiles = few ? some : std::max(slots / tile_rows, some);
+  int64_t want = std::max<int64_t>(1, tiles * groups / ((few ? 8 : 20) * (int64_t)cu_count()));
+  if (test_repeat > 0) want = test_repeat;
+  *n_groups = (int32_t)((groups + std::min(want, groups) - 1) / std::min(want, groups));
+  *repeat = (int32_t)((groups + *n_groups - 1) / *n_groups);
 }
 
 template <int NV, bool DUAL>
@@ -1606,7 +1611,6 @@ static hipError_t launch_few(ExpertArgs &a, bool fma, hipStream_t s) {
   const int64_t tiles = a.plan ? a.max_tiles
                         : NV == 1 ? a.slots
                                   : a.slots / (4 * NV) + std::min(a.slots, a.experts + 1);
-  set_repeat(a, std::min(a.slots, a.experts), DUAL ? 32 : 64, 8);
   const int64_t wgs = tiles * a.n_groups;
   // HIP bounds a grid's work-items by 2^32 - 1
   if (wgs * 256 > 0xFFFFFFFFll) return hipErrorInvalidConfiguration;
@@ -1620,7 +1624,6 @@ static hipError_t launch_few(ExpertArgs &a, bool fma, hipStream_t s) {
 
 template <int TT, bool DUAL>
 static hipError_t launch_many(ExpertArgs &a, bool fma, hipStream_t s) {
-  set_repeat(a, std::max(a.slots / (32 * TT), std::min(a.slots, a.experts)), DUAL ? 64 : 128, 20);
   const int64_t wgs = (int64_t)a.max_tiles * a.n_groups;
   if (wgs * 256 > 0xFFFFFFFFll) return hipErrorInvalidConfiguration;
   if (fma)
@@ -1664,6 +1667,7 @@ static ExpertArgs expert_args(const ExpertLaunch &l) {
 hipError_t launch_experts(const ExpertLaunch &l, hipStream_t s) {
   ExpertArgs a = expert_args(l);
   const bool dual = l.up != nullptr;
+  expert_ranges(l.slots, l.experts, l.tile_rows, l.rows, dual, l.test_repeat, &a.n_groups, &a.repeat);
   switch (l.tile_rows) {
     case 4:
       return dual ? launch_few<1, true>(a, l.fma, s) : launch_few<1, false>(a, l.fma, s);

@@ -251,6 +251,10 @@ int32_t expert_tile_rows(int64_t slots, int64_t experts, int64_t widest);
 bool expert_planned(int64_t slots, int64_t experts, int32_t tile_rows);
 int64_t expert_max_tiles(int64_t slots, int64_t experts, int32_t tile_rows);
 int64_t expert_plan_ints(int64_t slots, int64_t experts, int32_t tile_rows);
+// Workgroups side by side over an expert's `rows` columns and the column ranges
+// that each takes one after another (test_repeat > 0: so many, for tests).
+void expert_ranges(int64_t slots, int64_t experts, int32_t tile_rows, int64_t rows, bool dual,
+                   int32_t test_repeat, int32_t *n_groups, int32_t *repeat);
 // The plan and, x non-null, the Q8_1 of its m rows into qa / sa (dense).
 hipError_t launch_expert_prepare(const int32_t *ids, int64_t slots, int32_t experts,
                                  int32_t tile_rows, int32_t *plan, int32_t *err_flag, const void *x,
@@ -283,6 +287,7 @@ struct ExpertLaunch {
   int64_t ldy = 0;
   int8_t *hq = nullptr;          // [slots, rows]
   float *hs = nullptr;           // [slots, rows / 32]
+  int32_t test_repeat = 0;       // expert_ranges
 };
 hipError_t launch_experts(const ExpertLaunch &l, hipStream_t s);
 

@@ -117,6 +117,9 @@ struct llmcp_q8_ctx {
   // Tests only (llmcp_q8_test_ctx_gemm_splits): K splits forced on every
   // splittable GEMM of this context in SPLIT_K mode; 0 = chosen by shape.
   int32_t test_splits = 0;
+  // Tests only (llmcp_q8_test_ctx_expert_repeat): column ranges forced on every
+  // workgroup of the experts' products that share tiles; 0 = chosen by size.
+  int32_t test_repeat = 0;
   // Mixture of experts, grown on demand: the slots sorted by expert, the
   // SwiGLU's rows as Q8_1 and the experts' outputs.
   int32_t *plan = nullptr;
@@ -783,6 +786,31 @@ int32_t llmcp_q8_test_gemm_plan(int64_t m, const int64_t *rows, int32_t count, i
   gemm16_instance(m, rows, count, cols, dual != 0, seg, row_tiles, col_tiles);
   *splits = gemm_splits_for(m, rows[0], cols, 0);
   return gemm16_takes(m, rows, count, cols, dual != 0) ? 1 : 0;
+}
+
+// Test hook, declared in no header of the product (no counterpart in the
+// reference): forces `repeat` column ranges (clamped to what there is; 0 = the
+// size's own choice) on the workgroups of this context's expert products.
+int llmcp_q8_test_ctx_expert_repeat(llmcp_q8_ctx *ctx, int32_t repeat) {
+  if (!ctx) return fail(LLMCP_Q8_EINVAL, "null context");
+  if (repeat < 0) return fail(LLMCP_Q8_EINVAL, "negative range count %d", repeat);
+  ctx->test_repeat = repeat;
+  return LLMCP_Q8_OK;
+}
+
+// Test hook, declared in no header of the product (no counterpart in the
+// reference): what `slots` slots over `experts` experts of `rows` columns run on
+// (dual: the SwiGLU's products; weights and rows up to `widest` wide).  Returns
+// the column ranges per workgroup; `tile_rows`: slots per tile, `planned`: whether
+// the tiles come from a plan, `n_groups`: workgroups side by side per tile.
+int32_t llmcp_q8_test_expert_ranges(int64_t slots, int64_t experts, int64_t rows, int64_t widest,
+                                    int32_t dual, int32_t test_repeat, int32_t *tile_rows,
+                                    int32_t *planned, int32_t *n_groups) {
+  int32_t repeat = 0;
+  *tile_rows = expert_tile_rows(slots, experts, widest);
+  *planned = expert_planned(slots, experts, *tile_rows) ? 1 : 0;
+  expert_ranges(slots, experts, *tile_rows, rows, dual != 0, test_repeat, n_groups, &repeat);
+  return repeat;
 }
 
 // Test hook, declared in no header of the product (no counterpart in the
@@ -1771,6 +1799,7 @@ static int expert_prepare(llmcp_q8_ctx *ctx, const ExpertRows &in, const int32_t
   l.experts = (int32_t)count;
   l.err_flag = ctx->err_flag;
   l.fma = ctx->fma();
+  l.test_repeat = ctx->test_repeat;
   const bool planned = !token && expert_planned(slots, count, l.tile_rows);
   const bool aligned = in.x && (uintptr_t)in.x->data % (in.x->bf16 ? 8 : 16) == 0 && in.x->ld % 4 == 0;
   const int64_t blocks = in.cols / kBlock;
