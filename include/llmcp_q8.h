@@ -390,9 +390,10 @@ typedef struct {
  * both; sum and normed may each take the memory of input or residual (same
  * strides), but not each other's.  No counterpart in the reference, which
  * has llmcp.add and llmcp.rms_norm apart: the sum of squares is taken in
- * f64, so the bits do not depend on its order and are not those of
- * llmcp_q8_rmsnorm, whose f32 sum is serial (they agree to about H * 2^-24;
- * this one is the nearer to the exact norm).  The weight must be 16 B
+ * f64, in an order that H alone sets (another order would give another rstd for
+ * one row in some 10^8), so the bits are not those of llmcp_q8_rmsnorm, whose
+ * f32 sum is serial (they agree to about H * 2^-24; this one is the nearer to
+ * the exact norm).  The weight must be 16 B
  * aligned (8 B for bf16), quantized->values 16 B; declines otherwise. */
 int llmcp_q8_add_rmsnorm(llmcp_q8_ctx *ctx, const llmcp_memref_f32_2d *input,
                          const llmcp_memref_f32_2d *residual,
@@ -453,9 +454,10 @@ int llmcp_q8_mlp_bf16(llmcp_q8_ctx *ctx, const llmcp_memref_bf16_2d *input,
  * and rows (the input, and a row as wide as an expert's N or K per slot)
  * whose Q8_1 values stay below 4 GiB, and (slots / 16 + 1025) * (W / 32 + 1)
  * below 2^24, W the wider of N and K rounded up to 32 (one launch's column
- * ranges); more is declined.  Which kernels run,
- * and so the time, depends on the numbers of slots and experts, never on the
- * ids: results are the same bits whichever run. */
+ * ranges); more is declined.  Which kernels run depends on the numbers of slots
+ * and experts, the widths and the rows' alignment, never on the ids, and results
+ * are the same bits whichever run.  (How long they take depends on the ids
+ * too: on how many experts they touch, and how evenly.) */
 
 /* Most experts of a stack and most choices per token. */
 #define LLMCP_Q8_MAX_EXPERTS 1024

@@ -8,9 +8,9 @@
 // about 2^29 below f32's rounding, so a tree gives the same rstd as a serial
 // sum but for one row in some 10^8, and no step of a quantizer hangs on how
 // the row is split over lanes.  (The f64 work is a multiply and an add per
-// value of a row that is bound by memory.)  Measured in bf16, H = 2560, sum and
-// Q8_1 out: one row 3.9 us (the latency of two passes over the workgroup),
-// 4096 rows 19.4 us for 96 MB (4.9 TB/s; a copy reaches 5.3; 20.7 with the
+// value of a row that is bound by memory.)  Measured in bf16, H = 2560, sum, norm
+// and Q8_1 out: one row 3.9 us (the latency of two passes over the workgroup),
+// 4096 rows 19.2 us for 96 MB (5.0 TB/s; a copy reaches 5.3; 20.7 with the
 // loads one by one and the sum by LDS permutes).
 #include "q8_kernels.h"
 

@@ -4,8 +4,8 @@
 // The function per row is the other GEMMs': exact int32 block dots, acc =
 // fma(f32(I), sa * dw, acc) or acc + f32(I) * (sa * dw) in block order, so a
 // slot's result is bit for bit what the linear of its expert gives.  A
-// workgroup takes up to 16, 32 or 64 slots of one expert and a range of the
-// weight's columns.
+// workgroup takes up to 4, 8, 16, 32 or 64 slots of one expert (a token's
+// alone: one) and a range of the weight's columns.
 #include "q8_kernels.h"
 
 #include <algorithm>
@@ -87,8 +87,8 @@ __device__ __forceinline__ int wave_scan(int v) {
 // An id that is neither an expert nor -1 sets the error flag.  The order of a
 // group's slots is that of the atomics; no result depends on it.
 // Bound by latency, one workgroup's passes over the ids: with the rows' Q8_1
-// beside it 3.9 us for 640 slots (and as many rows of 768), 5.0 for 2664 (333
-// rows of 2560), 15 for 32768 (4096 rows).
+// beside it 4.0 us for 640 slots (and as many rows of 768), 4.9 for 2664 (333
+// rows of 2560), 14 for 32768 (4096 rows).
 __device__ void expert_plan(const int32_t *__restrict__ ids, int32_t slots, int32_t experts,
                             int32_t tile_rows, int32_t max_tiles, int32_t *__restrict__ plan,
                             int32_t *__restrict__ err) {
@@ -412,8 +412,8 @@ __device__ __forceinline__ void store_h(const ExpertArgs &p, const float *hb, in
 // from tile to tile; the rows stay in LDS for all of them.  A step issues its
 // MFMAs, reads the next step's rows and then runs the epilogue of the step
 // before, so that a lone wave waits for none of them.  Measured: 16 tokens
-// through 8 of 128 experts of [768, 2560], gate and up 62 us (344 MB, 5.5
-// TB/s), down 37 us (172 MB, 4.7 TB/s); what is missing to the 6.4 TB/s of a
+// through 8 of 128 experts of [768, 2560], gate and up 64 us (344 MB, 5.3
+// TB/s), down 38 us (172 MB, 4.5 TB/s); what is missing to the 6.4 TB/s of a
 // plain read is the launch and the last workgroups.
 //
 // LDS: [slots][a_ld] values (a block pair's 64 B: quarter, block parity,
@@ -836,7 +836,7 @@ struct TokenRow {
 // together give every lane a block's dot, which goes to LDS with the scale
 // product, and sixteen lanes run the chains over them in block order.  h is
 // left in the output's type; the down products quantize it.  Measured: 8
-// experts of [768, 2560], 33 MB, 8.1 us (11 to 12 on tiles of 16 columns, 32
+// experts of [768, 2560], 33 MB, 8.0 us (11 to 12 on tiles of 16 columns, 32
 // per workgroup and 192 workgroups; a plain read of as much 7.1).
 
 constexpr int kUpPairs = 5;  // pairs of steps of a wave in flight
@@ -992,7 +992,7 @@ __global__ __launch_bounds__(256) void expert_token_up_kernel(const ExpertArgs p
 // beyond eight): each streams its expert's tile with its one row of h,
 // quantized to LDS, and the results, rounded to the output's type, are added in slot
 // order by sixteen lanes (expert_combine_kernel's sum).  An expert that two
-// tokens share is read twice.  Measured: 8 experts of [2560, 768], 17 MB, 6.3
+// tokens share is read twice.  Measured: 8 experts of [2560, 768], 17 MB, 6.8
 // us: 160 workgroups that each read 104 KB at what a CU takes.
 
 constexpr int kTokenWaves = 8;
@@ -1088,8 +1088,8 @@ __global__ __launch_bounds__(64 * kTokenWaves) void expert_token_kernel(
 // blocks, loaded a step before they are stored there, one barrier a step; a
 // workgroup takes `repeat` column ranges without a pause in either stream.
 // Measured with 128 experts of [768, 2560], 8 per token: 4096 tokens, gate and
-// up 440 .. 460 us and down 265 us (258 + 129 GFLOP, 570 and 490 TOPS, where
-// convert, FMA and MFMAs alone reach 880); 333 tokens, TT = 1, 101 and 58 us
+// up 439 us and down 262 us (258 + 129 GFLOP, 590 and 490 TOPS, where
+// convert, FMA and MFMAs alone reach 880); 333 tokens, TT = 1, 102 and 59 us
 // (538 and 269 MB of weights, 5.3 and 4.6 TB/s).
 
 template <int TT>
@@ -1469,7 +1469,7 @@ __device__ __forceinline__ float wave_sum(float v) {
 // rounds, each the wave's largest key and the lowest index that has it; then
 // the chosen ones' exponentials side by side, one per lane.  Latency bound
 // for few rows: a round is six lane moves and a ballot per 64 logits.
-// Measured: the 8 largest of 128, one row 3.4 us, 4096 rows 5.0.
+// Measured: the 8 largest of 128, one row 3.6 us, 4096 rows 5.3.
 template <bool BF16, int PER>
 __global__ __launch_bounds__(256) void route_kernel(const void *__restrict__ logits, int64_t ld,
                                                     int64_t m, int32_t experts, int32_t top_k,
@@ -1728,7 +1728,7 @@ hipError_t launch_expert_combine(const void *o, const int32_t *ids, const float 
                                  int32_t experts, int64_t m, int64_t cols, const void *residual,
                                  int64_t ldr, void *y, int64_t ldy, bool bf16, hipStream_t s) {
   // Eight bf16 columns (16 B) per thread once that fills the chip (2048 lanes
-  // per CU), four before: 4096 rows of 8 x 2560 35.6 us (5.9 TB/s) against 41,
+  // per CU), four before: 4096 rows of 8 x 2560 35.1 us (6.0 TB/s) against 41,
   // 333 rows 7.0 against 6.4, 16 rows 5.2 against 4.5.
   const int v = bf16 && m * (cols / 8) >= (int64_t)cu_count() * 2048 ? 8 : 4;
   const int64_t wgs = (m * (cols / v) + 255) / 256;
