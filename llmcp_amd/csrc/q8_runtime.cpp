@@ -160,7 +160,7 @@ struct GraphInfo {
 // hipGraphLaunch does.  Host time of a replay of 1 / 2 / 4 / 6 / 7 / 8 linears
 // of 2560 x 2560 into an idle queue, us: 2.6 / 4.7 / 8.8 / 12.8 / 15.0 / 22.8 by
 // launches, 16.7 / 17.4 / 17.7 / 18.1 / 17.7 / 18.0 as a graph; of 256 x 2560 and
-// of 65536 x 2560 the same within 2 us.  The replays also follow each other more
+// of 65536 x 2560 the same within 3 us.  The replays also follow each other more
 // closely (2.9 / 5.6 / 11.0 / 16.2 / 18.9 / 21.9 us each against 13.3 / 13.5 /
 // 17.1 / 21.8 / 24.5 / 27.3; seven of 65536 x 2560 174 against 178).
 constexpr size_t kMaxChain = 7;
