@@ -44,8 +44,9 @@ extern "C" {
  * weight budget, graph staleness check, grouped linears; 5: RMSNorm, gated
  * RMSNorm and RMSNorm + grouped linears; 6: their MLIR C-interface entries
  * and the bf16 group entries; 7: the accumulation switch, later joined by
- * the residual-add norm and the mixture-of-experts entries, which change
- * nothing that was there).  The model ABI of
+ * the residual-add norm, the mixture-of-experts entries and those of the
+ * key/value cache, attention and the delta rule, which change nothing that
+ * was there).  The model ABI of
  * the AOT library (llmcp_model_abi_version() == 2,
  * include/llmcp/Support/AotAbi.h:12) is not changed by this library. */
 #define LLMCP_Q8_ABI_VERSION 7
@@ -172,6 +173,24 @@ typedef struct {
   int64_t sizes[1];
   int64_t strides[1];
 } llmcp_memref_bf16_1d;
+
+/* Rows of heads [rows, heads, dim] (memref<?x?x?xf32> / bf16): queries, keys,
+ * values and what a mixer gives. */
+typedef struct {
+  float *base;
+  float *data;
+  int64_t offset;
+  int64_t sizes[3];
+  int64_t strides[3];
+} llmcp_memref_f32_3d;
+
+typedef struct {
+  uint16_t *base;
+  uint16_t *data;
+  int64_t offset;
+  int64_t sizes[3];
+  int64_t strides[3];
+} llmcp_memref_bf16_3d;
 
 typedef struct llmcp_q8_ctx llmcp_q8_ctx;
 
@@ -549,6 +568,100 @@ int llmcp_q8_expert_mlp_rows_bf16(llmcp_q8_ctx *ctx, const llmcp_q8_rows *input,
                                   const llmcp_memref_i8_1d *w_down,
                                   const llmcp_memref_bf16_2d *residual,
                                   llmcp_memref_bf16_2d *output);
+
+/* ---- key/value cache, attention and the delta rule: what stands between the
+ * q/k/v (or qkv/z/a/b) linears and the output projection.  The reference's
+ * model has both mixers, with a bf16 cache and an f32 state
+ * (AotRuntime.cpp:87-118), as loops of its own lowering; these entries have
+ * their own numerics (f32 sums, in an order of their own).
+ *
+ * Rows of heads are [rows, heads, dim] with dense values (strides[2] == 1),
+ * a row's heads next to each other or further apart (strides[1] >= dim,
+ * strides[0] >= heads * strides[1] where rows > 1) and every head 16 B
+ * aligned, so that q, k and v may be parts of one linear's output; declined
+ * otherwise.  Outputs must not share memory with inputs.
+ *
+ * A call takes the rows of several sequences, one sequence after another:
+ * sequence s has the rows row_starts[s] .. row_starts[s + 1] - 1, none where
+ * the two are equal.  row_starts ascends within 0 .. rows (bounds outside are
+ * taken as 0 or rows; where it descends, rows of several sequences hold the
+ * result of one of them); rows before the first and from the last on are left as
+ * they were.  Up to 2^23 rows, 65536 sequences and 1024 heads; more is
+ * declined. */
+
+/* How a cache keeps a row of head_dim values: as bf16 (rounded to nearest
+ * even), or as int8 with an f32 scale s = max|x| / 127, value q * s with q = x *
+ * (1 / s) rounded to nearest even (llmcp_q8_quantize_activations' arithmetic
+ * over the whole row).  Q8: a row whose largest value is below 2^-118 is kept as
+ * zeros; a row with an infinity or NaN reads back as NaN. */
+enum llmcp_q8_cache_format { LLMCP_Q8_CACHE_BF16 = 0, LLMCP_Q8_CACHE_Q8 = 1 };
+
+/* Pages of keys and values in device memory, each [pages, kv_heads, page_size,
+ * head_dim] dense and 16 B aligned; Q8: int8 with the scales [pages, kv_heads,
+ * page_size].  head_dim 64, 128 or 256; page_size up to 2^20, of any value (a
+ * contiguous cache is one page per sequence), and max_pages * page_size and
+ * pages * kv_heads * page_size below 2^31; declined otherwise. */
+typedef struct {
+  void *keys, *values;
+  float *key_scales, *value_scales; /* Q8, else null */
+  int64_t pages;
+  int32_t page_size, kv_heads, head_dim;
+  int32_t format; /* llmcp_q8_cache_format */
+} llmcp_q8_kv_cache;
+
+/* The sequences of a call, in device memory.  lengths[s] counts the keys of
+ * sequence s with those of the call's rows: row i of its n rows is at
+ * position lengths[s] - n + i.  Position p is in slot p % page_size of page
+ * page_table[s * max_pages + p / page_size]; -1 there stands for no page, any
+ * other id that is no page counts as -1 and sets the context's error flag
+ * (llmcp_q8_ctx_check).  Positions below 0 or from max_pages * page_size on
+ * have no slot. */
+typedef struct {
+  const int32_t *row_starts; /* [sequences + 1] */
+  const int32_t *lengths;    /* [sequences] */
+  const int32_t *page_table; /* [sequences, max_pages] */
+  int32_t sequences, max_pages;
+} llmcp_q8_kv_batch;
+
+/* Keys and values [rows, kv_heads, head_dim] into their slots; a row without
+ * one is dropped.  (Two rows of one slot, by a page that two sequences share,
+ * leave it undefined.) */
+int llmcp_q8_kv_write(llmcp_q8_ctx *ctx, const llmcp_memref_f32_3d *keys,
+                      const llmcp_memref_f32_3d *values, const llmcp_q8_kv_batch *batch,
+                      const llmcp_q8_kv_cache *cache);
+int llmcp_q8_kv_write_bf16(llmcp_q8_ctx *ctx, const llmcp_memref_bf16_3d *keys,
+                           const llmcp_memref_bf16_3d *values, const llmcp_q8_kv_batch *batch,
+                           const llmcp_q8_kv_cache *cache);
+
+/* The values that the rows' slots stand for, rounded to the rows' type (q * s
+ * rounded once to f32, then to bf16); zeros for a row without a slot. */
+int llmcp_q8_kv_read(llmcp_q8_ctx *ctx, const llmcp_q8_kv_cache *cache,
+                     const llmcp_q8_kv_batch *batch, llmcp_memref_f32_3d *keys,
+                     llmcp_memref_f32_3d *values);
+int llmcp_q8_kv_read_bf16(llmcp_q8_ctx *ctx, const llmcp_q8_kv_cache *cache,
+                          const llmcp_q8_kv_batch *batch, llmcp_memref_bf16_3d *keys,
+                          llmcp_memref_bf16_3d *values);
+
+/* Attention of the rows over their sequences' keys (which the call's own rows
+ * are among: write them first): query head h of the row at position p gives
+ * sum over j <= p of softmax_j(scale * q . k_j) v_j with the keys and values of
+ * kv head h / (heads / kv_heads) that the slots stand for.  heads is a multiple
+ * of kv_heads, queries and output are [rows, heads, head_dim].  Positions
+ * without a slot are not seen, whatever their memory holds; a row that sees no key,
+ * or only scores of -inf, gives zeros.  Scores, softmax and sums are f32; of
+ * bf16 rows the probabilities (times a Q8 value's scale) are rounded to bf16
+ * before they meet the values, f32 rows take products exact to f32.
+ * Workspaces grow on the first call of a size: make it eagerly before
+ * capturing it into a graph.  How keys are split over workgroups, and with it the
+ * sums' order, depends on the numbers of rows, sequences, heads and pages of the
+ * call and on the sequence's own rows and length, not on what the other sequences
+ * hold. */
+int llmcp_q8_attention(llmcp_q8_ctx *ctx, const llmcp_memref_f32_3d *queries,
+                       const llmcp_q8_kv_cache *cache, const llmcp_q8_kv_batch *batch,
+                       float scale, llmcp_memref_f32_3d *output);
+int llmcp_q8_attention_bf16(llmcp_q8_ctx *ctx, const llmcp_memref_bf16_3d *queries,
+                            const llmcp_q8_kv_cache *cache, const llmcp_q8_kv_batch *batch,
+                            float scale, llmcp_memref_bf16_3d *output);
 
 /* llmcp.lm_head (LowerToLinalg.cpp:729-765): f32 logits [M,V] over the tied
  * table, plus the first-maximum index of the last row written to

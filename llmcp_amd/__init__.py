@@ -24,6 +24,7 @@ MODE = {"prefill": 0, "decode": 1}
 # computes: fma on aarch64 (SDOT emitters), mul+add on x86 (scalar path).
 PLATFORM = {"x86": 0, "aarch64": 1}
 ACCUM = {"exact": 0, "split_k": 1}
+CACHE_FORMAT = {"bf16": 0, "q8": 1}
 EPILOGUE = {"x86": "scalar", "aarch64": "fma"}
 
 _lib = None
@@ -100,6 +101,8 @@ EXPORTS = [
     "llmcp_q8_expert_linear", "llmcp_q8_expert_linear_bf16",
     "llmcp_q8_expert_mlp", "llmcp_q8_expert_mlp_bf16",
     "llmcp_q8_expert_mlp_rows", "llmcp_q8_expert_mlp_rows_bf16",
+    "llmcp_q8_kv_write", "llmcp_q8_kv_write_bf16", "llmcp_q8_kv_read", "llmcp_q8_kv_read_bf16",
+    "llmcp_q8_attention", "llmcp_q8_attention_bf16",
 ]
 
 
@@ -220,6 +223,9 @@ def lib():
         sig["llmcp_q8_expert_linear" + t] = (I, [P, P, P, I32, P, P, I32])
         sig["llmcp_q8_expert_mlp" + t] = (I, [P, P, P, P, I32, P, P, P, P, P])
         sig["llmcp_q8_expert_mlp_rows" + t] = (I, [P, P, P, P, I32, P, P, P, P, P])
+        sig["llmcp_q8_kv_write" + t] = (I, [P] * 5)
+        sig["llmcp_q8_kv_read" + t] = (I, [P] * 5)
+        sig["llmcp_q8_attention" + t] = (I, [P, P, P, P, ctypes.c_float, P])
     for name, (res, args) in sig.items():
         fn = getattr(L, name)
         fn.restype = res
@@ -309,6 +315,74 @@ class Q8Rows:
 
     def memref(self):
         return MemRefRows(_ptr(self.values), _ptr(self.scales), self.rows, self.cols)
+
+
+class MemRefHeads(ctypes.Structure):
+    """memref<?x?x?xf32> or bf16 (the same layout)."""
+    _fields_ = [("base", ctypes.c_void_p), ("data", ctypes.c_void_p),
+                ("offset", ctypes.c_int64), ("sizes", ctypes.c_int64 * 3),
+                ("strides", ctypes.c_int64 * 3)]
+
+
+def heads_memref(ptr, rows, heads, dim, row_stride=None):
+    """Rows of heads [rows, heads, dim], `row_stride` elements apart (None: dense)."""
+    d = MemRefHeads()
+    d.base = d.data = ptr
+    d.offset = 0
+    d.sizes[0], d.sizes[1], d.sizes[2] = rows, heads, dim
+    d.strides[0] = heads * dim if row_stride is None else row_stride
+    d.strides[1], d.strides[2] = dim, 1
+    return d
+
+
+class MemRefKVCache(ctypes.Structure):
+    """llmcp_q8_kv_cache."""
+    _fields_ = [("keys", ctypes.c_void_p), ("values", ctypes.c_void_p),
+                ("key_scales", ctypes.c_void_p), ("value_scales", ctypes.c_void_p),
+                ("pages", ctypes.c_int64), ("page_size", ctypes.c_int32),
+                ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("format", ctypes.c_int32)]
+
+
+class MemRefKVBatch(ctypes.Structure):
+    """llmcp_q8_kv_batch."""
+    _fields_ = [("row_starts", ctypes.c_void_p), ("lengths", ctypes.c_void_p),
+                ("page_table", ctypes.c_void_p), ("sequences", ctypes.c_int32),
+                ("max_pages", ctypes.c_int32)]
+
+
+class KVCache:
+    """Pages of keys and values in device memory, each [pages, kv_heads,
+    page_size, head_dim]: bf16, or int8 with f32 scales [pages, kv_heads,
+    page_size] where those are given."""
+
+    def __init__(self, keys, values, pages, page_size, kv_heads, head_dim, key_scales=None,
+                 value_scales=None):
+        self.keys, self.values = keys, values
+        self.key_scales, self.value_scales = key_scales, value_scales
+        self.pages, self.page_size = pages, page_size
+        self.kv_heads, self.head_dim = kv_heads, head_dim
+
+    def memref(self):
+        q8 = self.key_scales is not None
+        return MemRefKVCache(_ptr(self.keys), _ptr(self.values),
+                             _ptr(self.key_scales) if q8 else None,
+                             _ptr(self.value_scales) if q8 else None, self.pages, self.page_size,
+                             self.kv_heads, self.head_dim, CACHE_FORMAT["q8" if q8 else "bf16"])
+
+
+class KVBatch:
+    """The sequences of a call (int32, device memory): row_starts [sequences +
+    1], lengths [sequences] (keys, those of the call's rows among them) and
+    page_table [sequences, max_pages]."""
+
+    def __init__(self, row_starts, lengths, page_table, sequences, max_pages):
+        self.row_starts, self.lengths, self.page_table = row_starts, lengths, page_table
+        self.sequences, self.max_pages = sequences, max_pages
+
+    def memref(self):
+        return MemRefKVBatch(_ptr(self.row_starts), _ptr(self.lengths), _ptr(self.page_table),
+                             self.sequences, self.max_pages)
 
 
 def _ptr(buf):
@@ -634,6 +708,36 @@ class Context:
             _ptr(weights) if weights is not None else None, int(top_k),
             ctypes.byref(wg.memref()), ctypes.byref(wu.memref()), ctypes.byref(wd.memref()),
             ctypes.byref(ri) if ri is not None else None, ctypes.byref(yo)))
+
+    def kv_write(self, k, v, cache, batch, rows, strides=(None, None), dtype="f32"):
+        """Keys and values [rows, kv_heads, head_dim] (of dtype, `strides`
+        elements from row to row) into their slots of the cache (a KVCache)."""
+        ki, vi = (heads_memref(_ptr(b), rows, cache.kv_heads, cache.head_dim, st)
+                  for b, st in zip((k, v), strides))
+        check(self._entry("llmcp_q8_kv_write", dtype)(
+            self.handle, ctypes.byref(ki), ctypes.byref(vi), ctypes.byref(batch.memref()),
+            ctypes.byref(cache.memref())))
+
+    def kv_read(self, cache, batch, k, v, rows, strides=(None, None), dtype="f32"):
+        """The values that the rows' slots stand for into k and v [rows,
+        kv_heads, head_dim]."""
+        ko, vo = (heads_memref(_ptr(b), rows, cache.kv_heads, cache.head_dim, st)
+                  for b, st in zip((k, v), strides))
+        check(self._entry("llmcp_q8_kv_read", dtype)(
+            self.handle, ctypes.byref(cache.memref()), ctypes.byref(batch.memref()),
+            ctypes.byref(ko), ctypes.byref(vo)))
+
+    def attention(self, q, cache, batch, y, rows, heads, scale=None, strides=(None, None),
+                  dtype="f32"):
+        """y = attention of the queries q (both [rows, heads, head_dim]) over
+        their sequences' keys and values in the cache; scale None:
+        head_dim ** -0.5."""
+        qi, yo = (heads_memref(_ptr(b), rows, heads, cache.head_dim, st)
+                  for b, st in zip((q, y), strides))
+        check(self._entry("llmcp_q8_attention", dtype)(
+            self.handle, ctypes.byref(qi), ctypes.byref(cache.memref()),
+            ctypes.byref(batch.memref()),
+            float(cache.head_dim ** -0.5 if scale is None else scale), ctypes.byref(yo)))
 
     def swiglu(self, x, wg, wu, h, m, mode="decode", dtype="f32"):
         xi = f32_memref(x.ptr if hasattr(x, "ptr") else x, m, wg.cols)

@@ -221,6 +221,49 @@ hipError_t launch_add_rmsnorm(const void *x, int64_t ldx, const void *r, int64_t
                               void *s, int64_t lds, void *y, int64_t ldy, int8_t *q, float *qs,
                               hipStream_t stream);
 
+// ---- token mixers (q8_cache.hip, q8_attention.hip, q8_delta.hip)
+
+// Rows of heads: value d of head h of row r at data + r * row_ld + h * head_ld
+// + d (elements), every head 16 B aligned.
+struct HeadRows {
+  void *data = nullptr;
+  int64_t row_ld = 0, head_ld = 0;
+  bool bf16 = false;
+};
+
+// llmcp_q8_kv_cache and llmcp_q8_kv_batch, checked.
+struct KvPages {
+  void *k = nullptr, *v = nullptr;           // [pages, heads, page_size, dim]
+  float *ks = nullptr, *vs = nullptr;        // [pages, heads, page_size] (q8)
+  int32_t pages = 0, page_size = 0, heads = 0, dim = 0;
+  bool q8 = false;
+};
+struct KvBatch {
+  const int32_t *starts = nullptr, *lengths = nullptr, *table = nullptr;
+  int32_t sequences = 0, max_pages = 0;
+};
+constexpr int64_t kMaxMixerRows = 1 << 23;
+constexpr int32_t kMaxSequences = 65536, kMaxHeads = 1024, kMaxPageSize = 1 << 20;
+
+// Rows of keys and values to their slots, and back.
+hipError_t launch_kv_write(const HeadRows &k, const HeadRows &v, int64_t rows, const KvBatch &b,
+                           const KvPages &c, int32_t *err_flag, hipStream_t s);
+hipError_t launch_kv_read(const HeadRows &k, const HeadRows &v, int64_t rows, const KvBatch &b,
+                          const KvPages &c, int32_t *err_flag, hipStream_t s);
+
+// Attention of rows of `heads` query heads.  attention_plan chooses the
+// kernel and how many parts a sequence's keys are split into at most (rule and
+// measurements there), and gives the floats of workspace that takes.
+struct AttentionPlan {
+  int32_t tiles = 0;   // row tiles of all sequences, at most
+  int32_t splits = 1;  // parts of the keys, at most
+  int64_t part_floats = 0;
+};
+AttentionPlan attention_plan(int64_t rows, int32_t heads, const KvBatch &b, const KvPages &c);
+hipError_t launch_attention(const HeadRows &q, const HeadRows &o, int64_t rows, int32_t heads,
+                            const KvBatch &b, const KvPages &c, float scale, const AttentionPlan &plan,
+                            float *part, int32_t *err_flag, hipStream_t s);
+
 // ---- experts (q8_experts.hip)
 
 // p4 bytes (device) of a stack of experts [rows, cols] -> ExpertLayout.

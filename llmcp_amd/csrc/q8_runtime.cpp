@@ -127,6 +127,9 @@ struct llmcp_q8_ctx {
   float *expert_hs = nullptr;
   uint8_t *expert_out = nullptr;
   uint64_t plan_bytes = 0, expert_hq_bytes = 0, expert_hs_bytes = 0, expert_out_bytes = 0;
+  // Attention's parts of split keys, grown on demand.
+  float *attention_part = nullptr;
+  uint64_t attention_part_bytes = 0;
   // Cap on device bytes of registered weights (0: none).
   uint64_t weight_budget = 0;
   uint64_t weight_bytes = 0;
@@ -236,6 +239,30 @@ bool view_of(const M *d, bool bf16, Rows &r) {
   r.ld = d->sizes[0] <= 1 ? d->sizes[1] : d->strides[0];
   r.bf16 = bf16;
   return true;
+}
+
+// A [rows, heads, dim] view in device memory; every head 16 B aligned.
+struct Heads {
+  HeadRows h;
+  int64_t rows = 0, heads = 0, dim = 0;
+};
+
+template <class M>
+static bool heads_of(const M *d, bool bf16, Heads &r) {
+  if (!d || !d->data || d->sizes[0] < 0 || d->sizes[1] < 1 || d->sizes[2] < 1 ||
+      (d->sizes[2] > 1 && d->strides[2] != 1))
+    return false;
+  const int64_t per = bf16 ? 8 : 4;  // elements of 16 B
+  r.rows = d->sizes[0];
+  r.heads = d->sizes[1];
+  r.dim = d->sizes[2];
+  r.h.data = (void *)(d->data + d->offset);
+  r.h.bf16 = bf16;
+  r.h.head_ld = r.heads > 1 ? d->strides[1] : r.dim;
+  r.h.row_ld = r.rows > 1 ? d->strides[0] : 0;
+  if ((uintptr_t)r.h.data % 16 || r.h.head_ld < r.dim || (r.heads > 1 && r.h.head_ld % per)) return false;
+  // (a row ends with its last head)
+  return r.rows <= 1 || (r.h.row_ld % per == 0 && r.h.row_ld >= (r.heads - 1) * r.h.head_ld + r.dim);
 }
 
 // A norm's weight vector (dense 1-D memref of f32 or bf16).
@@ -673,6 +700,7 @@ int llmcp_q8_ctx_destroy(llmcp_q8_ctx *ctx) {
     if (ctx->expert_hq) (void)hipFree(ctx->expert_hq);
     if (ctx->expert_hs) (void)hipFree(ctx->expert_hs);
     if (ctx->expert_out) (void)hipFree(ctx->expert_out);
+    if (ctx->attention_part) (void)hipFree(ctx->attention_part);
     {
       std::lock_guard<std::mutex> lock(g_graph_mutex);
       for (auto it = g_graphs.begin(); it != g_graphs.end();) {
@@ -1953,6 +1981,106 @@ static int expert_mlp_impl(llmcp_q8_ctx *ctx, const ExpertRows &in, const int32_
   return LLMCP_Q8_OK;
 }
 
+// ---------------------------------------------------------- token mixers --
+
+static const char *kHeadsMsg = "rows of heads must be [rows, heads, dim] with dense, 16 B aligned heads";
+
+static int check_rows(const Heads &x) {
+  if (x.rows > kMaxMixerRows || x.heads > kMaxHeads)
+    return fail(LLMCP_Q8_DECLINED, "too many rows or heads for one launch (%lld of %lld)",
+                (long long)x.rows, (long long)x.heads);
+  return LLMCP_Q8_OK;
+}
+
+// The cache and batch of a call, checked.
+static int check_cache(const llmcp_q8_kv_cache *cache, const llmcp_q8_kv_batch *batch, KvPages &c,
+                       KvBatch &b) {
+  if (!cache || !batch || !cache->keys || !cache->values || !batch->row_starts || !batch->lengths ||
+      !batch->page_table)
+    return fail(LLMCP_Q8_EINVAL, "null cache, batch or one of their buffers");
+  if (cache->format != LLMCP_Q8_CACHE_BF16 && cache->format != LLMCP_Q8_CACHE_Q8)
+    return fail(LLMCP_Q8_EINVAL, "unknown cache format %d", cache->format);
+  const bool q8 = cache->format == LLMCP_Q8_CACHE_Q8;
+  if (q8 ? !cache->key_scales || !cache->value_scales : cache->key_scales || cache->value_scales)
+    return fail(LLMCP_Q8_EINVAL, "scales belong to a Q8 cache, and to it alone");
+  if (cache->head_dim != 64 && cache->head_dim != 128 && cache->head_dim != 256)
+    return fail(LLMCP_Q8_DECLINED, "head dim %d (64, 128 or 256)", cache->head_dim);
+  if (cache->kv_heads < 1 || cache->kv_heads > kMaxHeads || cache->page_size < 1 ||
+      cache->page_size > kMaxPageSize || cache->pages < 1 ||
+      cache->pages > 0x7FFFFFFFll / ((int64_t)cache->kv_heads * cache->page_size))
+    return fail(LLMCP_Q8_DECLINED, "a cache of %lld pages of %d slots of %d heads",
+                (long long)cache->pages, cache->page_size, cache->kv_heads);
+  if (batch->sequences < 1 || batch->sequences > kMaxSequences || batch->max_pages < 1 ||
+      (int64_t)batch->max_pages * cache->page_size > 0x7FFFFFFFll)
+    return fail(LLMCP_Q8_DECLINED, "%d sequences of up to %d pages", batch->sequences,
+                batch->max_pages);
+  if ((uintptr_t)cache->keys % 16 || (uintptr_t)cache->values % 16)
+    return fail(LLMCP_Q8_DECLINED, "a cache's keys and values must be 16 B aligned");
+  c.k = cache->keys;
+  c.v = cache->values;
+  c.ks = cache->key_scales;
+  c.vs = cache->value_scales;
+  c.pages = (int32_t)cache->pages;
+  c.page_size = cache->page_size;
+  c.heads = cache->kv_heads;
+  c.dim = cache->head_dim;
+  c.q8 = q8;
+  b.starts = batch->row_starts;
+  b.lengths = batch->lengths;
+  b.table = batch->page_table;
+  b.sequences = batch->sequences;
+  b.max_pages = batch->max_pages;
+  return LLMCP_Q8_OK;
+}
+
+static int kv_impl(llmcp_q8_ctx *ctx, const Heads &k, const Heads &v, const llmcp_q8_kv_batch *batch,
+                   const llmcp_q8_kv_cache *cache, bool write) {
+  KvPages c;
+  KvBatch b;
+  int rc = check_cache(cache, batch, c, b);
+  if (!rc) rc = check_rows(k);
+  if (rc) return rc;
+  if (k.rows != v.rows || k.heads != c.heads || v.heads != c.heads || k.dim != c.dim || v.dim != c.dim)
+    return fail(LLMCP_Q8_DECLINED, "keys and values must be [rows, %d, %d] like the cache", c.heads, c.dim);
+  if (!write && k.h.data == v.h.data && k.rows)
+    return fail(LLMCP_Q8_EINVAL, "keys and values must not share memory");
+  if (k.rows == 0) return LLMCP_Q8_OK;
+  if ((rc = set_device(ctx))) return rc;
+  hipError_t e = write ? launch_kv_write(k.h, v.h, k.rows, b, c, ctx->err_flag, ctx->stream)
+                       : launch_kv_read(k.h, v.h, k.rows, b, c, ctx->err_flag, ctx->stream);
+  if (e != hipSuccess) return hip_fail(e, "cache launch");
+  return LLMCP_Q8_OK;
+}
+
+static int attention_impl(llmcp_q8_ctx *ctx, const Heads &q, const llmcp_q8_kv_cache *cache,
+                          const llmcp_q8_kv_batch *batch, float scale, const Heads &out) {
+  KvPages c;
+  KvBatch b;
+  int rc = check_cache(cache, batch, c, b);
+  if (!rc) rc = check_rows(q);
+  if (rc) return rc;
+  if (q.dim != c.dim || q.heads % c.heads != 0)
+    return fail(LLMCP_Q8_DECLINED, "queries must be [rows, n * %d, %d] like the cache", c.heads, c.dim);
+  if (out.rows != q.rows || out.heads != q.heads || out.dim != q.dim)
+    return fail(LLMCP_Q8_DECLINED, "the output must be [rows, heads, dim] like the queries");
+  if (q.rows == 0) return LLMCP_Q8_OK;
+  if (q.h.data == out.h.data)
+    return fail(LLMCP_Q8_EINVAL, "attention's output must not take its queries' memory");
+  if (q.rows * q.heads > 1ll << 26)
+    return fail(LLMCP_Q8_DECLINED, "too many rows of heads for one launch (%lld)",
+                (long long)(q.rows * q.heads));
+  if ((rc = set_device(ctx))) return rc;
+  const AttentionPlan plan = attention_plan(q.rows, (int32_t)q.heads, b, c);
+  if (plan.part_floats &&
+      (rc = grow(ctx, ctx->attention_part, ctx->attention_part_bytes, (uint64_t)plan.part_floats * 4,
+                 "attention's parts")))
+    return rc;
+  hipError_t e = launch_attention(q.h, out.h, q.rows, (int32_t)q.heads, b, c, scale, plan,
+                                  ctx->attention_part, ctx->err_flag, ctx->stream);
+  if (e != hipSuccess) return hip_fail(e, "attention launch");
+  return LLMCP_Q8_OK;
+}
+
 static int lm_head_impl(llmcp_q8_ctx *ctx, const Rows &in,
                         const llmcp_memref_i8_1d *table, const Rows &logits,
                         int64_t *argmax_dev, int32_t execution_mode,
@@ -2485,6 +2613,74 @@ int llmcp_q8_expert_mlp_rows_bf16(llmcp_q8_ctx *ctx, const llmcp_q8_rows *input,
     in.cols = input->cols;
     return expert_mlp_impl(ctx, in, experts, weights, top_k, w_gate, w_up, w_down,
                            residual ? &r : nullptr, out);
+  });
+}
+
+int llmcp_q8_kv_write(llmcp_q8_ctx *ctx, const llmcp_memref_f32_3d *keys,
+                      const llmcp_memref_f32_3d *values, const llmcp_q8_kv_batch *batch,
+                      const llmcp_q8_kv_cache *cache) {
+  return guarded([&]() -> int {
+    if (!ctx) return fail(LLMCP_Q8_EINVAL, "null context");
+    Heads k, v;
+    if (!heads_of(keys, false, k) || !heads_of(values, false, v)) return fail(LLMCP_Q8_DECLINED, "%s", kHeadsMsg);
+    return kv_impl(ctx, k, v, batch, cache, true);
+  });
+}
+
+int llmcp_q8_kv_read(llmcp_q8_ctx *ctx, const llmcp_q8_kv_cache *cache,
+                     const llmcp_q8_kv_batch *batch, llmcp_memref_f32_3d *keys,
+                     llmcp_memref_f32_3d *values) {
+  return guarded([&]() -> int {
+    if (!ctx) return fail(LLMCP_Q8_EINVAL, "null context");
+    Heads k, v;
+    if (!heads_of(keys, false, k) || !heads_of(values, false, v)) return fail(LLMCP_Q8_DECLINED, "%s", kHeadsMsg);
+    return kv_impl(ctx, k, v, batch, cache, false);
+  });
+}
+
+int llmcp_q8_attention(llmcp_q8_ctx *ctx, const llmcp_memref_f32_3d *queries,
+                       const llmcp_q8_kv_cache *cache, const llmcp_q8_kv_batch *batch, float scale,
+                       llmcp_memref_f32_3d *output) {
+  return guarded([&]() -> int {
+    if (!ctx) return fail(LLMCP_Q8_EINVAL, "null context");
+    Heads q, o;
+    if (!heads_of(queries, false, q) || !heads_of(output, false, o))
+      return fail(LLMCP_Q8_DECLINED, "%s", kHeadsMsg);
+    return attention_impl(ctx, q, cache, batch, scale, o);
+  });
+}
+
+int llmcp_q8_kv_write_bf16(llmcp_q8_ctx *ctx, const llmcp_memref_bf16_3d *keys,
+                      const llmcp_memref_bf16_3d *values, const llmcp_q8_kv_batch *batch,
+                      const llmcp_q8_kv_cache *cache) {
+  return guarded([&]() -> int {
+    if (!ctx) return fail(LLMCP_Q8_EINVAL, "null context");
+    Heads k, v;
+    if (!heads_of(keys, true, k) || !heads_of(values, true, v)) return fail(LLMCP_Q8_DECLINED, "%s", kHeadsMsg);
+    return kv_impl(ctx, k, v, batch, cache, true);
+  });
+}
+
+int llmcp_q8_kv_read_bf16(llmcp_q8_ctx *ctx, const llmcp_q8_kv_cache *cache,
+                     const llmcp_q8_kv_batch *batch, llmcp_memref_bf16_3d *keys,
+                     llmcp_memref_bf16_3d *values) {
+  return guarded([&]() -> int {
+    if (!ctx) return fail(LLMCP_Q8_EINVAL, "null context");
+    Heads k, v;
+    if (!heads_of(keys, true, k) || !heads_of(values, true, v)) return fail(LLMCP_Q8_DECLINED, "%s", kHeadsMsg);
+    return kv_impl(ctx, k, v, batch, cache, false);
+  });
+}
+
+int llmcp_q8_attention_bf16(llmcp_q8_ctx *ctx, const llmcp_memref_bf16_3d *queries,
+                       const llmcp_q8_kv_cache *cache, const llmcp_q8_kv_batch *batch, float scale,
+                       llmcp_memref_bf16_3d *output) {
+  return guarded([&]() -> int {
+    if (!ctx) return fail(LLMCP_Q8_EINVAL, "null context");
+    Heads q, o;
+    if (!heads_of(queries, true, q) || !heads_of(output, true, o))
+      return fail(LLMCP_Q8_DECLINED, "%s", kHeadsMsg);
+    return attention_impl(ctx, q, cache, batch, scale, o);
   });
 }
 
