@@ -663,6 +663,34 @@ int llmcp_q8_attention_bf16(llmcp_q8_ctx *ctx, const llmcp_memref_bf16_3d *queri
                             const llmcp_q8_kv_cache *cache, const llmcp_q8_kv_batch *batch,
                             float scale, llmcp_memref_bf16_3d *output);
 
+/* The gated delta rule of the linear-attention layers, over the rows of each
+ * sequence in order: with a = exp(log_decay) and beta of the row and value
+ * head (f32 [rows, value_heads], rows dense or further apart), k and q of key head h / (value_heads /
+ * key_heads) and the state S [key_dim, value_dim] of value head h,
+ *   u = beta * (v - a * S^T k),  S <- a * S + k u^T,  output = scale * S^T q,
+ * k and q over sqrt(their sum of squares + eps) when normalize, else as they
+ * are.  queries and keys [rows, key_heads, key_dim], key_dim 64 or 128; values and
+ * output [rows, value_heads, value_dim], value_dim a multiple of 16 up to 1024,
+ * value_heads a multiple of key_heads, sequences * value_heads * value_dim up to
+ * 2^26; declined otherwise.  row_starts [sequences + 1] in device
+ * memory as for the cache's entries (null: one sequence of all rows).  state and
+ * new_state [sequences, value_heads, key_dim, value_dim] f32, dense, 16 B
+ * aligned: where each sequence starts (null: from zeros) and what its rows
+ * leave, which may be the same memory; a sequence without rows keeps its state.
+ * States and sums are f32, products of f32 precision. */
+int llmcp_q8_delta_rule(llmcp_q8_ctx *ctx, const llmcp_memref_f32_3d *queries,
+                        const llmcp_memref_f32_3d *keys, const llmcp_memref_f32_3d *values,
+                        const llmcp_memref_f32_2d *log_decay, const llmcp_memref_f32_2d *beta,
+                        float scale, int32_t normalize, float eps, const int32_t *row_starts,
+                        int32_t sequences, const float *state, float *new_state,
+                        llmcp_memref_f32_3d *output);
+int llmcp_q8_delta_rule_bf16(llmcp_q8_ctx *ctx, const llmcp_memref_bf16_3d *queries,
+                             const llmcp_memref_bf16_3d *keys, const llmcp_memref_bf16_3d *values,
+                             const llmcp_memref_f32_2d *log_decay, const llmcp_memref_f32_2d *beta,
+                             float scale, int32_t normalize, float eps, const int32_t *row_starts,
+                             int32_t sequences, const float *state, float *new_state,
+                             llmcp_memref_bf16_3d *output);
+
 /* llmcp.lm_head (LowerToLinalg.cpp:729-765): f32 logits [M,V] over the tied
  * table, plus the first-maximum index of the last row written to
  * `argmax_dev` (device int64, nullable) -- the host std::max_element of

@@ -103,6 +103,7 @@ EXPORTS = [
     "llmcp_q8_expert_mlp_rows", "llmcp_q8_expert_mlp_rows_bf16",
     "llmcp_q8_kv_write", "llmcp_q8_kv_write_bf16", "llmcp_q8_kv_read", "llmcp_q8_kv_read_bf16",
     "llmcp_q8_attention", "llmcp_q8_attention_bf16",
+    "llmcp_q8_delta_rule", "llmcp_q8_delta_rule_bf16",
 ]
 
 
@@ -226,6 +227,8 @@ def lib():
         sig["llmcp_q8_kv_write" + t] = (I, [P] * 5)
         sig["llmcp_q8_kv_read" + t] = (I, [P] * 5)
         sig["llmcp_q8_attention" + t] = (I, [P, P, P, P, ctypes.c_float, P])
+        sig["llmcp_q8_delta_rule" + t] = (I, [P, P, P, P, P, P, ctypes.c_float, I32,
+                                              ctypes.c_float, P, I32, P, P, P])
     for name, (res, args) in sig.items():
         fn = getattr(L, name)
         fn.restype = res
@@ -738,6 +741,26 @@ class Context:
             self.handle, ctypes.byref(qi), ctypes.byref(cache.memref()),
             ctypes.byref(batch.memref()),
             float(cache.head_dim ** -0.5 if scale is None else scale), ctypes.byref(yo)))
+
+    def delta_rule(self, q, k, v, log_decay, beta, y, rows, key_heads, value_heads, key_dim,
+                   value_dim, state=None, new_state=None, row_starts=None, sequences=1,
+                   scale=None, eps=1e-6, strides=(None, None, None), dtype="f32"):
+        """y [rows, value_heads, value_dim] of the gated delta rule over q, k
+        [rows, key_heads, key_dim] and v (of dtype, `strides` elements from row to
+        row), log_decay and beta f32 [rows, value_heads], from state (None:
+        zeros) to new_state, f32 [sequences, value_heads, key_dim, value_dim].
+        eps None: q and k as they are; scale None: key_dim ** -0.5."""
+        qi, ki = (heads_memref(_ptr(b), rows, key_heads, key_dim, st)
+                  for b, st in zip((q, k), strides))
+        vi = heads_memref(_ptr(v), rows, value_heads, value_dim, strides[2])
+        yo = heads_memref(_ptr(y), rows, value_heads, value_dim)
+        di, bi = (f32_memref(_ptr(b), rows, value_heads) for b in (log_decay, beta))
+        check(self._entry("llmcp_q8_delta_rule", dtype)(
+            self.handle, ctypes.byref(qi), ctypes.byref(ki), ctypes.byref(vi), ctypes.byref(di),
+            ctypes.byref(bi), float(key_dim ** -0.5 if scale is None else scale),
+            0 if eps is None else 1, 0.0 if eps is None else float(eps),
+            _ptr(row_starts) if row_starts is not None else None, int(sequences),
+            _ptr(state) if state is not None else None, _ptr(new_state), ctypes.byref(yo)))
 
     def swiglu(self, x, wg, wu, h, m, mode="decode", dtype="f32"):
         xi = f32_memref(x.ptr if hasattr(x, "ptr") else x, m, wg.cols)

@@ -15,7 +15,7 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 SOURCES = ["q8_kernels.hip", "q8_gemv_fma.hip", "q8_gemm.hip", "q8_gemm16.hip",
            "q8_experts.hip", "q8_add_rmsnorm.hip", "q8_cache.hip",
-           "q8_attention.hip", "q8_microbench.hip",
+           "q8_attention.hip", "q8_delta.hip", "q8_microbench.hip",
            "q8_runtime.cpp"]
 
 ROOT = os.path.dirname(HERE)

@@ -264,6 +264,23 @@ hipError_t launch_attention(const HeadRows &q, const HeadRows &o, int64_t rows, 
                             const KvBatch &b, const KvPages &c, float scale, const AttentionPlan &plan,
                             float *part, int32_t *err_flag, hipStream_t s);
 
+// The gated delta rule.
+struct DeltaLaunch {
+  HeadRows q, k, v, o;             // key_heads of key_dim; heads of value_dim
+  const float *decay = nullptr, *beta = nullptr;  // [rows, heads]
+  int64_t decay_ld = 0, beta_ld = 0;
+  int64_t rows = 0;
+  int32_t key_heads = 0, heads = 0, key_dim = 0, value_dim = 0;
+  float scale = 1.0f, eps = 0.0f;
+  bool normalize = false;
+  const int32_t *starts = nullptr; // null: one sequence
+  int32_t sequences = 1;
+  const float *state = nullptr;    // null: zeros
+  float *new_state = nullptr;
+};
+constexpr int32_t kMaxValueDim = 1024;
+hipError_t launch_delta(const DeltaLaunch &l, hipStream_t s);
+
 // ---- experts (q8_experts.hip)
 
 // p4 bytes (device) of a stack of experts [rows, cols] -> ExpertLayout.

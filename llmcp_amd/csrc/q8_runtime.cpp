@@ -241,6 +241,8 @@ bool view_of(const M *d, bool bf16, Rows &r) {
   return true;
 }
 
+const char *kHeadsMsg = "rows of heads must be [rows, heads, dim] with dense, 16 B aligned heads";
+
 // A [rows, heads, dim] view in device memory; every head 16 B aligned.
 struct Heads {
   HeadRows h;
@@ -263,6 +265,54 @@ static bool heads_of(const M *d, bool bf16, Heads &r) {
   if ((uintptr_t)r.h.data % 16 || r.h.head_ld < r.dim || (r.heads > 1 && r.h.head_ld % per)) return false;
   // (a row ends with its last head)
   return r.rows <= 1 || (r.h.row_ld % per == 0 && r.h.row_ld >= (r.heads - 1) * r.h.head_ld + r.dim);
+}
+
+int check_rows(const Heads &x) {
+  if (x.rows > kMaxMixerRows || x.heads > kMaxHeads)
+    return fail(LLMCP_Q8_DECLINED, "too many rows or heads for one launch (%lld of %lld)",
+                (long long)x.rows, (long long)x.heads);
+  return LLMCP_Q8_OK;
+}
+
+// The cache and batch of a call, checked.
+int check_cache(const llmcp_q8_kv_cache *cache, const llmcp_q8_kv_batch *batch, KvPages &c,
+                       KvBatch &b) {
+  if (!cache || !batch || !cache->keys || !cache->values || !batch->row_starts || !batch->lengths ||
+      !batch->page_table)
+    return fail(LLMCP_Q8_EINVAL, "null cache, batch or one of their buffers");
+  if (cache->format != LLMCP_Q8_CACHE_BF16 && cache->format != LLMCP_Q8_CACHE_Q8)
+    return fail(LLMCP_Q8_EINVAL, "unknown cache format %d", cache->format);
+  const bool q8 = cache->format == LLMCP_Q8_CACHE_Q8;
+  if (q8 ? !cache->key_scales || !cache->value_scales : cache->key_scales || cache->value_scales)
+    return fail(LLMCP_Q8_EINVAL, "scales belong to a Q8 cache, and to it alone");
+  if (cache->head_dim != 64 && cache->head_dim != 128 && cache->head_dim != 256)
+    return fail(LLMCP_Q8_DECLINED, "head dim %d (64, 128 or 256)", cache->head_dim);
+  if (cache->kv_heads < 1 || cache->kv_heads > kMaxHeads || cache->page_size < 1 ||
+      cache->page_size > kMaxPageSize || cache->pages < 1 ||
+      cache->pages > 0x7FFFFFFFll / ((int64_t)cache->kv_heads * cache->page_size))
+    return fail(LLMCP_Q8_DECLINED, "a cache of %lld pages of %d slots of %d heads",
+                (long long)cache->pages, cache->page_size, cache->kv_heads);
+  if (batch->sequences < 1 || batch->sequences > kMaxSequences || batch->max_pages < 1 ||
+      (int64_t)batch->max_pages * cache->page_size > 0x7FFFFFFFll)
+    return fail(LLMCP_Q8_DECLINED, "%d sequences of up to %d pages", batch->sequences,
+                batch->max_pages);
+  if ((uintptr_t)cache->keys % 16 || (uintptr_t)cache->values % 16)
+    return fail(LLMCP_Q8_DECLINED, "a cache's keys and values must be 16 B aligned");
+  c.k = cache->keys;
+  c.v = cache->values;
+  c.ks = cache->key_scales;
+  c.vs = cache->value_scales;
+  c.pages = (int32_t)cache->pages;
+  c.page_size = cache->page_size;
+  c.heads = cache->kv_heads;
+  c.dim = cache->head_dim;
+  c.q8 = q8;
+  b.starts = batch->row_starts;
+  b.lengths = batch->lengths;
+  b.table = batch->page_table;
+  b.sequences = batch->sequences;
+  b.max_pages = batch->max_pages;
+  return LLMCP_Q8_OK;
 }
 
 // A norm's weight vector (dense 1-D memref of f32 or bf16).
@@ -845,6 +895,28 @@ int32_t llmcp_q8_test_expert_ranges(int64_t slots, int64_t experts, int64_t rows
 // reference): whether a stack of experts of this shape would be registered.
 int llmcp_q8_test_expert_stack(int64_t experts, int64_t rows, int64_t cols) {
   return check_stack(experts, rows, cols);
+}
+
+// Test hook, declared in no header of the product (no counterpart in the
+// reference): what the cache's entries answer to this cache and batch before they
+// touch the device.
+int llmcp_q8_test_kv_check(const llmcp_q8_kv_cache *cache, const llmcp_q8_kv_batch *batch) {
+  return guarded([&]() -> int {
+    KvPages c;
+    KvBatch b;
+    return check_cache(cache, batch, c, b);
+  });
+}
+
+// Test hook, likewise: whether these are rows of heads that the mixers take.
+int llmcp_q8_test_heads(const void *rows, int32_t bf16) {
+  return guarded([&]() -> int {
+    Heads h;
+    if (!(bf16 ? heads_of((const llmcp_memref_bf16_3d *)rows, true, h)
+               : heads_of((const llmcp_memref_f32_3d *)rows, false, h)))
+      return fail(LLMCP_Q8_DECLINED, "%s", kHeadsMsg);
+    return check_rows(h);
+  });
 }
 
 int32_t llmcp_q8_get_platform(llmcp_q8_ctx *ctx) {
@@ -1983,56 +2055,6 @@ static int expert_mlp_impl(llmcp_q8_ctx *ctx, const ExpertRows &in, const int32_
 
 // ---------------------------------------------------------- token mixers --
 
-static const char *kHeadsMsg = "rows of heads must be [rows, heads, dim] with dense, 16 B aligned heads";
-
-static int check_rows(const Heads &x) {
-  if (x.rows > kMaxMixerRows || x.heads > kMaxHeads)
-    return fail(LLMCP_Q8_DECLINED, "too many rows or heads for one launch (%lld of %lld)",
-                (long long)x.rows, (long long)x.heads);
-  return LLMCP_Q8_OK;
-}
-
-// The cache and batch of a call, checked.
-static int check_cache(const llmcp_q8_kv_cache *cache, const llmcp_q8_kv_batch *batch, KvPages &c,
-                       KvBatch &b) {
-  if (!cache || !batch || !cache->keys || !cache->values || !batch->row_starts || !batch->lengths ||
-      !batch->page_table)
-    return fail(LLMCP_Q8_EINVAL, "null cache, batch or one of their buffers");
-  if (cache->format != LLMCP_Q8_CACHE_BF16 && cache->format != LLMCP_Q8_CACHE_Q8)
-    return fail(LLMCP_Q8_EINVAL, "unknown cache format %d", cache->format);
-  const bool q8 = cache->format == LLMCP_Q8_CACHE_Q8;
-  if (q8 ? !cache->key_scales || !cache->value_scales : cache->key_scales || cache->value_scales)
-    return fail(LLMCP_Q8_EINVAL, "scales belong to a Q8 cache, and to it alone");
-  if (cache->head_dim != 64 && cache->head_dim != 128 && cache->head_dim != 256)
-    return fail(LLMCP_Q8_DECLINED, "head dim %d (64, 128 or 256)", cache->head_dim);
-  if (cache->kv_heads < 1 || cache->kv_heads > kMaxHeads || cache->page_size < 1 ||
-      cache->page_size > kMaxPageSize || cache->pages < 1 ||
-      cache->pages > 0x7FFFFFFFll / ((int64_t)cache->kv_heads * cache->page_size))
-    return fail(LLMCP_Q8_DECLINED, "a cache of %lld pages of %d slots of %d heads",
-                (long long)cache->pages, cache->page_size, cache->kv_heads);
-  if (batch->sequences < 1 || batch->sequences > kMaxSequences || batch->max_pages < 1 ||
-      (int64_t)batch->max_pages * cache->page_size > 0x7FFFFFFFll)
-    return fail(LLMCP_Q8_DECLINED, "%d sequences of up to %d pages", batch->sequences,
-                batch->max_pages);
-  if ((uintptr_t)cache->keys % 16 || (uintptr_t)cache->values % 16)
-    return fail(LLMCP_Q8_DECLINED, "a cache's keys and values must be 16 B aligned");
-  c.k = cache->keys;
-  c.v = cache->values;
-  c.ks = cache->key_scales;
-  c.vs = cache->value_scales;
-  c.pages = (int32_t)cache->pages;
-  c.page_size = cache->page_size;
-  c.heads = cache->kv_heads;
-  c.dim = cache->head_dim;
-  c.q8 = q8;
-  b.starts = batch->row_starts;
-  b.lengths = batch->lengths;
-  b.table = batch->page_table;
-  b.sequences = batch->sequences;
-  b.max_pages = batch->max_pages;
-  return LLMCP_Q8_OK;
-}
-
 static int kv_impl(llmcp_q8_ctx *ctx, const Heads &k, const Heads &v, const llmcp_q8_kv_batch *batch,
                    const llmcp_q8_kv_cache *cache, bool write) {
   KvPages c;
@@ -2078,6 +2100,61 @@ static int attention_impl(llmcp_q8_ctx *ctx, const Heads &q, const llmcp_q8_kv_c
   hipError_t e = launch_attention(q.h, out.h, q.rows, (int32_t)q.heads, b, c, scale, plan,
                                   ctx->attention_part, ctx->err_flag, ctx->stream);
   if (e != hipSuccess) return hip_fail(e, "attention launch");
+  return LLMCP_Q8_OK;
+}
+
+static int delta_impl(llmcp_q8_ctx *ctx, const Heads &q, const Heads &k, const Heads &v,
+                      const Rows &decay, const Rows &beta, float scale, int32_t normalize, float eps,
+                      const int32_t *row_starts, int32_t sequences, const float *state,
+                      float *new_state, const Heads &out) {
+  if (!new_state) return fail(LLMCP_Q8_EINVAL, "null state");
+  int rc = check_rows(q);
+  if (!rc) rc = check_rows(v);
+  if (rc) return rc;
+  if (k.rows != q.rows || k.heads != q.heads || k.dim != q.dim || v.rows != q.rows)
+    return fail(LLMCP_Q8_DECLINED, "queries and keys must be [rows, key heads, key dim], values have their rows");
+  if (q.dim != 64 && q.dim != 128)
+    return fail(LLMCP_Q8_DECLINED, "key dim %lld (64 or 128)", (long long)q.dim);
+  if (v.dim % 16 || v.dim > kMaxValueDim || v.heads % q.heads)
+    return fail(LLMCP_Q8_DECLINED, "values [%lld, %lld] for %lld key heads", (long long)v.heads,
+                (long long)v.dim, (long long)q.heads);
+  if (out.rows != v.rows || out.heads != v.heads || out.dim != v.dim)
+    return fail(LLMCP_Q8_DECLINED, "the output must be [rows, value heads, value dim] like the values");
+  if (decay.rows != v.rows || decay.cols != v.heads || beta.rows != v.rows || beta.cols != v.heads)
+    return fail(LLMCP_Q8_DECLINED, "log decay and beta must be [rows, value heads]");
+  if (sequences < 1 || sequences > kMaxSequences || (!row_starts && sequences != 1))
+    return fail(LLMCP_Q8_DECLINED, "%d sequences (up to %d; without row starts one)", sequences, kMaxSequences);
+  if (sequences * v.heads * v.dim > 1ll << 26)
+    return fail(LLMCP_Q8_DECLINED, "too many states for one launch (%d of %lld x %lld columns)",
+                sequences, (long long)v.heads, (long long)v.dim);
+  if ((uintptr_t)state % 16 || (uintptr_t)new_state % 16)
+    return fail(LLMCP_Q8_DECLINED, "states must be 16 B aligned");
+  if (v.rows && (out.h.data == q.h.data || out.h.data == k.h.data || out.h.data == v.h.data))
+    return fail(LLMCP_Q8_EINVAL, "the delta rule's output must not take its inputs' memory");
+  if ((rc = set_device(ctx))) return rc;
+  DeltaLaunch l;
+  l.q = q.h;
+  l.k = k.h;
+  l.v = v.h;
+  l.o = out.h;
+  l.decay = (const float *)decay.data;
+  l.beta = (const float *)beta.data;
+  l.decay_ld = decay.ld;
+  l.beta_ld = beta.ld;
+  l.rows = q.rows;
+  l.key_heads = (int32_t)q.heads;
+  l.heads = (int32_t)v.heads;
+  l.key_dim = (int32_t)q.dim;
+  l.value_dim = (int32_t)v.dim;
+  l.scale = scale;
+  l.eps = eps;
+  l.normalize = normalize != 0;
+  l.starts = row_starts;
+  l.sequences = sequences;
+  l.state = state;
+  l.new_state = new_state;
+  hipError_t e = launch_delta(l, ctx->stream);
+  if (e != hipSuccess) return hip_fail(e, "delta rule launch");
   return LLMCP_Q8_OK;
 }
 
@@ -2681,6 +2758,46 @@ int llmcp_q8_attention_bf16(llmcp_q8_ctx *ctx, const llmcp_memref_bf16_3d *queri
     if (!heads_of(queries, true, q) || !heads_of(output, true, o))
       return fail(LLMCP_Q8_DECLINED, "%s", kHeadsMsg);
     return attention_impl(ctx, q, cache, batch, scale, o);
+  });
+}
+
+int llmcp_q8_delta_rule(llmcp_q8_ctx *ctx, const llmcp_memref_f32_3d *queries,
+                        const llmcp_memref_f32_3d *keys, const llmcp_memref_f32_3d *values,
+                        const llmcp_memref_f32_2d *log_decay, const llmcp_memref_f32_2d *beta,
+                        float scale, int32_t normalize, float eps, const int32_t *row_starts,
+                        int32_t sequences, const float *state, float *new_state,
+                        llmcp_memref_f32_3d *output) {
+  return guarded([&]() -> int {
+    if (!ctx) return fail(LLMCP_Q8_EINVAL, "null context");
+    Heads q, k, v, o;
+    if (!heads_of(queries, false, q) || !heads_of(keys, false, k) || !heads_of(values, false, v) ||
+        !heads_of(output, false, o))
+      return fail(LLMCP_Q8_DECLINED, "%s", kHeadsMsg);
+    Rows d, w;
+    if (!view_of(log_decay, false, d) || !view_of(beta, false, w))
+      return fail(LLMCP_Q8_DECLINED, kDenseMsg);
+    return delta_impl(ctx, q, k, v, d, w, scale, normalize, eps, row_starts, sequences, state,
+                      new_state, o);
+  });
+}
+
+int llmcp_q8_delta_rule_bf16(llmcp_q8_ctx *ctx, const llmcp_memref_bf16_3d *queries,
+                        const llmcp_memref_bf16_3d *keys, const llmcp_memref_bf16_3d *values,
+                        const llmcp_memref_f32_2d *log_decay, const llmcp_memref_f32_2d *beta,
+                        float scale, int32_t normalize, float eps, const int32_t *row_starts,
+                        int32_t sequences, const float *state, float *new_state,
+                        llmcp_memref_bf16_3d *output) {
+  return guarded([&]() -> int {
+    if (!ctx) return fail(LLMCP_Q8_EINVAL, "null context");
+    Heads q, k, v, o;
+    if (!heads_of(queries, true, q) || !heads_of(keys, true, k) || !heads_of(values, true, v) ||
+        !heads_of(output, true, o))
+      return fail(LLMCP_Q8_DECLINED, "%s", kHeadsMsg);
+    Rows d, w;
+    if (!view_of(log_decay, false, d) || !view_of(beta, false, w))
+      return fail(LLMCP_Q8_DECLINED, kDenseMsg);
+    return delta_impl(ctx, q, k, v, d, w, scale, normalize, eps, row_starts, sequences, state,
+                      new_state, o);
   });
 }
 
