@@ -1,6 +1,24 @@
 // q8_delta.hip -- the gated delta rule: per value head a state S [key_dim,
 // value_dim], and per row of a sequence
 //   u = beta (v - a S^T k),  S = a S + k u^T,  o = scale S^T q,  a = exp(g).
+//
+// Few rows go one after another (delta_rows_kernel). Many bf16 rows go in chunks
+// of 64: with G the running sum of g in the chunk, S0 the state before it, and
+//   L_ij = beta_i exp(G_i - G_j) k_i . k_j  (j < i),      T = (I + L)^-1,
+//   A_ij = exp(G_i - G_j) q_i . k_j         (j <= i),
+// the chunk's u, outputs and state are
+//   U = T diag(beta) (V - diag(exp G) K S0),
+//   O = diag(exp G) Q S0 + A U,
+//   S = exp(G_63) S0 + K^T diag(exp(G_63 - G)) U.
+// T and A do not depend on the state: delta_chunk_kernel makes them for all
+// chunks side by side. delta_scan_kernel then walks a sequence's chunks with
+// 16 columns of a head's state per workgroup.
+//
+// States and sums are f32 on bf16 matrix instructions: rows of q and k are
+// exact in bf16 (their norms, the scale and the decays multiply f32 results),
+// and an f32 factor goes in as parts of 8 bits: three of S0 towards U and of U
+// towards the state (exact products), two of what only reaches a bf16 output. T
+// meets V - K S0 in f32 matrix instructions.
 #include <algorithm>
 
 #include "q8_gemv.h"
@@ -154,6 +172,618 @@ hipError_t launch_delta_rows(const DeltaLaunch &l, hipStream_t s) {
   return hipGetLastError();
 }
 
+// ------------------------------------------------------------- chunks --
+
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef short v8s __attribute__((ext_vector_type(8)));
+
+constexpr int kChunk = 64;
+
+// What a chunk of a head leaves for the scan, each block in the order in which
+// a wave's lanes take it as an operand.
+struct ChunkData {
+  v4f t[10][64];        // T diag(beta): block (w, t <= w) at w (w + 1) / 2 + t
+  v4u a[6][2][64];      // A in two parts: 16 rows w by 32 columns s <= w / 2
+  float k_in[kChunk];   // exp(G_i) over |k_i|
+  float q_in[kChunk];   // exp(G_i) scale over |q_i|
+  float k_out[kChunk];  // exp(G_63 - G_i) over |k_i|
+  float decay;          // exp(G_63)
+  int32_t odd;          // an infinity or NaN among q, k, decay or beta
+  float pad[62];
+};
+static_assert(sizeof(ChunkData) % 256 == 0, "aligned");
+__device__ constexpr int a_block(int w, int s) { return (w / 2) * 2 + (w % 2) + (w / 2) * s + (w / 2 ? (w % 2) : 0); }
+static_assert(a_block(0, 0) == 0 && a_block(1, 0) == 1 && a_block(2, 0) == 2 && a_block(2, 1) == 3 &&
+              a_block(3, 0) == 4 && a_block(3, 1) == 5, "blocks of A");
+
+struct ChunkArgs {
+  DeltaLaunch l;
+  ChunkData *data;     // [chunks of the window][heads]
+  int32_t first, count; // the window's chunks
+  int32_t slices;
+};
+
+// A chunk of the call: its sequence, the chunk's number there and its rows.
+struct Chunk {
+  int32_t seq = -1, index = 0, row = 0, live = 0;
+};
+
+// Chunk number c, sequences in order, each in whole chunks.
+__device__ __forceinline__ Chunk find_chunk(const DeltaLaunch &l, int32_t c, int lane) {
+  Chunk r;
+  int32_t sum = 0;
+  for (int32_t at = 0; at < l.sequences; at += 64) {
+    RowRange range = {0, 0};
+    if (at + lane < l.sequences) range = delta_range(l, at + lane);
+    int32_t incl = (range.hi - range.lo + kChunk - 1) / kChunk;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int32_t o = __shfl_up(incl, d);
+      if (lane >= d) incl += o;
+    }
+    const int n = __popcll(__builtin_amdgcn_ballot_w64(sum + incl <= c));
+    if (n < 64) {
+      r.seq = at + n;
+      r.index = c - (n ? sum + __builtin_amdgcn_readlane(incl, n - 1) : sum);
+      r.row = __builtin_amdgcn_readlane(range.lo, n) + r.index * kChunk;
+      r.live = min(kChunk, __builtin_amdgcn_readlane(range.hi, n) - r.row);
+      break;
+    }
+    sum += __builtin_amdgcn_readlane(incl, 63);
+  }
+  return r;
+}
+
+// Chunks of the sequences before s.
+__device__ __forceinline__ int32_t chunks_before(const DeltaLaunch &l, int32_t s, int lane) {
+  int32_t sum = 0;
+  for (int32_t at = 0; at < s; at += 64) {
+    if (at + lane < s) {
+      const RowRange range = delta_range(l, at + lane);
+      sum += (range.hi - range.lo + kChunk - 1) / kChunk;
+    }
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
+  return __builtin_amdgcn_readfirstlane(sum);
+}
+
+__device__ __forceinline__ float low_half(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float high_half(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+// The upper halves of two words: their leading 8 bits as bf16.
+__device__ __forceinline__ uint32_t upper2(float lo, float hi) {
+  return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+}
+__device__ __forceinline__ float below(float x) { return x - high_half(__float_as_uint(x)); }
+
+// Four values as PARTS bf16 parts of 8 bits each.
+template <int PARTS>
+__device__ __forceinline__ void split4(v4f x, v2u (&part)[PARTS]) {
+#pragma unroll
+  for (int n = 0; n < PARTS; ++n) {
+    part[n] = v2u{upper2(x[0], x[1]), upper2(x[2], x[3])};
+    if (n + 1 < PARTS) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = below(x[i]);
+    }
+  }
+}
+
+__device__ __forceinline__ v8bf join(v2u a, v2u b) {
+  return __builtin_bit_cast(v8bf, v4u{a[0], a[1], b[0], b[1]});
+}
+
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) < __builtin_inff(); }
+
+// T and A of a chunk and head. The products K K^T and Q K^T are exact products
+// in f32 sums; wave w has rows 16 w .. 16 w + 15 of both. The inverse goes
+// by 16 x 16 blocks: those on the diagonal by substitution, a column per lane,
+// then wave j has column j of the blocks below, T_ij = -T_ii sum L_ik T_kj, a
+// result's registers being the next product's operand.
+template <int KD>
+__global__ __launch_bounds__(256) void delta_chunk_kernel(const ChunkArgs p) {
+  constexpr int KS = KD / 32, LD = 68;
+  __shared__ __align__(16) v4u kt[4][KS][64];
+  __shared__ __align__(16) float lm[kChunk][LD], am[kChunk][LD], tm[kChunk][LD];
+  __shared__ double run[kChunk];
+  __shared__ float kn[kChunk], qn[kChunk], bt[kChunk];
+  __shared__ int odd;
+  const DeltaLaunch &l = p.l;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
+  const int32_t c = blockIdx.x / l.heads, head = blockIdx.x - c * l.heads;
+  const int32_t key_head = head / (l.heads / l.key_heads);
+  const Chunk ch = find_chunk(l, p.first + c, lane);
+  if (ch.seq < 0) return;
+  if (threadIdx.x == 0) odd = 0;
+  __syncthreads();
+  const int my = 16 * wave + col;
+  v8bf kr[KS], qr[KS];
+  {
+    const bool live = my < ch.live;
+    const int64_t row = ch.row + (live ? my : 0);
+    float kk = 0, qq = 0;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      v4u a = *(const v4u *)((const uint16_t *)l.k.data + row * l.k.row_ld + key_head * l.k.head_ld + 32 * s + 8 * g);
+      v4u b = *(const v4u *)((const uint16_t *)l.q.data + row * l.q.row_ld + key_head * l.q.head_ld + 32 * s + 8 * g);
+      if (!live) a = v4u{0, 0, 0, 0}, b = a;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        kk = __builtin_fmaf(low_half(a[i]), low_half(a[i]), kk);
+        kk = __builtin_fmaf(high_half(a[i]), high_half(a[i]), kk);
+        qq = __builtin_fmaf(low_half(b[i]), low_half(b[i]), qq);
+        qq = __builtin_fmaf(high_half(b[i]), high_half(b[i]), qq);
+      }
+      kt[wave][s][lane] = a;
+      kr[s] = __builtin_bit_cast(v8bf, a);
+      qr[s] = __builtin_bit_cast(v8bf, b);
+    }
+    kk += __shfl_xor(kk, 16);
+    qq += __shfl_xor(qq, 16);
+    kk += __shfl_xor(kk, 32);
+    qq += __shfl_xor(qq, 32);
+    float k1 = 1.0f, q1 = l.scale;
+    if (l.normalize) {
+      k1 = 1.0f / sqrtf(kk + l.eps);
+      q1 = l.scale * (1.0f / sqrtf(qq + l.eps));
+    }
+    if (!live) k1 = 0.0f, q1 = 0.0f;
+    if (g == 0) {
+      kn[my] = k1;
+      qn[my] = q1;
+      if (!finite(kk) || !finite(qq) || !finite(k1) || !finite(q1)) odd = 1;
+    }
+  }
+  if (wave == 0) {
+    const bool live = lane < ch.live;
+    const int64_t row = ch.row + (live ? lane : 0);
+    float d = live ? l.decay[row * l.decay_ld + head] : 0.0f;
+    const float b = live ? l.beta[row * l.beta_ld + head] : 0.0f;
+    // what decays below e^-10000 is nothing; the sum stays finite
+    if (d < -1e4f) d = -1e4f;
+    if (!finite(d) || !finite(b)) odd = 1;
+    double sum = (double)d;
+#pragma unroll
+    for (int n = 1; n < 64; n *= 2) {
+      const double o = __shfl_up(sum, n);
+      if (lane >= n) sum += o;
+    }
+    run[lane] = sum;
+    bt[lane] = b;
+  }
+  __syncthreads();
+  // rows 16 wave + 4 g + i by columns 16 t + col
+  double gi[4];
+  float bi[4], ki[4], qi[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = 16 * wave + 4 * g + i;
+    gi[i] = run[r];
+    ki[i] = kn[r];
+    qi[i] = qn[r];
+    bi[i] = bt[r] * ki[i];
+  }
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    if (t > wave) continue;
+    v4f kk = v4f{0, 0, 0, 0}, qk = kk;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const v8bf b = __builtin_bit_cast(v8bf, kt[t][s][lane]);
+      kk = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kr[s], b, kk, 0, 0, 0);
+      qk = __builtin_amdgcn_mfma_f32_16x16x32_bf16(qr[s], b, qk, 0, 0, 0);
+    }
+    const int j = 16 * t + col;
+    const double gj = run[j];
+    const float kj = kn[j];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 16 * wave + 4 * g + i;
+      const float e = j <= r ? expf((float)(gi[i] - gj)) : 0.0f;
+      lm[r][j] = j < r ? (bi[i] * kj) * (e * kk[i]) : 0.0f;
+      am[r][j] = j <= r ? (qi[i] * kj) * (e * qk[i]) : 0.0f;
+    }
+  }
+  __syncthreads();
+  {
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float v = i == col ? 1.0f : 0.0f;
+#pragma unroll
+      for (int k = 0; k < i; ++k) v = __builtin_fmaf(-lm[16 * wave + i][16 * wave + k], x[k], v);
+      x[i] = v;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if ((i >> 2) == g) tm[16 * wave + i][my] = x[i];
+  }
+  __syncthreads();
+  if (wave < 3) {
+    v4f tc[4];  // column `wave` of T's blocks: rows 4 g + i, column col
+#pragma unroll
+    for (int i = 0; i < 4; ++i) tc[0][i] = tm[16 * wave + 4 * g + i][my];
+#pragma unroll
+    for (int d = 1; d < 4; ++d) {
+      const int bi_ = wave + d;
+      if (bi_ > 3) continue;
+      v4f sum = v4f{0, 0, 0, 0}, out = sum;
+#pragma unroll
+      for (int k = 0; k < d; ++k) {
+        const v4f a = *(const v4f *)&lm[16 * bi_ + col][16 * (wave + k) + 4 * g];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], tc[k][i], sum, 0, 0, 0);
+      }
+      const v4f a = *(const v4f *)&tm[16 * bi_ + col][16 * bi_ + 4 * g];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) out = __builtin_amdgcn_mfma_f32_16x16x4f32(-a[i], sum[i], out, 0, 0, 0);
+      tc[d] = out;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) tm[16 * bi_ + 4 * g + i][my] = out[i];
+    }
+  }
+  __syncthreads();
+  ChunkData &to = p.data[(int64_t)c * l.heads + head];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    if (t > wave) continue;
+    v4f x = *(const v4f *)&tm[my][16 * t + 4 * g];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] *= bt[16 * t + 4 * g + i];
+    to.t[wave * (wave + 1) / 2 + t][lane] = x;
+  }
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    if (s > wave / 2) continue;
+    v2u part[2][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      v4f x = v4f{0, 0, 0, 0};
+      if (2 * s + h <= wave) x = *(const v4f *)&am[my][16 * (2 * s + h) + 4 * g];
+      split4<2>(x, part[h]);
+    }
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+      to.a[a_block(wave, s)][n][lane] = v4u{part[0][n][0], part[0][n][1], part[1][n][0], part[1][n][1]};
+  }
+  if (wave == 0) {
+    const double last = run[kChunk - 1];
+    const float e = expf((float)run[lane]);
+    to.k_in[lane] = e * kn[lane];
+    to.q_in[lane] = e * qn[lane];
+    to.k_out[lane] = expf((float)(last - run[lane])) * kn[lane];
+    if (lane == 0) {
+      to.decay = expf((float)last);
+      to.odd = odd;
+    }
+  }
+}
+
+// What a wave holds of a chunk before it is needed.
+template <int KD>
+struct ScanLoads {
+  static constexpr int KS = KD / 32;
+  v2u q[KS][2];        // row 16 w + col: values 32 s + 16 h + 4 g ..
+  v4u k[KD / 32];      // 16 B of K's rows for LDS
+  v4f t[4];
+  v4u a[2][2];
+  float v[4], k_in[4], q_in[4], k_out[4];
+  float decay;
+  int32_t odd;
+};
+
+template <int KD>
+__device__ __forceinline__ void scan_load(const ChunkArgs &p, const ChunkData &d, int32_t row,
+                                          int32_t live, int32_t head, int32_t key_head, int32_t column,
+                                          int wave, int lane, ScanLoads<KD> &x) {
+  const DeltaLaunch &l = p.l;
+  const int col = lane & 15, g = lane >> 4;
+  {
+    const int my = 16 * wave + col;
+    const uint16_t *const q = (const uint16_t *)l.q.data + (int64_t)(row + min(my, live - 1)) * l.q.row_ld + key_head * l.q.head_ld;
+#pragma unroll
+    for (int s = 0; s < KD / 32; ++s) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) x.q[s][h] = *(const v2u *)(q + 32 * s + 16 * h + 4 * g);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < KD / 32; ++i) {
+    constexpr int PER = KD / 8;  // threads a row
+    const int n = i * 256 + threadIdx.x, r = n / PER, c = n % PER;
+    x.k[i] = *(const v4u *)((const uint16_t *)l.k.data + (int64_t)(row + min(r, live - 1)) * l.k.row_ld +
+                            key_head * l.k.head_ld + 8 * c);
+    if (r >= live) x.k[i] = v4u{0, 0, 0, 0};
+  }
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+    if (t <= wave) x.t[t] = d.t[wave * (wave + 1) / 2 + t][lane];
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    if (s <= wave / 2) {
+#pragma unroll
+      for (int n = 0; n < 2; ++n) x.a[s][n] = d.a[a_block(wave, s)][n][lane];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = 16 * wave + 4 * g + i;
+    const uint16_t b = ((const uint16_t *)l.v.data)[(int64_t)(row + min(r, live - 1)) * l.v.row_ld +
+                                                    head * l.v.head_ld + column];
+    x.v[i] = r < live ? bf16_to_float(b) : 0.0f;
+    x.k_in[i] = d.k_in[r];
+    x.q_in[i] = d.q_in[r];
+    x.k_out[i] = d.k_out[r];
+  }
+  x.decay = d.decay;
+  x.odd = d.odd;
+}
+
+// A sequence's chunks of the window, 16 columns of a head's state per
+// workgroup. Wave w has rows 16 w .. of the chunk and, of the state, tiles
+// of 16 key dims; between the waves everything passes through LDS in the order
+// of the lanes, since a result's registers (rows 4 g + i, column col) are a lane's
+// part of the next product's operand when the summed index is taken in that
+// order.
+template <int KD>
+__global__ __launch_bounds__(256) void delta_scan_kernel(const ChunkArgs p) {
+  constexpr int KS = KD / 32, TILES = KD / 16, TW = TILES / 4;
+  __shared__ __align__(16) uint8_t kl[2][kChunk * KD * 2];
+  __shared__ __align__(16) v2u sp[3][TILES][64], up[2][4][64], uo[3][4][64];
+  __shared__ __align__(16) v4f bl[4][64];
+  __shared__ float red[2][4][2][16];
+  __shared__ float red3[2][4][3];
+  __shared__ int odd_v[2][16];  // columns with an infinity or NaN among the chunk's values
+  const DeltaLaunch &l = p.l;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
+  const int32_t slice = blockIdx.x % p.slices, sh = blockIdx.x / p.slices;
+  const int32_t seq = sh / l.heads, head = sh - seq * l.heads;
+  const int32_t key_head = head / (l.heads / l.key_heads);
+  const int32_t column = slice * 16 + col;
+  const RowRange range = delta_range(l, seq);
+  const int32_t chunks = (range.hi - range.lo + kChunk - 1) / kChunk;
+  const int32_t base = chunks_before(l, seq, lane) - p.first;  // the first chunk's place in the window
+  const int32_t from = max(0, -base), to = min(chunks, p.count - base);
+  // (a sequence without rows hands its state on in the first window)
+  if (from >= to && !(chunks == 0 && p.first == 0 && l.state != l.new_state)) return;
+  const int64_t at = (int64_t)sh * KD * l.value_dim + column;
+  const float *const before = from > 0 ? l.new_state : l.state;
+  v4f state[TW];
+#pragma unroll
+  for (int t = 0; t < TW; ++t) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      state[t][i] = before ? before[at + (int64_t)(16 * (TW * wave + t) + 4 * g + i) * l.value_dim] : 0.0f;
+  }
+  ScanLoads<KD> now;
+  auto place = [](int r, int c) { return r * KD * 2 + ((c ^ ((r & 7) << 1 | (r >> 3 & 1))) & (KD / 8 - 1)) * 16; };
+  auto keep_k = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < KD / 32; ++i) {
+      constexpr int PER = KD / 8;
+      const int n = i * 256 + threadIdx.x;
+      *(v4u *)(kl[buf] + place(n / PER, n % PER)) = now.k[i];
+    }
+  };
+  auto keep_state = [&]() {
+#pragma unroll
+    for (int t = 0; t < TW; ++t) {
+      v2u part[3];
+      split4<3>(state[t], part);
+#pragma unroll
+      for (int n = 0; n < 3; ++n) sp[n][TW * wave + t][lane] = part[n];
+    }
+  };
+  if (threadIdx.x < 32) odd_v[threadIdx.x / 16][threadIdx.x % 16] = 0;
+  __syncthreads();
+  if (from < to) {
+    scan_load<KD>(p, p.data[(int64_t)(base + from) * l.heads + head], range.lo + from * kChunk,
+                  min(kChunk, range.hi - range.lo - from * kChunk), head, key_head, column, wave, lane, now);
+    keep_k(from & 1);
+  }
+  keep_state();
+  for (int32_t n = from; n < to; ++n) {
+    const int32_t row = range.lo + n * kChunk, live = min(kChunk, range.hi - row);
+    const int buf = n & 1;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bad |= !finite(now.v[i]);
+    if (bad) odd_v[buf][col] = 1;
+    __syncthreads();  // the state's parts, K's rows and the vote are there
+    // An infinity or NaN would reach rows before its own, by 0 times it: its
+    // column (every column, if it is not in the values) goes row by row below.
+    const bool mine_odd = now.odd || odd_v[buf][col];
+    const bool slow = __builtin_amdgcn_ballot_w64(mine_odd) != 0;
+    if (threadIdx.x < 16) odd_v[buf ^ 1][threadIdx.x] = 0;  // (read before this barrier, set after the next)
+    v4f old[TW];
+#pragma unroll
+    for (int t = 0; t < TW; ++t) old[t] = state[t];
+    ScanLoads<KD> next = now;
+    if (n + 1 < to)
+      scan_load<KD>(p, p.data[(int64_t)(base + n + 1) * l.heads + head], row + kChunk,
+                    min(kChunk, range.hi - row - kChunk), head, key_head, column, wave, lane, next);
+    if (!now.odd) {
+      // K S0 and Q S0
+      v4f ks[3], qs[2];
+#pragma unroll
+      for (int i = 0; i < 3; ++i) ks[i] = v4f{0, 0, 0, 0};
+      qs[0] = qs[1] = ks[0];
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        v2u kh[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          kh[h] = *(const v2u *)(kl[buf] + place(16 * wave + col, 4 * s + 2 * h + (g >> 1)) + (g & 1) * 8);
+        const v8bf a = join(kh[0], kh[1]), b = join(now.q[s][0], now.q[s][1]);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+          const v8bf x = join(sp[i][2 * s][lane], sp[i][2 * s + 1][lane]);
+          ks[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, x, ks[i], 0, 0, 0);
+          if (i < 2) qs[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, x, qs[i], 0, 0, 0);
+        }
+      }
+      {
+        v4f x = (ks[2] + ks[1]) + ks[0];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = __builtin_fmaf(-now.k_in[i], x[i], now.v[i]);
+        bl[wave][lane] = x;
+      }
+      __syncthreads();
+      // U
+      v4f u = v4f{0, 0, 0, 0}, u2 = u;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        if (t > wave) continue;
+        const v4f b = bl[t][lane];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (i % 2 == 0) u = __builtin_amdgcn_mfma_f32_16x16x4f32(now.t[t][i], b[i], u, 0, 0, 0);
+          else u2 = __builtin_amdgcn_mfma_f32_16x16x4f32(now.t[t][i], b[i], u2, 0, 0, 0);
+        }
+      }
+      u = u + u2;
+      {
+        v2u part[2], out[3];
+        split4<2>(u, part);
+        v4f x = u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] *= now.k_out[i];
+        split4<3>(x, out);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) up[i][wave][lane] = part[i];
+#pragma unroll
+        for (int i = 0; i < 3; ++i) uo[i][wave][lane] = out[i];
+      }
+      __syncthreads();
+      // the state after the chunk
+#pragma unroll
+      for (int t = 0; t < TW; ++t) {
+        v4f sum[3];
+#pragma unroll
+        for (int i = 0; i < 3; ++i) sum[i] = v4f{0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          v4s half[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int r = 16 * (2 * s + h) + 4 * g + (col >> 2);
+            half[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) v4s *)(kl[buf] + place(r, 2 * (TW * wave + t) + (col >> 1 & 1)) + (col & 1) * 8));
+          }
+          const v8s both = __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7);
+          const v8bf a = __builtin_bit_cast(v8bf, both);
+#pragma unroll
+          for (int i = 0; i < 3; ++i)
+            sum[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, join(uo[i][2 * s][lane], uo[i][2 * s + 1][lane]), sum[i], 0, 0, 0);
+        }
+        const v4f x = (sum[2] + sum[1]) + sum[0];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) state[t][i] = __builtin_fmaf(now.decay, state[t][i], x[i]);
+      }
+      // the outputs
+      v4f o = v4f{0, 0, 0, 0}, o2 = o;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        if (s > wave / 2) continue;
+        const v8bf u0 = join(up[0][2 * s][lane], up[0][2 * s + 1][lane]);
+        const v8bf u1 = join(up[1][2 * s][lane], up[1][2 * s + 1][lane]);
+        const v8bf a0 = __builtin_bit_cast(v8bf, now.a[s][0]), a1 = __builtin_bit_cast(v8bf, now.a[s][1]);
+        o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a0, u0, o, 0, 0, 0);
+        o2 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a0, u1, o2, 0, 0, 0);
+        o2 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a1, u0, o2, 0, 0, 0);
+      }
+      o = o + o2;
+      const v4f q0 = qs[0] + qs[1];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = 16 * wave + 4 * g + i;
+        if (r < live && !mine_odd)
+          ((uint16_t *)l.o.data)[(int64_t)(row + r) * l.o.row_ld + head * l.o.head_ld + column] =
+              float_to_bf16(__builtin_fmaf(now.q_in[i], q0[i], o[i]));
+      }
+    }
+    if (slow) {
+      for (int32_t r = 0; r < live; ++r) {
+        const int64_t rr = row + r;
+        const uint16_t *const kp = (const uint16_t *)l.k.data + rr * l.k.row_ld + key_head * l.k.head_ld;
+        const uint16_t *const qp = (const uint16_t *)l.q.data + rr * l.q.row_ld + key_head * l.q.head_ld;
+        float k[TW][4], pk = 0, pq = 0, kk = 0, qq = 0, kq = 0;
+#pragma unroll
+        for (int t = 0; t < TW; ++t) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int d = 16 * (TW * wave + t) + 4 * g + i;
+            const float q = bf16_to_float(qp[d]);
+            k[t][i] = bf16_to_float(kp[d]);
+            pk = __builtin_fmaf(old[t][i], k[t][i], pk);
+            pq = __builtin_fmaf(old[t][i], q, pq);
+            kk = __builtin_fmaf(k[t][i], k[t][i], kk);
+            qq = __builtin_fmaf(q, q, qq);
+            kq = __builtin_fmaf(k[t][i], q, kq);
+          }
+        }
+#pragma unroll
+        for (int d = 16; d < 64; d *= 2) {
+          pk += __shfl_xor(pk, d);
+          pq += __shfl_xor(pq, d);
+          kk += __shfl_xor(kk, d);
+          qq += __shfl_xor(qq, d);
+          kq += __shfl_xor(kq, d);
+        }
+        const int b = r & 1;
+        if (g == 0) {
+          red[b][wave][0][col] = pk;
+          red[b][wave][1][col] = pq;
+        }
+        if (lane == 0) {
+          red3[b][wave][0] = kk;
+          red3[b][wave][1] = qq;
+          red3[b][wave][2] = kq;
+        }
+        __syncthreads();
+        pk = pq = kk = qq = kq = 0;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          pk += red[b][w][0][col];
+          pq += red[b][w][1][col];
+          kk += red3[b][w][0];
+          qq += red3[b][w][1];
+          kq += red3[b][w][2];
+        }
+        const float rk = l.normalize ? 1.0f / sqrtf(kk + l.eps) : 1.0f;
+        const float rq = l.scale * (l.normalize ? 1.0f / sqrtf(qq + l.eps) : 1.0f);
+        const float a = expf(l.decay[rr * l.decay_ld + head]), beta = l.beta[rr * l.beta_ld + head];
+        const float v = bf16_to_float(((const uint16_t *)l.v.data)[rr * l.v.row_ld + head * l.v.head_ld + column]);
+        const float u = (v - pk * (a * rk)) * beta;
+        const float o = pq * (a * rq) + u * (kq * rk * rq);
+#pragma unroll
+        for (int t = 0; t < TW; ++t) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) old[t][i] = __builtin_fmaf(k[t][i] * rk, u, a * old[t][i]);
+        }
+        if (wave == 0 && g == 0 && mine_odd)
+          ((uint16_t *)l.o.data)[rr * l.o.row_ld + head * l.o.head_ld + column] = float_to_bf16(o);
+      }
+#pragma unroll
+      for (int t = 0; t < TW; ++t) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) state[t][i] = mine_odd ? old[t][i] : state[t][i];
+      }
+    }
+    now = next;
+    keep_state();
+    if (n + 1 < to) keep_k(buf ^ 1);
+  }
+#pragma unroll
+  for (int t = 0; t < TW; ++t) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      l.new_state[at + (int64_t)(16 * (TW * wave + t) + 4 * g + i) * l.value_dim] = state[t][i];
+  }
+}
+
 template <bool BF16, int KD>
 hipError_t launch_delta_k(const DeltaLaunch &l, hipStream_t s) {
   if (l.value_dim % 32 || (int64_t)l.sequences * l.heads * l.value_dim < 256 * 32)
@@ -161,9 +791,51 @@ hipError_t launch_delta_k(const DeltaLaunch &l, hipStream_t s) {
   return launch_delta_rows<BF16, KD, 32>(l, s);
 }
 
+// Chunks of all sequences, at most, and those of one window: what the
+// workspace holds at a time (up to 192 MiB, a chunk of all heads at least).
+int64_t delta_chunks(const DeltaLaunch &l) {
+  return l.rows / kChunk + std::min<int64_t>(l.sequences, l.rows);
+}
+int64_t delta_window(const DeltaLaunch &l) {
+  const int64_t fit = (192ll << 20) / ((int64_t)sizeof(ChunkData) * l.heads);
+  return std::max<int64_t>(1, std::min(delta_chunks(l), fit));
+}
+
+template <int KD>
+hipError_t launch_delta_chunks(const DeltaLaunch &l, void *workspace, hipStream_t s) {
+  const int64_t total = delta_chunks(l), window = delta_window(l);
+  ChunkArgs a = {l, (ChunkData *)workspace, 0, 0, l.value_dim / 16};
+  const int64_t scan = (int64_t)l.sequences * l.heads * a.slices;
+  if (window * l.heads > 0x7FFFFF || scan > 0x7FFFFF) return hipErrorInvalidConfiguration;
+  for (int64_t first = 0; first < total; first += window) {
+    a.first = (int32_t)first;
+    a.count = (int32_t)std::min(window, total - first);
+    hipLaunchKernelGGL((delta_chunk_kernel<KD>), dim3((unsigned)(a.count * l.heads)), dim3(256), 0, s, a);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((delta_scan_kernel<KD>), dim3((unsigned)scan), dim3(256), 0, s, a);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
 }  // namespace
 
-hipError_t launch_delta(const DeltaLaunch &l, hipStream_t s) {
+bool delta_chunked(const DeltaLaunch &l) {
+  return l.q.bf16 && l.rows >= 16 * (int64_t)l.sequences;
+}
+
+int64_t delta_workspace(const DeltaLaunch &l) {
+  return delta_chunked(l) ? delta_window(l) * l.heads * (int64_t)sizeof(ChunkData) : 0;
+}
+
+hipError_t launch_delta(const DeltaLaunch &l, void *workspace, hipStream_t s) {
+  if (delta_chunked(l)) {
+    if (!workspace) return hipErrorInvalidConfiguration;
+    return l.key_dim == 128 ? launch_delta_chunks<128>(l, workspace, s)
+           : l.key_dim == 64 ? launch_delta_chunks<64>(l, workspace, s)
+                             : hipErrorInvalidConfiguration;
+  }
   if (l.key_dim == 128) return l.q.bf16 ? launch_delta_k<true, 128>(l, s) : launch_delta_k<false, 128>(l, s);
   if (l.key_dim == 64) return l.q.bf16 ? launch_delta_k<true, 64>(l, s) : launch_delta_k<false, 64>(l, s);
   return hipErrorInvalidConfiguration;

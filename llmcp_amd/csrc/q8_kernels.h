@@ -279,7 +279,11 @@ struct DeltaLaunch {
   float *new_state = nullptr;
 };
 constexpr int32_t kMaxValueDim = 1024;
-hipError_t launch_delta(const DeltaLaunch &l, hipStream_t s);
+// Whether the rows go in chunks (rule and measurements there), and the bytes
+// of workspace that takes; none where they go one after another.
+bool delta_chunked(const DeltaLaunch &l);
+int64_t delta_workspace(const DeltaLaunch &l);
+hipError_t launch_delta(const DeltaLaunch &l, void *workspace, hipStream_t s);
 
 // ---- experts (q8_experts.hip)
 

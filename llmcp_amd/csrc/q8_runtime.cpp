@@ -130,6 +130,9 @@ struct llmcp_q8_ctx {
   // Attention's parts of split keys, grown on demand.
   float *attention_part = nullptr;
   uint64_t attention_part_bytes = 0;
+  // What the delta rule's chunks hold, grown on demand.
+  uint8_t *delta_work = nullptr;
+  uint64_t delta_work_bytes = 0;
   // Cap on device bytes of registered weights (0: none).
   uint64_t weight_budget = 0;
   uint64_t weight_bytes = 0;
@@ -751,6 +754,7 @@ int llmcp_q8_ctx_destroy(llmcp_q8_ctx *ctx) {
     if (ctx->expert_hs) (void)hipFree(ctx->expert_hs);
     if (ctx->expert_out) (void)hipFree(ctx->expert_out);
     if (ctx->attention_part) (void)hipFree(ctx->attention_part);
+    if (ctx->delta_work) (void)hipFree(ctx->delta_work);
     {
       std::lock_guard<std::mutex> lock(g_graph_mutex);
       for (auto it = g_graphs.begin(); it != g_graphs.end();) {
@@ -2153,7 +2157,10 @@ static int delta_impl(llmcp_q8_ctx *ctx, const Heads &q, const Heads &k, const H
   l.sequences = sequences;
   l.state = state;
   l.new_state = new_state;
-  hipError_t e = launch_delta(l, ctx->stream);
+  if ((rc = grow(ctx, ctx->delta_work, ctx->delta_work_bytes, (uint64_t)delta_workspace(l),
+                 "delta rule's chunks")))
+    return rc;
+  hipError_t e = launch_delta(l, ctx->delta_work, ctx->stream);
   if (e != hipSuccess) return hip_fail(e, "delta rule launch");
   return LLMCP_Q8_OK;
 }
