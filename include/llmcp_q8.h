@@ -672,7 +672,7 @@ int llmcp_q8_attention_bf16(llmcp_q8_ctx *ctx, const llmcp_memref_bf16_3d *queri
  * are.  queries and keys [rows, key_heads, key_dim], key_dim 64 or 128; values and
  * output [rows, value_heads, value_dim], value_dim a multiple of 16 up to 1024,
  * value_heads a multiple of key_heads, sequences * value_heads * value_dim up to
- * 2^26; declined otherwise.  row_starts [sequences + 1] in device
+ * 2^26, rows less than 2^22 values apart; declined otherwise.  row_starts [sequences + 1] in device
  * memory as for the cache's entries (null: one sequence of all rows).  state and
  * new_state [sequences, value_heads, key_dim, value_dim] f32, dense, 16 B
  * aligned: where each sequence starts (null: from zeros) and what its rows

@@ -189,9 +189,8 @@ struct ChunkData {
   float k_in[kChunk];   // exp(G_i) over |k_i|
   float q_in[kChunk];   // exp(G_i) scale over |q_i|
   float k_out[kChunk];  // exp(G_63 - G_i) over |k_i|
-  float decay;          // exp(G_63)
-  int32_t odd;          // an infinity or NaN among q, k, decay or beta
-  float pad[62];
+  float decay[64];      // exp(G_63), for every lane
+  int32_t odd[64];      // whether an infinity or NaN is among q, k, decay or beta
 };
 static_assert(sizeof(ChunkData) % 256 == 0, "aligned");
 __device__ constexpr int a_block(int w, int s) { return (w / 2) * 2 + (w % 2) + (w / 2) * s + (w / 2 ? (w % 2) : 0); }
@@ -454,71 +453,17 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(const ChunkArgs p) {
     to.k_in[lane] = e * kn[lane];
     to.q_in[lane] = e * qn[lane];
     to.k_out[lane] = expf((float)(last - run[lane])) * kn[lane];
-    if (lane == 0) {
-      to.decay = expf((float)last);
-      to.odd = odd;
-    }
+    to.decay[lane] = expf((float)last);
+    to.odd[lane] = odd;
   }
 }
 
-// What a wave holds of a chunk before it is needed.
-template <int KD>
-struct ScanLoads {
-  static constexpr int KS = KD / 32;
-  v2u q[KS][2];        // row 16 w + col: values 32 s + 16 h + 4 g ..
-  v4u k[KD / 32];      // 16 B of K's rows for LDS
-  v4f t[4];
-  v4u a[2][2];
-  float v[4], k_in[4], q_in[4], k_out[4];
-  float decay;
-  int32_t odd;
-};
-
-template <int KD>
-__device__ __forceinline__ void scan_load(const ChunkArgs &p, const ChunkData &d, int32_t row,
-                                          int32_t live, int32_t head, int32_t key_head, int32_t column,
-                                          int wave, int lane, ScanLoads<KD> &x) {
-  const DeltaLaunch &l = p.l;
-  const int col = lane & 15, g = lane >> 4;
-  {
-    const int my = 16 * wave + col;
-    const uint16_t *const q = (const uint16_t *)l.q.data + (int64_t)(row + min(my, live - 1)) * l.q.row_ld + key_head * l.q.head_ld;
-#pragma unroll
-    for (int s = 0; s < KD / 32; ++s) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) x.q[s][h] = *(const v2u *)(q + 32 * s + 16 * h + 4 * g);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < KD / 32; ++i) {
-    constexpr int PER = KD / 8;  // threads a row
-    const int n = i * 256 + threadIdx.x, r = n / PER, c = n % PER;
-    x.k[i] = *(const v4u *)((const uint16_t *)l.k.data + (int64_t)(row + min(r, live - 1)) * l.k.row_ld +
-                            key_head * l.k.head_ld + 8 * c);
-    if (r >= live) x.k[i] = v4u{0, 0, 0, 0};
-  }
-#pragma unroll
-  for (int t = 0; t < 4; ++t)
-    if (t <= wave) x.t[t] = d.t[wave * (wave + 1) / 2 + t][lane];
-#pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    if (s <= wave / 2) {
-#pragma unroll
-      for (int n = 0; n < 2; ++n) x.a[s][n] = d.a[a_block(wave, s)][n][lane];
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = 16 * wave + 4 * g + i;
-    const uint16_t b = ((const uint16_t *)l.v.data)[(int64_t)(row + min(r, live - 1)) * l.v.row_ld +
-                                                    head * l.v.head_ld + column];
-    x.v[i] = r < live ? bf16_to_float(b) : 0.0f;
-    x.k_in[i] = d.k_in[r];
-    x.q_in[i] = d.q_in[r];
-    x.k_out[i] = d.k_out[r];
-  }
-  x.decay = d.decay;
-  x.odd = d.odd;
+// Blocks of a sequence in an order in which consecutive ones are on one XCD (the
+// hardware deals them out over 8), so that a head's slices share its operands in
+// one L2.
+__device__ __forceinline__ int32_t on_one_xcd(int32_t block, int32_t blocks) {
+  const int32_t x = block % 8, each = blocks / 8, rest = blocks % 8;
+  return x * each + min(x, rest) + block / 8;
 }
 
 // A sequence's chunks of the window, 16 columns of a head's state per
@@ -526,7 +471,9 @@ __device__ __forceinline__ void scan_load(const ChunkArgs &p, const ChunkData &d
 // of 16 key dims; between the waves everything passes through LDS in the order
 // of the lanes, since a result's registers (rows 4 g + i, column col) are a lane's
 // part of the next product's operand when the summed index is taken in that
-// order.
+// order. What a phase takes from memory is asked for a phase or two ahead, as it
+// comes (a conversion or a row's mask there would wait for it; rows past the
+// chunk's last repeat that one); what it takes from LDS, together.
 template <int KD>
 __global__ __launch_bounds__(256) void delta_scan_kernel(const ChunkArgs p) {
   constexpr int KS = KD / 32, TILES = KD / 16, TW = TILES / 4;
@@ -537,9 +484,11 @@ __global__ __launch_bounds__(256) void delta_scan_kernel(const ChunkArgs p) {
   __shared__ float red3[2][4][3];
   __shared__ int odd_v[2][16];  // columns with an infinity or NaN among the chunk's values
   const DeltaLaunch &l = p.l;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
-  const int32_t slice = blockIdx.x % p.slices, sh = blockIdx.x / p.slices;
-  const int32_t seq = sh / l.heads, head = sh - seq * l.heads;
+  const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int32_t seq = blockIdx.x / (l.heads * p.slices);
+  const int32_t block = on_one_xcd(blockIdx.x - seq * (l.heads * p.slices), l.heads * p.slices);
+  const int32_t head = block / p.slices, slice = block - head * p.slices, sh = seq * l.heads + head;
   const int32_t key_head = head / (l.heads / l.key_heads);
   const int32_t column = slice * 16 + col;
   const RowRange range = delta_range(l, seq);
@@ -557,14 +506,77 @@ __global__ __launch_bounds__(256) void delta_scan_kernel(const ChunkArgs p) {
     for (int i = 0; i < 4; ++i)
       state[t][i] = before ? before[at + (int64_t)(16 * (TW * wave + t) + 4 * g + i) * l.value_dim] : 0.0f;
   }
-  ScanLoads<KD> now;
+  auto rows_of = [&](int32_t n) { return min(kChunk, range.hi - range.lo - n * kChunk); };
+  auto data_of = [&](int32_t n) -> const ChunkData & { return p.data[(int64_t)(base + n) * l.heads + head]; };
   auto place = [](int r, int c) { return r * KD * 2 + ((c ^ ((r & 7) << 1 | (r >> 3 & 1))) & (KD / 8 - 1)) * 16; };
-  auto keep_k = [&](int buf) {
+  // Places in a chunk are 32-bit lane offsets from the chunk's first row (rows
+  // are less than 2^22 values apart).
+  const uint32_t q_ld = 2 * (uint32_t)l.q.row_ld, k_ld = 2 * (uint32_t)l.k.row_ld,
+                 v_ld = 2 * (uint32_t)l.v.row_ld, o_ld = 2 * (uint32_t)l.o.row_ld;
+  auto row_at = [&](const HeadRows &x, int32_t n, int32_t h) {
+    return (uint8_t *)x.data + 2 * ((int64_t)(range.lo + n * kChunk) * x.row_ld + (int64_t)h * x.head_ld);
+  };
+  // rows 16 w + col of q (values 32 s + 16 h + 4 g ..), rows 16 w + 4 g + i of v
+  v2u q[KS][2];
+  uint16_t vb[4];
+  v4f k_in;
+  int32_t odd_chunk = 0;
+  auto ask_rows = [&](int32_t n) {
+    const uint32_t last = rows_of(n) - 1;
+    const uint8_t *const qp = row_at(l.q, n, key_head) + (min(16u * wave + col, last) * q_ld + 8 * g);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) q[s][h] = *(const v2u *)(qp + 64 * s + 32 * h);
+    }
+    const uint8_t *const vp = row_at(l.v, n, head);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      vb[i] = *(const uint16_t *)(vp + (min(16u * wave + 4 * g + i, last) * v_ld + 2 * column));
+    const ChunkData &d = data_of(n);
+    k_in = *(const v4f *)&d.k_in[16 * wave + 4 * g];
+    odd_chunk = d.odd[lane];
+  };
+  // K's rows, 16 B at a time, for LDS
+  v4u kv[KD / 32];
+  auto ask_k = [&](int32_t n) {
+    const uint32_t last = rows_of(n) - 1;
+    const uint8_t *const kp = row_at(l.k, n, key_head);
+#pragma unroll
+    for (int i = 0; i < KD / 32; ++i) {
+      constexpr int PER = KD / 8;  // threads a row
+      const uint32_t x = i * 256 + threadIdx.x;
+      kv[i] = *(const v4u *)(kp + (min(x / PER, last) * k_ld + 16 * (x % PER)));
+    }
+  };
+  // T's and A's rows 16 w .. of the chunk, with what goes with them (the blocks
+  // above the diagonal are the last one again: as many loads on every path, so
+  // that a wait counts those that came after it right)
+  v4f tr[4], q_in, k_out;
+  v4u ar[2][2];
+  float decay = 0.0f;
+  auto ask_t = [&](int32_t n) {
+    const ChunkData &d = data_of(n);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) tr[t] = d.t[wave * (wave + 1) / 2 + min(t, wave)][lane];
+    k_out = *(const v4f *)&d.k_out[16 * wave + 4 * g];
+  };
+  auto ask_a = [&](int32_t n) {
+    const ChunkData &d = data_of(n);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) ar[s][i] = d.a[a_block(wave, min(s, wave / 2))][i][lane];
+    }
+    q_in = *(const v4f *)&d.q_in[16 * wave + 4 * g];
+    decay = d.decay[lane];
+  };
+  auto keep_k = [&](int32_t n) {
 #pragma unroll
     for (int i = 0; i < KD / 32; ++i) {
       constexpr int PER = KD / 8;
-      const int n = i * 256 + threadIdx.x;
-      *(v4u *)(kl[buf] + place(n / PER, n % PER)) = now.k[i];
+      const int x = i * 256 + threadIdx.x;
+      *(v4u *)(kl[n & 1] + place(x / PER, x % PER)) = x / PER < rows_of(n) ? kv[i] : v4u{0, 0, 0, 0};
     }
   };
   auto keep_state = [&]() {
@@ -579,131 +591,179 @@ __global__ __launch_bounds__(256) void delta_scan_kernel(const ChunkArgs p) {
   if (threadIdx.x < 32) odd_v[threadIdx.x / 16][threadIdx.x % 16] = 0;
   __syncthreads();
   if (from < to) {
-    scan_load<KD>(p, p.data[(int64_t)(base + from) * l.heads + head], range.lo + from * kChunk,
-                  min(kChunk, range.hi - range.lo - from * kChunk), head, key_head, column, wave, lane, now);
-    keep_k(from & 1);
+    ask_k(from);
+    ask_rows(from);
+    ask_t(from);
+    ask_a(from);
+    keep_k(from);
+    ask_k(min(from + 1, to - 1));
   }
   keep_state();
   for (int32_t n = from; n < to; ++n) {
-    const int32_t row = range.lo + n * kChunk, live = min(kChunk, range.hi - row);
+    const int32_t after = min(n + 1, to - 1);  // (the last chunk asks for itself again)
+    const int32_t row = range.lo + n * kChunk, live = rows_of(n);
     const int buf = n & 1;
     bool bad = false;
+    float v[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) bad |= !finite(now.v[i]);
+    for (int i = 0; i < 4; ++i) {
+      v[i] = 16 * wave + 4 * g + i < live ? bf16_to_float(vb[i]) : 0.0f;
+      bad |= !finite(v[i]);
+    }
     if (bad) odd_v[buf][col] = 1;
+    const bool odd_all = __builtin_amdgcn_readfirstlane(odd_chunk) != 0;
     __syncthreads();  // the state's parts, K's rows and the vote are there
     // An infinity or NaN would reach rows before its own, by 0 times it: its
     // column (every column, if it is not in the values) goes row by row below.
-    const bool mine_odd = now.odd || odd_v[buf][col];
+    const bool mine_odd = odd_all || odd_v[buf][col];
     const bool slow = __builtin_amdgcn_ballot_w64(mine_odd) != 0;
     if (threadIdx.x < 16) odd_v[buf ^ 1][threadIdx.x] = 0;  // (read before this barrier, set after the next)
     v4f old[TW];
 #pragma unroll
     for (int t = 0; t < TW; ++t) old[t] = state[t];
-    ScanLoads<KD> next = now;
-    if (n + 1 < to)
-      scan_load<KD>(p, p.data[(int64_t)(base + n + 1) * l.heads + head], row + kChunk,
-                    min(kChunk, range.hi - row - kChunk), head, key_head, column, wave, lane, next);
-    if (!now.odd) {
+    v4f q0;
+    {
       // K S0 and Q S0
       v4f ks[3], qs[2];
 #pragma unroll
       for (int i = 0; i < 3; ++i) ks[i] = v4f{0, 0, 0, 0};
       qs[0] = qs[1] = ks[0];
+      v2u kh[KS][2], sv[3][TILES];
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
-        v2u kh[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-          kh[h] = *(const v2u *)(kl[buf] + place(16 * wave + col, 4 * s + 2 * h + (g >> 1)) + (g & 1) * 8);
-        const v8bf a = join(kh[0], kh[1]), b = join(now.q[s][0], now.q[s][1]);
+          kh[s][h] = *(const v2u *)(kl[buf] + place(16 * wave + col, 4 * s + 2 * h + (g >> 1)) + (g & 1) * 8);
 #pragma unroll
         for (int i = 0; i < 3; ++i) {
-          const v8bf x = join(sp[i][2 * s][lane], sp[i][2 * s + 1][lane]);
+          sv[i][2 * s] = sp[i][2 * s][lane];
+          sv[i][2 * s + 1] = sp[i][2 * s + 1][lane];
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const v8bf a = join(kh[s][0], kh[s][1]), b = join(q[s][0], q[s][1]);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+          const v8bf x = join(sv[i][2 * s], sv[i][2 * s + 1]);
           ks[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, x, ks[i], 0, 0, 0);
           if (i < 2) qs[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, x, qs[i], 0, 0, 0);
         }
       }
-      {
-        v4f x = (ks[2] + ks[1]) + ks[0];
+      v4f x = (ks[2] + ks[1]) + ks[0];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = __builtin_fmaf(-now.k_in[i], x[i], now.v[i]);
-        bl[wave][lane] = x;
-      }
-      __syncthreads();
+      for (int i = 0; i < 4; ++i) x[i] = __builtin_fmaf(-k_in[i], x[i], mine_odd ? 0.0f : v[i]);
+      bl[wave][lane] = x;
+      q0 = qs[0] + qs[1];
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    ask_rows(after);
+    __builtin_amdgcn_sched_barrier(0);
+    __syncthreads();
+    {
       // U
+      v4f b[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) b[t] = bl[t][lane];
       v4f u = v4f{0, 0, 0, 0}, u2 = u;
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         if (t > wave) continue;
-        const v4f b = bl[t][lane];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          if (i % 2 == 0) u = __builtin_amdgcn_mfma_f32_16x16x4f32(now.t[t][i], b[i], u, 0, 0, 0);
-          else u2 = __builtin_amdgcn_mfma_f32_16x16x4f32(now.t[t][i], b[i], u2, 0, 0, 0);
+          if (i % 2 == 0) u = __builtin_amdgcn_mfma_f32_16x16x4f32(tr[t][i], b[t][i], u, 0, 0, 0);
+          else u2 = __builtin_amdgcn_mfma_f32_16x16x4f32(tr[t][i], b[t][i], u2, 0, 0, 0);
         }
       }
       u = u + u2;
       {
         v2u part[2], out[3];
-        split4<2>(u, part);
         v4f x = u;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] *= now.k_out[i];
+        for (int i = 0; i < 4; ++i) x[i] *= k_out[i];
         split4<3>(x, out);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) up[i][wave][lane] = part[i];
-#pragma unroll
         for (int i = 0; i < 3; ++i) uo[i][wave][lane] = out[i];
+        split4<2>(u, part);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) up[i][wave][lane] = part[i];
       }
-      __syncthreads();
-      // the state after the chunk
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    ask_t(after);
+    __builtin_amdgcn_sched_barrier(0);
+    __syncthreads();
+    {
+      // the state after the chunk, and the outputs
+      v4s kt[TW][2][2];
+      v2u ul[2][4], ol[3][4];
 #pragma unroll
       for (int t = 0; t < TW; ++t) {
-        v4f sum[3];
-#pragma unroll
-        for (int i = 0; i < 3; ++i) sum[i] = v4f{0, 0, 0, 0};
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-          v4s half[2];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int r = 16 * (2 * s + h) + 4 * g + (col >> 2);
-            half[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            kt[t][s][h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                 (__attribute__((address_space(3))) v4s *)(kl[buf] + place(r, 2 * (TW * wave + t) + (col >> 1 & 1)) + (col & 1) * 8));
           }
-          const v8s both = __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+#pragma unroll
+        for (int i = 0; i < 3; ++i) ol[i][t] = uo[i][t][lane];
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) ul[i][t] = up[i][t][lane];
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      v4f sum[TW][3];
+#pragma unroll
+      for (int t = 0; t < TW; ++t) {
+#pragma unroll
+        for (int i = 0; i < 3; ++i) sum[t][i] = v4f{0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const v8s both = __builtin_shufflevector(kt[t][s][0], kt[t][s][1], 0, 1, 2, 3, 4, 5, 6, 7);
           const v8bf a = __builtin_bit_cast(v8bf, both);
 #pragma unroll
           for (int i = 0; i < 3; ++i)
-            sum[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, join(uo[i][2 * s][lane], uo[i][2 * s + 1][lane]), sum[i], 0, 0, 0);
+            sum[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, join(ol[i][2 * s], ol[i][2 * s + 1]), sum[t][i], 0, 0, 0);
         }
-        const v4f x = (sum[2] + sum[1]) + sum[0];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) state[t][i] = __builtin_fmaf(now.decay, state[t][i], x[i]);
       }
-      // the outputs
       v4f o = v4f{0, 0, 0, 0}, o2 = o;
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         if (s > wave / 2) continue;
-        const v8bf u0 = join(up[0][2 * s][lane], up[0][2 * s + 1][lane]);
-        const v8bf u1 = join(up[1][2 * s][lane], up[1][2 * s + 1][lane]);
-        const v8bf a0 = __builtin_bit_cast(v8bf, now.a[s][0]), a1 = __builtin_bit_cast(v8bf, now.a[s][1]);
+        const v8bf u0 = join(ul[0][2 * s], ul[0][2 * s + 1]), u1 = join(ul[1][2 * s], ul[1][2 * s + 1]);
+        const v8bf a0 = __builtin_bit_cast(v8bf, ar[s][0]), a1 = __builtin_bit_cast(v8bf, ar[s][1]);
         o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a0, u0, o, 0, 0, 0);
         o2 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a0, u1, o2, 0, 0, 0);
         o2 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a1, u0, o2, 0, 0, 0);
       }
+#pragma unroll
+      for (int t = 0; t < TW; ++t) {
+        const v4f x = (sum[t][2] + sum[t][1]) + sum[t][0];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) state[t][i] = __builtin_fmaf(decay, state[t][i], x[i]);
+      }
       o = o + o2;
-      const v4f q0 = qs[0] + qs[1];
+      // (rows past the last are out of the buffer's range, without a branch)
+      const auto to_o = __builtin_amdgcn_make_buffer_rsrc(row_at(l.o, n, head), 0, 0x7fffffff, 0x00020000);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int r = 16 * wave + 4 * g + i;
-        if (r < live && !mine_odd)
-          ((uint16_t *)l.o.data)[(int64_t)(row + r) * l.o.row_ld + head * l.o.head_ld + column] =
-              float_to_bf16(__builtin_fmaf(now.q_in[i], q0[i], o[i]));
+        const uint32_t off = r < live && !mine_odd ? (uint32_t)r * o_ld + 2 * column : 0xffffff00u;
+        __builtin_amdgcn_raw_buffer_store_b16(float_to_bf16(__builtin_fmaf(q_in[i], q0[i], o[i])), to_o, off, 0, 0);
       }
     }
+    __builtin_amdgcn_sched_barrier(0);
+    ask_a(after);
+    __builtin_amdgcn_sched_barrier(0);
     if (slow) {
       for (int32_t r = 0; r < live; ++r) {
         const int64_t rr = row + r;
@@ -714,23 +774,23 @@ __global__ __launch_bounds__(256) void delta_scan_kernel(const ChunkArgs p) {
         for (int t = 0; t < TW; ++t) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int d = 16 * (TW * wave + t) + 4 * g + i;
-            const float q = bf16_to_float(qp[d]);
-            k[t][i] = bf16_to_float(kp[d]);
+            const int x = 16 * (TW * wave + t) + 4 * g + i;
+            const float qv = bf16_to_float(qp[x]);
+            k[t][i] = bf16_to_float(kp[x]);
             pk = __builtin_fmaf(old[t][i], k[t][i], pk);
-            pq = __builtin_fmaf(old[t][i], q, pq);
+            pq = __builtin_fmaf(old[t][i], qv, pq);
             kk = __builtin_fmaf(k[t][i], k[t][i], kk);
-            qq = __builtin_fmaf(q, q, qq);
-            kq = __builtin_fmaf(k[t][i], q, kq);
+            qq = __builtin_fmaf(qv, qv, qq);
+            kq = __builtin_fmaf(k[t][i], qv, kq);
           }
         }
 #pragma unroll
-        for (int d = 16; d < 64; d *= 2) {
-          pk += __shfl_xor(pk, d);
-          pq += __shfl_xor(pq, d);
-          kk += __shfl_xor(kk, d);
-          qq += __shfl_xor(qq, d);
-          kq += __shfl_xor(kq, d);
+        for (int x = 16; x < 64; x *= 2) {
+          pk += __shfl_xor(pk, x);
+          pq += __shfl_xor(pq, x);
+          kk += __shfl_xor(kk, x);
+          qq += __shfl_xor(qq, x);
+          kq += __shfl_xor(kq, x);
         }
         const int b = r & 1;
         if (g == 0) {
@@ -755,8 +815,8 @@ __global__ __launch_bounds__(256) void delta_scan_kernel(const ChunkArgs p) {
         const float rk = l.normalize ? 1.0f / sqrtf(kk + l.eps) : 1.0f;
         const float rq = l.scale * (l.normalize ? 1.0f / sqrtf(qq + l.eps) : 1.0f);
         const float a = expf(l.decay[rr * l.decay_ld + head]), beta = l.beta[rr * l.beta_ld + head];
-        const float v = bf16_to_float(((const uint16_t *)l.v.data)[rr * l.v.row_ld + head * l.v.head_ld + column]);
-        const float u = (v - pk * (a * rk)) * beta;
+        const float vv = bf16_to_float(((const uint16_t *)l.v.data)[rr * l.v.row_ld + head * l.v.head_ld + column]);
+        const float u = (vv - pk * (a * rk)) * beta;
         const float o = pq * (a * rq) + u * (kq * rk * rq);
 #pragma unroll
         for (int t = 0; t < TW; ++t) {
@@ -772,9 +832,9 @@ __global__ __launch_bounds__(256) void delta_scan_kernel(const ChunkArgs p) {
         for (int i = 0; i < 4; ++i) state[t][i] = mine_odd ? old[t][i] : state[t][i];
       }
     }
-    now = next;
     keep_state();
-    if (n + 1 < to) keep_k(buf ^ 1);
+    if (n + 1 < to) keep_k(n + 1);
+    ask_k(min(n + 2, to - 1));
   }
 #pragma unroll
   for (int t = 0; t < TW; ++t) {

@@ -2128,6 +2128,8 @@ static int delta_impl(llmcp_q8_ctx *ctx, const Heads &q, const Heads &k, const H
     return fail(LLMCP_Q8_DECLINED, "log decay and beta must be [rows, value heads]");
   if (sequences < 1 || sequences > kMaxSequences || (!row_starts && sequences != 1))
     return fail(LLMCP_Q8_DECLINED, "%d sequences (up to %d; without row starts one)", sequences, kMaxSequences);
+  if (q.h.row_ld >= 1 << 22 || k.h.row_ld >= 1 << 22 || v.h.row_ld >= 1 << 22 || out.h.row_ld >= 1 << 22)
+    return fail(LLMCP_Q8_DECLINED, "rows 2^22 values apart or more");
   if (sequences * v.heads * v.dim > 1ll << 26)
     return fail(LLMCP_Q8_DECLINED, "too many states for one launch (%d of %lld x %lld columns)",
                 sequences, (long long)v.heads, (long long)v.dim);
