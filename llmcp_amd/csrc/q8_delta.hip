@@ -19,6 +19,8 @@
 // and an f32 factor goes in as parts of 8 bits: three of S0 towards U and of U
 // towards the state (exact products), two of what only reaches a bf16 output. T
 // meets V - K S0 in f32 matrix instructions.
+#include <stddef.h>
+
 #include <algorithm>
 
 #include "q8_gemv.h"
@@ -467,16 +469,19 @@ __device__ __forceinline__ int32_t on_one_xcd(int32_t block, int32_t blocks) {
 }
 
 // A sequence's chunks of the window, 16 columns of a head's state per
-// workgroup. Wave w has rows 16 w .. of the chunk and, of the state, tiles
-// of 16 key dims; between the waves everything passes through LDS in the order
-// of the lanes, since a result's registers (rows 4 g + i, column col) are a lane's
-// part of the next product's operand when the summed index is taken in that
-// order. What a phase takes from memory is asked for a phase or two ahead, as it
-// comes (a conversion or a row's mask there would wait for it; rows past the
-// chunk's last repeat that one); what it takes from LDS, together.
+// workgroup of eight waves. Waves 0 to 3 carry the state: wave w has rows 16 w ..
+// of the chunk's U and tiles of 16 key dims of the state. Waves 4 to 7 have the
+// same rows of the outputs, and bring K's rows to LDS. Between the waves
+// everything passes through LDS in the order of the lanes, since a result's
+// registers (rows 4 g + i, column col) are a lane's part of the next product's
+// operand when the summed index is taken in that order. What a phase takes from
+// memory is asked for a phase or more ahead, as it comes (a conversion or a row's
+// mask there would wait for it; rows past the chunk's last repeat that one, and
+// what a wave needs no block of is another's again: as many loads on every path,
+// so that a wait counts those after it right); what it takes from LDS, together.
 template <int KD>
-__global__ __launch_bounds__(256) void delta_scan_kernel(const ChunkArgs p) {
-  constexpr int KS = KD / 32, TILES = KD / 16, TW = TILES / 4;
+__global__ __launch_bounds__(512) void delta_scan_kernel(const ChunkArgs p) {
+  constexpr int KS = KD / 32, TILES = KD / 16, TW = TILES / 4, KL = KD / 32;
   __shared__ __align__(16) uint8_t kl[2][kChunk * KD * 2];
   __shared__ __align__(16) v2u sp[3][TILES][64], up[2][4][64], uo[3][4][64];
   __shared__ __align__(16) v4f bl[4][64];
@@ -485,7 +490,9 @@ __global__ __launch_bounds__(256) void delta_scan_kernel(const ChunkArgs p) {
   __shared__ int odd_v[2][16];  // columns with an infinity or NaN among the chunk's values
   const DeltaLaunch &l = p.l;
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int which = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const bool carries = which < 4;
+  const int wave = which & 3, t256 = threadIdx.x & 255;
   const int32_t seq = blockIdx.x / (l.heads * p.slices);
   const int32_t block = on_one_xcd(blockIdx.x - seq * (l.heads * p.slices), l.heads * p.slices);
   const int32_t head = block / p.slices, slice = block - head * p.slices, sh = seq * l.heads + head;
@@ -504,11 +511,9 @@ __global__ __launch_bounds__(256) void delta_scan_kernel(const ChunkArgs p) {
   for (int t = 0; t < TW; ++t) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      state[t][i] = before ? before[at + (int64_t)(16 * (TW * wave + t) + 4 * g + i) * l.value_dim] : 0.0f;
+      state[t][i] = before && carries ? before[at + (int64_t)(16 * (TW * wave + t) + 4 * g + i) * l.value_dim] : 0.0f;
   }
   auto rows_of = [&](int32_t n) { return min(kChunk, range.hi - range.lo - n * kChunk); };
-  auto data_of = [&](int32_t n) -> const ChunkData & { return p.data[(int64_t)(base + n) * l.heads + head]; };
-  auto place = [](int r, int c) { return r * KD * 2 + ((c ^ ((r & 7) << 1 | (r >> 3 & 1))) & (KD / 8 - 1)) * 16; };
   // Places in a chunk are 32-bit lane offsets from the chunk's first row (rows
   // are less than 2^22 values apart).
   const uint32_t q_ld = 2 * (uint32_t)l.q.row_ld, k_ld = 2 * (uint32_t)l.k.row_ld,
@@ -516,118 +521,71 @@ __global__ __launch_bounds__(256) void delta_scan_kernel(const ChunkArgs p) {
   auto row_at = [&](const HeadRows &x, int32_t n, int32_t h) {
     return (uint8_t *)x.data + 2 * ((int64_t)(range.lo + n * kChunk) * x.row_ld + (int64_t)h * x.head_ld);
   };
-  // rows 16 w + col of q (values 32 s + 16 h + 4 g ..), rows 16 w + 4 g + i of v
-  v2u q[KS][2];
-  uint16_t vb[4];
-  v4f k_in;
-  int32_t odd_chunk = 0;
-  auto ask_rows = [&](int32_t n) {
-    const uint32_t last = rows_of(n) - 1;
-    const uint8_t *const qp = row_at(l.q, n, key_head) + (min(16u * wave + col, last) * q_ld + 8 * g);
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) q[s][h] = *(const v2u *)(qp + 64 * s + 32 * h);
-    }
-    const uint8_t *const vp = row_at(l.v, n, head);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      vb[i] = *(const uint16_t *)(vp + (min(16u * wave + 4 * g + i, last) * v_ld + 2 * column));
-    const ChunkData &d = data_of(n);
-    k_in = *(const v4f *)&d.k_in[16 * wave + 4 * g];
-    odd_chunk = d.odd[lane];
-  };
-  // K's rows, 16 B at a time, for LDS
-  v4u kv[KD / 32];
-  auto ask_k = [&](int32_t n) {
-    const uint32_t last = rows_of(n) - 1;
-    const uint8_t *const kp = row_at(l.k, n, key_head);
-#pragma unroll
-    for (int i = 0; i < KD / 32; ++i) {
-      constexpr int PER = KD / 8;  // threads a row
-      const uint32_t x = i * 256 + threadIdx.x;
-      kv[i] = *(const v4u *)(kp + (min(x / PER, last) * k_ld + 16 * (x % PER)));
-    }
-  };
-  // T's and A's rows 16 w .. of the chunk, with what goes with them (the blocks
-  // above the diagonal are the last one again: as many loads on every path, so
-  // that a wait counts those that came after it right)
-  v4f tr[4], q_in, k_out;
-  v4u ar[2][2];
-  float decay = 0.0f;
-  auto ask_t = [&](int32_t n) {
-    const ChunkData &d = data_of(n);
-#pragma unroll
-    for (int t = 0; t < 4; ++t) tr[t] = d.t[wave * (wave + 1) / 2 + min(t, wave)][lane];
-    k_out = *(const v4f *)&d.k_out[16 * wave + 4 * g];
-  };
-  auto ask_a = [&](int32_t n) {
-    const ChunkData &d = data_of(n);
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) ar[s][i] = d.a[a_block(wave, min(s, wave / 2))][i][lane];
-    }
-    q_in = *(const v4f *)&d.q_in[16 * wave + 4 * g];
-    decay = d.decay[lane];
-  };
-  auto keep_k = [&](int32_t n) {
-#pragma unroll
-    for (int i = 0; i < KD / 32; ++i) {
-      constexpr int PER = KD / 8;
-      const int x = i * 256 + threadIdx.x;
-      *(v4u *)(kl[n & 1] + place(x / PER, x % PER)) = x / PER < rows_of(n) ? kv[i] : v4u{0, 0, 0, 0};
-    }
-  };
-  auto keep_state = [&]() {
-#pragma unroll
-    for (int t = 0; t < TW; ++t) {
-      v2u part[3];
-      split4<3>(state[t], part);
-#pragma unroll
-      for (int n = 0; n < 3; ++n) sp[n][TW * wave + t][lane] = part[n];
-    }
-  };
+  auto data_of = [&](int32_t n) { return (const uint8_t *)(p.data + ((int64_t)(base + n) * l.heads + head)); };
+  const int64_t data_step = (int64_t)l.heads * sizeof(ChunkData);
+  constexpr uint32_t kA = offsetof(ChunkData, a), kKIn = offsetof(ChunkData, k_in),
+                     kQIn = offsetof(ChunkData, q_in), kKOut = offsetof(ChunkData, k_out),
+                     kDecay = offsetof(ChunkData, decay), kOdd = offsetof(ChunkData, odd);
+  // K in LDS: 16 B of a row by a swizzle that spreads both ways it is read
+  auto place = [](int r, int c) { return r * KD * 2 + ((c ^ ((r & 7) << 1 | (r >> 3 & 1))) & (KD / 8 - 1)) * 16; };
   if (threadIdx.x < 32) odd_v[threadIdx.x / 16][threadIdx.x % 16] = 0;
   __syncthreads();
-  if (from < to) {
-    ask_k(from);
-    ask_rows(from);
-    ask_t(from);
-    ask_a(from);
-    keep_k(from);
-    ask_k(min(from + 1, to - 1));
-  }
-  keep_state();
-  for (int32_t n = from; n < to; ++n) {
-    const int32_t after = min(n + 1, to - 1);  // (the last chunk asks for itself again)
-    const int32_t row = range.lo + n * kChunk, live = rows_of(n);
-    const int buf = n & 1;
-    bool bad = false;
-    float v[4];
+  const int32_t first = min(from, max(to - 1, 0));
+
+  if (carries) {
+    uint16_t vb[4];
+    v4f k_in = v4f{0, 0, 0, 0}, tr[4], k_out = k_in;
+    int32_t odd_chunk = 0;
+    float decay = 0.0f;
+    const uint8_t *vp = row_at(l.v, first, head), *dp = data_of(first);
+    const uint32_t v_full = (16 * wave + 4 * g) * v_ld + 2 * column;
+    auto ask_v = [&](uint32_t last) {
+      if (last == kChunk - 1) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[i] = 16 * wave + 4 * g + i < live ? bf16_to_float(vb[i]) : 0.0f;
-      bad |= !finite(v[i]);
+        for (int i = 0; i < 4; ++i) vb[i] = *(const uint16_t *)(vp + (v_full + i * v_ld));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          vb[i] = *(const uint16_t *)(vp + (min(16u * wave + 4 * g + i, last) * v_ld + 2 * column));
+      }
+      k_in = *(const v4f *)(dp + kKIn + 64 * wave + 16 * g);
+      odd_chunk = *(const int32_t *)(dp + kOdd + 4 * lane);
+      decay = *(const float *)(dp + kDecay + 4 * lane);
+    };
+    auto ask_t = [&]() {
+      const uint8_t *const tp = dp + wave * (wave + 1) / 2 * 1024 + lane * 16;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) tr[t] = *(const v4f *)(tp + min(t, wave) * 1024);
+      k_out = *(const v4f *)(dp + kKOut + 64 * wave + 16 * g);
+    };
+    auto keep_state = [&]() {
+#pragma unroll
+      for (int t = 0; t < TW; ++t) {
+        v2u part[3];
+        split4<3>(state[t], part);
+#pragma unroll
+        for (int n = 0; n < 3; ++n) sp[n][TW * wave + t][lane] = part[n];
+      }
+    };
+    if (from < to) {
+      ask_v(rows_of(from) - 1);
+      ask_t();
     }
-    if (bad) odd_v[buf][col] = 1;
-    const bool odd_all = __builtin_amdgcn_readfirstlane(odd_chunk) != 0;
-    __syncthreads();  // the state's parts, K's rows and the vote are there
-    // An infinity or NaN would reach rows before its own, by 0 times it: its
-    // column (every column, if it is not in the values) goes row by row below.
-    const bool mine_odd = odd_all || odd_v[buf][col];
-    const bool slow = __builtin_amdgcn_ballot_w64(mine_odd) != 0;
-    if (threadIdx.x < 16) odd_v[buf ^ 1][threadIdx.x] = 0;  // (read before this barrier, set after the next)
-    v4f old[TW];
+    keep_state();
+    for (int32_t n = from; n < to; ++n) {
+      const int32_t live = rows_of(n);
+      const int buf = n & 1;
+      bool bad = false;
+      float v[4];
 #pragma unroll
-    for (int t = 0; t < TW; ++t) old[t] = state[t];
-    v4f q0;
-    {
-      // K S0 and Q S0
-      v4f ks[3], qs[2];
-#pragma unroll
-      for (int i = 0; i < 3; ++i) ks[i] = v4f{0, 0, 0, 0};
-      qs[0] = qs[1] = ks[0];
+      for (int i = 0; i < 4; ++i) {
+        v[i] = 16 * wave + 4 * g + i < live ? bf16_to_float(vb[i]) : 0.0f;
+        bad |= !finite(v[i]);
+      }
+      if (bad) odd_v[buf][col] = 1;
+      const bool odd_all = __builtin_amdgcn_readfirstlane(odd_chunk) != 0;
+      const float decay_now = decay;
+      __syncthreads();  // the state's parts, K's rows and the vote are there
       v2u kh[KS][2], sv[3][TILES];
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
@@ -640,44 +598,54 @@ __global__ __launch_bounds__(256) void delta_scan_kernel(const ChunkArgs p) {
           sv[i][2 * s + 1] = sp[i][2 * s + 1][lane];
         }
       }
+      // An infinity or NaN would reach rows before its own, by 0 times it: its
+      // column (every column, if it is not in the values) goes row by row below.
+      const bool mine_odd = odd_all || odd_v[buf][col];
       __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const v8bf a = join(kh[s][0], kh[s][1]), b = join(q[s][0], q[s][1]);
-#pragma unroll
-        for (int i = 0; i < 3; ++i) {
-          const v8bf x = join(sv[i][2 * s], sv[i][2 * s + 1]);
-          ks[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, x, ks[i], 0, 0, 0);
-          if (i < 2) qs[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, x, qs[i], 0, 0, 0);
-        }
-      }
-      v4f x = (ks[2] + ks[1]) + ks[0];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = __builtin_fmaf(-k_in[i], x[i], mine_odd ? 0.0f : v[i]);
-      bl[wave][lane] = x;
-      q0 = qs[0] + qs[1];
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    ask_rows(after);
-    __builtin_amdgcn_sched_barrier(0);
-    __syncthreads();
-    {
-      // U
-      v4f b[4];
-#pragma unroll
-      for (int t = 0; t < 4; ++t) b[t] = bl[t][lane];
-      v4f u = v4f{0, 0, 0, 0}, u2 = u;
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        if (t > wave) continue;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (i % 2 == 0) u = __builtin_amdgcn_mfma_f32_16x16x4f32(tr[t][i], b[t][i], u, 0, 0, 0);
-          else u2 = __builtin_amdgcn_mfma_f32_16x16x4f32(tr[t][i], b[t][i], u2, 0, 0, 0);
-        }
-      }
-      u = u + u2;
+      // V - diag(k_in) K S0
       {
+        v4f ks[3];
+#pragma unroll
+        for (int i = 0; i < 3; ++i) ks[i] = v4f{0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+#pragma unroll
+          for (int i = 0; i < 3; ++i)
+            ks[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(join(kh[s][0], kh[s][1]),
+                                                            join(sv[i][2 * s], sv[i][2 * s + 1]), ks[i], 0, 0, 0);
+        }
+        v4f x = (ks[2] + ks[1]) + ks[0];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = __builtin_fmaf(-k_in[i], x[i], mine_odd ? 0.0f : v[i]);
+        bl[wave][lane] = x;
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      // (the last chunk asks for itself again)
+      if (n + 1 < to) {
+        dp += data_step;
+        vp += (int64_t)kChunk * v_ld;
+      }
+      ask_v(rows_of(min(n + 1, to - 1)) - 1);
+      __builtin_amdgcn_sched_barrier(0);
+      const bool slow = __builtin_amdgcn_ballot_w64(mine_odd) != 0;
+      __syncthreads();
+      if (threadIdx.x < 16) odd_v[buf ^ 1][threadIdx.x] = 0;  // (set after the next barrier but one)
+      // U
+      {
+        v4f b[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) b[t] = bl[t][lane];
+        v4f u = v4f{0, 0, 0, 0}, u2 = u;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          if (t > wave) continue;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (i % 2 == 0) u = __builtin_amdgcn_mfma_f32_16x16x4f32(tr[t][i], b[t][i], u, 0, 0, 0);
+            else u2 = __builtin_amdgcn_mfma_f32_16x16x4f32(tr[t][i], b[t][i], u2, 0, 0, 0);
+          }
+        }
+        u = u + u2;
         v2u part[2], out[3];
         v4f x = u;
 #pragma unroll
@@ -689,158 +657,252 @@ __global__ __launch_bounds__(256) void delta_scan_kernel(const ChunkArgs p) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) up[i][wave][lane] = part[i];
       }
+      __builtin_amdgcn_sched_barrier(0);
+      ask_t();
+      __builtin_amdgcn_sched_barrier(0);
+      __syncthreads();
+      // the state after the chunk
+      v4f old[TW];
+      {
+        v4s kt[TW][2][2];
+        v2u ol[3][4];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+#pragma unroll
+          for (int t = 0; t < TW; ++t) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int r = 16 * (2 * s + h) + 4 * g + (col >> 2);
+              kt[t][s][h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                  (__attribute__((address_space(3))) v4s *)(kl[buf] + place(r, 2 * (TW * wave + t) + (col >> 1 & 1)) + (col & 1) * 8));
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 3; ++i) {
+            ol[i][2 * s] = uo[i][2 * s][lane];
+            ol[i][2 * s + 1] = uo[i][2 * s + 1][lane];
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        v4f sum[TW][3];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+#pragma unroll
+          for (int t = 0; t < TW; ++t) {
+            const v8s both = __builtin_shufflevector(kt[t][s][0], kt[t][s][1], 0, 1, 2, 3, 4, 5, 6, 7);
+            const v8bf a = __builtin_bit_cast(v8bf, both);
+#pragma unroll
+            for (int i = 0; i < 3; ++i)
+              sum[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, join(ol[i][2 * s], ol[i][2 * s + 1]),
+                                                                  s ? sum[t][i] : v4f{0, 0, 0, 0}, 0, 0, 0);
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < TW; ++t) {
+          const v4f x = (sum[t][2] + sum[t][1]) + sum[t][0];
+          old[t] = state[t];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) state[t][i] = __builtin_fmaf(decay_now, state[t][i], x[i]);
+        }
+      }
+      if (slow) {
+        for (int32_t r = 0; r < live; ++r) {
+          const int64_t rr = range.lo + n * kChunk + r;
+          const uint16_t *const kp = (const uint16_t *)l.k.data + rr * l.k.row_ld + key_head * l.k.head_ld;
+          const uint16_t *const qp = (const uint16_t *)l.q.data + rr * l.q.row_ld + key_head * l.q.head_ld;
+          float k[TW][4], pk = 0, pq = 0, kk = 0, qq = 0, kq = 0;
+#pragma unroll
+          for (int t = 0; t < TW; ++t) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int x = 16 * (TW * wave + t) + 4 * g + i;
+              const float qv = bf16_to_float(qp[x]);
+              k[t][i] = bf16_to_float(kp[x]);
+              pk = __builtin_fmaf(old[t][i], k[t][i], pk);
+              pq = __builtin_fmaf(old[t][i], qv, pq);
+              kk = __builtin_fmaf(k[t][i], k[t][i], kk);
+              qq = __builtin_fmaf(qv, qv, qq);
+              kq = __builtin_fmaf(k[t][i], qv, kq);
+            }
+          }
+#pragma unroll
+          for (int x = 16; x < 64; x *= 2) {
+            pk += __shfl_xor(pk, x);
+            pq += __shfl_xor(pq, x);
+            kk += __shfl_xor(kk, x);
+            qq += __shfl_xor(qq, x);
+            kq += __shfl_xor(kq, x);
+          }
+          const int b = r & 1;
+          if (g == 0) {
+            red[b][wave][0][col] = pk;
+            red[b][wave][1][col] = pq;
+          }
+          if (lane == 0) {
+            red3[b][wave][0] = kk;
+            red3[b][wave][1] = qq;
+            red3[b][wave][2] = kq;
+          }
+          __syncthreads();
+          pk = pq = kk = qq = kq = 0;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            pk += red[b][w][0][col];
+            pq += red[b][w][1][col];
+            kk += red3[b][w][0];
+            qq += red3[b][w][1];
+            kq += red3[b][w][2];
+          }
+          const float rk = l.normalize ? 1.0f / sqrtf(kk + l.eps) : 1.0f;
+          const float rq = l.scale * (l.normalize ? 1.0f / sqrtf(qq + l.eps) : 1.0f);
+          const float a = expf(l.decay[rr * l.decay_ld + head]), beta = l.beta[rr * l.beta_ld + head];
+          const float vv = bf16_to_float(((const uint16_t *)l.v.data)[rr * l.v.row_ld + head * l.v.head_ld + column]);
+          const float u = (vv - pk * (a * rk)) * beta;
+          const float o = pq * (a * rq) + u * (kq * rk * rq);
+#pragma unroll
+          for (int t = 0; t < TW; ++t) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) old[t][i] = __builtin_fmaf(k[t][i] * rk, u, a * old[t][i]);
+          }
+          if (wave == 0 && g == 0 && mine_odd)
+            ((uint16_t *)l.o.data)[rr * l.o.row_ld + head * l.o.head_ld + column] = float_to_bf16(o);
+        }
+#pragma unroll
+        for (int t = 0; t < TW; ++t) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) state[t][i] = mine_odd ? old[t][i] : state[t][i];
+        }
+      }
+      keep_state();
+    }
+#pragma unroll
+    for (int t = 0; t < TW; ++t) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        l.new_state[at + (int64_t)(16 * (TW * wave + t) + 4 * g + i) * l.value_dim] = state[t][i];
+    }
+    return;
+  }
+
+  // ---- waves 4 to 7
+  v2u q[KS][2];
+  v4u kv[KL], ar[2][2];
+  v4f q_in = v4f{0, 0, 0, 0};
+  int32_t odd_chunk = 0;
+  const uint8_t *qp = row_at(l.q, first, key_head), *kp = row_at(l.k, first, key_head), *dp = data_of(first);
+  uint8_t *op = row_at(l.o, first, head);
+  constexpr int PER = KD / 8, EACH = 256 / PER;  // threads a row of K, rows at a time
+  const uint32_t q_full = (16 * wave + col) * q_ld + 8 * g, k_full = t256 / PER * k_ld + 16 * (t256 % PER);
+  auto ask_q = [&](uint32_t last) {
+    const uint8_t *const x = qp + (last == kChunk - 1 ? q_full : min(16u * wave + col, last) * q_ld + 8 * g);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) q[s][h] = *(const v2u *)(x + 64 * s + 32 * h);
+    }
+  };
+  auto ask_k = [&](uint32_t last) {
+    if (last == kChunk - 1) {
+#pragma unroll
+      for (int i = 0; i < KL; ++i) kv[i] = *(const v4u *)(kp + i * EACH * k_ld + k_full);
+    } else {
+#pragma unroll
+      for (int i = 0; i < KL; ++i)
+        kv[i] = *(const v4u *)(kp + (min((uint32_t)(i * EACH + t256 / PER), last) * k_ld + 16 * (t256 % PER)));
+    }
+  };
+  auto keep_k = [&](int32_t n) {
+    const int32_t live = rows_of(n);
+#pragma unroll
+    for (int i = 0; i < KL; ++i) {
+      const int r = i * EACH + t256 / PER;
+      *(v4u *)(kl[n & 1] + place(r, t256 % PER)) = r < live ? kv[i] : v4u{0, 0, 0, 0};
+    }
+  };
+  auto ask_a = [&]() {
+    const uint8_t *const x = dp + kA + a_block(wave, 0) * 2048 + lane * 16;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) ar[s][i] = *(const v4u *)(x + min(s, wave / 2) * 2048 + i * 1024);
+    }
+    q_in = *(const v4f *)(dp + kQIn + 64 * wave + 16 * g);
+    odd_chunk = *(const int32_t *)(dp + kOdd + 4 * lane);
+  };
+  if (from < to) {
+    ask_k(rows_of(from) - 1);
+    ask_q(rows_of(from) - 1);
+    ask_a();
+    keep_k(from);
+    if (from + 1 < to) kp += (int64_t)kChunk * k_ld;
+    ask_k(rows_of(min(from + 1, to - 1)) - 1);
+  }
+  for (int32_t n = from; n < to; ++n) {
+    const int32_t live = rows_of(n);
+    const int buf = n & 1;
+    const bool odd_all = __builtin_amdgcn_readfirstlane(odd_chunk) != 0;
+    const uint32_t last_next = rows_of(min(n + 1, to - 1)) - 1;
+    __syncthreads();
+    v2u sv[2][TILES];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) sv[i][t] = sp[i][t][lane];
+    }
+    const bool mine_odd = odd_all || odd_v[buf][col];
+    const bool slow = __builtin_amdgcn_ballot_w64(mine_odd) != 0;
+    __builtin_amdgcn_sched_barrier(0);
+    v4f qs[2];
+    qs[0] = qs[1] = v4f{0, 0, 0, 0};
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        qs[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(join(q[s][0], q[s][1]), join(sv[i][2 * s], sv[i][2 * s + 1]), qs[i], 0, 0, 0);
     }
     __builtin_amdgcn_sched_barrier(0);
-    ask_t(after);
+    if (n + 1 < to) qp += (int64_t)kChunk * q_ld;
+    ask_q(last_next);
     __builtin_amdgcn_sched_barrier(0);
     __syncthreads();
-    {
-      // the state after the chunk, and the outputs
-      v4s kt[TW][2][2];
-      v2u ul[2][4], ol[3][4];
+    if (n + 1 < to) keep_k(n + 1);  // (the other buffer was read for the last time a chunk ago)
+    if (n + 2 < to) kp += (int64_t)kChunk * k_ld;
+    ask_k(rows_of(min(n + 2, to - 1)) - 1);
+    __builtin_amdgcn_sched_barrier(0);
+    __syncthreads();
+    v2u ul[2][4];
 #pragma unroll
-      for (int t = 0; t < TW; ++t) {
+    for (int t = 0; t < 4; ++t) {
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int r = 16 * (2 * s + h) + 4 * g + (col >> 2);
-            kt[t][s][h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) v4s *)(kl[buf] + place(r, 2 * (TW * wave + t) + (col >> 1 & 1)) + (col & 1) * 8));
-          }
-        }
-      }
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-#pragma unroll
-        for (int i = 0; i < 3; ++i) ol[i][t] = uo[i][t][lane];
-      }
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) ul[i][t] = up[i][t][lane];
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      v4f sum[TW][3];
-#pragma unroll
-      for (int t = 0; t < TW; ++t) {
-#pragma unroll
-        for (int i = 0; i < 3; ++i) sum[t][i] = v4f{0, 0, 0, 0};
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          const v8s both = __builtin_shufflevector(kt[t][s][0], kt[t][s][1], 0, 1, 2, 3, 4, 5, 6, 7);
-          const v8bf a = __builtin_bit_cast(v8bf, both);
-#pragma unroll
-          for (int i = 0; i < 3; ++i)
-            sum[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, join(ol[i][2 * s], ol[i][2 * s + 1]), sum[t][i], 0, 0, 0);
-        }
-      }
-      v4f o = v4f{0, 0, 0, 0}, o2 = o;
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        if (s > wave / 2) continue;
-        const v8bf u0 = join(ul[0][2 * s], ul[0][2 * s + 1]), u1 = join(ul[1][2 * s], ul[1][2 * s + 1]);
-        const v8bf a0 = __builtin_bit_cast(v8bf, ar[s][0]), a1 = __builtin_bit_cast(v8bf, ar[s][1]);
-        o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a0, u0, o, 0, 0, 0);
-        o2 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a0, u1, o2, 0, 0, 0);
-        o2 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a1, u0, o2, 0, 0, 0);
-      }
-#pragma unroll
-      for (int t = 0; t < TW; ++t) {
-        const v4f x = (sum[t][2] + sum[t][1]) + sum[t][0];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) state[t][i] = __builtin_fmaf(decay, state[t][i], x[i]);
-      }
-      o = o + o2;
-      // (rows past the last are out of the buffer's range, without a branch)
-      const auto to_o = __builtin_amdgcn_make_buffer_rsrc(row_at(l.o, n, head), 0, 0x7fffffff, 0x00020000);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = 16 * wave + 4 * g + i;
-        const uint32_t off = r < live && !mine_odd ? (uint32_t)r * o_ld + 2 * column : 0xffffff00u;
-        __builtin_amdgcn_raw_buffer_store_b16(float_to_bf16(__builtin_fmaf(q_in[i], q0[i], o[i])), to_o, off, 0, 0);
-      }
+      for (int i = 0; i < 2; ++i) ul[i][t] = up[i][t][lane];
     }
     __builtin_amdgcn_sched_barrier(0);
-    ask_a(after);
-    __builtin_amdgcn_sched_barrier(0);
+    v4f o = v4f{0, 0, 0, 0}, o2 = o;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      if (s > wave / 2) continue;
+      const v8bf u0 = join(ul[0][2 * s], ul[0][2 * s + 1]), u1 = join(ul[1][2 * s], ul[1][2 * s + 1]);
+      const v8bf a0 = __builtin_bit_cast(v8bf, ar[s][0]), a1 = __builtin_bit_cast(v8bf, ar[s][1]);
+      o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a0, u0, o, 0, 0, 0);
+      o2 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a0, u1, o2, 0, 0, 0);
+      o2 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a1, u0, o2, 0, 0, 0);
+    }
+    o = o + o2;
+    const v4f q0 = qs[0] + qs[1];
+    // (rows past the last are out of the buffer's range, without a branch)
+    const auto to_o = __builtin_amdgcn_make_buffer_rsrc(op, 0, 0x7fffffff, 0x00020000);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 16 * wave + 4 * g + i;
+      const uint32_t off = r < live && !mine_odd ? (uint32_t)r * o_ld + 2 * column : 0xffffff00u;
+      __builtin_amdgcn_raw_buffer_store_b16(float_to_bf16(__builtin_fmaf(q_in[i], q0[i], o[i])), to_o, off, 0, 0);
+    }
+    op += (int64_t)kChunk * o_ld;
+    if (n + 1 < to) dp += data_step;
+    ask_a();
     if (slow) {
-      for (int32_t r = 0; r < live; ++r) {
-        const int64_t rr = row + r;
-        const uint16_t *const kp = (const uint16_t *)l.k.data + rr * l.k.row_ld + key_head * l.k.head_ld;
-        const uint16_t *const qp = (const uint16_t *)l.q.data + rr * l.q.row_ld + key_head * l.q.head_ld;
-        float k[TW][4], pk = 0, pq = 0, kk = 0, qq = 0, kq = 0;
-#pragma unroll
-        for (int t = 0; t < TW; ++t) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int x = 16 * (TW * wave + t) + 4 * g + i;
-            const float qv = bf16_to_float(qp[x]);
-            k[t][i] = bf16_to_float(kp[x]);
-            pk = __builtin_fmaf(old[t][i], k[t][i], pk);
-            pq = __builtin_fmaf(old[t][i], qv, pq);
-            kk = __builtin_fmaf(k[t][i], k[t][i], kk);
-            qq = __builtin_fmaf(qv, qv, qq);
-            kq = __builtin_fmaf(k[t][i], qv, kq);
-          }
-        }
-#pragma unroll
-        for (int x = 16; x < 64; x *= 2) {
-          pk += __shfl_xor(pk, x);
-          pq += __shfl_xor(pq, x);
-          kk += __shfl_xor(kk, x);
-          qq += __shfl_xor(qq, x);
-          kq += __shfl_xor(kq, x);
-        }
-        const int b = r & 1;
-        if (g == 0) {
-          red[b][wave][0][col] = pk;
-          red[b][wave][1][col] = pq;
-        }
-        if (lane == 0) {
-          red3[b][wave][0] = kk;
-          red3[b][wave][1] = qq;
-          red3[b][wave][2] = kq;
-        }
-        __syncthreads();
-        pk = pq = kk = qq = kq = 0;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          pk += red[b][w][0][col];
-          pq += red[b][w][1][col];
-          kk += red3[b][w][0];
-          qq += red3[b][w][1];
-          kq += red3[b][w][2];
-        }
-        const float rk = l.normalize ? 1.0f / sqrtf(kk + l.eps) : 1.0f;
-        const float rq = l.scale * (l.normalize ? 1.0f / sqrtf(qq + l.eps) : 1.0f);
-        const float a = expf(l.decay[rr * l.decay_ld + head]), beta = l.beta[rr * l.beta_ld + head];
-        const float vv = bf16_to_float(((const uint16_t *)l.v.data)[rr * l.v.row_ld + head * l.v.head_ld + column]);
-        const float u = (vv - pk * (a * rk)) * beta;
-        const float o = pq * (a * rq) + u * (kq * rk * rq);
-#pragma unroll
-        for (int t = 0; t < TW; ++t) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) old[t][i] = __builtin_fmaf(k[t][i] * rk, u, a * old[t][i]);
-        }
-        if (wave == 0 && g == 0 && mine_odd)
-          ((uint16_t *)l.o.data)[rr * l.o.row_ld + head * l.o.head_ld + column] = float_to_bf16(o);
-      }
-#pragma unroll
-      for (int t = 0; t < TW; ++t) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) state[t][i] = mine_odd ? old[t][i] : state[t][i];
-      }
+      for (int32_t r = 0; r < live; ++r) __syncthreads();  // (with the rows of the other waves)
     }
-    keep_state();
-    if (n + 1 < to) keep_k(n + 1);
-    ask_k(min(n + 2, to - 1));
-  }
-#pragma unroll
-  for (int t = 0; t < TW; ++t) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      l.new_state[at + (int64_t)(16 * (TW * wave + t) + 4 * g + i) * l.value_dim] = state[t][i];
   }
 }
 
@@ -873,7 +935,7 @@ hipError_t launch_delta_chunks(const DeltaLaunch &l, void *workspace, hipStream_
     hipLaunchKernelGGL((delta_chunk_kernel<KD>), dim3((unsigned)(a.count * l.heads)), dim3(256), 0, s, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((delta_scan_kernel<KD>), dim3((unsigned)scan), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((delta_scan_kernel<KD>), dim3((unsigned)scan), dim3(512), 0, s, a);
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
   return hipSuccess;
