@@ -123,6 +123,7 @@ def lib():
         "llmcp_q8_abi_version": (I32, []),
         "llmcp_q8_test_ctx_rmsnorm_skew": (I, [P, I32]),
         "llmcp_q8_test_ctx_gemm_splits": (I, [P, I32]),
+        "llmcp_q8_test_ctx_attention": (I, [P, I32, I32]),
         "llmcp_q8_test_gemm_plan": (I32, [I64, P, I32, I64, I32, P, P, P, P]),
         "llmcp_q8_test_dma_stage": (None, [I32, I32, ctypes.c_uint32, P, P]),
         "llmcp_q8_set_accumulation": (I, [P, I32]),

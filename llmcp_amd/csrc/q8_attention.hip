@@ -32,7 +32,8 @@ struct AttnArgs {
   KvPages c;
   float scale2;  // scale * log2(e)
   int32_t rows, group, tiles, splits;
-  float *part;   // [unit][split][16] rows of dim + 4: the sum, maximum, total
+  int32_t snake;           // attention_many: order of the units
+  float *part;   // [unit][split][tile rows] rows of dim + 4: the sum, maximum, total
   int32_t *err_flag;
 };
 
@@ -440,27 +441,409 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttnArgs p)
   }
 }
 
+// ------------------------------------------------------- many rows (bf16) --
+
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef short v8s __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) void lds_void;
+
+constexpr int kManyRows = 128;  // rows of a tile, 32 for each wave
+
+// Unit and part of a workgroup: the longest tiles (a sequence's last) first, a
+// kv head's tiles on few XCDs; with up to two workgroups per CU in all, the
+// second half in ascending order, so that a CU's two add up to the same.
+__device__ __forceinline__ int32_t many_unit(const AttnArgs &p, int32_t block, int32_t &split) {
+  const int32_t head = block % p.c.heads, rest = block / p.c.heads;
+  split = rest % p.splits;
+  int32_t tile = rest / p.splits;
+  if (p.snake && 2 * tile >= p.tiles) tile = p.tiles + (p.tiles + 1) / 2 - 1 - tile;
+  return head * p.tiles + (p.tiles - 1 - tile);
+}
+
+// Two f32 as bf16 to nearest even, in one word.
+__device__ __forceinline__ uint32_t round2(float lo, float hi) {
+  typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+  typedef float v2f __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f{lo, hi}), v2bf));
+}
+
+// Tiles of 128 rows, 32 per wave, over keys that the workgroup brings to LDS
+// in steps of 32 KT, a step ahead: bf16 pages directly, Q8 ones through
+// registers, widened. S^T = K Q^T and O^T += V^T P^T on 32 x 32 x 16 products. The
+// maximum that exponents refer to moves only when one would pass 2^8 (f32
+// sums and bf16's 8 bits are the same at any such scale), so that the
+// accumulator is seldom rescaled.
+template <int D, bool Q8, int KT>
+__global__ __launch_bounds__(256, 2) void attention_many_kernel(const AttnArgs p) {
+  constexpr int STEPS = D / 16, DT = D / 32, KEYS = 32 * KT;
+  constexpr int CHUNKS = D / 8, ROW = 2 * D;
+  constexpr int LOADS = KEYS * CHUNKS / 256 / (Q8 ? 2 : 1);  // 16 B of a page per thread, of K and of V
+  constexpr int PER = Q8 ? D / 16 : D / 8;                   // lanes a row
+  constexpr int TILE = KEYS * ROW;
+  __shared__ __align__(16) uint8_t lds[2][2][TILE];
+  __shared__ __align__(16) float scale_lds[2][2][KEYS];
+  __shared__ int odd_lds;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 31, h = lane >> 5;
+  int32_t split;
+  const int32_t unit = many_unit(p, blockIdx.x, split);
+  const Unit u = find_unit(p, unit, kManyRows, lane);
+  if (u.seq < 0) return;
+  const int32_t step_keys = part_keys(u.seen, p.splits);
+  const int32_t k_lo = split * step_keys, k_hi = min(u.seen, k_lo + step_keys);
+  const int32_t parts = max(1, step_keys ? (u.seen + step_keys - 1) / step_keys : 0);
+  if (split >= parts) return;
+
+  const int32_t packed = u.row + 32 * wave + col;
+  const bool live = packed < u.n * p.group;
+  const int32_t i_row = live ? packed / p.group : 0;
+  const int32_t head = u.head * p.group + (live ? packed - i_row * p.group : 0);
+  auto seen_by = [&](int32_t pk) {
+    return (int32_t)min(max(u.first + pk / p.group + 1, (int64_t)0), (int64_t)u.keys);
+  };
+  const int32_t sees = live ? seen_by(packed) : 0;
+  const int32_t all_see = seen_by(u.row);  // what every row of the tile sees
+  const int32_t last = u.n * p.group - 1;
+  const int32_t wave_all = seen_by(min(u.row + 32 * wave, last));
+  const int32_t wave_seen = u.row + 32 * wave > last ? 0 : seen_by(min(u.row + 32 * wave + 31, last));
+
+  v8bf q[STEPS];
+  {
+    const uint16_t *const at = (const uint16_t *)p.q.data + (int64_t)(u.lo + i_row) * p.q.row_ld + (int64_t)head * p.q.head_ld;
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      v4u w = *(const v4u *)(at + 16 * s + 8 * h);
+      if (!live) w = v4u{0, 0, 0, 0};
+      q[s] = __builtin_bit_cast(v8bf, w);
+    }
+  }
+  float m = -__builtin_inff(), l = 0.0f;
+  v16f acc[DT];
+#pragma unroll
+  for (int t = 0; t < DT; ++t) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[t][i] = 0.0f;
+  }
+
+  // 16 B of a row in LDS: K's swizzle spreads the rows of one chunk, V's the
+  // pairs of chunks of four rows
+  auto k_place = [](int r, int c) { return r * ROW + (c ^ (r & (CHUNKS - 1) & 15)) * 16; };
+  auto v_place = [](int r, int c) { return r * ROW + (c ^ (2 * (r & (CHUNKS / 2 - 1) & 7))) * 16; };
+
+  // Where this lane's operands are in a step's rows: chunk 2 k + h of K's row 32 t
+  // + col at ka[k % 8] (a swizzle by exclusive or: 32 k at once), and of V's row 32
+  // t + 16 c + 8 n + .. the columns 32 d + .. at va[d % 4]; what is left is a
+  // constant offset.
+  constexpr int KV_A = STEPS < 8 ? STEPS : 8, VV_A = DT < 4 ? DT : 4;
+  uint32_t ka[KV_A], va[VV_A];
+  {
+    const int r = 4 * h + (lane >> 2 & 3), b = 2 * (lane >> 4 & 1) + (lane >> 1 & 1);
+    const uint32_t kb = k_place(col, h), vb = v_place(r, b) + (lane & 1) * 8;
+    const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)&lds[0][0][0];
+#pragma unroll
+    for (int k = 0; k < KV_A; ++k) ka[k] = base + (kb ^ (32u * k));
+#pragma unroll
+    for (int d = 0; d < VV_A; ++d) va[d] = base + TILE + (vb ^ (64u * d));
+  }
+
+  // The cache's row of key k0 + lane (of KEYS; -1 for none).
+  auto slot_of_key = [&](int32_t k0) {
+    int32_t slot = -1;
+    const int32_t key = k0 + (lane & (KEYS - 1));
+    if (key < k_hi) {
+      const int32_t index = key / p.c.page_size;
+      const int32_t page = page_at(p.b, p.c, u.seq, index, p.err_flag);
+      if (page >= 0) slot = (page * p.c.heads + u.head) * p.c.page_size + (key - index * p.c.page_size);
+    }
+    return slot;
+  };
+  auto mask_of = [&](int32_t slot) { return (uint64_t)__builtin_amdgcn_ballot_w64(slot >= 0); };
+
+  v4u kr[Q8 ? LOADS : 1], vr[Q8 ? LOADS : 1];
+  float ks_r = 0.0f, vs_r = 0.0f;
+  // A step's rows on their way (a row of the cache stands for those without one).
+  auto ask = [&](int32_t slot, int buf) {
+    const int32_t at = max(slot, 0);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int x = (wave * LOADS + i) * 64;  // the load's first 16 B
+      const int r = x / PER + lane / PER, c = lane % PER;
+      const int64_t row = __shfl(at, r);
+      if constexpr (Q8) {
+        kr[i] = *(const v4u *)((const int8_t *)p.c.k + row * D + c * 16);
+        vr[i] = *(const v4u *)((const int8_t *)p.c.v + row * D + c * 16);
+      } else {
+        const int kc = c ^ (r & (CHUNKS - 1) & 15), vc = c ^ (2 * (r & (CHUNKS / 2 - 1) & 7));
+        __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void *)((const uint16_t *)p.c.k + row * D + kc * 8),
+                                         (lds_void *)(lds[buf][0] + x * 16), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void *)((const uint16_t *)p.c.v + row * D + vc * 8),
+                                         (lds_void *)(lds[buf][1] + x * 16), 16, 0, 0);
+      }
+    }
+    if (Q8 && wave == 0 && lane < KEYS) {
+      ks_r = p.c.ks[at];
+      vs_r = p.c.vs[at];
+    }
+  };
+  // A step's rows in LDS, as far as they were not brought there.
+  auto keep = [&](uint64_t valid, int buf) {
+    if constexpr (Q8) {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int x = (wave * LOADS + i) * 64;
+        const int r = x / PER + lane / PER, c = lane % PER;
+        const bool has = valid >> r & 1;
+        if (!has) vr[i] = v4u{0, 0, 0, 0};
+        *(v8bf *)(lds[buf][0] + k_place(r, 2 * c)) = widen8(kr[i][0], kr[i][1]);
+        *(v8bf *)(lds[buf][0] + k_place(r, 2 * c + 1)) = widen8(kr[i][2], kr[i][3]);
+        *(v8bf *)(lds[buf][1] + v_place(r, 2 * c)) = widen8(vr[i][0], vr[i][1]);
+        *(v8bf *)(lds[buf][1] + v_place(r, 2 * c + 1)) = widen8(vr[i][2], vr[i][3]);
+      }
+      if (wave == 0 && lane < KEYS) {
+        scale_lds[buf][0][lane] = ks_r * p.scale2;
+        scale_lds[buf][1][lane] = vs_r;
+      }
+    }
+  };
+
+  constexpr uint64_t kAll = KEYS == 64 ? ~0ull : (1ull << 32) - 1;
+  int32_t slot = slot_of_key(k_lo);
+  uint64_t valid = mask_of(slot) & kAll;
+  ask(slot, 0);
+  slot = slot_of_key(k_lo + KEYS);
+  keep(valid, 0);
+  if (threadIdx.x == 0) odd_lds = 0;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  int buf = 0;
+  for (int32_t k0 = k_lo; k0 < k_hi; k0 += KEYS, buf ^= 1) {
+    const uint64_t next_valid = mask_of(slot) & kAll;
+    if (k0 + KEYS < k_hi) ask(slot, buf ^ 1);
+    slot = slot_of_key(k0 + 2 * KEYS);
+    uint8_t *const vl = lds[buf][1];
+    const uint32_t at_buf = buf * (2 * TILE);
+    const bool edge_all = k0 + KEYS > all_see || valid != kAll;  // the same in the workgroup
+    bool odd = false;
+    if (!Q8 && edge_all) {
+      // rows without a key to zeros; infinities and NaN, which some rows may
+      // not see, out of the product
+      constexpr int EACH = KEYS * CHUNKS / 256;
+#pragma unroll 1
+      for (int i = 0; i < EACH; ++i) {
+        const int x = i * 256 + threadIdx.x, r = x / CHUNKS;
+        v4u w = *(const v4u *)(vl + x * 16);
+        const bool has = valid >> r & 1;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const bool lo = (w[k] & 0x7f80u) == 0x7f80u, hi = (w[k] & 0x7f800000u) == 0x7f800000u;
+          odd |= has && (lo || hi);
+          w[k] = has ? w[k] & (lo ? 0xffff0000u : 0xffffffffu) & (hi ? 0x0000ffffu : 0xffffffffu) : 0u;
+        }
+        *(v4u *)(vl + x * 16) = w;
+      }
+      if (odd) odd_lds = 1;
+      __syncthreads();
+    }
+    const bool edge = k0 + KEYS > wave_all || valid != kAll;
+    const bool idle = k0 >= wave_seen;  // (the causal end of the wave's rows)
+    v16f s[KT];
+    if (!idle) {
+#pragma unroll
+      for (int t = 0; t < KT; ++t) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[t][i] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < STEPS; ++k) {
+          const v8bf a = *(__attribute__((address_space(3))) const v8bf *)(uintptr_t)(
+              ka[k % KV_A] + at_buf + 32 * t * ROW + k / KV_A * 256);
+          s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, q[k], s[t], 0, 0, 0);
+        }
+      }
+      float top = -__builtin_inff();
+#pragma unroll
+      for (int t = 0; t < KT; ++t) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          v4f ks = v4f{p.scale2, p.scale2, p.scale2, p.scale2};
+          if (Q8) ks = *(const v4f *)&scale_lds[buf][0][32 * t + 8 * j + 4 * h];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float x = s[t][4 * j + i] * ks[i];
+            if (edge) {
+              const int k = 32 * t + 8 * j + 4 * h + i;
+              if (!(k0 + k < sees && (valid >> k & 1))) x = -__builtin_inff();
+            }
+            s[t][4 * j + i] = x;
+            top = fmaxf(top, x);
+          }
+        }
+      }
+      top = fmaxf(top, __shfl_xor(top, 32));
+      if (__builtin_amdgcn_ballot_w64(top > m + 8.0f)) {
+        const float m_new = top > m + 8.0f ? top : m;
+        const float alpha = exp2_f32(m - finite_max(m_new));
+        m = m_new;
+        l *= alpha;
+#pragma unroll
+        for (int t = 0; t < DT; ++t) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[t][i] *= alpha;
+        }
+      }
+      const float mf = finite_max(m);
+#pragma unroll
+      for (int t = 0; t < KT; ++t) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const float e = exp2_f32(s[t][j] - mf);
+          l += e;
+          s[t][j] = e;
+        }
+        if constexpr (Q8) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const v4f vs = *(const v4f *)&scale_lds[buf][1][32 * t + 8 * j + 4 * h];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float x = s[t][4 * j + i] * vs[i];
+              // (a masked key's scale may be anything)
+              s[t][4 * j + i] = edge && s[t][4 * j + i] == 0.0f ? 0.0f : x;
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < KT; ++t) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          v4u w;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) w[k] = round2(s[t][8 * c + 2 * k], s[t][8 * c + 2 * k + 1]);
+          const v8bf pb = __builtin_bit_cast(v8bf, w);
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            v4s half[2];
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+              half[n] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                  (__attribute__((address_space(3))) v4s *)(uintptr_t)(
+                      va[d % VV_A] + at_buf + (32 * t + 16 * c + 8 * n) * ROW + d / VV_A * 256));
+            }
+            const v8s both = __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7);
+            acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, both), pb, acc[d], 0, 0, 0);
+          }
+        }
+      }
+    }
+    if (!Q8 && edge_all && odd_lds) {
+      // Infinities and NaN among the values: added key by key, to the rows
+      // that see them. (K's rows make room for the probabilities.)
+      __syncthreads();
+      float *const pl = (float *)lds[buf][0] + wave * 1024;
+#pragma unroll 1
+      for (int t = 0; t < KT; ++t) {
+        if (!idle) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            pl[(8 * (j / 4) + 4 * h + j % 4) * 32 + col] = KT > 1 && t ? s[KT - 1][j] : s[0][j];
+        }
+        __builtin_amdgcn_wave_barrier();
+        const int32_t mine = slot_of_key(k0);
+#pragma unroll 1
+        for (int k = 0; k < 32 && !idle; ++k) {
+          if (!(valid >> (32 * t + k) & 1)) continue;
+          const int64_t row = __builtin_amdgcn_readlane(mine, 32 * t + k);
+          const float pk = pl[k * 32 + col];
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const v2u w = *(const v2u *)((const uint16_t *)p.c.v + row * D + 32 * d + 8 * j + 4 * h);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float v = bf16_to_float(i % 2 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu);
+                if (!(fabsf(v) < __builtin_inff()) && k0 + 32 * t + k < sees) acc[d][4 * j + i] += pk * v;
+              }
+            }
+          }
+        }
+        __builtin_amdgcn_wave_barrier();
+      }
+      __syncthreads();
+      if (threadIdx.x == 0) odd_lds = 0;
+    }
+    if (k0 + KEYS < k_hi) keep(next_valid, buf ^ 1);
+    valid = next_valid;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  }
+
+  l += __shfl_xor(l, 32);
+  if (parts > 1) {
+    if (!live) return;
+    float *const to = p.part + ((int64_t)(unit * p.splits + split) * kManyRows + 32 * wave + col) * (D + 4);
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *(v4f *)(to + 32 * d + 8 * j + 4 * h) = v4f{acc[d][4 * j], acc[d][4 * j + 1], acc[d][4 * j + 2], acc[d][4 * j + 3]};
+    }
+    if (h == 0) {
+      to[D] = m;
+      to[D + 1] = l;
+    }
+    return;
+  }
+  // through LDS, for whole rows
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  uint8_t *const mine = &lds[0][0][0] + wave * (4 * TILE / kWaves);
+  constexpr int FIT = 4 * TILE / kWaves / ROW;  // rows of a wave's share of LDS
+  static_assert(FIT >= 32, "the outputs fit");
+#pragma unroll
+  for (int d = 0; d < DT; ++d) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const v2u w = v2u{round2(acc[d][4 * j] * inv, acc[d][4 * j + 1] * inv),
+                        round2(acc[d][4 * j + 2] * inv, acc[d][4 * j + 3] * inv)};
+      *(v2u *)(mine + k_place(col, 4 * d + j) + 8 * h) = w;
+    }
+  }
+  __builtin_amdgcn_wave_barrier();
+  constexpr int LANES = D / 8, AT_ONCE = 64 / LANES;
+#pragma unroll 4
+  for (int r0 = 0; r0 < 32; r0 += AT_ONCE) {
+    const int r = r0 + lane / LANES, c = lane % LANES;
+    const int32_t pk = u.row + 32 * wave + r;
+    if (pk > last) continue;
+    const int32_t row = pk / p.group, hd = u.head * p.group + pk - row * p.group;
+    *(v4u *)((uint16_t *)p.o.data + (int64_t)(u.lo + row) * p.o.row_ld + (int64_t)hd * p.o.head_ld + 8 * c) =
+        *(const v4u *)(mine + k_place(r, c));
+  }
+}
+
 // The parts of the units whose keys were split, joined in order.
-template <int D>
+template <int D, int TILE>
 __global__ __launch_bounds__(256) void attention_join_kernel(const AttnArgs p) {
-  const Unit u = find_unit(p, blockIdx.x, kTileRows, threadIdx.x & 63);
+  const int32_t unit = blockIdx.x / (TILE / 16), sub = blockIdx.x % (TILE / 16);
+  const Unit u = find_unit(p, unit, TILE, threadIdx.x & 63);
   if (u.seq < 0) return;
   const int32_t step_keys = part_keys(u.seen, p.splits);
   const int32_t parts = step_keys ? (u.seen + step_keys - 1) / step_keys : 0;
   if (parts <= 1) return;
-  const float *const from = p.part + (int64_t)blockIdx.x * p.splits * kTileRows * (D + 4);
-  for (int i = threadIdx.x; i < kTileRows * (D / 4); i += 256) {
+  const float *const from = p.part + ((int64_t)unit * p.splits * TILE + 16 * sub) * (D + 4);
+  for (int i = threadIdx.x; i < 16 * (D / 4); i += 256) {
     const int r = i / (D / 4), c = i % (D / 4);
-    const int32_t pk = u.row + r;
+    const int32_t pk = u.row + 16 * sub + r;
     if (pk >= u.n * p.group) break;
     float top = -__builtin_inff();
-    for (int32_t s = 0; s < parts; ++s) top = fmaxf(top, from[(int64_t)(s * kTileRows + r) * (D + 4) + D]);
+    for (int32_t s = 0; s < parts; ++s) top = fmaxf(top, from[(int64_t)(s * TILE + r) * (D + 4) + D]);
     const float mf = finite_max(top);
     v4f sum = v4f{0, 0, 0, 0};
     float total = 0.0f;
 #pragma unroll 4
     for (int32_t s = 0; s < parts; ++s) {
-      const float *const at = from + (int64_t)(s * kTileRows + r) * (D + 4);
+      const float *const at = from + (int64_t)(s * TILE + r) * (D + 4);
       const float f = exp2_f32(at[D] - mf);
       total += f * at[D + 1];
       sum = sum + *(const v4f *)(at + 4 * c) * f;
@@ -475,26 +858,33 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttnArgs p) {
 }
 
 template <int D, bool Q8>
-hipError_t launch_attention_d(const AttnArgs &a, bool bf16, int32_t units, hipStream_t s) {
+hipError_t launch_attention_d(const AttnArgs &a, bool bf16, bool many, int32_t units, hipStream_t s) {
   const dim3 grid((unsigned)(units * a.splits)), wg(64 * kWaves);
-  if (bf16) hipLaunchKernelGGL((attention_few_kernel<D, Q8, 1>), grid, wg, 0, s, a);
+  if (many) hipLaunchKernelGGL((attention_many_kernel<D, Q8, D == 256 ? 1 : 2>), grid, wg, 0, s, a);
+  else if (bf16) hipLaunchKernelGGL((attention_few_kernel<D, Q8, 1>), grid, wg, 0, s, a);
   else hipLaunchKernelGGL((attention_few_kernel<D, Q8, 3>), grid, wg, 0, s, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.splits == 1) return e;
-  hipLaunchKernelGGL((attention_join_kernel<D>), dim3((unsigned)units), wg, 0, s, a);
+  if (many) hipLaunchKernelGGL((attention_join_kernel<D, kManyRows>), dim3((unsigned)units * (kManyRows / 16)), wg, 0, s, a);
+  else hipLaunchKernelGGL((attention_join_kernel<D, kTileRows>), dim3((unsigned)units), wg, 0, s, a);
   return hipGetLastError();
 }
 
 }  // namespace
 
-AttentionPlan attention_plan(int64_t rows, int32_t heads, const KvBatch &b, const KvPages &c) {
+AttentionPlan attention_plan(int64_t rows, int32_t heads, bool bf16, const KvBatch &b, const KvPages &c,
+                             int32_t test_kernel, int32_t test_splits) {
   AttentionPlan plan;
   const int64_t group = heads / c.heads;
-  plan.tiles = (int32_t)(rows * group / kTileRows + std::min<int64_t>(b.sequences, rows));
-  const int64_t units = (int64_t)plan.tiles * c.heads;
   const int64_t steps = ((int64_t)b.max_pages * c.page_size + kWaves * kBlockKeys - 1) / (kWaves * kBlockKeys);
-  plan.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({steps, 2048 / units, 64}));
-  if (plan.splits > 1) plan.part_floats = units * plan.splits * kTileRows * (c.dim + 4);
+  plan.many = bf16 && rows * group >= 64 * (int64_t)b.sequences && rows * heads >= 16384;
+  if (test_kernel && bf16) plan.many = test_kernel == 2;
+  const int64_t tile = plan.many ? kManyRows : kTileRows;
+  plan.tiles = (int32_t)(rows * group / tile + std::min<int64_t>(b.sequences, rows));
+  const int64_t units = (int64_t)plan.tiles * c.heads;
+  plan.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({steps, (plan.many ? 512 : 2048) / units, 64}));
+  if (test_splits > 0) plan.splits = (int32_t)std::min<int64_t>(steps, test_splits);
+  if (plan.splits > 1) plan.part_floats = units * plan.splits * tile * (c.dim + 4);
   return plan;
 }
 
@@ -505,16 +895,13 @@ hipError_t launch_attention(const HeadRows &q, const HeadRows &o, int64_t rows, 
   if (rows < 1 || units < 1 || units * plan.splits > 0x7FFFFF || (plan.splits > 1 && !part))
     return hipErrorInvalidConfiguration;
   AttnArgs a = {q, o, b, c, (float)((double)scale * 1.4426950408889634), (int32_t)rows,
-                heads / c.heads, plan.tiles, plan.splits, part, err_flag};
-  switch (c.dim) {
-    case 64: return c.q8 ? launch_attention_d<64, true>(a, q.bf16, (int32_t)units, s)
-                         : launch_attention_d<64, false>(a, q.bf16, (int32_t)units, s);
-    case 128: return c.q8 ? launch_attention_d<128, true>(a, q.bf16, (int32_t)units, s)
-                          : launch_attention_d<128, false>(a, q.bf16, (int32_t)units, s);
-    case 256: return c.q8 ? launch_attention_d<256, true>(a, q.bf16, (int32_t)units, s)
-                          : launch_attention_d<256, false>(a, q.bf16, (int32_t)units, s);
-    default: return hipErrorInvalidConfiguration;
-  }
+                heads / c.heads, plan.tiles, plan.splits,
+                units * plan.splits <= 2 * cu_count() ? 1 : 0, part, err_flag};
+  const auto launch = c.dim == 64    ? (c.q8 ? launch_attention_d<64, true> : launch_attention_d<64, false>)
+                      : c.dim == 128 ? (c.q8 ? launch_attention_d<128, true> : launch_attention_d<128, false>)
+                      : c.dim == 256 ? (c.q8 ? launch_attention_d<256, true> : launch_attention_d<256, false>)
+                                     : nullptr;
+  return launch ? launch(a, q.bf16, plan.many, (int32_t)units, s) : hipErrorInvalidConfiguration;
 }
 
 }  // namespace llmcp_q8

@@ -255,11 +255,15 @@ hipError_t launch_kv_read(const HeadRows &k, const HeadRows &v, int64_t rows, co
 // kernel and how many parts a sequence's keys are split into at most (rule and
 // measurements there), and gives the floats of workspace that takes.
 struct AttentionPlan {
+  bool many = false;   // tiles of 128 rows
   int32_t tiles = 0;   // row tiles of all sequences, at most
   int32_t splits = 1;  // parts of the keys, at most
   int64_t part_floats = 0;
 };
-AttentionPlan attention_plan(int64_t rows, int32_t heads, const KvBatch &b, const KvPages &c);
+// (test_kernel 1 / 2: tiles of 16 / 128 rows forced, test_splits > 0: so many
+// parts; for tests.)
+AttentionPlan attention_plan(int64_t rows, int32_t heads, bool bf16, const KvBatch &b, const KvPages &c,
+                             int32_t test_kernel, int32_t test_splits);
 hipError_t launch_attention(const HeadRows &q, const HeadRows &o, int64_t rows, int32_t heads,
                             const KvBatch &b, const KvPages &c, float scale, const AttentionPlan &plan,
                             float *part, int32_t *err_flag, hipStream_t s);

@@ -120,6 +120,9 @@ struct llmcp_q8_ctx {
   // Tests only (llmcp_q8_test_ctx_expert_repeat): column ranges forced on every
   // workgroup of the experts' products that share tiles; 0 = chosen by size.
   int32_t test_repeat = 0;
+  // Tests only (llmcp_q8_test_ctx_attention): the kernel (1: tiles of 16 rows, 2: of
+  // 128) and the parts of the keys forced on attention; 0 = chosen by size.
+  int32_t test_attention = 0, test_attention_splits = 0;
   // Mixture of experts, grown on demand: the slots sorted by expert, the
   // SwiGLU's rows as Q8_1 and the experts' outputs.
   int32_t *plan = nullptr;
@@ -899,6 +902,17 @@ int32_t llmcp_q8_test_expert_ranges(int64_t slots, int64_t experts, int64_t rows
 // reference): whether a stack of experts of this shape would be registered.
 int llmcp_q8_test_expert_stack(int64_t experts, int64_t rows, int64_t cols) {
   return check_stack(experts, rows, cols);
+}
+
+// Test hook, declared in no header of the product (no counterpart in the
+// reference): forces attention's kernel and parts on this context.
+int llmcp_q8_test_ctx_attention(llmcp_q8_ctx *ctx, int32_t kernel, int32_t splits) {
+  if (!ctx) return fail(LLMCP_Q8_EINVAL, "null context");
+  if (kernel < 0 || kernel > 2 || splits < 0 || splits > 64)
+    return fail(LLMCP_Q8_EINVAL, "kernel %d, %d splits", kernel, splits);
+  ctx->test_attention = kernel;
+  ctx->test_attention_splits = splits;
+  return LLMCP_Q8_OK;
 }
 
 // Test hook, declared in no header of the product (no counterpart in the
@@ -2096,7 +2110,8 @@ static int attention_impl(llmcp_q8_ctx *ctx, const Heads &q, const llmcp_q8_kv_c
     return fail(LLMCP_Q8_DECLINED, "too many rows of heads for one launch (%lld)",
                 (long long)(q.rows * q.heads));
   if ((rc = set_device(ctx))) return rc;
-  const AttentionPlan plan = attention_plan(q.rows, (int32_t)q.heads, b, c);
+  const AttentionPlan plan = attention_plan(q.rows, (int32_t)q.heads, q.h.bf16, b, c,
+                                            ctx->test_attention, ctx->test_attention_splits);
   if (plan.part_floats &&
       (rc = grow(ctx, ctx->attention_part, ctx->attention_part_bytes, (uint64_t)plan.part_floats * 4,
                  "attention's parts")))

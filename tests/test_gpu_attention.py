@@ -98,6 +98,57 @@ def test_attention(q8, ctx, oracle, shape, dtype, fmt):
     assert ctx.check_flag() == 0
 
 
+@pytest.fixture
+def forced(q8, ctx):
+    """Forces the kernel (1: tiles of 16 rows, 2: of 128) and the parts of the
+    keys on the context; undone afterwards."""
+    yield lambda kernel, splits=0: q8.check(
+        q8.lib().llmcp_q8_test_ctx_attention(ctx.handle, kernel, splits))
+    q8.check(q8.lib().llmcp_q8_test_ctx_attention(ctx.handle, 0, 0))
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "q8"])
+@pytest.mark.parametrize("kernel,splits", [(1, 1), (1, 5), (2, 1), (2, 3)])
+@pytest.mark.parametrize("shape", range(len(SHAPES)))
+def test_each_kernel(q8, ctx, oracle, forced, shape, kernel, splits, fmt):
+    ns, lengths, page, heads, kvh, dim = SHAPES[shape]
+    rng = np.random.default_rng(300 + shape)
+    c = filled(q8, ctx, oracle, rng, lengths, page, kvh, dim, fmt)
+    _, q = rows_of(oracle, rng, sum(ns) + 2, heads, dim, "bf16", 2.0)
+    forced(kernel, splits)
+    run(q8, ctx, oracle, c, ns, lengths, q, "bf16", dim ** -0.5, pad=2)
+    assert ctx.check_flag() == 0
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "q8"])
+@pytest.mark.parametrize("ns,lengths,page,heads,kvh,dim", [
+    ([1100], [1100], 64, 16, 4, 64), ([700, 500], [900, 500], 40, 16, 2, 128),
+    ([1050], [1300], 1300, 16, 4, 256), ([1030, 3, 0], [1030, 40, 7], 16, 16, 16, 64)])
+def test_long_chunks(q8, ctx, oracle, ns, lengths, page, heads, kvh, dim, fmt):
+    rng = np.random.default_rng(23)
+    c = filled(q8, ctx, oracle, rng, lengths, page, kvh, dim, fmt)
+    _, q = rows_of(oracle, rng, sum(ns), heads, dim, "bf16", 2.0)
+    run(q8, ctx, oracle, c, ns, lengths, q, "bf16", dim ** -0.5)
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "q8"])
+@pytest.mark.parametrize("kernel", [1, 2])
+def test_growing_scores(q8, ctx, oracle, forced, kernel, fmt):
+    """Scores that rise by hundreds along the keys, and fall: the running
+    maximum moves at every step, or never again."""
+    rng = np.random.default_rng(29)
+    n, length, dim = 70, 390, 64
+    q = np.abs(rows_of(oracle, rng, n, 2, dim, "bf16", 1.0)[1])
+    for sign in (1.0, -1.0):
+        c = Cache(q8, ctx, rng, [length], 16, 1, dim, fmt)
+        k = np.abs(rng.standard_normal((length, 1, dim))).astype(F32)
+        k *= (sign * np.linspace(-3, 3, length)).astype(F32)[:, None, None]
+        c.put(oracle, 0, 0, k, rng.standard_normal((length, 1, dim)).astype(F32))
+        c.upload()
+        forced(kernel, 2)
+        run(q8, ctx, oracle, c, [n], [length], q, "bf16", 4.0)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("fmt", ["bf16", "q8"])
 @pytest.mark.parametrize("scale", [0.0, -0.3, 3.0])
@@ -111,12 +162,15 @@ def test_scales(q8, ctx, oracle, dtype, fmt, scale):
 
 @pytest.mark.parametrize("n", [1, 40, 200])
 @pytest.mark.parametrize("fmt", ["bf16", "q8"])
-def test_odd_values_out_of_sight(q8, ctx, oracle, n, fmt):
+@pytest.mark.parametrize("kernel", [1, 2])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_odd_values_out_of_sight(q8, ctx, oracle, forced, n, fmt, kernel, dim):
     """Infinities and NaN at positions that a row does not see leave it alone:
     behind the last key, in the chunk's later rows, on no page; the rows that
     see them are NaN or infinite."""
+    forced(kernel)
     rng = np.random.default_rng(n)
-    length, kvh, dim, page = 260, 2, 64, 16
+    length, kvh, page = 260, 2, 16
     c = filled(q8, ctx, oracle, rng, [length + 30], page, kvh, dim, fmt)
     k, v = (rng.standard_normal((1, kvh, dim)).astype(F32) for _ in range(2))
     odd = length - 5 if n > 1 else length + 3
@@ -146,8 +200,10 @@ def test_odd_values_out_of_sight(q8, ctx, oracle, n, fmt):
         assert (np.abs(got[i] - want[0]) <= bound[0]).all()
 
 
-def test_rows_without_sight(q8, ctx, oracle):
+@pytest.mark.parametrize("kernel", [1, 2])
+def test_rows_without_sight(q8, ctx, oracle, forced, kernel):
     """No page at all, no key, and scores of -inf alone give zeros."""
+    forced(kernel)
     rng = np.random.default_rng(3)
     c = filled(q8, ctx, oracle, rng, [40, 40, 8], 8, 1, 64, "bf16")
     c.table[0, :] = -1
