@@ -447,11 +447,16 @@ typedef float v16f __attribute__((ext_vector_type(16)));
 typedef short v8s __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) void lds_void;
 
-constexpr int kManyRows = 128;  // rows of a tile, 32 for each wave
+constexpr int kManyRows = 128;  // rows of a tile, 32 for each of four waves
+constexpr int kManyThreads = 256;
+// Workgroups of a CU: at dim 256 a wave's accumulator and queries alone take 192
+// registers, and one workgroup of up to 512 each (no spills) is faster than
+// two of 256.
+constexpr int many_resident(int dim) { return dim == 256 ? 1 : 2; }
 
 // Unit and part of a workgroup: the longest tiles (a sequence's last) first, a
-// kv head's tiles on few XCDs; with up to two workgroups per CU in all, the
-// second half in ascending order, so that a CU's two add up to the same.
+// kv head's tiles on few XCDs; where all workgroups are resident at once, two per
+// CU, the second half in ascending order, so that a CU's two add up to the same.
 __device__ __forceinline__ int32_t many_unit(const AttnArgs &p, int32_t block, int32_t &split) {
   const int32_t head = block % p.c.heads, rest = block / p.c.heads;
   split = rest % p.splits;
@@ -467,18 +472,19 @@ __device__ __forceinline__ uint32_t round2(float lo, float hi) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f{lo, hi}), v2bf));
 }
 
-// Tiles of 128 rows, 32 per wave, over keys that the workgroup brings to LDS
-// in steps of 32 KT, a step ahead: bf16 pages directly, Q8 ones through
-// registers, widened. S^T = K Q^T and O^T += V^T P^T on 32 x 32 x 16 products. The
-// maximum that exponents refer to moves only when one would pass 2^8 (f32
-// sums and bf16's 8 bits are the same at any such scale), so that the
-// accumulator is seldom rescaled.
-template <int D, bool Q8, int KT>
-__global__ __launch_bounds__(256, 2) void attention_many_kernel(const AttnArgs p) {
+// Tiles of 128 rows, 32 per wave, over keys that the workgroup brings to LDS in
+// steps of 32 KT, a step ahead: bf16 pages directly, Q8 ones through registers,
+// widened. S^T = K Q^T and O^T += V^T P^T on 32 x 32 x 16 products. The
+// maximum that exponents refer to moves only when one would pass 2^8 (f32 sums and
+// bf16's 8 bits are the same at any such scale), so that the accumulator is
+// seldom rescaled. WHOLE: a page is a multiple of a step, so a step's rows follow
+// each other.
+template <int D, bool Q8, int KT, bool WHOLE>
+__global__ __launch_bounds__(kManyThreads, many_resident(D)) void attention_many_kernel(const AttnArgs p) {
   constexpr int STEPS = D / 16, DT = D / 32, KEYS = 32 * KT;
   constexpr int CHUNKS = D / 8, ROW = 2 * D;
-  constexpr int LOADS = KEYS * CHUNKS / 256 / (Q8 ? 2 : 1);  // 16 B of a page per thread, of K and of V
-  constexpr int PER = Q8 ? D / 16 : D / 8;                   // lanes a row
+  constexpr int LOADS = KEYS * CHUNKS / kManyThreads / (Q8 ? 2 : 1);  // 16 B of a page per thread, of K and of V
+  constexpr int PER = Q8 ? D / 16 : D / 8;                            // lanes a row
   constexpr int TILE = KEYS * ROW;
   __shared__ __align__(16) uint8_t lds[2][2][TILE];
   __shared__ __align__(16) float scale_lds[2][2][KEYS];
@@ -495,27 +501,28 @@ __global__ __launch_bounds__(256, 2) void attention_many_kernel(const AttnArgs p
   const int32_t parts = max(1, step_keys ? (u.seen + step_keys - 1) / step_keys : 0);
   if (split >= parts) return;
 
-  const int32_t packed = u.row + 32 * wave + col;
-  const bool live = packed < u.n * p.group;
-  const int32_t i_row = live ? packed / p.group : 0;
-  const int32_t head = u.head * p.group + (live ? packed - i_row * p.group : 0);
   auto seen_by = [&](int32_t pk) {
     return (int32_t)min(max(u.first + pk / p.group + 1, (int64_t)0), (int64_t)u.keys);
   };
+  const int32_t last = u.n * p.group - 1, row0 = u.row + 32 * wave, packed = row0 + col;
+  const bool live = packed <= last;
   const int32_t sees = live ? seen_by(packed) : 0;
   const int32_t all_see = seen_by(u.row);  // what every row of the tile sees
-  const int32_t last = u.n * p.group - 1;
-  const int32_t wave_all = seen_by(min(u.row + 32 * wave, last));
-  const int32_t wave_seen = u.row + 32 * wave > last ? 0 : seen_by(min(u.row + 32 * wave + 31, last));
-
+  const int32_t wave_all = seen_by(min(row0, last));
+  const int32_t wave_seen = row0 > last ? 0 : seen_by(min(row0 + 31, last));
+  // (the scale's sign goes into q; a scale of 0 is next to it, so that a masked
+  // score stays -inf)
+  const float scale2 = fmaxf(fabsf(p.scale2), 0x1p-126f);
   v8bf q[STEPS];
   {
+    const int32_t i_row = live ? packed / p.group : 0;
+    const int32_t head = u.head * p.group + (live ? packed - i_row * p.group : 0);
     const uint16_t *const at = (const uint16_t *)p.q.data + (int64_t)(u.lo + i_row) * p.q.row_ld + (int64_t)head * p.q.head_ld;
+    const uint32_t sign = p.scale2 < 0.0f ? 0x80008000u : 0u;
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
-      v4u w = *(const v4u *)(at + 16 * s + 8 * h);
-      if (!live) w = v4u{0, 0, 0, 0};
-      q[s] = __builtin_bit_cast(v8bf, w);
+      const v4u w = *(const v4u *)(at + 16 * s + 8 * h);
+      q[s] = __builtin_bit_cast(v8bf, live ? w ^ sign : v4u{0, 0, 0, 0});
     }
   }
   float m = -__builtin_inff(), l = 0.0f;
@@ -528,9 +535,8 @@ __global__ __launch_bounds__(256, 2) void attention_many_kernel(const AttnArgs p
 
   // 16 B of a row in LDS: K's swizzle spreads the rows of one chunk, V's the
   // pairs of chunks of four rows
-  auto k_place = [](int r, int c) { return r * ROW + (c ^ (r & (CHUNKS - 1) & 15)) * 16; };
-  auto v_place = [](int r, int c) { return r * ROW + (c ^ (2 * (r & (CHUNKS / 2 - 1) & 7))) * 16; };
-
+  auto k_swap = [](int r) { return r & (CHUNKS - 1) & 15; };
+  auto v_swap = [](int r) { return 2 * (r & (CHUNKS / 2 - 1) & 7); };
   // Where this lane's operands are in a step's rows: chunk 2 k + h of K's row 32 t
   // + col at ka[k % 8] (a swizzle by exclusive or: 32 k at once), and of V's row 32
   // t + 16 c + 8 n + .. the columns 32 d + .. at va[d % 4]; what is left is a
@@ -539,7 +545,7 @@ __global__ __launch_bounds__(256, 2) void attention_many_kernel(const AttnArgs p
   uint32_t ka[KV_A], va[VV_A];
   {
     const int r = 4 * h + (lane >> 2 & 3), b = 2 * (lane >> 4 & 1) + (lane >> 1 & 1);
-    const uint32_t kb = k_place(col, h), vb = v_place(r, b) + (lane & 1) * 8;
+    const uint32_t kb = col * ROW + (h ^ k_swap(col)) * 16, vb = r * ROW + (b ^ v_swap(r)) * 16 + (lane & 1) * 8;
     const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)&lds[0][0][0];
 #pragma unroll
     for (int k = 0; k < KV_A; ++k) ka[k] = base + (kb ^ (32u * k));
@@ -547,43 +553,86 @@ __global__ __launch_bounds__(256, 2) void attention_many_kernel(const AttnArgs p
     for (int d = 0; d < VV_A; ++d) va[d] = base + TILE + (vb ^ (64u * d));
   }
 
-  // The cache's row of key k0 + lane (of KEYS; -1 for none).
+  // The cache's row of key k0 + lane (of KEYS; -1 for none), or (WHOLE) of key k0.
+  // Lane i holds the page after i others: a load and its wait per 64 pages.
+  int32_t pages = -1, pages_from = -64;
   auto slot_of_key = [&](int32_t k0) {
-    int32_t slot = -1;
-    const int32_t key = k0 + (lane & (KEYS - 1));
-    if (key < k_hi) {
-      const int32_t index = key / p.c.page_size;
-      const int32_t page = page_at(p.b, p.c, u.seq, index, p.err_flag);
-      if (page >= 0) slot = (page * p.c.heads + u.head) * p.c.page_size + (key - index * p.c.page_size);
+    const int32_t end = max(min(k0 + KEYS, k_hi) - 1, 0) / p.c.page_size;
+    if (end >= pages_from + 64) {
+      pages_from = k0 / p.c.page_size;
+      pages = p.b.table[(int64_t)u.seq * p.b.max_pages + min(pages_from + lane, p.b.max_pages - 1)];
     }
-    return slot;
+    const int32_t key = WHOLE ? k0 : k0 + (lane & (KEYS - 1));
+    const int32_t index = min(key, max(k_hi - 1, 0)) / p.c.page_size;
+    const int32_t page = WHOLE ? __builtin_amdgcn_readlane(pages, index - pages_from) : __shfl(pages, index - pages_from);
+    int32_t slot = -1;
+    if (key < k_hi) {
+      if ((uint32_t)page < (uint32_t)p.c.pages)
+        slot = (page * p.c.heads + u.head) * p.c.page_size + (key - index * p.c.page_size);
+      else if (page != -1)
+        *p.err_flag = 1;
+    }
+    return WHOLE ? __builtin_amdgcn_readfirstlane(slot) : slot;
   };
-  auto mask_of = [&](int32_t slot) { return (uint64_t)__builtin_amdgcn_ballot_w64(slot >= 0); };
+  constexpr uint64_t kAll = KEYS == 64 ? ~0ull : (1ull << 32) - 1;
+  // Which of the step's keys there are.
+  auto mask_of = [&](int32_t slot, int32_t k0) -> uint64_t {
+    if (!WHOLE) return __builtin_amdgcn_ballot_w64(slot >= 0) & kAll;
+    const int32_t n = k_hi - k0;
+    return slot < 0 || n <= 0 ? 0 : n >= KEYS ? kAll : (1ull << n) - 1;
+  };
 
   v4u kr[Q8 ? LOADS : 1], vr[Q8 ? LOADS : 1];
   float ks_r = 0.0f, vs_r = 0.0f;
   // A step's rows on their way (a row of the cache stands for those without one).
+  // The chunk that a lane brings is the one whose place in LDS is the lane's.
+  const int lr = lane / PER, lc = lane % PER;
+  const uint32_t k_lane = lr * ROW + (lc ^ k_swap(lr)) * 16, v_lane = lr * ROW + (lc ^ v_swap(lr)) * 16;
   auto ask = [&](int32_t slot, int buf) {
     const int32_t at = max(slot, 0);
+    if constexpr (WHOLE) {
+      const uint8_t *const kp = (const uint8_t *)p.c.k + (int64_t)at * (Q8 ? D : ROW);
+      const uint8_t *const vp = (const uint8_t *)p.c.v + (int64_t)at * (Q8 ? D : ROW);
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      const int x = (wave * LOADS + i) * 64;  // the load's first 16 B
-      const int r = x / PER + lane / PER, c = lane % PER;
-      const int64_t row = __shfl(at, r);
-      if constexpr (Q8) {
-        kr[i] = *(const v4u *)((const int8_t *)p.c.k + row * D + c * 16);
-        vr[i] = *(const v4u *)((const int8_t *)p.c.v + row * D + c * 16);
-      } else {
-        const int kc = c ^ (r & (CHUNKS - 1) & 15), vc = c ^ (2 * (r & (CHUNKS / 2 - 1) & 7));
-        __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void *)((const uint16_t *)p.c.k + row * D + kc * 8),
-                                         (lds_void *)(lds[buf][0] + x * 16), 16, 0, 0);
-        __builtin_amdgcn_global_load_lds((__attribute__((address_space(1))) void *)((const uint16_t *)p.c.v + row * D + vc * 8),
-                                         (lds_void *)(lds[buf][1] + x * 16), 16, 0, 0);
+      for (int i = 0; i < LOADS; ++i) {
+        const int x = (wave * LOADS + i) * 64, r0 = x / PER;  // the load's first 16 B and row
+        if constexpr (Q8) {
+          kr[i] = *(const v4u *)(kp + r0 * D + lane * 16);
+          vr[i] = *(const v4u *)(vp + r0 * D + lane * 16);
+        } else {
+          __builtin_amdgcn_global_load_lds(
+              (__attribute__((address_space(1))) void *)(kp + r0 * ROW + (k_lane ^ (uint32_t)(k_swap(r0) * 16))),
+              (lds_void *)(lds[buf][0] + x * 16), 16, 0, 0);
+          __builtin_amdgcn_global_load_lds(
+              (__attribute__((address_space(1))) void *)(vp + r0 * ROW + (v_lane ^ (uint32_t)(v_swap(r0) * 16))),
+              (lds_void *)(lds[buf][1] + x * 16), 16, 0, 0);
+        }
       }
-    }
-    if (Q8 && wave == 0 && lane < KEYS) {
-      ks_r = p.c.ks[at];
-      vs_r = p.c.vs[at];
+      if (Q8 && wave == 0 && lane < KEYS) {
+        ks_r = p.c.ks[at + lane];
+        vs_r = p.c.vs[at + lane];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int x = (wave * LOADS + i) * 64, r = x / PER + lr;
+        const int64_t row = __shfl(at, r);
+        if constexpr (Q8) {
+          kr[i] = *(const v4u *)((const int8_t *)p.c.k + row * D + lc * 16);
+          vr[i] = *(const v4u *)((const int8_t *)p.c.v + row * D + lc * 16);
+        } else {
+          __builtin_amdgcn_global_load_lds(
+              (__attribute__((address_space(1))) void *)((const uint16_t *)p.c.k + row * D + (lc ^ k_swap(r)) * 8),
+              (lds_void *)(lds[buf][0] + x * 16), 16, 0, 0);
+          __builtin_amdgcn_global_load_lds(
+              (__attribute__((address_space(1))) void *)((const uint16_t *)p.c.v + row * D + (lc ^ v_swap(r)) * 8),
+              (lds_void *)(lds[buf][1] + x * 16), 16, 0, 0);
+        }
+      }
+      if (Q8 && wave == 0 && lane < KEYS) {
+        ks_r = p.c.ks[at];
+        vs_r = p.c.vs[at];
+      }
     }
   };
   // A step's rows in LDS, as far as they were not brought there.
@@ -592,35 +641,34 @@ __global__ __launch_bounds__(256, 2) void attention_many_kernel(const AttnArgs p
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
         const int x = (wave * LOADS + i) * 64;
-        const int r = x / PER + lane / PER, c = lane % PER;
+        const int r = x / PER + lr;
         const bool has = valid >> r & 1;
         if (!has) vr[i] = v4u{0, 0, 0, 0};
-        *(v8bf *)(lds[buf][0] + k_place(r, 2 * c)) = widen8(kr[i][0], kr[i][1]);
-        *(v8bf *)(lds[buf][0] + k_place(r, 2 * c + 1)) = widen8(kr[i][2], kr[i][3]);
-        *(v8bf *)(lds[buf][1] + v_place(r, 2 * c)) = widen8(vr[i][0], vr[i][1]);
-        *(v8bf *)(lds[buf][1] + v_place(r, 2 * c + 1)) = widen8(vr[i][2], vr[i][3]);
+        uint8_t *const kl = lds[buf][0] + r * ROW, *const vl = lds[buf][1] + r * ROW;
+        *(v8bf *)(kl + (2 * lc ^ k_swap(r)) * 16) = widen8(kr[i][0], kr[i][1]);
+        *(v8bf *)(kl + ((2 * lc + 1) ^ k_swap(r)) * 16) = widen8(kr[i][2], kr[i][3]);
+        *(v8bf *)(vl + (2 * lc ^ v_swap(r)) * 16) = widen8(vr[i][0], vr[i][1]);
+        *(v8bf *)(vl + ((2 * lc + 1) ^ v_swap(r)) * 16) = widen8(vr[i][2], vr[i][3]);
       }
       if (wave == 0 && lane < KEYS) {
-        scale_lds[buf][0][lane] = ks_r * p.scale2;
+        scale_lds[buf][0][lane] = ks_r;
         scale_lds[buf][1][lane] = vs_r;
       }
     }
   };
 
-  constexpr uint64_t kAll = KEYS == 64 ? ~0ull : (1ull << 32) - 1;
   int32_t slot = slot_of_key(k_lo);
-  uint64_t valid = mask_of(slot) & kAll;
+  uint64_t valid = mask_of(slot, k_lo);
   ask(slot, 0);
-  slot = slot_of_key(k_lo + KEYS);
   keep(valid, 0);
   if (threadIdx.x == 0) odd_lds = 0;
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   int buf = 0;
   for (int32_t k0 = k_lo; k0 < k_hi; k0 += KEYS, buf ^= 1) {
-    const uint64_t next_valid = mask_of(slot) & kAll;
+    slot = slot_of_key(k0 + KEYS);
+    const uint64_t next_valid = mask_of(slot, k0 + KEYS);
     if (k0 + KEYS < k_hi) ask(slot, buf ^ 1);
-    slot = slot_of_key(k0 + 2 * KEYS);
     uint8_t *const vl = lds[buf][1];
     const uint32_t at_buf = buf * (2 * TILE);
     const bool edge_all = k0 + KEYS > all_see || valid != kAll;  // the same in the workgroup
@@ -628,10 +676,10 @@ __global__ __launch_bounds__(256, 2) void attention_many_kernel(const AttnArgs p
     if (!Q8 && edge_all) {
       // rows without a key to zeros; infinities and NaN, which some rows may
       // not see, out of the product
-      constexpr int EACH = KEYS * CHUNKS / 256;
+      constexpr int EACH = KEYS * CHUNKS / kManyThreads;
 #pragma unroll 1
       for (int i = 0; i < EACH; ++i) {
-        const int x = i * 256 + threadIdx.x, r = x / CHUNKS;
+        const int x = i * kManyThreads + threadIdx.x, r = x / CHUNKS;
         v4u w = *(const v4u *)(vl + x * 16);
         const bool has = valid >> r & 1;
 #pragma unroll
@@ -660,29 +708,40 @@ __global__ __launch_bounds__(256, 2) void attention_many_kernel(const AttnArgs p
           s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, q[k], s[t], 0, 0, 0);
         }
       }
-      float top = -__builtin_inff();
+      if constexpr (Q8) {
 #pragma unroll
-      for (int t = 0; t < KT; ++t) {
+        for (int t = 0; t < KT; ++t) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          v4f ks = v4f{p.scale2, p.scale2, p.scale2, p.scale2};
-          if (Q8) ks = *(const v4f *)&scale_lds[buf][0][32 * t + 8 * j + 4 * h];
+          for (int j = 0; j < 4; ++j) {
+            const v4f ks = *(const v4f *)&scale_lds[buf][0][32 * t + 8 * j + 4 * h];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float x = s[t][4 * j + i] * ks[i];
-            if (edge) {
-              const int k = 32 * t + 8 * j + 4 * h + i;
-              if (!(k0 + k < sees && (valid >> k & 1))) x = -__builtin_inff();
-            }
-            s[t][4 * j + i] = x;
-            top = fmaxf(top, x);
+            for (int i = 0; i < 4; ++i) s[t][4 * j + i] *= ks[i];
           }
         }
       }
-      top = fmaxf(top, __shfl_xor(top, 32));
+      if (edge) {
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+          // this lane's keys are 8 (i / 4) + i % 4 from here
+          const uint32_t has = (uint32_t)(valid >> (32 * t)) >> (4 * h);
+          const int32_t ends = sees - k0 - 32 * t - 4 * h;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int k = 8 * (i / 4) + i % 4;
+            s[t][i] = (has >> k & 1) && k < ends ? s[t][i] : -__builtin_inff();
+          }
+        }
+      }
+      float top = s[0][0];
+#pragma unroll
+      for (int t = 0; t < KT; ++t) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[t][i]);
+      }
+      top = fmaxf(top, __shfl_xor(top, 32)) * scale2;
       if (__builtin_amdgcn_ballot_w64(top > m + 8.0f)) {
         const float m_new = top > m + 8.0f ? top : m;
-        const float alpha = exp2_f32(m - finite_max(m_new));
+        const float alpha = m_new == m ? 1.0f : exp2_f32(m - finite_max(m_new));
         m = m_new;
         l *= alpha;
 #pragma unroll
@@ -692,13 +751,13 @@ __global__ __launch_bounds__(256, 2) void attention_many_kernel(const AttnArgs p
         }
       }
       const float mf = finite_max(m);
+      v8bf pb[2 * KT];
 #pragma unroll
       for (int t = 0; t < KT; ++t) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const float e = exp2_f32(s[t][j] - mf);
-          l += e;
-          s[t][j] = e;
+        for (int i = 0; i < 16; ++i) {
+          s[t][i] = exp2_f32(__builtin_fmaf(s[t][i], scale2, -mf));
+          l += s[t][i];
         }
         if constexpr (Q8) {
 #pragma unroll
@@ -706,39 +765,37 @@ __global__ __launch_bounds__(256, 2) void attention_many_kernel(const AttnArgs p
             const v4f vs = *(const v4f *)&scale_lds[buf][1][32 * t + 8 * j + 4 * h];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const float x = s[t][4 * j + i] * vs[i];
+              const float e = s[t][4 * j + i];
               // (a masked key's scale may be anything)
-              s[t][4 * j + i] = edge && s[t][4 * j + i] == 0.0f ? 0.0f : x;
+              s[t][4 * j + i] = edge && e == 0.0f ? 0.0f : e * vs[i];
             }
           }
         }
-      }
-#pragma unroll
-      for (int t = 0; t < KT; ++t) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           v4u w;
 #pragma unroll
           for (int k = 0; k < 4; ++k) w[k] = round2(s[t][8 * c + 2 * k], s[t][8 * c + 2 * k + 1]);
-          const v8bf pb = __builtin_bit_cast(v8bf, w);
+          pb[2 * t + c] = __builtin_bit_cast(v8bf, w);
+        }
+      }
 #pragma unroll
-          for (int d = 0; d < DT; ++d) {
-            v4s half[2];
+      for (int tc = 0; tc < 2 * KT; ++tc) {
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
-              half[n] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                  (__attribute__((address_space(3))) v4s *)(uintptr_t)(
-                      va[d % VV_A] + at_buf + (32 * t + 16 * c + 8 * n) * ROW + d / VV_A * 256));
-            }
-            const v8s both = __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7);
-            acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, both), pb, acc[d], 0, 0, 0);
-          }
+        for (int d = 0; d < DT; ++d) {
+          v4s half[2];
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+            half[n] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s *)(uintptr_t)(
+                va[d % VV_A] + at_buf + (16 * tc + 8 * n) * ROW + d / VV_A * 256));
+          const v8s both = __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7);
+          acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, both), pb[tc], acc[d], 0, 0, 0);
         }
       }
     }
     if (!Q8 && edge_all && odd_lds) {
       // Infinities and NaN among the values: added key by key, to the rows
-      // that see them. (K's rows make room for the probabilities.)
+      // that see them. (K's and V's rows make room for the probabilities.)
       __syncthreads();
       float *const pl = (float *)lds[buf][0] + wave * 1024;
 #pragma unroll 1
@@ -749,12 +806,15 @@ __global__ __launch_bounds__(256, 2) void attention_many_kernel(const AttnArgs p
             pl[(8 * (j / 4) + 4 * h + j % 4) * 32 + col] = KT > 1 && t ? s[KT - 1][j] : s[0][j];
         }
         __builtin_amdgcn_wave_barrier();
+        pages_from = -64;  // (they are asked for again)
         const int32_t mine = slot_of_key(k0);
+        pages_from = -64;
 #pragma unroll 1
         for (int k = 0; k < 32 && !idle; ++k) {
           if (!(valid >> (32 * t + k) & 1)) continue;
-          const int64_t row = __builtin_amdgcn_readlane(mine, 32 * t + k);
+          const int64_t row = WHOLE ? mine + 32 * t + k : __builtin_amdgcn_readlane(mine, 32 * t + k);
           const float pk = pl[k * 32 + col];
+          const bool sees_it = k0 + 32 * t + k < sees;
 #pragma unroll
           for (int d = 0; d < DT; ++d) {
 #pragma unroll
@@ -763,7 +823,7 @@ __global__ __launch_bounds__(256, 2) void attention_many_kernel(const AttnArgs p
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const float v = bf16_to_float(i % 2 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu);
-                if (!(fabsf(v) < __builtin_inff()) && k0 + 32 * t + k < sees) acc[d][4 * j + i] += pk * v;
+                if (!(fabsf(v) < __builtin_inff()) && sees_it) acc[d][4 * j + i] += pk * v;
               }
             }
           }
@@ -795,18 +855,17 @@ __global__ __launch_bounds__(256, 2) void attention_many_kernel(const AttnArgs p
     }
     return;
   }
-  // through LDS, for whole rows
+  // through LDS (each wave its share), for whole rows
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  uint8_t *const mine = &lds[0][0][0] + wave * (4 * TILE / kWaves);
-  constexpr int FIT = 4 * TILE / kWaves / ROW;  // rows of a wave's share of LDS
-  static_assert(FIT >= 32, "the outputs fit");
+  uint8_t *const mine = &lds[0][0][0] + wave * TILE;
+  static_assert(TILE >= 32 * ROW, "the outputs fit");
 #pragma unroll
   for (int d = 0; d < DT; ++d) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const v2u w = v2u{round2(acc[d][4 * j] * inv, acc[d][4 * j + 1] * inv),
                         round2(acc[d][4 * j + 2] * inv, acc[d][4 * j + 3] * inv)};
-      *(v2u *)(mine + k_place(col, 4 * d + j) + 8 * h) = w;
+      *(v2u *)(mine + col * ROW + ((4 * d + j) ^ k_swap(col)) * 16 + 8 * h) = w;
     }
   }
   __builtin_amdgcn_wave_barrier();
@@ -814,11 +873,11 @@ __global__ __launch_bounds__(256, 2) void attention_many_kernel(const AttnArgs p
 #pragma unroll 4
   for (int r0 = 0; r0 < 32; r0 += AT_ONCE) {
     const int r = r0 + lane / LANES, c = lane % LANES;
-    const int32_t pk = u.row + 32 * wave + r;
+    const int32_t pk = row0 + r;
     if (pk > last) continue;
     const int32_t row = pk / p.group, hd = u.head * p.group + pk - row * p.group;
     *(v4u *)((uint16_t *)p.o.data + (int64_t)(u.lo + row) * p.o.row_ld + (int64_t)hd * p.o.head_ld + 8 * c) =
-        *(const v4u *)(mine + k_place(r, c));
+        *(const v4u *)(mine + r * ROW + (c ^ k_swap(r)) * 16);
   }
 }
 
@@ -860,7 +919,11 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttnArgs p) {
 template <int D, bool Q8>
 hipError_t launch_attention_d(const AttnArgs &a, bool bf16, bool many, int32_t units, hipStream_t s) {
   const dim3 grid((unsigned)(units * a.splits)), wg(64 * kWaves);
-  if (many) hipLaunchKernelGGL((attention_many_kernel<D, Q8, D == 256 ? 1 : 2>), grid, wg, 0, s, a);
+  constexpr int KT = D == 256 ? 1 : 2;
+  if (many && a.c.page_size % (32 * KT) == 0)
+    hipLaunchKernelGGL((attention_many_kernel<D, Q8, KT, true>), grid, dim3(kManyThreads), 0, s, a);
+  else if (many)
+    hipLaunchKernelGGL((attention_many_kernel<D, Q8, KT, false>), grid, dim3(kManyThreads), 0, s, a);
   else if (bf16) hipLaunchKernelGGL((attention_few_kernel<D, Q8, 1>), grid, wg, 0, s, a);
   else hipLaunchKernelGGL((attention_few_kernel<D, Q8, 3>), grid, wg, 0, s, a);
   hipError_t e = hipGetLastError();
@@ -896,7 +959,7 @@ hipError_t launch_attention(const HeadRows &q, const HeadRows &o, int64_t rows, 
     return hipErrorInvalidConfiguration;
   AttnArgs a = {q, o, b, c, (float)((double)scale * 1.4426950408889634), (int32_t)rows,
                 heads / c.heads, plan.tiles, plan.splits,
-                units * plan.splits <= 2 * cu_count() ? 1 : 0, part, err_flag};
+                many_resident(c.dim) == 2 && units * plan.splits <= 2 * cu_count() ? 1 : 0, part, err_flag};
   const auto launch = c.dim == 64    ? (c.q8 ? launch_attention_d<64, true> : launch_attention_d<64, false>)
                       : c.dim == 128 ? (c.q8 ? launch_attention_d<128, true> : launch_attention_d<128, false>)
                       : c.dim == 256 ? (c.q8 ? launch_attention_d<256, true> : launch_attention_d<256, false>)
