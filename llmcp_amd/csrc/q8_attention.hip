@@ -99,6 +99,44 @@ __device__ __forceinline__ int32_t part_keys(int32_t seen, int32_t splits) {
   return ((seen + splits - 1) / splits + step - 1) / step * step;
 }
 
+// The pages of a sequence from one on, a lane each: a load and its wait for 64 of
+// them.
+struct PageWindow {
+  int32_t pages = -1, from = -64;
+};
+
+// The cache's row of key k0 + lane (of KEYS; -1 for none), or (WHOLE: a page is a
+// multiple of KEYS) of key k0; there are keys up to k_hi.
+template <int KEYS, bool WHOLE>
+__device__ __forceinline__ int32_t slot_of_key(const AttnArgs &p, const Unit &u, int32_t k_hi, int lane,
+                                               int32_t k0, PageWindow &w) {
+  const int32_t end = max(min(k0 + KEYS, k_hi) - 1, 0) / p.c.page_size;
+  if (end >= w.from + 64) {
+    w.from = k0 / p.c.page_size;
+    w.pages = p.b.table[(int64_t)u.seq * p.b.max_pages + min(w.from + lane, p.b.max_pages - 1)];
+  }
+  const int32_t key = WHOLE ? k0 : k0 + (lane & (KEYS - 1));
+  const int32_t index = min(key, max(k_hi - 1, 0)) / p.c.page_size;
+  const int32_t page = WHOLE ? __builtin_amdgcn_readlane(w.pages, index - w.from) : __shfl(w.pages, index - w.from);
+  int32_t slot = -1;
+  if (key < k_hi) {
+    if ((uint32_t)page < (uint32_t)p.c.pages)
+      slot = (page * p.c.heads + u.head) * p.c.page_size + (key - index * p.c.page_size);
+    else if (page != -1)
+      *p.err_flag = 1;
+  }
+  return WHOLE ? __builtin_amdgcn_readfirstlane(slot) : slot;
+}
+
+// Which of a step's keys there are.
+template <int KEYS, bool WHOLE>
+__device__ __forceinline__ uint64_t keys_of(int32_t slot, int32_t k0, int32_t k_hi) {
+  constexpr uint64_t all = KEYS == 64 ? ~0ull : (1ull << 32) - 1;
+  if (!WHOLE) return __builtin_amdgcn_ballot_w64(slot >= 0) & all;
+  const int32_t n = k_hi - k0;
+  return slot < 0 || n <= 0 ? 0 : n >= KEYS ? all : (1ull << n) - 1;
+}
+
 // f32 as three bf16 parts, the sum exactly x (parts of an infinity or NaN: itself).
 __device__ __forceinline__ void split3(float x, uint32_t (&part)[3]) {
   const uint32_t b = __float_as_uint(x);
@@ -139,7 +177,7 @@ __device__ __forceinline__ float finite_max(float m) { return m == -__builtin_in
 // statistics and accumulator; they meet at the end.  K goes from memory to the
 // operand's registers, V through LDS (written row by row, read
 // transposed), each wave in its own 64 * D bytes.
-template <int D, bool Q8, int PARTS>
+template <int D, bool Q8, int PARTS, bool WHOLE>
 __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttnArgs p) {
   constexpr int STEPS = D / 32, DT = D / 16;
   constexpr int CHUNKS = D / 8;                // 16 B of bf16 in a row
@@ -201,49 +239,45 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttnArgs p)
 #pragma unroll
   for (int t = 0; t < DT; ++t) acc[t] = v4f{0, 0, 0, 0};
   uint8_t *const lds = tile_lds[wave];
+  PageWindow window;
 
   for (int32_t k0 = k_lo + wave * kBlockKeys; k0 < k_hi; k0 += kWaves * kBlockKeys) {
-    // lane k (and k + 32): the row of key k0 + k in the cache, -1 for none
-    int32_t slot = -1;
-    {
-      const int32_t key = k0 + (lane & 31);
-      if (key < k_hi) {
-        const int32_t index = key / p.c.page_size;
-        const int32_t page = page_at(p.b, p.c, u.seq, index, p.err_flag);
-        if (page >= 0)
-          slot = (page * p.c.heads + u.head) * p.c.page_size + (key - index * p.c.page_size);
-      }
-    }
-    const uint32_t valid = (uint32_t)__builtin_amdgcn_ballot_w64(slot >= 0);
+    // lane k (and k + 32): the row of key k0 + k in the cache (WHOLE: the first's)
+    const int32_t slot = slot_of_key<kBlockKeys, WHOLE>(p, u, k_hi, lane, k0, window);
+    const uint32_t valid = (uint32_t)keys_of<kBlockKeys, WHOLE>(slot, k0, k_hi);
     const int32_t at = max(slot, 0);  // (a row of the cache for those without one)
-    if (Q8) {
-      if (lane < 32) {
-        scale_lds[wave][0][lane] = p.c.ks[at] * p.scale2;
-        scale_lds[wave][1][lane] = p.c.vs[at];
-      }
+    constexpr int BYTES = Q8 ? D : 2 * D;
+    const uint8_t *const kp = (const uint8_t *)p.c.k + (WHOLE ? (int64_t)at * BYTES : 0);
+    const uint8_t *const vp = (const uint8_t *)p.c.v + (WHOLE ? (int64_t)at * BYTES : 0);
+    float ks_r = 0.0f, vs_r = 0.0f;
+    if (Q8 && lane < 32) {
+      ks_r = p.c.ks[WHOLE ? at + lane : at];
+      vs_r = p.c.vs[WHOLE ? at + lane : at];
     }
     // V on its way
     v4u vr[VL];
-    bool has[VL];
 #pragma unroll
     for (int i = 0; i < VL; ++i) {
       constexpr int PER = Q8 ? D / 16 : D / 8;  // lanes a row
-      const int r = i * (64 / PER) + lane / PER;
-      const int32_t row = __shfl(at, r);
-      has[i] = valid >> r & 1;
-      vr[i] = *(const v4u *)((const uint8_t *)p.c.v + (int64_t)row * (Q8 ? D : 2 * D) + lane % PER * 16);
+      if constexpr (WHOLE) {
+        vr[i] = *(const v4u *)(vp + i * 1024 + lane * 16);
+      } else {
+        const int32_t row = __shfl(at, i * (64 / PER) + lane / PER);
+        vr[i] = *(const v4u *)(vp + (int64_t)row * BYTES + lane % PER * 16);
+      }
     }
     // scores
     v4f s[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const int32_t row = __shfl(at, 16 * t + col);
+      const uint8_t *const kr = WHOLE ? kp + (16 * t + col) * BYTES + g * 16
+                                      : kp + (int64_t)__shfl(at, 16 * t + col) * BYTES + g * 16;
       s[t] = v4f{0, 0, 0, 0};
       if constexpr (Q8) {
         v4u w[D / 64];
 #pragma unroll
         for (int k = 0; k < D / 64; ++k)
-          w[k] = *(const v4u *)((const int8_t *)p.c.k + (int64_t)row * D + k * 64 + g * 16);
+          w[k] = *(const v4u *)(kr + k * 64);
 #pragma unroll
         for (int k = 0; k < STEPS; ++k) {
           const v8bf a = widen8(w[k / 2][k % 2 * 2], w[k / 2][k % 2 * 2 + 1]);
@@ -255,7 +289,7 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttnArgs p)
         v4u w[STEPS];
 #pragma unroll
         for (int k = 0; k < STEPS; ++k)
-          w[k] = *(const v4u *)((const uint16_t *)p.c.k + (int64_t)row * D + k * 32 + g * 8);
+          w[k] = *(const v4u *)(kr + k * 64);
 #pragma unroll
         for (int k = 0; k < STEPS; ++k) {
 #pragma unroll
@@ -269,7 +303,14 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttnArgs p)
     float vs[2][4];
     const bool edge = k0 + kBlockKeys > all_see || valid != 0xffffffffu;
     float top = -__builtin_inff();
+    if (Q8 && lane < 32) {
+      scale_lds[wave][0][lane] = ks_r * p.scale2;
+      scale_lds[wave][1][lane] = vs_r;
+    }
     __builtin_amdgcn_wave_barrier();
+    // this lane's keys are 16 t + i from here
+    const uint32_t has = valid >> (4 * g);
+    const int32_t ends = sees - k0 - 4 * g;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       v4f ks = v4f{p.scale2, p.scale2, p.scale2, p.scale2}, vv = v4f{1, 1, 1, 1};
@@ -279,16 +320,23 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttnArgs p)
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int k = 16 * t + 4 * g + i;
         s[t][i] = s[t][i] * ks[i];
         vs[t][i] = vv[i];
-        if (edge && !(k0 + k < sees && (valid >> k & 1))) {
-          s[t][i] = -__builtin_inff();
-          vs[t][i] = 0.0f;
-        }
-        top = fmaxf(top, s[t][i]);
       }
     }
+    if (edge) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool in = (has >> (16 * t + i) & 1) && 16 * t + i < ends;
+          s[t][i] = in ? s[t][i] : -__builtin_inff();
+          vs[t][i] = in ? vs[t][i] : 0.0f;
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = fmaxf(top, s[j / 4][j % 4]);
     top = fmaxf(top, __shfl_xor(top, 16));
     top = fmaxf(top, __shfl_xor(top, 32));
     const float m_new = fmaxf(m, top), mf = finite_max(m_new);
@@ -333,7 +381,7 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttnArgs p)
       constexpr int PER = Q8 ? D / 16 : D / 8;
       const int r = i * (64 / PER) + lane / PER, c = lane % PER;
       const int swap = 2 * (r & (CHUNKS / 2 - 1) & 7);
-      if (!has[i]) vr[i] = v4u{0, 0, 0, 0};
+      if (edge && !(valid >> r & 1)) vr[i] = v4u{0, 0, 0, 0};
       if constexpr (Q8) {
         *(v8bf *)(lds + r * 2 * D + ((2 * c) ^ swap) * 16) = widen8(vr[i][0], vr[i][1]);
         *(v8bf *)(lds + r * 2 * D + ((2 * c + 1) ^ swap) * 16) = widen8(vr[i][2], vr[i][3]);
@@ -361,11 +409,11 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttnArgs p)
 #pragma unroll 1
       for (int k = 0; k < kBlockKeys; ++k) {
         if (!(valid >> k & 1)) continue;
-        const int32_t row = __builtin_amdgcn_readlane(at, k);
+        const int64_t row = WHOLE ? at + k : __builtin_amdgcn_readlane(at, k);
         const float pk = odd_lds[wave][k * kTileRows + col];
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
-          const v2u w = *(const v2u *)((const uint16_t *)p.c.v + (int64_t)row * D + 16 * t + 4 * g);
+          const v2u w = *(const v2u *)((const uint16_t *)p.c.v + row * D + 16 * t + 4 * g);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float v = bf16_to_float(i % 2 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu);
@@ -553,34 +601,10 @@ __global__ __launch_bounds__(kManyThreads, many_resident(D)) void attention_many
     for (int d = 0; d < VV_A; ++d) va[d] = base + TILE + (vb ^ (64u * d));
   }
 
-  // The cache's row of key k0 + lane (of KEYS; -1 for none), or (WHOLE) of key k0.
-  // Lane i holds the page after i others: a load and its wait per 64 pages.
-  int32_t pages = -1, pages_from = -64;
-  auto slot_of_key = [&](int32_t k0) {
-    const int32_t end = max(min(k0 + KEYS, k_hi) - 1, 0) / p.c.page_size;
-    if (end >= pages_from + 64) {
-      pages_from = k0 / p.c.page_size;
-      pages = p.b.table[(int64_t)u.seq * p.b.max_pages + min(pages_from + lane, p.b.max_pages - 1)];
-    }
-    const int32_t key = WHOLE ? k0 : k0 + (lane & (KEYS - 1));
-    const int32_t index = min(key, max(k_hi - 1, 0)) / p.c.page_size;
-    const int32_t page = WHOLE ? __builtin_amdgcn_readlane(pages, index - pages_from) : __shfl(pages, index - pages_from);
-    int32_t slot = -1;
-    if (key < k_hi) {
-      if ((uint32_t)page < (uint32_t)p.c.pages)
-        slot = (page * p.c.heads + u.head) * p.c.page_size + (key - index * p.c.page_size);
-      else if (page != -1)
-        *p.err_flag = 1;
-    }
-    return WHOLE ? __builtin_amdgcn_readfirstlane(slot) : slot;
-  };
+  PageWindow window;
+  auto slot_at = [&](int32_t k0) { return slot_of_key<KEYS, WHOLE>(p, u, k_hi, lane, k0, window); };
+  auto mask_of = [&](int32_t slot, int32_t k0) { return keys_of<KEYS, WHOLE>(slot, k0, k_hi); };
   constexpr uint64_t kAll = KEYS == 64 ? ~0ull : (1ull << 32) - 1;
-  // Which of the step's keys there are.
-  auto mask_of = [&](int32_t slot, int32_t k0) -> uint64_t {
-    if (!WHOLE) return __builtin_amdgcn_ballot_w64(slot >= 0) & kAll;
-    const int32_t n = k_hi - k0;
-    return slot < 0 || n <= 0 ? 0 : n >= KEYS ? kAll : (1ull << n) - 1;
-  };
 
   v4u kr[Q8 ? LOADS : 1], vr[Q8 ? LOADS : 1];
   float ks_r = 0.0f, vs_r = 0.0f;
@@ -657,7 +681,7 @@ __global__ __launch_bounds__(kManyThreads, many_resident(D)) void attention_many
     }
   };
 
-  int32_t slot = slot_of_key(k_lo);
+  int32_t slot = slot_at(k_lo);
   uint64_t valid = mask_of(slot, k_lo);
   ask(slot, 0);
   keep(valid, 0);
@@ -666,7 +690,7 @@ __global__ __launch_bounds__(kManyThreads, many_resident(D)) void attention_many
   __syncthreads();
   int buf = 0;
   for (int32_t k0 = k_lo; k0 < k_hi; k0 += KEYS, buf ^= 1) {
-    slot = slot_of_key(k0 + KEYS);
+    slot = slot_at(k0 + KEYS);
     const uint64_t next_valid = mask_of(slot, k0 + KEYS);
     if (k0 + KEYS < k_hi) ask(slot, buf ^ 1);
     uint8_t *const vl = lds[buf][1];
@@ -806,9 +830,9 @@ __global__ __launch_bounds__(kManyThreads, many_resident(D)) void attention_many
             pl[(8 * (j / 4) + 4 * h + j % 4) * 32 + col] = KT > 1 && t ? s[KT - 1][j] : s[0][j];
         }
         __builtin_amdgcn_wave_barrier();
-        pages_from = -64;  // (they are asked for again)
-        const int32_t mine = slot_of_key(k0);
-        pages_from = -64;
+        window.from = -64;  // (the pages are asked for again)
+        const int32_t mine = slot_at(k0);
+        window.from = -64;
 #pragma unroll 1
         for (int k = 0; k < 32 && !idle; ++k) {
           if (!(valid >> (32 * t + k) & 1)) continue;
@@ -891,24 +915,33 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const AttnArgs p) {
   const int32_t parts = step_keys ? (u.seen + step_keys - 1) / step_keys : 0;
   if (parts <= 1) return;
   const float *const from = p.part + ((int64_t)unit * p.splits * TILE + 16 * sub) * (D + 4);
-  for (int i = threadIdx.x; i < 16 * (D / 4); i += 256) {
+  const int32_t live = min(16, u.n * p.group - u.row - 16 * sub);
+  // a part's weight in its row: a lane per part
+  __shared__ float weight[16][64], whole[16];
+  const int lane = threadIdx.x & 63;
+  for (int r = threadIdx.x >> 6; r < live; r += 4) {
+    v2u st = v2u{0xff800000u, 0u};  // (-inf, 0)
+    if (lane < parts) st = *(const v2u *)(from + (int64_t)(lane * TILE + r) * (D + 4) + D);
+    const float m = __uint_as_float(st[0]);
+    float top = m;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+    const float f = exp2_f32(m - finite_max(top));
+    float total = f * __uint_as_float(st[1]);
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) total += __shfl_xor(total, d);
+    weight[r][lane] = f;
+    if (lane == 0) whole[r] = total == 0.0f ? 0.0f : 1.0f / total;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < live * (D / 4); i += 256) {
     const int r = i / (D / 4), c = i % (D / 4);
     const int32_t pk = u.row + 16 * sub + r;
-    if (pk >= u.n * p.group) break;
-    float top = -__builtin_inff();
-    for (int32_t s = 0; s < parts; ++s) top = fmaxf(top, from[(int64_t)(s * TILE + r) * (D + 4) + D]);
-    const float mf = finite_max(top);
     v4f sum = v4f{0, 0, 0, 0};
-    float total = 0.0f;
-#pragma unroll 4
-    for (int32_t s = 0; s < parts; ++s) {
-      const float *const at = from + (int64_t)(s * TILE + r) * (D + 4);
-      const float f = exp2_f32(at[D] - mf);
-      total += f * at[D + 1];
-      sum = sum + *(const v4f *)(at + 4 * c) * f;
-    }
-    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-    sum = sum * inv;
+#pragma unroll 8
+    for (int32_t s = 0; s < parts; ++s)
+      sum = sum + *(const v4f *)(from + (int64_t)(s * TILE + r) * (D + 4) + 4 * c) * weight[r][s];
+    sum = sum * whole[r];
     const int32_t row = pk / p.group, h = u.head * p.group + pk - row * p.group;
     const int64_t to = (int64_t)(u.lo + row) * p.o.row_ld + (int64_t)h * p.o.head_ld + 4 * c;
     if (p.o.bf16) *(v2u *)((uint16_t *)p.o.data + to) = v2u{pack2(sum[0], sum[1]), pack2(sum[2], sum[3])};
@@ -924,8 +957,12 @@ hipError_t launch_attention_d(const AttnArgs &a, bool bf16, bool many, int32_t u
     hipLaunchKernelGGL((attention_many_kernel<D, Q8, KT, true>), grid, dim3(kManyThreads), 0, s, a);
   else if (many)
     hipLaunchKernelGGL((attention_many_kernel<D, Q8, KT, false>), grid, dim3(kManyThreads), 0, s, a);
-  else if (bf16) hipLaunchKernelGGL((attention_few_kernel<D, Q8, 1>), grid, wg, 0, s, a);
-  else hipLaunchKernelGGL((attention_few_kernel<D, Q8, 3>), grid, wg, 0, s, a);
+  else if (bf16 && a.c.page_size % kBlockKeys == 0)
+    hipLaunchKernelGGL((attention_few_kernel<D, Q8, 1, true>), grid, wg, 0, s, a);
+  else if (bf16) hipLaunchKernelGGL((attention_few_kernel<D, Q8, 1, false>), grid, wg, 0, s, a);
+  else if (a.c.page_size % kBlockKeys == 0)
+    hipLaunchKernelGGL((attention_few_kernel<D, Q8, 3, true>), grid, wg, 0, s, a);
+  else hipLaunchKernelGGL((attention_few_kernel<D, Q8, 3, false>), grid, wg, 0, s, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.splits == 1) return e;
   if (many) hipLaunchKernelGGL((attention_join_kernel<D, kManyRows>), dim3((unsigned)units * (kManyRows / 16)), wg, 0, s, a);
