@@ -761,7 +761,8 @@ class Context:
             ctypes.byref(bi), float(key_dim ** -0.5 if scale is None else scale),
             0 if eps is None else 1, 0.0 if eps is None else float(eps),
             _ptr(row_starts) if row_starts is not None else None, int(sequences),
-            _ptr(state) if state is not None else None, _ptr(new_state), ctypes.byref(yo)))
+            _ptr(state) if state is not None else None,
+            _ptr(new_state) if new_state is not None else None, ctypes.byref(yo)))
 
     def swiglu(self, x, wg, wu, h, m, mode="decode", dtype="f32"):
         xi = f32_memref(x.ptr if hasattr(x, "ptr") else x, m, wg.cols)
