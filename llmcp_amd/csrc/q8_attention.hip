@@ -977,12 +977,22 @@ AttentionPlan attention_plan(int64_t rows, int32_t heads, bool bf16, const KvBat
   AttentionPlan plan;
   const int64_t group = heads / c.heads;
   const int64_t steps = ((int64_t)b.max_pages * c.page_size + kWaves * kBlockKeys - 1) / (kWaves * kBlockKeys);
-  plan.many = bf16 && rows * group >= 64 * (int64_t)b.sequences && rows * heads >= 16384;
+  // Tiles of 128 rows where a sequence's rows (times the group) fill one on
+  // average. Measured, us with tiles of 16 against 128: 16 heads over 4 of 256, 2048
+  // keys, one sequence of 16 / 32 / 64 rows 28 / 30 / 44 against 30 / 32 / 37, eight
+  // of them 59 / 110 / 135 against 40 / 45 / 92; 8192 Q8 keys, eight sequences of 16 /
+  // 32 rows 107 / 195 against 154 / 101; 8 heads of 64, 1024 keys, one sequence of
+  // 128 / 512 rows 15 / 25 against 17 / 22. (f32 rows, of three times the operands,
+  // always take tiles of 16.)
+  plan.many = bf16 && rows * group >= kManyRows * (int64_t)b.sequences;
   if (test_kernel && bf16) plan.many = test_kernel == 2;
   const int64_t tile = plan.many ? kManyRows : kTileRows;
   plan.tiles = (int32_t)(rows * group / tile + std::min<int64_t>(b.sequences, rows));
   const int64_t units = (int64_t)plan.tiles * c.heads;
-  plan.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({steps, (plan.many ? 512 : 2048) / units, 64}));
+  // Parts of the keys until there are 2 workgroups per CU (tiles of 128 rows) or 8
+  // (of 16, two resident at a time: the rest evens out sequences of unlike lengths),
+  // up to a lane each in the kernel that joins them.
+  plan.splits = (int32_t)std::max<int64_t>(1, std::min<int64_t>({steps, (plan.many ? 2 : 8) * cu_count() / units, 64}));
   if (test_splits > 0) plan.splits = (int32_t)std::min<int64_t>(steps, test_splits);
   if (plan.splits > 1) plan.part_floats = units * plan.splits * tile * (c.dim + 4);
   return plan;

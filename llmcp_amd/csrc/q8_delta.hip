@@ -286,8 +286,10 @@ __device__ __forceinline__ bool finite(float v) { return fabsf(v) < __builtin_in
 template <int KD>
 __global__ __launch_bounds__(256) void delta_chunk_kernel(const ChunkArgs p) {
   constexpr int KS = KD / 32, LD = 68;
-  __shared__ __align__(16) v4u kt[4][KS][64];
+  // K's rows make room for T: 53.5 KB, three workgroups per CU
   __shared__ __align__(16) float lm[kChunk][LD], am[kChunk][LD], tm[kChunk][LD];
+  v4u (*const kt)[KS][64] = (v4u (*)[KS][64])&tm[0][0];
+  static_assert(sizeof(v4u) * 4 * KS * 64 <= sizeof(float) * kChunk * LD, "K's rows fit");
   __shared__ double run[kChunk];
   __shared__ float kn[kChunk], qn[kChunk], bt[kChunk];
   __shared__ int odd;
@@ -943,8 +945,15 @@ hipError_t launch_delta_chunks(const DeltaLaunch &l, void *workspace, hipStream_
 
 }  // namespace
 
+// Chunks from a mean of 10 rows per sequence on where the scan's workgroups are
+// resident at once, of 16 where they are not. Measured on 32 heads of 128 x 128, us
+// of 8 / 12 / 16 / 24 rows one after another against in chunks: one sequence 15 /
+// 20 / 25 / 34 against 15 for all; 8 sequences 29 / 40 / 51 / 72 against 51; 32
+// sequences 84 / 119 / 155 / 235 against 172. (f32 rows always go one after another:
+// their products would not be exact in bf16.)
 bool delta_chunked(const DeltaLaunch &l) {
-  return l.q.bf16 && l.rows >= 16 * (int64_t)l.sequences;
+  const int64_t least = (int64_t)l.sequences * l.heads * (l.value_dim / 16) <= cu_count() ? 10 : 16;
+  return l.q.bf16 && l.rows >= least * l.sequences;
 }
 
 int64_t delta_workspace(const DeltaLaunch &l) {
