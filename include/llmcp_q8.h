@@ -599,8 +599,8 @@ enum llmcp_q8_cache_format { LLMCP_Q8_CACHE_BF16 = 0, LLMCP_Q8_CACHE_Q8 = 1 };
 /* Pages of keys and values in device memory, each [pages, kv_heads, page_size,
  * head_dim] dense and 16 B aligned; Q8: int8 with the scales [pages, kv_heads,
  * page_size].  head_dim 64, 128 or 256; page_size up to 2^20, of any value (a
- * contiguous cache is one page per sequence), and max_pages * page_size and
- * pages * kv_heads * page_size below 2^31; declined otherwise. */
+ * contiguous cache is one page per sequence), and max_pages * page_size below 2^30
+ * and pages * kv_heads * page_size below 2^31; declined otherwise. */
 typedef struct {
   void *keys, *values;
   float *key_scales, *value_scales; /* Q8, else null */

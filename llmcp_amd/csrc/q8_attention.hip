@@ -1002,7 +1002,7 @@ hipError_t launch_attention(const HeadRows &q, const HeadRows &o, int64_t rows, 
                             const KvBatch &b, const KvPages &c, float scale, const AttentionPlan &plan,
                             float *part, int32_t *err_flag, hipStream_t s) {
   const int64_t units = (int64_t)plan.tiles * c.heads;
-  if (rows < 1 || units < 1 || units * plan.splits > 0x7FFFFF || (plan.splits > 1 && !part))
+  if (rows < 1 || units < 1 || units * plan.splits > kMaxMixerBlocks || (plan.splits > 1 && !part))
     return hipErrorInvalidConfiguration;
   AttnArgs a = {q, o, b, c, (float)((double)scale * 1.4426950408889634), (int32_t)rows,
                 heads / c.heads, plan.tiles, plan.splits,

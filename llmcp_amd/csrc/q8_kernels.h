@@ -242,7 +242,7 @@ struct KvBatch {
   const int32_t *starts = nullptr, *lengths = nullptr, *table = nullptr;
   int32_t sequences = 0, max_pages = 0;
 };
-constexpr int64_t kMaxMixerRows = 1 << 23;
+constexpr int64_t kMaxMixerRows = 1 << 23, kMaxMixerBlocks = 0x7FFFFF;
 constexpr int32_t kMaxSequences = 65536, kMaxHeads = 1024, kMaxPageSize = 1 << 20;
 
 // Rows of keys and values to their slots, and back.

@@ -299,7 +299,7 @@ int check_cache(const llmcp_q8_kv_cache *cache, const llmcp_q8_kv_batch *batch, 
     return fail(LLMCP_Q8_DECLINED, "a cache of %lld pages of %d slots of %d heads",
                 (long long)cache->pages, cache->page_size, cache->kv_heads);
   if (batch->sequences < 1 || batch->sequences > kMaxSequences || batch->max_pages < 1 ||
-      (int64_t)batch->max_pages * cache->page_size > 0x7FFFFFFFll)
+      (int64_t)batch->max_pages * cache->page_size >= 1ll << 30)
     return fail(LLMCP_Q8_DECLINED, "%d sequences of up to %d pages", batch->sequences,
                 batch->max_pages);
   if ((uintptr_t)cache->keys % 16 || (uintptr_t)cache->values % 16)
@@ -2112,6 +2112,9 @@ static int attention_impl(llmcp_q8_ctx *ctx, const Heads &q, const llmcp_q8_kv_c
   if ((rc = set_device(ctx))) return rc;
   const AttentionPlan plan = attention_plan(q.rows, (int32_t)q.heads, q.h.bf16, b, c,
                                             ctx->test_attention, ctx->test_attention_splits);
+  if ((int64_t)plan.tiles * c.heads * plan.splits > kMaxMixerBlocks)
+    return fail(LLMCP_Q8_DECLINED, "too many rows or sequences for one launch (%lld, %d)", (long long)q.rows,
+                b.sequences);
   if (plan.part_floats &&
       (rc = grow(ctx, ctx->attention_part, ctx->attention_part_bytes, (uint64_t)plan.part_floats * 4,
                  "attention's parts")))

@@ -49,9 +49,9 @@ def test_caches_invalid(q8, kw):
 
 def test_batches(q8):
     assert status(q8, cache(q8), batch(q8, sequences=65536)) == q8.OK
-    assert status(q8, cache(q8), batch(q8, max_pages=(1 << 27) - 1)) == q8.OK
+    assert status(q8, cache(q8), batch(q8, max_pages=(1 << 26) - 1)) == q8.OK
     for kw in ({"sequences": 0}, {"sequences": -1}, {"sequences": 65537}, {"max_pages": 0},
-               {"max_pages": 1 << 27}, {"max_pages": -4}):
+               {"max_pages": 1 << 26}, {"max_pages": -4}):
         assert status(q8, cache(q8), batch(q8, **kw)) == q8.DECLINED
     for name in ("row_starts", "lengths", "page_table"):
         assert status(q8, cache(q8), batch(q8, **{name: None})) == q8.EINVAL
