@@ -584,8 +584,8 @@ int llmcp_q8_expert_mlp_rows_bf16(llmcp_q8_ctx *ctx, const llmcp_q8_rows *input,
  * A call takes the rows of several sequences, one sequence after another:
  * sequence s has the rows row_starts[s] .. row_starts[s + 1] - 1, none where
  * the two are equal.  row_starts ascends within 0 .. rows (bounds outside are
- * taken as 0 or rows; where it descends, rows of several sequences hold the
- * result of one of them); rows before the first and from the last on are left as
+ * taken as 0 or rows; where it descends, what the calls leave for the sequences
+ * is undefined, and nothing outside their memory is touched); rows before the first and from the last on are left as
  * they were.  Up to 2^23 rows, 65536 sequences and 1024 heads; more is
  * declined. */
 
@@ -644,7 +644,7 @@ int llmcp_q8_kv_read_bf16(llmcp_q8_ctx *ctx, const llmcp_q8_kv_cache *cache,
 
 /* Attention of the rows over their sequences' keys (which the call's own rows
  * are among: write them first): query head h of the row at position p gives
- * sum over j <= p of softmax_j(scale * q . k_j) v_j with the keys and values of
+ * sum over j <= p of softmax_j(scale * q . k_j) v_j (|scale| up to 1e38) with the keys and values of
  * kv head h / (heads / kv_heads) that the slots stand for.  heads is a multiple
  * of kv_heads, queries and output are [rows, heads, head_dim].  Positions
  * without a slot are not seen, whatever their memory holds; a row that sees no key,

@@ -2106,6 +2106,7 @@ static int attention_impl(llmcp_q8_ctx *ctx, const Heads &q, const llmcp_q8_kv_c
   if (q.rows == 0) return LLMCP_Q8_OK;
   if (q.h.data == out.h.data)
     return fail(LLMCP_Q8_EINVAL, "attention's output must not take its queries' memory");
+  if (!(std::fabs(scale) <= 1e38f)) return fail(LLMCP_Q8_EINVAL, "attention's scale must be finite, up to 1e38");
   if (q.rows * q.heads > 1ll << 26)
     return fail(LLMCP_Q8_DECLINED, "too many rows of heads for one launch (%lld)",
                 (long long)(q.rows * q.heads));

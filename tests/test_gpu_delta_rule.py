@@ -237,3 +237,35 @@ def test_replayed(q8, ctx, oracle, n):
         c.check(ctx, 0.1, 1e-6, y, s)
         other.call(ctx, 0.1, 1e-6)
     ctx.graph_destroy(graph)
+
+
+@pytest.mark.parametrize("inplace", [False, True])
+def test_more_chunks_than_the_workspace_holds(q8, ctx, oracle, inplace):
+    """1024 heads leave room for 8 chunks at a time: sequences that end, begin and
+    go on in a later window, and one without rows."""
+    if ctx.platform != "aarch64":
+        pytest.skip("the same kernels on either platform")
+    rng = np.random.default_rng(31)
+    c = Case(oracle, rng, [530, 0, 40, 200], 1, 1024, 64, 16, "bf16").upload(ctx)
+    if inplace:
+        c.call(ctx, 0.125, 1e-6, new_state=c.ds)
+        c.check(ctx, 0.125, 1e-6, *c.results(ctx, c.ds))
+    else:
+        c.call(ctx, 0.125, 1e-6)
+        c.check(ctx, 0.125, 1e-6, *c.results(ctx))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_descending_starts_stay_in_bounds(q8, ctx, oracle, dtype):
+    """Bounds that descend give every other sequence all rows: nothing behind
+    the states and the output is touched."""
+    rng = np.random.default_rng(37)
+    c = Case(oracle, rng, [40] * 30, 1, 1, 64, 16, dtype)
+    c.rows, c.starts = 40, np.asarray([0, 40] * 15 + [0], np.int32)
+    c.upload(ctx)
+    guard = ctx.to_device(np.full((31,) + c.shape[1:], 5, F32))
+    y = ctx.to_device(np.full((44, 1, 16), 7, c.bits.dtype))
+    c.y = y
+    c.call(ctx, 0.125, 1e-6, new_state=guard)
+    assert (ctx.to_host(guard, (31,) + c.shape[1:], F32)[30] == 5).all()
+    assert (ctx.to_host(y, (44, 1, 16), c.bits.dtype)[40:] == 7).all()

@@ -241,6 +241,8 @@ def test_refusals(q8, ctx, oracle):
     refused(q8.DECLINED, ctx.attention, x, cache, batch, y, 4, 3, dtype="bf16")  # 3 heads over 2
     refused(q8.EINVAL, ctx.attention, x, cache, batch, x, 4, 4, dtype="bf16")
     refused(q8.EINVAL, ctx.kv_read, cache, batch, x, x, 4, dtype="bf16")
+    for scale in (np.nan, np.inf, -np.inf):
+        refused(q8.EINVAL, ctx.attention, x, cache, batch, y, 4, 4, scale=scale, dtype="bf16")
     refused(q8.DECLINED, ctx.attention, x.ptr + 2, cache, batch, y, 4, 4, dtype="bf16")
     wrong = Cache(q8, ctx, rng, [20], 16, 2, 128, "bf16").cache()
     wrong.head_dim = 96
