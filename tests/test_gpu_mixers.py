@@ -259,3 +259,40 @@ def test_refusals(q8, ctx, oracle):
         full.update(kw)
         refused(code, ctx.delta_rule, *args, ctx.alloc(1 << 16), **full)
     refused(q8.EINVAL, ctx.delta_rule, x, y, x, g, g, x, 4, 2, 2, 64, 32, new_state=s, dtype="bf16")
+
+
+@pytest.mark.parametrize("n", [150, 1])
+@pytest.mark.parametrize("fmt", ["bf16", "q8"])
+def test_caches_above_4_gib(q8, ctx, oracle, fmt, n):
+    """Pages whose bytes lie past 32 bits: written, read back and attended."""
+    if ctx.platform != "aarch64":
+        pytest.skip("the same kernels on either platform")
+    rng = np.random.default_rng(61)
+    kvh, dim, page, length = 4, 256, 64, 200
+    pages = 40000 if fmt == "bf16" else 80000  # 5.2 GB of keys, as much of values
+    each = pages * kvh * page * dim * (2 if fmt == "bf16" else 1)
+    assert each > 1 << 32
+    bufs = [ctx.alloc(each) for _ in range(2)]
+    scales = [ctx.alloc(pages * kvh * page * 4) for _ in range(2)] if fmt == "q8" else [None, None]
+    cache = q8.KVCache(*bufs, pages, page, kvh, dim, key_scales=scales[0], value_scales=scales[1])
+    table = np.asarray([[pages - 1, 0, pages - 3, pages // 2 + 9000]], np.int32)
+    keep = [ctx.to_device(np.asarray(a, np.int32)) for a in ([0, length], [length], table, [0, n])]
+    fill = q8.KVBatch(keep[0], keep[1], keep[2], 1, 4)
+    kb, vb, qb = (oracle.f32_to_bf16_bits(rng.standard_normal(shape).astype(F32))
+                  for shape in ((length, kvh, dim), (length, kvh, dim), (n, 16, dim)))
+    ctx.kv_write(ctx.to_device(kb), ctx.to_device(vb), cache, fill, length, dtype="bf16")
+    out = [ctx.to_device(np.zeros(kb.shape, F32)) for _ in range(2)]
+    ctx.kv_read(cache, fill, out[0], out[1], length)
+    k, v = (ctx.to_host(o, kb.shape, F32) for o in out)
+    for got, bits in ((k, kb), (v, vb)):
+        want = oracle.bf16_bits_to_f32(bits)
+        step = 0 if fmt == "bf16" else np.abs(want).max(-1, keepdims=True) / 127 * (0.5 + 2.0 ** -10)
+        assert (np.abs(got - want) <= step).all()
+    y = ctx.to_device(np.zeros(qb.shape, np.uint16))
+    ctx.attention(ctx.to_device(qb), cache, q8.KVBatch(keep[3], keep[1], keep[2], 1, 4), y, n, 16,
+                  dtype="bf16")
+    want, bound = attention_reference(oracle.bf16_bits_to_f32(qb), k, v, dim ** -0.5, length - n, True)
+    got = oracle.bf16_bits_to_f32(ctx.to_host(y, qb.shape, np.uint16))
+    assert (np.abs(got - want) <= bound).all()
+    for b in bufs + [s for s in scales if s]:
+        b.free()
