@@ -454,6 +454,78 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttnArgs p)
     __builtin_amdgcn_wave_barrier();
   }
 
+  if constexpr (!Q8 && PARTS > 1) {
+    // An infinity among the keys or values times a part of q or p that is 0 is NaN,
+    // and stays in the sums: f32 rows whose sums are not finite take the wave's steps
+    // again, key by key in f32. (The same steps once more, with a look at every
+    // value, cost all calls registers: 12 to 24 % at dim 256.)
+    float worst = 0.0f;
+#pragma unroll
+    for (int t = 0; t < DT; ++t) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) worst = __builtin_fmaf(acc[t][i], 0.0f, worst);
+    }
+    worst += __shfl_xor(worst, 16);
+    worst += __shfl_xor(worst, 32);
+    if (__builtin_amdgcn_ballot_w64(!(worst == 0.0f))) {
+      // (the tile's other rows keep theirs)
+      const float m_had = m, l_had = l;
+      m = -__builtin_inff(), l = 0.0f;
+#pragma unroll
+      for (int t = 0; t < DT; ++t) {
+        *(v4f *)(lds + (t * 64 + lane) * 16) = acc[t];
+        acc[t] = v4f{0, 0, 0, 0};
+      }
+      window = PageWindow();
+      // a quarter of the row's dims, g's
+      const float *const mine = (const float *)p.q.data + (int64_t)(u.lo + i_row) * p.q.row_ld +
+                                (int64_t)head * p.q.head_ld + g * (D / 4);
+#pragma unroll 1
+      for (int32_t k0 = k_lo + wave * kBlockKeys; k0 < k_hi; k0 += kWaves * kBlockKeys) {
+        const int32_t slot = slot_of_key<kBlockKeys, WHOLE>(p, u, k_hi, lane, k0, window);
+        const uint32_t valid = (uint32_t)keys_of<kBlockKeys, WHOLE>(slot, k0, k_hi);
+        const int32_t at = max(slot, 0);
+#pragma unroll 1
+        for (int k = 0; k < kBlockKeys; ++k) {
+          if (!(valid >> k & 1)) continue;
+          const int64_t row = (WHOLE ? at + k : __builtin_amdgcn_readlane(at, k)) * (int64_t)D;
+          const bool in = k0 + k < sees;
+          float score = 0.0f;
+#pragma unroll 4
+          for (int d = 0; d < D / 4; d += 4) {
+            const v4f x = *(const v4f *)(mine + d);
+            const v2u w = *(const v2u *)((const uint16_t *)p.c.k + row + g * (D / 4) + d);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              score = __builtin_fmaf(x[i], bf16_to_float(i % 2 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu), score);
+          }
+          score += __shfl_xor(score, 16);
+          score += __shfl_xor(score, 32);
+          score = in ? score * p.scale2 : -__builtin_inff();
+          const float m_new = fmaxf(m, score), mf = finite_max(m_new);
+          const float alpha = exp2_f32(m - mf), e = exp2_f32(score - mf);
+          m = m_new;
+          l = l * alpha + e;
+#pragma unroll
+          for (int t = 0; t < DT; ++t) {
+            const v2u w = *(const v2u *)((const uint16_t *)p.c.v + row + 16 * t + 4 * g);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float v = bf16_to_float(i % 2 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu);
+              acc[t][i] = __builtin_fmaf(e, in ? v : 0.0f, acc[t][i] * alpha);
+            }
+          }
+        }
+      }
+      l = g == 0 ? l : 0.0f;  // (each lane has the row's whole sum)
+      if (worst == 0.0f) {
+        m = m_had, l = l_had;
+#pragma unroll
+        for (int t = 0; t < DT; ++t) acc[t] = *(const v4f *)(lds + (t * 64 + lane) * 16);
+      }
+    }
+  }
+
   // the four waves' sums meet
   l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);

@@ -1,0 +1,139 @@
+"""llmcp_q8_attention with infinities and NaN among the keys and values that rows
+see, with scores that leave f32, and where the low bits of f32 rows decide.
+
+What is expected comes row by row from the definition in float64 over the keys
+that the row sees, with IEEE's rules for infinities: a score of -inf is a weight
+of 0, one of +inf or NaN makes the row NaN, an infinite value that has a weight
+makes its column infinite.  Finite results keep to the bound of
+test_gpu_attention.py."""
+import numpy as np
+import pytest
+
+from kv_reference import F32, Cache, rows_of
+from test_gpu_attention import filled, forced, reference  # noqa: F401 (a fixture)
+
+pytestmark = pytest.mark.gpu
+
+U32 = 2.0 ** -24  # half a step of f32
+
+# (dtype, kernel, splits): f32 rows always take tiles of 16
+KINDS = [("f32", 0, 0), ("f32", 1, 3), ("bf16", 1, 1), ("bf16", 1, 3), ("bf16", 2, 1), ("bf16", 2, 2)]
+
+
+@pytest.fixture(autouse=True)
+def once(ctx):
+    if ctx.platform != "aarch64":
+        pytest.skip("the same kernels on either platform")
+
+
+def some(n):
+    """Rows of n that are looked at, those around the middle and the ends among them."""
+    return sorted({i for i in range(n) if i % 7 == 0 or abs(i - n // 2) < 3 or n - i < 4})
+
+
+def attend(q8, ctx, oracle, c, ns, lengths, q, dtype, scale):
+    """Rows q (values of dtype) [sum ns, heads, dim] through the call, as f32."""
+    bits = oracle.f32_to_bf16_bits(q) if dtype == "bf16" else q
+    y = ctx.to_device(np.full(q.shape, 7, bits.dtype))
+    ctx.attention(ctx.to_device(bits), c.cache(), c.batch(np.concatenate([[0], np.cumsum(ns)]), lengths),
+                  y, q.shape[0], q.shape[1], scale=scale, dtype=dtype)
+    got = ctx.to_host(y, q.shape, bits.dtype)
+    return oracle.bf16_bits_to_f32(got) if dtype == "bf16" else got
+
+
+@pytest.mark.parametrize("page", [16, 20, 64])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("n", [1, 75])
+@pytest.mark.parametrize("kind", KINDS)
+def test_infinite_keys(q8, ctx, oracle, forced, kind, n, dim, page):
+    """Keys whose score is -inf have no weight, wherever they stand; one whose
+    score is +inf makes the rows that see it NaN; the other kv head's rows keep
+    their values.  The queries fit bf16, so f32 rows have parts that are 0."""
+    dtype, kernel, splits = kind
+    forced(kernel, splits)
+    rng = np.random.default_rng(dim + n)
+    length = 400
+    c = filled(q8, ctx, oracle, rng, [length], page, 2, dim, "bf16")
+    _, q = rows_of(oracle, rng, n, 4, dim, "bf16", 2.0)
+    q[:, :, 1], q[:, 1, 1] = 1.0, 1.5
+    lowest = [3, 40, 41, 200, 319, length - n, length - 1]
+    for at in lowest:
+        c.k[c.table[0, at // page], 0, at % page, 1] = 0xFF80
+    c.upload()
+    kk, vv = c.values(oracle, 0, 0, length)
+    keep = np.ones(length, bool)
+    keep[lowest] = False
+    got = attend(q8, ctx, oracle, c, [n], [length], q, dtype, 0.2)
+    for i in some(n):
+        use = np.arange(length) <= length - n + i
+        want, bound = reference(q[i:i + 1, 2:], kk[use, 1:], vv[use, 1:], 0.2, length, dtype == "bf16")
+        assert (np.abs(got[i, 2:] - want[0]) <= bound[0]).all()
+        use &= keep
+        want, bound = reference(q[i:i + 1, :2], kk[use, :1], vv[use, :1], 0.2, length, dtype == "bf16")
+        assert (np.abs(got[i, :2] - want[0]) <= bound[0]).all()
+    at = length - (n + 1) // 2
+    c.k[c.table[0, at // page], 0, at % page, 1] = 0x7F80
+    c.upload()
+    again = attend(q8, ctx, oracle, c, [n], [length], q, dtype, 0.2)
+    sees = length - n + np.arange(n) >= at
+    assert np.isnan(again[sees, :2]).all()
+    assert np.array_equal(again[:, 2:], got[:, 2:]) and np.array_equal(again[~sees], got[~sees])
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_scores_of_minus_infinity_alone(q8, ctx, oracle, forced, kind):
+    """Give zeros, also of f32 rows whose values fit bf16."""
+    dtype, kernel, splits = kind
+    forced(kernel, splits)
+    rng = np.random.default_rng(5)
+    c = filled(q8, ctx, oracle, rng, [200, 200], 16, 1, 64, "bf16")
+    c.k[c.table[0], 0, :, 1] = 0xFF80
+    c.upload()
+    _, q = rows_of(oracle, rng, 4, 2, 64, "bf16")
+    q[:, :, 1] = 1.0
+    got = attend(q8, ctx, oracle, c, [2, 2], [200, 200], q, dtype, 0.1)
+    assert (got[:2] == 0).all() and np.isfinite(got).all() and (got[2:] != 0).all()
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "q8"])
+@pytest.mark.parametrize("page", [16, 20, 64])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("n", [1, 75])
+@pytest.mark.parametrize("kind", KINDS)
+def test_odd_values(q8, ctx, oracle, forced, kind, n, dim, page, fmt):
+    """Infinite and NaN values, seen by all rows and by some: an infinity keeps
+    its sign, in its column and head alone (of a Q8 row with one, whose values
+    read back as NaN, in all columns); all else keeps to the bound."""
+    dtype, kernel, splits = kind
+    forced(kernel, splits)
+    rng = np.random.default_rng(dim + n)
+    length, kvh = 400, 3
+    c = filled(q8, ctx, oracle, rng, [length + 30], page, kvh, dim, fmt)
+    _, q = rows_of(oracle, rng, n, 6, dim, dtype, 1.0)
+    clean_k, clean_v = c.values(oracle, 0, 0, length)
+    # (position, kv head, column, value); the two of kv head 0's column 9 meet
+    odd = [(37, 0, 9, np.inf), (length - n // 2 - 1, 0, 20, -np.inf), (length - 2, 0, 9, -np.inf),
+           (length - 1, 1, 0, np.inf), (length - n, 1, dim - 1, np.nan), (length, 2, 4, np.inf)]
+    if fmt == "q8":
+        odd = [o for o in odd if o[0] != 37]
+    for at, h, col, x in odd:
+        slot = c.table[0, at // page], h, at % page
+        if fmt == "bf16":
+            c.v[slot][col] = {np.inf: 0x7F80, -np.inf: 0xFF80}.get(x, 0x7FC0)
+        else:
+            c.vs[slot] = np.nan
+    c.upload()
+    got = attend(q8, ctx, oracle, c, [n], [length], q, dtype, 0.05)
+    for i in some(n):
+        last = length - n + i
+        want, bound = reference(q[i:i + 1], clean_k[:last + 1], clean_v[:last + 1], 0.05, length, dtype == "bf16")
+        expect, loose = want[0].copy(), bound[0].copy()
+        for at, h, col, x in odd:
+            if at <= last:
+                here = np.s_[2 * h:2 * h + 2, col] if fmt == "bf16" else np.s_[2 * h:2 * h + 2]
+                value = x if fmt == "bf16" else np.nan
+                with np.errstate(invalid="ignore"):
+                    expect[here] = expect[here] + value
+        fine = np.isfinite(expect)
+        assert np.array_equal(got[i][~fine], expect[~fine].astype(F32), equal_nan=True)
+        assert (np.abs(got[i][fine] - expect[fine]) <= loose[fine]).all()
