@@ -648,8 +648,9 @@ int llmcp_q8_kv_read_bf16(llmcp_q8_ctx *ctx, const llmcp_q8_kv_cache *cache,
  * kv head h / (heads / kv_heads) that the slots stand for.  heads is a multiple
  * of kv_heads, queries and output are [rows, heads, head_dim].  Positions
  * without a slot are not seen, whatever their memory holds; a row that sees no key,
- * or only scores of -inf, gives zeros.  Scores, softmax and sums are f32; of
- * bf16 rows the probabilities (times a Q8 value's scale) are rounded to bf16
+ * or only scores of -inf, gives zeros.  Scores, softmax and sums are f32 (a score
+ * past f32 counts as infinite: below, the key has no weight; above, or NaN, the row
+ * is NaN); of bf16 rows the probabilities (times a Q8 value's scale) are rounded to bf16
  * before they meet the values, f32 rows take products exact to f32.
  * Workspaces grow on the first call of a size: make it eagerly before
  * capturing it into a graph.  How keys are split over workgroups, and with it the

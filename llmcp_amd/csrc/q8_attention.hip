@@ -314,7 +314,7 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttnArgs p)
     const bool edge = k0 + kBlockKeys > all_see || valid != 0xffffffffu;
     float top = -__builtin_inff();
     if (Q8 && lane < 32) {
-      scale_lds[wave][0][lane] = ks_r * p.scale2;
+      scale_lds[wave][0][lane] = ks_r;
       scale_lds[wave][1][lane] = vs_r;
     }
     __builtin_amdgcn_wave_barrier();
@@ -323,16 +323,14 @@ __global__ __launch_bounds__(256, 2) void attention_few_kernel(const AttnArgs p)
     const int32_t ends = sees - k0 - 4 * g;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      v4f ks = v4f{p.scale2, p.scale2, p.scale2, p.scale2}, vv = v4f{1, 1, 1, 1};
+      v4f vv = v4f{1, 1, 1, 1};
       if (Q8) {
-        ks = *(const v4f *)&scale_lds[wave][0][16 * t + 4 * g];
+        s[t] = s[t] * *(const v4f *)&scale_lds[wave][0][16 * t + 4 * g];
         vv = *(const v4f *)&scale_lds[wave][1][16 * t + 4 * g];
       }
+      s[t] = s[t] * p.scale2;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s[t][i] = s[t][i] * ks[i];
-        vs[t][i] = vv[i];
-      }
+      for (int i = 0; i < 4; ++i) vs[t][i] = vv[i];
     }
     if (edge) {
 #pragma unroll
@@ -656,6 +654,7 @@ __global__ __launch_bounds__(kManyThreads, many_resident(D)) void attention_many
     }
   }
   float m = -__builtin_inff(), l = 0.0f;
+  bool far = false;  // whether |m| is 2^20 or more
   v16f acc[DT];
 #pragma unroll
   for (int t = 0; t < DT; ++t) {
@@ -845,7 +844,11 @@ __global__ __launch_bounds__(kManyThreads, many_resident(D)) void attention_many
         for (int i = 0; i < 16; ++i) top = fmaxf(top, s[t][i]);
       }
       top = fmaxf(top, __shfl_xor(top, 32)) * scale2;
-      if (__builtin_amdgcn_ballot_w64(top > m + 8.0f)) {
+      // Exponents are s * scale2 - m in one rounding. What m's own rounding leaves is the
+      // same for all keys and small, but of scores from 2^20 on may grow past exp2:
+      // those, and infinite ones, are rounded before m is taken off.
+      float by = scale2, from = far ? 0.0f : finite_max(m);
+      if (__builtin_amdgcn_ballot_w64(top > m + 8.0f || far)) {
         const float m_new = top > m + 8.0f ? top : m;
         const float alpha = m_new == m ? 1.0f : exp2_f32(m - finite_max(m_new));
         m = m_new;
@@ -855,14 +858,24 @@ __global__ __launch_bounds__(kManyThreads, many_resident(D)) void attention_many
 #pragma unroll
           for (int i = 0; i < 16; ++i) acc[t][i] *= alpha;
         }
+        from = finite_max(m);
+        far = !(fabsf(from) < 0x1p20f);
+        if (__builtin_amdgcn_ballot_w64(far)) {
+#pragma unroll
+          for (int t = 0; t < KT; ++t) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[t][i] = far ? s[t][i] * scale2 - from : s[t][i];
+          }
+          by = far ? 1.0f : by;
+          from = far ? 0.0f : from;
+        }
       }
-      const float mf = finite_max(m);
       v8bf pb[2 * KT];
 #pragma unroll
       for (int t = 0; t < KT; ++t) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          s[t][i] = exp2_f32(__builtin_fmaf(s[t][i], scale2, -mf));
+          s[t][i] = exp2_f32(__builtin_fmaf(s[t][i], by, -from));
           l += s[t][i];
         }
         if constexpr (Q8) {

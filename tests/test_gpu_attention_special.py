@@ -137,3 +137,44 @@ def test_odd_values(q8, ctx, oracle, forced, kind, n, dim, page, fmt):
         fine = np.isfinite(expect)
         assert np.array_equal(got[i][~fine], expect[~fine].astype(F32), equal_nan=True)
         assert (np.abs(got[i][fine] - expect[fine]) <= loose[fine]).all()
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "q8"])
+@pytest.mark.parametrize("scale", [1e30, -1e30, 1e38, 3e37, 100.0, -1e4])
+@pytest.mark.parametrize("kind", KINDS)
+def test_scores_past_f32(q8, ctx, oracle, forced, kind, scale, fmt):
+    """A score that f32 has no number for counts as infinite: above, the row is
+    NaN; below, the key has no weight.  Queries and keys of one value each, so that
+    q . k is exact: 127 * 2^20, which 1e30 takes to 1.3e38 (times log2 e 1.9e38),
+    a number still, and the others past 3.4e38."""
+    dtype, kernel, splits = kind
+    forced(kernel, splits)
+    rng = np.random.default_rng(8)
+    length, n, dim = 300, 40, 64
+    sign = 1.0 if scale > 0 else -1.0
+    c = Cache(q8, ctx, rng, [length], 16, 1, dim, fmt)
+    k = np.zeros((length, 1, dim), F32)
+    k[::3, 0, 5] = -127.0 * 2.0 ** 10 * sign  # scores of -inf
+    k[270, 0, 5] = 127.0 * 2.0 ** 10 * sign   # of +inf where q is positive
+    v = rng.standard_normal((length, 1, dim)).astype(F32)
+    c.put(oracle, 0, 0, k, v)
+    c.upload()
+    q = np.zeros((n, 2, dim), F32)
+    q[:, 0, 5] = 2.0 ** 10
+    got = attend(q8, ctx, oracle, c, [n], [length], q, dtype, scale)
+    _, vv = c.values(oracle, 0, 0, length)
+    for i in range(n):
+        last = length - n + i
+        even = np.zeros((1, 1, dim), F32)
+        use = np.arange(length) <= last
+        want, bound = reference(even, np.zeros((use.sum(), 1, dim)), vv[use], 1.0, length, dtype == "bf16")
+        assert (np.abs(got[i, 1] - want[0, 0]) <= bound[0, 0]).all()
+        if last >= 270 and abs(scale) > 1e30:
+            assert np.isnan(got[i, 0]).all()
+            continue
+        if last >= 270:  # that key alone
+            assert (np.abs(got[i, 0] - vv[270, 0]) <= (2.0 ** -7 if dtype == "bf16" else 2 * U32) * np.abs(vv[270, 0])).all()
+            continue
+        use &= k[:, 0, 5] == 0
+        want, bound = reference(even, np.zeros((use.sum(), 1, dim)), vv[use], 1.0, length, dtype == "bf16")
+        assert (np.abs(got[i, 0] - want[0, 0]) <= bound[0, 0]).all()
