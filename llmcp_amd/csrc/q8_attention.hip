@@ -638,9 +638,8 @@ __global__ __launch_bounds__(kManyThreads, many_resident(D)) void attention_many
   const int32_t all_see = seen_by(u.row);  // what every row of the tile sees
   const int32_t wave_all = seen_by(min(row0, last));
   const int32_t wave_seen = row0 > last ? 0 : seen_by(min(row0 + 31, last));
-  // (the scale's sign goes into q; a scale of 0 is next to it, so that a masked
-  // score stays -inf)
-  const float scale2 = fmaxf(fabsf(p.scale2), 0x1p-126f);
+  // (the scale's sign goes into q; it is not 0, so that a masked score stays -inf)
+  const float scale2 = fabsf(p.scale2);
   v8bf q[STEPS];
   {
     const int32_t i_row = live ? packed / p.group : 0;
@@ -1068,7 +1067,7 @@ hipError_t launch_attention_d(const AttnArgs &a, bool bf16, bool many, int32_t u
 }  // namespace
 
 AttentionPlan attention_plan(int64_t rows, int32_t heads, bool bf16, const KvBatch &b, const KvPages &c,
-                             int32_t test_kernel, int32_t test_splits) {
+                             float scale, int32_t test_kernel, int32_t test_splits) {
   AttentionPlan plan;
   const int64_t group = heads / c.heads;
   const int64_t steps = ((int64_t)b.max_pages * c.page_size + kWaves * kBlockKeys - 1) / (kWaves * kBlockKeys);
@@ -1081,6 +1080,9 @@ AttentionPlan attention_plan(int64_t rows, int32_t heads, bool bf16, const KvBat
   // always take tiles of 16.)
   plan.many = bf16 && rows * group >= kManyRows * (int64_t)b.sequences;
   if (test_kernel && bf16) plan.many = test_kernel == 2;
+  // Tiles of 128 rows mask before they scale: a scale of 0 would make a masked score
+  // NaN, one next to it is not a normal number once it meets log2 e.
+  if (!(fabsf(scale) >= 0x1p-100f)) plan.many = false;
   const int64_t tile = plan.many ? kManyRows : kTileRows;
   plan.tiles = (int32_t)(rows * group / tile + std::min<int64_t>(b.sequences, rows));
   const int64_t units = (int64_t)plan.tiles * c.heads;

@@ -263,7 +263,7 @@ struct AttentionPlan {
 // (test_kernel 1 / 2: tiles of 16 / 128 rows forced, test_splits > 0: so many
 // parts; for tests.)
 AttentionPlan attention_plan(int64_t rows, int32_t heads, bool bf16, const KvBatch &b, const KvPages &c,
-                             int32_t test_kernel, int32_t test_splits);
+                             float scale, int32_t test_kernel, int32_t test_splits);
 hipError_t launch_attention(const HeadRows &q, const HeadRows &o, int64_t rows, int32_t heads,
                             const KvBatch &b, const KvPages &c, float scale, const AttentionPlan &plan,
                             float *part, int32_t *err_flag, hipStream_t s);

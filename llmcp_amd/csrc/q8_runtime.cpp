@@ -2111,7 +2111,7 @@ static int attention_impl(llmcp_q8_ctx *ctx, const Heads &q, const llmcp_q8_kv_c
     return fail(LLMCP_Q8_DECLINED, "too many rows of heads for one launch (%lld)",
                 (long long)(q.rows * q.heads));
   if ((rc = set_device(ctx))) return rc;
-  const AttentionPlan plan = attention_plan(q.rows, (int32_t)q.heads, q.h.bf16, b, c,
+  const AttentionPlan plan = attention_plan(q.rows, (int32_t)q.heads, q.h.bf16, b, c, scale,
                                             ctx->test_attention, ctx->test_attention_splits);
   if ((int64_t)plan.tiles * c.heads * plan.splits > kMaxMixerBlocks)
     return fail(LLMCP_Q8_DECLINED, "too many rows or sequences for one launch (%lld, %d)", (long long)q.rows,

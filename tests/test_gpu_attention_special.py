@@ -178,3 +178,29 @@ def test_scores_past_f32(q8, ctx, oracle, forced, kind, scale, fmt):
         use &= k[:, 0, 5] == 0
         want, bound = reference(even, np.zeros((use.sum(), 1, dim)), vv[use], 1.0, length, dtype == "bf16")
         assert (np.abs(got[i, 0] - want[0, 0]) <= bound[0, 0]).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("scale", [0.0, -0.0, 1e-38, 1e-45])
+def test_scales_next_to_zero(q8, ctx, oracle, forced, kind, scale):
+    """A scale of 0 weighs every key alike, however large q . k; 0 times an
+    infinite one is NaN.  q . k is 2^127 here, so a scale of 1e-38 or 1e-45 still
+    gives scores of 1.7 and 2.4e-7."""
+    dtype, kernel, splits = kind
+    forced(kernel, splits)
+    rng = np.random.default_rng(9)
+    length, n, dim = 150, 36, 64
+    c = Cache(q8, ctx, rng, [length], 32, 2, dim, "bf16")
+    k = np.zeros((length, 2, dim), F32)
+    k[::2, :, 3] = 2.0 ** 64
+    v = rng.standard_normal((length, 2, dim)).astype(F32)
+    c.put(oracle, 0, 0, k, v)
+    c.k[c.table[0, 0], 1, 7, 3] = 0x7F80
+    c.upload()
+    q = np.zeros((n, 4, dim), F32)
+    q[:, :, 3] = 2.0 ** 63
+    got = attend(q8, ctx, oracle, c, [n], [length], q, dtype, scale)
+    kk, vv = c.values(oracle, 0, 0, length)
+    want, bound = reference(q[:, :2], kk[:, :1], vv[:, :1], float(F32(scale)), length - n, dtype == "bf16")
+    assert (np.abs(got[:, :2] - want) <= bound).all()
+    assert np.isnan(got[:, 2:]).all()
