@@ -197,7 +197,7 @@ struct ChunkData {
   float q_in[kChunk];   // exp(G_i) scale over |q_i|
   float k_out[kChunk];  // exp(G_63 - G_i) over |k_i|
   float decay[64];      // exp(G_63), for every lane
-  int32_t odd[64];      // whether an infinity or NaN is among q, k, decay or beta
+  int32_t odd[64];      // whether the chunk has to go row by row
 };
 static_assert(sizeof(ChunkData) % 256 == 0, "aligned");
 __device__ constexpr int a_block(int w, int s) { return (w / 2) * 2 + (w % 2) + (w / 2) * s + (w / 2 ? (w % 2) : 0); }
@@ -351,7 +351,11 @@ __global__ __launch_bounds__(256) void delta_chunk_kernel(const ChunkArgs p) {
     const float b = live ? l.beta[row * l.beta_ld + head] : 0.0f;
     // what decays below e^-10000 is nothing; the sum stays finite
     if (d < -1e4f) d = -1e4f;
-    if (!finite(d) || !finite(b)) odd = 1;
+    // Where decays grow the state, what is written over later still stands in exp(G)
+    // and in T, times up to e to the sum of the rises, and has to cancel there: by
+    // e at most (two bits), else row by row.
+    const float rise = wave_sum(fmaxf(d, 0.0f));
+    if (!finite(d) || !finite(b) || !(rise <= 1.0f)) odd = 1;
     double sum = (double)d;
 #pragma unroll
     for (int n = 1; n < 64; n *= 2) {
