@@ -498,7 +498,7 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const ChunkArgs p) {
   __shared__ __align__(16) v4f bl[4][64];
   __shared__ float red[2][4][2][16];
   __shared__ float red3[2][4][3];
-  __shared__ int odd_v[2][16];  // columns with an infinity or NaN among the chunk's values
+  __shared__ int odd_v[2][16];  // columns with an infinity or NaN among the chunk's values or U
   const DeltaLaunch &l = p.l;
   const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
   const int which = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -611,7 +611,7 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const ChunkArgs p) {
       }
       // An infinity or NaN would reach rows before its own, by 0 times it: its
       // column (every column, if it is not in the values) goes row by row below.
-      const bool mine_odd = odd_all || odd_v[buf][col];
+      bool mine_odd = odd_all || odd_v[buf][col];
       __builtin_amdgcn_sched_barrier(0);
       // V - diag(k_in) K S0
       {
@@ -638,7 +638,6 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const ChunkArgs p) {
       }
       ask_v(rows_of(min(n + 1, to - 1)) - 1);
       __builtin_amdgcn_sched_barrier(0);
-      const bool slow = __builtin_amdgcn_ballot_w64(mine_odd) != 0;
       __syncthreads();
       if (threadIdx.x < 16) odd_v[buf ^ 1][threadIdx.x] = 0;  // (set after the next barrier but one)
       // U
@@ -667,12 +666,16 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const ChunkArgs p) {
         split4<2>(u, part);
 #pragma unroll
         for (int i = 0; i < 2; ++i) up[i][wave][lane] = part[i];
+        // (as would U where it left f32, parts of an infinity being none; x is not
+        // finite where u is not)
+        if (!finite((x[0] + x[1]) + (x[2] + x[3]))) odd_v[buf][col] = 1;
       }
       __builtin_amdgcn_sched_barrier(0);
       ask_t();
       __builtin_amdgcn_sched_barrier(0);
       __syncthreads();
       // the state after the chunk
+      mine_odd |= odd_v[buf][col] != 0;
       v4f old[TW];
       {
         v4s kt[TW][2][2];
@@ -716,7 +719,7 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const ChunkArgs p) {
           for (int i = 0; i < 4; ++i) state[t][i] = __builtin_fmaf(decay_now, state[t][i], x[i]);
         }
       }
-      if (slow) {
+      if (__builtin_amdgcn_ballot_w64(mine_odd)) {
         for (int32_t r = 0; r < live; ++r) {
           const int64_t rr = range.lo + n * kChunk + r;
           const uint16_t *const kp = (const uint16_t *)l.k.data + rr * l.k.row_ld + key_head * l.k.head_ld;
@@ -851,7 +854,6 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const ChunkArgs p) {
   for (int32_t n = from; n < to; ++n) {
     const int32_t live = rows_of(n);
     const int buf = n & 1;
-    const bool odd_all = __builtin_amdgcn_readfirstlane(odd_chunk) != 0;
     const uint32_t last_next = rows_of(min(n + 1, to - 1)) - 1;
     __syncthreads();
     v2u sv[2][TILES];
@@ -860,8 +862,6 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const ChunkArgs p) {
 #pragma unroll
       for (int t = 0; t < TILES; ++t) sv[i][t] = sp[i][t][lane];
     }
-    const bool mine_odd = odd_all || odd_v[buf][col];
-    const bool slow = __builtin_amdgcn_ballot_w64(mine_odd) != 0;
     __builtin_amdgcn_sched_barrier(0);
     v4f qs[2];
     qs[0] = qs[1] = v4f{0, 0, 0, 0};
@@ -887,6 +887,7 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const ChunkArgs p) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) ul[i][t] = up[i][t][lane];
     }
+    const bool mine_odd = (__builtin_amdgcn_readfirstlane(odd_chunk) != 0) | (odd_v[buf][col] != 0);
     __builtin_amdgcn_sched_barrier(0);
     v4f o = v4f{0, 0, 0, 0}, o2 = o;
 #pragma unroll
@@ -911,7 +912,7 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const ChunkArgs p) {
     op += (int64_t)kChunk * o_ld;
     if (n + 1 < to) dp += data_step;
     ask_a();
-    if (slow) {
+    if (__builtin_amdgcn_ballot_w64(mine_odd)) {
       for (int32_t r = 0; r < live; ++r) __syncthreads();  // (with the rows of the other waves)
     }
   }

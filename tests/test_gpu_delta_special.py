@@ -129,3 +129,37 @@ def test_small_growth_keeps_its_digits(q8, ctx, oracle, dtype, n):
         chunked = dtype == "bf16" and n > 9
         most = np.exp(np.abs(c.x["decay"][i * n:(i + 1) * n]).sum(0)) * ref.rms(exact)
         assert ref.share(s[i], exact, f32, chunked, most, 6 if chunked else n).max() <= 1
+
+
+@pytest.mark.parametrize("dtype,n", CASES)
+@pytest.mark.parametrize("kind", ["beta", "difference", "sum"])
+def test_what_leaves_f32_on_the_way(q8, ctx, oracle, dtype, n, kind):
+    """Finite inputs whose u is infinite: by beta times a value, by the difference of
+    a large value and the state's, by the sum of a key with a state's column.  The
+    rows before and the other columns keep their values."""
+    c = Call(oracle, 11, n, dtype)
+    row = {150: 42, 8: 3, 40: 17}[n]
+    if kind == "beta":
+        c.x["v"][row, 1, 5], c.x["beta"][row, 1] = 3e38, 2.0
+    elif kind == "difference":
+        c.x["v"][row, 1, 5], c.x["v"][row + 1, 1, 5] = 3e38, -3e38
+        c.x["k"][row + 1] = c.x["k"][row]
+        c.x["beta"][row:row + 2, 1], c.x["decay"][row:row + 2, 1] = 1.0, 0.0
+    else:
+        # keys and queries of one dim each, large states where they are not
+        c.eps = None
+        for a in "qk":
+            c.x[a][:] = 0
+            for i in range(2 * n):
+                c.x[a][i, :, i % n % 40] = 1
+        c.x["k"][row, 0] = 0
+        c.x["k"][row, 0, 48:60] = 1
+        c.state[0, 1, 48:60, 5], c.x["decay"][:n, 1] = 2e38, 0.0
+    c.x["v"] = ref.bf16(c.x["v"])
+    y, s = c.run(q8, ctx)
+    c.check(y, 0, row)
+    c.check(y, 0, n, heads=np.arange(VH) != 1)
+    c.check(y, 0, n, columns=np.arange(VD) != 5)
+    c.check(y, 1, n)
+    assert not np.isfinite(y[n - 1, 1, 5]) or kind == "sum"
+    assert not np.isfinite(s[0, 1, :, 5]).all()
