@@ -204,3 +204,82 @@ def test_scales_next_to_zero(q8, ctx, oracle, forced, kind, scale):
     want, bound = reference(q[:, :2], kk[:, :1], vv[:, :1], float(F32(scale)), length - n, dtype == "bf16")
     assert (np.abs(got[:, :2] - want) <= bound).all()
     assert np.isnan(got[:, 2:]).all()
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "q8"])
+@pytest.mark.parametrize("page", [16, 20])
+def test_low_bits_of_f32_queries_decide(q8, ctx, oracle, page, fmt):
+    """q's values differ from 1 + 2^-8 by a few 2^-17 and meet keys of +-2^17 c, so
+    that a score is what the last 8 of q's 24 bits say; all products and sums are
+    exact in f32.  With the leading 16 bits alone every weight would be the same."""
+    rng = np.random.default_rng(21)
+    length, n, dim = 90, 3, 64
+    c = Cache(q8, ctx, rng, [length], page, 1, dim, fmt)
+    k = np.zeros((length, 1, dim), F32)
+    at = rng.integers(0, dim // 2, length)
+    size = rng.integers(1, 3, length).astype(F32) * F32(2.0 ** 17)
+    for j in range(length):
+        k[j, 0, 2 * at[j]], k[j, 0, 2 * at[j] + 1] = size[j], -size[j]
+    v = rng.standard_normal((length, 1, dim)).astype(F32)
+    c.put(oracle, 0, 0, k, v)
+    c.upload()
+    kk, vv = c.values(oracle, 0, 0, length)
+    q = np.full((n, 2, dim), 1 + 2.0 ** -8, F32)
+    q[:, :, ::2] += rng.integers(0, 4, (n, 2, dim // 2)).astype(F32) * F32(2.0 ** -17)
+    got = attend(q8, ctx, oracle, c, [n], [length], q, "f32", 0.5)
+    # exact scores but for their scale (and of Q8 a step's rounding, in kk): a
+    # rounding each for scale, scale * log2 e, a Q8 scale and the product, and the
+    # exponential's, the sums' and the result's
+    for i in range(n):
+        seen = length - n + i + 1
+        for h in range(2):
+            s = 0.5 * (kk[:seen, 0].astype(np.float64) @ q[i, h].astype(np.float64))
+            p = np.exp(s - s.max())
+            p /= p.sum()
+            want = p @ vv[:seen, 0].astype(np.float64)
+            ep = (8 * np.abs(s).max() + seen + 64) * U32
+            assert (np.abs(got[i, h] - want) <= ep * (p @ np.abs(vv[:seen, 0])) + U32 * np.abs(want)).all()
+            flat = vv[:seen, 0].mean(0)
+            assert np.abs(flat - want).max() > 0.05  # (what the leading 16 bits alone give)
+
+
+@pytest.mark.parametrize("page", [16, 20])
+def test_low_bits_of_f32_weights_decide(q8, ctx, oracle, page):
+    """Two keys of weights 1 and 1 - d, d a few 2^-19, with values +-V: the result is
+    V d / 2 next to V.  Two parts of a weight hold 16 bits, which would be off by up
+    to 2^-17 V."""
+    length, dim = 2, 64
+    rng = np.random.default_rng(22)
+    c = Cache(q8, ctx, rng, [length], page, 1, dim, "bf16")
+    k, v = np.zeros((2, length, 1, dim), F32)
+    k[1, 0, 0] = -1.0
+    v[0], v[1] = 1024.0, -1024.0
+    c.put(oracle, 0, 0, k, v)
+    c.upload()
+    q = np.zeros((1, 12, dim), F32)
+    d = (np.arange(12) + 0.37) * 2.0 ** -19
+    q[0, :, 0] = d.astype(F32)
+    got = attend(q8, ctx, oracle, c, [1], [length], q, "f32", 1.0)
+    p = np.exp(-d.astype(F32).astype(np.float64))
+    want = 1024.0 * (1 - p) / (1 + p)
+    # a step of f32 (2^-23) for each of the exponential, the rounded exponent and
+    # the sums, of weights next to 1
+    bound = 1024.0 * 4 * 2.0 ** -23 / 2
+    assert (np.abs(got[0] - want[:, None]) <= bound).all()
+    two = (np.floor(p * 2.0 ** 16) / 2.0 ** 16)
+    assert (np.abs(1024.0 * (1 - two) / (1 + two) - want) > bound).sum() > 6
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "q8"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("ns,lengths", [
+    ([260] + [1] * 9, [700] + [7 * i + 30 for i in range(9)]),
+    ([1] * 40 + [150], [11 * i + 1 for i in range(40)] + [150]),
+    ([1, 900, 0, 1, 2], [1300, 1000, 50, 3, 2])])
+def test_a_prompt_among_single_rows(q8, ctx, oracle, ns, lengths, dtype, fmt):
+    """One call of a chunk of many rows and sequences of one row, either way around."""
+    from test_gpu_attention import run
+    rng = np.random.default_rng(31)
+    c = filled(q8, ctx, oracle, rng, lengths, 32, 2, 64, fmt)
+    _, q = rows_of(oracle, rng, sum(ns), 8, 64, dtype, 2.0)
+    run(q8, ctx, oracle, c, ns, lengths, q, dtype, 0.125)

@@ -131,6 +131,50 @@ def test_small_growth_keeps_its_digits(q8, ctx, oracle, dtype, n):
         assert ref.share(s[i], exact, f32, chunked, most, 6 if chunked else n).max() <= 1
 
 
+@pytest.mark.parametrize("value", ["nan", "inf", "-inf"])
+@pytest.mark.parametrize("where", ["q", "k", "v", "decay", "beta", "state"])
+@pytest.mark.parametrize("dtype,n", CASES)
+def test_odd_inputs(q8, ctx, oracle, dtype, n, where, value):
+    """One infinity or NaN, of key head 0 (value heads 0 and 1) or value head 1:
+    rows before it, the other heads, the other sequence and, of a value or a
+    state's element, the other columns keep their values; a query's leaves the rows
+    after it and the state alone too."""
+    if where == "decay" and value == "-inf":
+        pytest.skip("a decay to nothing, not an odd value")
+    c = Call(oracle, 7, n, dtype)
+    base_y, base_s = c.run(q8, ctx)
+    row = {150: 74, 8: 3, 40: 17}[n]
+    clean = {a: x.copy() for a, x in c.x.items()}
+    states = c.state.copy()
+    x = {"nan": np.nan, "inf": np.inf, "-inf": -np.inf}[value]
+    heads = [0, 1] if where in "qk" else [1]
+    at = {"q": (row, 0, 9), "k": (row, 0, 9), "v": (row, 1, 5), "decay": (row, 1), "beta": (row, 1)}
+    if where == "state":
+        c.state[0, 1, 20, 5] = x
+        row = 0
+    else:
+        c.x[where][at[where]] = x
+    y, s = c.run(q8, ctx)
+    c.x, c.state = clean, states
+    others = np.array([h not in heads for h in range(VH)])
+    assert np.array_equal(y[:, others], base_y[:, others]) and np.array_equal(y[n:], base_y[n:])
+    assert np.array_equal(s[0, others], base_s[0, others]) and np.array_equal(s[1], base_s[1])
+    c.check(y, 0, row)
+    if where in ("v", "state"):
+        columns = np.arange(VD) != 5
+        assert np.array_equal(y[..., columns], base_y[..., columns])
+        assert np.array_equal(s[..., columns], base_s[..., columns])
+        assert not np.isfinite(y[row:n, 1, 5]).any() and not np.isfinite(s[0, 1, :, 5]).all()
+    elif where == "q":
+        assert not np.isfinite(y[row, heads]).any()
+        o, exact, most = c.exact(0, n)
+        later = ref.output_share(y[row + 1:n], o[row + 1:], most[row + 1:])
+        assert (later <= 1).all()
+        assert ref.share(s[0], exact, c.exact(0, n, F32)[1], False, ref.rms(c.state[0]) + 1, n).max() <= 1
+    else:
+        assert not np.isfinite(y[row + 1:n, heads]).any() and not np.isfinite(s[0, heads]).all((1, 2)).any()
+
+
 @pytest.mark.parametrize("dtype,n", CASES)
 @pytest.mark.parametrize("kind", ["beta", "difference", "sum"])
 def test_what_leaves_f32_on_the_way(q8, ctx, oracle, dtype, n, kind):
@@ -163,3 +207,19 @@ def test_what_leaves_f32_on_the_way(q8, ctx, oracle, dtype, n, kind):
     c.check(y, 1, n)
     assert not np.isfinite(y[n - 1, 1, 5]) or kind == "sum"
     assert not np.isfinite(s[0, 1, :, 5]).all()
+
+
+@pytest.mark.parametrize("n", [150])
+def test_rows_of_an_odd_column(q8, ctx, oracle, n):
+    """In a chunk with a NaN among the values, the rows before it in its column come
+    from the row-by-row form: next to the chunk form's, within both's roundings."""
+    c = Call(oracle, 13, n, "bf16", kd=128)
+    base, _ = c.run(q8, ctx)
+    c.x["v"][100, 2, 5] = np.nan
+    y, _ = c.run(q8, ctx)
+    c.x["v"][100, 2, 5] = 0
+    c.check(y, 0, 100)
+    assert np.isnan(y[100:n, 2, 5]).all()
+    _, _, most = c.exact(0, 100)
+    step = 2 * 2.0 ** -8 * np.abs(base[:100]) + 2.0 ** -13 * most
+    assert (np.abs(y[:100] - base[:100]) <= step).all()
