@@ -872,21 +872,23 @@ __global__ __launch_bounds__(kManyThreads, many_resident(D)) void attention_many
       v8bf pb[2 * KT];
 #pragma unroll
       for (int t = 0; t < KT; ++t) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          s[t][i] = exp2_f32(__builtin_fmaf(s[t][i], by, -from));
-          l += s[t][i];
-        }
         if constexpr (Q8) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const v4f vs = *(const v4f *)&scale_lds[buf][1][32 * t + 8 * j + 4 * h];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const float e = s[t][4 * j + i];
+              const float e = exp2_f32(__builtin_fmaf(s[t][4 * j + i], by, -from));
+              l += e;
               // (a masked key's scale may be anything)
-              s[t][4 * j + i] = edge && e == 0.0f ? 0.0f : e * vs[i];
+              s[t][4 * j + i] = edge && s[t][4 * j + i] == -__builtin_inff() ? 0.0f : e * vs[i];
             }
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            s[t][i] = exp2_f32(__builtin_fmaf(s[t][i], by, -from));
+            l += s[t][i];
           }
         }
 #pragma unroll

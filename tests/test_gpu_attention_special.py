@@ -283,3 +283,31 @@ def test_a_prompt_among_single_rows(q8, ctx, oracle, ns, lengths, dtype, fmt):
     c = filled(q8, ctx, oracle, rng, lengths, 32, 2, 64, fmt)
     _, q = rows_of(oracle, rng, sum(ns), 8, 64, dtype, 2.0)
     run(q8, ctx, oracle, c, ns, lengths, q, dtype, 0.125)
+
+
+@pytest.mark.parametrize("at", [20, 140, 195])
+@pytest.mark.parametrize("kind", KINDS)
+def test_nan_without_weight(q8, ctx, oracle, forced, kind, at):
+    """A Q8 row of NaN values whose key is seen and whose weight is 0 in f32 (its
+    score is 200 below the others) makes its rows NaN wherever it stands, as 0 times
+    NaN does; rows that do not see it keep their values."""
+    dtype, kernel, splits = kind
+    forced(kernel, splits)
+    rng = np.random.default_rng(at)
+    length, n, dim, page = 200, 40, 64, 64
+    c = Cache(q8, ctx, rng, [length], page, 1, dim, "q8")
+    k = np.zeros((length, 1, dim), F32)
+    k[at, 0, 0] = -200.0
+    v = rng.standard_normal((length, 1, dim)).astype(F32)
+    c.put(oracle, 0, 0, k, v)
+    c.vs[c.table[0, at // page], 0, at % page] = np.nan
+    c.upload()
+    q = np.zeros((n, 2, dim), F32)
+    q[:, :, 0] = 1.0
+    got = attend(q8, ctx, oracle, c, [n], [length], q, dtype, 1.0)
+    sees = length - n + np.arange(n) >= at
+    assert np.isnan(got[sees]).all()
+    if not sees.all():
+        kk, vv = c.values(oracle, 0, 0, at)
+        want, bound = reference(q[~sees], kk, vv, 1.0, length - n, dtype == "bf16")
+        assert (np.abs(got[~sees] - want) <= bound).all()
