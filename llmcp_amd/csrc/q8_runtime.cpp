@@ -255,6 +255,8 @@ struct Heads {
   int64_t rows = 0, heads = 0, dim = 0;
 };
 
+constexpr int64_t kMaxSpan = 1ll << 40;
+
 template <class M>
 static bool heads_of(const M *d, bool bf16, Heads &r) {
   if (!d || !d->data || d->sizes[0] < 0 || d->sizes[1] < 1 || d->sizes[2] < 1 ||
@@ -269,8 +271,11 @@ static bool heads_of(const M *d, bool bf16, Heads &r) {
   r.h.head_ld = r.heads > 1 ? d->strides[1] : r.dim;
   r.h.row_ld = r.rows > 1 ? d->strides[0] : 0;
   if ((uintptr_t)r.h.data % 16 || r.h.head_ld < r.dim || (r.heads > 1 && r.h.head_ld % per)) return false;
-  // (a row ends with its last head)
-  return r.rows <= 1 || (r.h.row_ld % per == 0 && r.h.row_ld >= (r.heads - 1) * r.h.head_ld + r.dim);
+  // a row ends with its last head; what it spans is memory (2^40 values at most)
+  const __int128 row = (__int128)(r.heads - 1) * r.h.head_ld + r.dim;
+  if (row > kMaxSpan) return false;
+  return r.rows <= 1 || (r.h.row_ld % per == 0 && r.h.row_ld >= (int64_t)row &&
+                         (__int128)(r.rows - 1) * r.h.row_ld + row <= kMaxSpan);
 }
 
 int check_rows(const Heads &x) {
