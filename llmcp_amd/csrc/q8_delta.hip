@@ -881,13 +881,13 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const ChunkArgs p) {
     ask_k(rows_of(min(n + 2, to - 1)) - 1);
     __builtin_amdgcn_sched_barrier(0);
     __syncthreads();
+    const int odd_here = odd_v[buf][col];
     v2u ul[2][4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) ul[i][t] = up[i][t][lane];
     }
-    const bool mine_odd = (__builtin_amdgcn_readfirstlane(odd_chunk) != 0) | (odd_v[buf][col] != 0);
     __builtin_amdgcn_sched_barrier(0);
     v4f o = v4f{0, 0, 0, 0}, o2 = o;
 #pragma unroll
@@ -901,6 +901,7 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const ChunkArgs p) {
     }
     o = o + o2;
     const v4f q0 = qs[0] + qs[1];
+    const bool mine_odd = (__builtin_amdgcn_readfirstlane(odd_chunk) != 0) | (odd_here != 0);
     // (rows past the last are out of the buffer's range, without a branch)
     const auto to_o = __builtin_amdgcn_make_buffer_rsrc(op, 0, 0x7fffffff, 0x00020000);
 #pragma unroll

@@ -223,3 +223,13 @@ def test_rows_of_an_odd_column(q8, ctx, oracle, n):
     _, _, most = c.exact(0, 100)
     step = 2 * 2.0 ** -8 * np.abs(base[:100]) + 2.0 ** -13 * most
     assert (np.abs(y[:100] - base[:100]) <= step).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("ns", [[200] + [1] * 30, [1] * 6 + [300], [1, 0, 90, 1, 1, 64]])
+def test_a_prompt_among_single_rows(q8, ctx, oracle, ns, dtype):
+    """One call of a prompt and sequences of one row, in either form."""
+    from test_gpu_delta_rule import Case
+    c = Case(oracle, np.random.default_rng(17), ns, 1, 2, KD, VD, dtype, pad=2).upload(ctx)
+    c.call(ctx, 0.125, 1e-6)
+    c.check(ctx, 0.125, 1e-6, *c.results(ctx))
