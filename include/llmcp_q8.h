@@ -576,31 +576,38 @@ int llmcp_q8_expert_mlp_rows_bf16(llmcp_q8_ctx *ctx, const llmcp_q8_rows *input,
  * their own numerics (f32 sums, in an order of their own).
  *
  * Rows of heads are [rows, heads, dim] with dense values (strides[2] == 1),
- * a row's heads next to each other or further apart (strides[1] >= dim,
- * strides[0] >= heads * strides[1] where rows > 1) and every head 16 B
- * aligned, so that q, k and v may be parts of one linear's output; declined
- * otherwise.  Outputs must not share memory with inputs.
+ * a row's heads next to each other or further apart (strides[1] >= dim where
+ * heads > 1, strides[0] no less than a row's extent where rows > 1) and every
+ * head 16 B aligned, so that q, k and v may be parts of one linear's output;
+ * declined otherwise.  Outputs must not share memory with inputs.
  *
  * A call takes the rows of several sequences, one sequence after another:
  * sequence s has the rows row_starts[s] .. row_starts[s + 1] - 1, none where
  * the two are equal.  row_starts ascends within 0 .. rows (bounds outside are
- * taken as 0 or rows; where it descends, what the calls leave for the sequences
- * is undefined, and nothing outside their memory is touched); rows before the first and from the last on are left as
- * they were.  Up to 2^23 rows, 65536 sequences and 1024 heads; more is
- * declined. */
+ * taken as 0 or rows; where it descends, what the calls leave for the
+ * sequences is undefined, and nothing outside their memory is touched); rows
+ * before the first and from the last on are left as they were.  Up to 2^23
+ * rows, 65536 sequences and 1024 heads; more is declined.
+ *
+ * One kernel takes a whole call, chosen by its rows per sequence on average:
+ * where a prompt and many single rows meet in one call, either part may take
+ * several times what it takes by itself (measured: the bf16 delta rule over a
+ * prompt of 4096 rows and 300 single rows 6.2 ms, in two calls 0.42; bf16
+ * attention of a prompt of 2048 rows and 31 single rows over up to 8192 keys
+ * 0.50 ms, in two calls 0.27).  Two calls, over the same cache, avoid that. */
 
 /* How a cache keeps a row of head_dim values: as bf16 (rounded to nearest
  * even), or as int8 with an f32 scale s = max|x| / 127, value q * s with q = x *
  * (1 / s) rounded to nearest even (llmcp_q8_quantize_activations' arithmetic
- * over the whole row).  Q8: a row whose largest value is below 2^-118 is kept as
- * zeros; a row with an infinity or NaN reads back as NaN. */
+ * over the whole row).  Q8: a row whose largest value is below 2^-118 is kept
+ * as zeros; a row with an infinity or NaN reads back as NaN. */
 enum llmcp_q8_cache_format { LLMCP_Q8_CACHE_BF16 = 0, LLMCP_Q8_CACHE_Q8 = 1 };
 
 /* Pages of keys and values in device memory, each [pages, kv_heads, page_size,
  * head_dim] dense and 16 B aligned; Q8: int8 with the scales [pages, kv_heads,
  * page_size].  head_dim 64, 128 or 256; page_size up to 2^20, of any value (a
- * contiguous cache is one page per sequence), and max_pages * page_size below 2^30
- * and pages * kv_heads * page_size below 2^31; declined otherwise. */
+ * contiguous cache is one page per sequence), and max_pages * page_size below
+ * 2^30 and pages * kv_heads * page_size below 2^31; declined otherwise. */
 typedef struct {
   void *keys, *values;
   float *key_scales, *value_scales; /* Q8, else null */
@@ -644,19 +651,22 @@ int llmcp_q8_kv_read_bf16(llmcp_q8_ctx *ctx, const llmcp_q8_kv_cache *cache,
 
 /* Attention of the rows over their sequences' keys (which the call's own rows
  * are among: write them first): query head h of the row at position p gives
- * sum over j <= p of softmax_j(scale * q . k_j) v_j (|scale| up to 1e38) with the keys and values of
- * kv head h / (heads / kv_heads) that the slots stand for.  heads is a multiple
- * of kv_heads, queries and output are [rows, heads, head_dim].  Positions
- * without a slot are not seen, whatever their memory holds; a row that sees no key,
- * or only scores of -inf, gives zeros.  Scores, softmax and sums are f32 (a score
- * past f32 counts as infinite: below, the key has no weight; above, or NaN, the row
- * is NaN); of bf16 rows the probabilities (times a Q8 value's scale) are rounded to bf16
+ * sum over j <= p of softmax_j(scale * q . k_j) v_j (|scale| up to 1e38) with
+ * the keys and values of kv head h / (heads / kv_heads) that the slots stand
+ * for.  heads is a multiple of kv_heads, queries and output are [rows, heads,
+ * head_dim]; rows * heads up to 2^26 and rows * heads / 16 + sequences * kv_heads
+ * below 2^23, declined otherwise.  Positions without a slot are not seen,
+ * whatever their memory holds; a row that sees no key, or only scores of -inf,
+ * gives zeros.  Scores, softmax and sums are f32 (a score past f32 counts as
+ * infinite: below, the key has no weight; above, or NaN, the row is NaN); of
+ * bf16 rows the probabilities (times a Q8 value's scale) are rounded to bf16
  * before they meet the values, f32 rows take products exact to f32.
- * Workspaces grow on the first call of a size: make it eagerly before
- * capturing it into a graph.  How keys are split over workgroups, and with it the
- * sums' order, depends on the numbers of rows, sequences, heads and pages of the
- * call and on the sequence's own rows and length, not on what the other sequences
- * hold. */
+ *
+ * Workspaces grow on the first call of a size: make it eagerly before capturing
+ * it into a graph.  The kernel, and how it splits keys over workgroups, and with
+ * them the sums' order, depend on the numbers of rows, sequences, heads and
+ * pages of the call, on the scale (0 or next to it) and on the sequence's own
+ * rows and length, not on what the other sequences hold. */
 int llmcp_q8_attention(llmcp_q8_ctx *ctx, const llmcp_memref_f32_3d *queries,
                        const llmcp_q8_kv_cache *cache, const llmcp_q8_kv_batch *batch,
                        float scale, llmcp_memref_f32_3d *output);
@@ -666,19 +676,31 @@ int llmcp_q8_attention_bf16(llmcp_q8_ctx *ctx, const llmcp_memref_bf16_3d *queri
 
 /* The gated delta rule of the linear-attention layers, over the rows of each
  * sequence in order: with a = exp(log_decay) and beta of the row and value
- * head (f32 [rows, value_heads], rows dense or further apart), k and q of key head h / (value_heads /
- * key_heads) and the state S [key_dim, value_dim] of value head h,
+ * head (f32 [rows, value_heads], rows dense or further apart), k and q of key
+ * head h / (value_heads / key_heads) and the state S [key_dim, value_dim] of
+ * value head h,
  *   u = beta * (v - a * S^T k),  S <- a * S + k u^T,  output = scale * S^T q,
  * k and q over sqrt(their sum of squares + eps) when normalize, else as they
- * are.  queries and keys [rows, key_heads, key_dim], key_dim 64 or 128; values and
- * output [rows, value_heads, value_dim], value_dim a multiple of 16 up to 1024,
- * value_heads a multiple of key_heads, sequences * value_heads * value_dim up to
- * 2^26, rows less than 2^22 values apart; declined otherwise.  row_starts [sequences + 1] in device
- * memory as for the cache's entries (null: one sequence of all rows).  state and
- * new_state [sequences, value_heads, key_dim, value_dim] f32, dense, 16 B
- * aligned: where each sequence starts (null: from zeros) and what its rows
- * leave, which may be the same memory; a sequence without rows keeps its state.
- * States and sums are f32, products of f32 precision. */
+ * are.  queries and keys [rows, key_heads, key_dim], key_dim 64 or 128; values
+ * and output [rows, value_heads, value_dim], value_dim a multiple of 16 up to
+ * 1024, value_heads a multiple of key_heads, sequences * value_heads * value_dim
+ * up to 2^26, rows less than 2^22 values apart; declined otherwise.  row_starts
+ * [sequences + 1] in device memory as for the cache's entries (null: one
+ * sequence of all rows).  state and new_state [sequences, value_heads, key_dim,
+ * value_dim] f32, dense, 16 B aligned: where each sequence starts (null: from
+ * zeros) and what its rows leave, which may be the same memory; a sequence
+ * without rows keeps its state.
+ *
+ * f32 rows, and few bf16 rows per sequence (less than 10, or 16 where the states
+ * are many, on average), go one after another in f32 (f32 rows at 1.4 us each
+ * however many there are).  More bf16 rows go in chunks of 64: what reaches the
+ * state keeps f32's bits (24 of the state and of u, decays summed in f64), what
+ * only reaches an output is taken with 16 bits of the state, of u and of exp(G_i -
+ * G_j) q_i . k_j, off by up to 2^-13 of the sum of its terms' magnitudes before it
+ * is rounded to bf16.  Log decays are meant to be 0 or less: a chunk whose rises add
+ * up to more than 1, or in which an infinity or NaN is met or made, goes row by
+ * row (in the columns concerned, where only values are), so that rows before and
+ * other columns, heads and sequences keep their values. */
 int llmcp_q8_delta_rule(llmcp_q8_ctx *ctx, const llmcp_memref_f32_3d *queries,
                         const llmcp_memref_f32_3d *keys, const llmcp_memref_f32_3d *values,
                         const llmcp_memref_f32_2d *log_decay, const llmcp_memref_f32_2d *beta,

@@ -21,10 +21,11 @@
 // meets V - K S0 in f32 matrix instructions.
 //
 // Bound by the states' stream (few rows: 32 sequences of one row and 32 heads of 128 x
-// 128 23 us for 135 MB), by latency of one row (4.6 us, about 1.3 for every further
+// 128 24 us for 135 MB), by latency of one row (4.2 us, 1.4 for every further
 // one) and of a chunk in the scan (2.2 us: three exchanges between the waves, whose
-// operands come from LDS). 4096 rows of 32 heads: 36 us for T and A (three
-// workgroups per CU), 143 for the scan's 64 chunks, its 256 workgroups one per CU.
+// operands come from LDS). 4096 rows of 32 heads: 168 us, traced apart (which takes
+// longer) 35 for T and A (three workgroups per CU) and 140 for the scan's 64 chunks,
+// its 256 workgroups one per CU.
 #include <stddef.h>
 
 #include <algorithm>
